@@ -219,6 +219,106 @@ int awqb_rmsnorm(const void* input, const void* weight, void* out, int64_t M, in
 int awqb_fused_add_rmsnorm(void* input, void* residual, const void* weight, int64_t M, int64_t N,
                            int64_t ld_in, int64_t ld_res, float eps, int dtype, void* stream);
 
+/* The norms around a block, fused with its gate and residual scale: the step
+ * between one block's projection output x and the next block's input. Per row,
+ * in fp32:
+ *   b = post_weight ? x * rsqrt(mean(x * x) + eps) * (weight_offset + post_weight) : x
+ *   h = residual + scale * act(gate) * b
+ *   residual_out = h (rounded to the residual's type)
+ *   out = h * rsqrt(mean(h * h) + eps) * (weight_offset + weight)
+ * where the second norm is taken over the unrounded h, as in
+ * awqb_fused_add_rmsnorm. post_weight, gate and weight (with out) may be null:
+ * no norm after the block, a gate of 1, no norm before the next block; one of
+ * post_weight and weight must be given. weight_offset is 0, or 1 for models
+ * that store their norm weights minus one. x, the weights, gate and out are of
+ * `dtype`; residual and residual_out are fp32 if residual_f32 != 0, else of
+ * `dtype`. Element (m, n) of the gate is gate[m * gate_row + n * gate_col]
+ * with gate_col 0 or 1 (0, 1: per channel; 1, 0: per row). gate_act: 0 none,
+ * 1 sigmoid, 2 tanh, 3 SiLU. N is a multiple of 8, at most 16384; row strides
+ * ld_* (and gate_row where gate_col is 1) are in elements, multiples of 8;
+ * pointers 16-byte aligned. out may equal x and residual_out may equal
+ * residual; other overlaps are not allowed. Extends RMSNormFused,
+ * srt/model_executor/layers/norm.py:28-47. */
+int awqb_gated_add_rmsnorm(const void* x, int64_t ld_x, const void* residual, int64_t ld_res, int residual_f32,
+                           const void* post_weight, const void* gate, int64_t gate_row, int64_t gate_col,
+                           int gate_act, float scale, const void* weight, float weight_offset, void* out,
+                           int64_t ld_out, void* residual_out, int64_t ld_res_out, int64_t M, int64_t N,
+                           float eps, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Rotary positions of q and k between the QKV projection and attention, with
+ * the per-head RMSNorm of q and k (if q_weight / k_weight are given) folded in.
+ * Head h of token m starts at q + m * q_row + h * q_head (elements), likewise
+ * k and the outputs, so q and k may be slices of the merged projection's
+ * output. Per head, in fp32 with one rounding at the end:
+ *   v = q_weight ? q * rsqrt(mean(q * q) + eps) * q_weight : q
+ *   pair j < rot_dim / 2 of v (elements j and j + rot_dim / 2, or 2j and 2j + 1
+ *   if interleaved) turns by the angle positions[m] * inv_freq[j]: (a, b) ->
+ *   scale * (a cos - b sin, a sin + b cos); elements from rot_dim on stay.
+ * inv_freq is fp64 and the angle is reduced in fp64, so far positions keep
+ * their accuracy; a long-context scaling enters through inv_freq and scale.
+ * positions are int32, or int64 if positions_i64 != 0. A token with a negative
+ * position is padding: its outputs are left as they were. Outputs may be the
+ * inputs (in place); other overlaps are not allowed. head_dim is a multiple of
+ * 8, at most 256; rot_dim is even, 2..head_dim; strides are multiples of 8
+ * and pointers of q, k, the weights and outputs 16-byte aligned. Hk may be 0
+ * (no k). Replaces the rotary call of RopeAttn, models/blocks.py:134-139 and
+ * layers/rotary.py. */
+int awqb_rotary(const void* q, int64_t q_row, int64_t q_head, int64_t Hq, const void* k, int64_t k_row,
+                int64_t k_head, int64_t Hk, const void* positions, int positions_i64, const double* inv_freq,
+                int64_t rot_dim, int64_t head_dim, int64_t M, int interleaved, float scale,
+                const void* q_weight, const void* k_weight, float eps, void* q_out, int64_t q_out_row,
+                int64_t q_out_head, void* k_out, int64_t k_out_row, int64_t k_out_head, int dtype,
+                void* stream);
+
+/* ------------------------------------------------------------------------
+ * Work on rows that belong to groups (experts, adapters).
+ * ------------------------------------------------------------------------ */
+/* Stable grouping of n ids: order [n] lists the indices whose id is begin, then
+ * those whose id is begin + 1, ..., then all others (in no group), each in
+ * index order; group g's indices are order[offsets[g] .. offsets[g + 1]),
+ * offsets [groups + 1], offsets[0] = 0. groups is 1..1024. The workspace
+ * (awqb_group_rows_workspace_bytes; none for small n) needs no zeroing.
+ * Replaces the sort of moe_align_block_size, fused.py:34-61, without padding. */
+int64_t awqb_group_rows_workspace_bytes(int64_t n, int64_t groups);
+int awqb_group_rows(const int32_t* ids, int64_t n, int64_t begin, int64_t groups, int32_t* order,
+                    int32_t* offsets, void* workspace, int64_t workspace_bytes, void* stream);
+/* Matrix products grouped by expert over 16-bit weights w [E][N][K]:
+ *   y[r] = x[r] w[e]^T for offsets[e] <= r < offsets[e + 1]
+ * (fp32 accumulation, one rounding), or with silu_mul != 0, w [E][2I][K] holding
+ * the gate rows and then the up rows (N = 2I), y[r] = silu(gate) * up (I
+ * features). offsets [E + 1] is on the device, does not decrease and stays in
+ * 0..rows (values outside are clamped); rows of x outside
+ * [offsets[0], offsets[E]) are not computed. With row_map, y[r] goes to row
+ * row_map[r] of out (rows that map outside 0..out_rows - 1 are dropped), else
+ * to row r; with row_scale (fp32) it is multiplied by row_scale[its out row].
+ * Rows of out that nothing maps to are left as they were. K is a multiple of 8,
+ * N of 8 (16 with silu_mul); ldx and ldo are in elements, multiples of 8;
+ * x, w and out 16-byte aligned. out must not overlap the inputs. E <= 1024.
+ * Replaces fused_moe_kernel over dense experts, kernels/triton/fused_moe.py:155-285. */
+int awqb_grouped_gemm(const void* x, int64_t rows, int64_t ldx, const void* w, int64_t E, int64_t K, int64_t N,
+                      const int32_t* offsets, int dtype, int silu_mul, const int32_t* row_map,
+                      const float* row_scale, void* out, int64_t out_rows, int64_t ldo, void* stream);
+/* Low-rank adapters of many requests beside a shared projection:
+ *   out[t] = base[t] + scales[a] * (x[t] a[a]^T) b[a]^T
+ * for the rows t = order[offsets[a] .. offsets[a + 1]) of adapter a; rows in no
+ * adapter (the rest of order) get out = base. A merged projection (QKV,
+ * gate_up) has num_slices > 1 slices of its N outputs (slices: their widths, on
+ * the host, adding up to N; null with num_slices 1), each with its own pair: a
+ * [L][num_slices * rank][K] stacks the slices' first factors, b [L][N][rank]
+ * their second ones. Sums are fp32; the product of the first factor is kept in
+ * fp32 (as two 16-bit halves in the tensor cores). scales [L] fp32 or null (1).
+ * order [M] and offsets [L + 1] as awqb_group_rows gives them: order is a
+ * permutation of the rows (an entry outside 0..M - 1 is skipped). out may
+ * equal base. K is a multiple of 8, the slice widths of 8, rank of 8 and at
+ * most 128, num_slices at most 4, L at most 1024; row strides are in elements,
+ * multiples of 8; pointers 16-byte aligned. No counterpart in the reference. */
+int awqb_lora_workspace_bytes(int64_t M, int64_t K, int64_t L, int64_t rank, int64_t num_slices, int64_t* bytes);
+int awqb_lora(const void* x, int64_t M, int64_t ldx, int64_t K, const void* a, const void* b, int64_t L,
+              int64_t rank, int64_t N, const int64_t* slices, int64_t num_slices, const int32_t* order,
+              const int32_t* offsets, const float* scales, const void* base, int64_t ld_base, void* out,
+              int64_t ld_out, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------
  * Tensor-parallel all-reduce. Replaces NCCLWrapper (create_nccl_uid, ctor,
  * all_reduce), kernels/csrc/src/pynccl.cu:75-189, used through

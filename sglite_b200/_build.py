@@ -28,6 +28,11 @@ SOURCES = [
     "awqb_gemm.cu",
     "awqb_moe.cu",
     "awqb_norm.cu",
+    "awqb_gated_norm.cu",
+    "awqb_rotary.cu",
+    "awqb_group.cu",
+    "awqb_grouped_gemm.cu",
+    "awqb_lora.cu",
     "awqb_nccl.cpp",
 ]
 

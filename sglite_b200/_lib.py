@@ -63,6 +63,21 @@ _SIGNATURES = {
     "awqb_rmsnorm": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, ctypes.c_float, c_int, c_vp]),
     "awqb_fused_add_rmsnorm": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, ctypes.c_float, c_int,
                                        c_vp]),
+    "awqb_gated_add_rmsnorm": (
+        c_int, [c_vp, c_i64, c_vp, c_i64, c_int, c_vp, c_vp, c_i64, c_i64, c_int, ctypes.c_float, c_vp, ctypes.c_float,
+                c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, ctypes.c_float, c_int, c_vp]),
+    "awqb_rotary": (
+        c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_i64, c_i64, c_i64, c_int,
+                ctypes.c_float, c_vp, c_vp, ctypes.c_float, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_vp]),
+    "awqb_group_rows_workspace_bytes": (c_i64, [c_i64, c_i64]),
+    "awqb_group_rows": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "awqb_grouped_gemm": (
+        c_int, [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_int, c_vp, c_vp, c_vp, c_i64, c_i64,
+                c_vp]),
+    "awqb_lora_workspace_bytes": (c_int, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64p]),
+    "awqb_lora": (
+        c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64,
+                c_vp, c_i64, c_int, c_vp, c_i64, c_vp]),
     "awqb_moe_topk_sum": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_vp, c_vp]),
     "awqb_nccl_unique_id_bytes": (c_int, []),
     "awqb_nccl_get_unique_id": (c_int, [c_vp]),

@@ -24,6 +24,10 @@ const char* get_last_error();
 
 int device_sm_count();  // of the current device, cached per device
 
+// The current device's error word (the one awqb_device_error reads; kernels OR
+// bits into it when a bounded wait gives up); nullptr if it cannot be found.
+uint32_t* device_error_word();
+
 }  // namespace awqb
 
 #define AWQB_REQUIRE(cond, code, ...)                        \

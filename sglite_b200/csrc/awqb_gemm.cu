@@ -14,16 +14,15 @@
 #include "awqb_common.h"
 #include "awqb_gemm.cuh"
 #include "awqb_gemv.cuh"
+#include "awqb_tma.h"
 
 namespace awqb {
 
 __device__ uint32_t g_awqb_err;  // OR of DeviceError bits, cleared by awqb_clear_device_error
 
-namespace {
-
 constexpr int kMaxDevices = 64;
 
-uint32_t* device_err_ptr() {
+uint32_t* device_error_word() {
   static uint32_t* ptrs[kMaxDevices] = {};
   static std::mutex mu;
   int dev = 0;
@@ -50,6 +49,8 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   });
   return fn;
 }
+
+namespace {
 
 // Activation tensor map, 128-byte swizzle, out-of-range elements read as zero.
 // K % 64 == 0: a 3-D view {64, rows, K/64} (strides K*2 and 128 bytes) whose box
@@ -587,7 +588,7 @@ int gemv_impl(const void* x, int64_t M, int64_t K, int64_t N, int64_t G, int dty
   int st = gemv_plan(M, K, N, G, F_req, W_req, ring_req, &gp);
   if (st != kOk) return st;
   AWQB_REQUIRE(K % 32 == 0, kUnsupported, "K=%lld must be a multiple of 32", (long long)K);
-  uint32_t* err = device_err_ptr();
+  uint32_t* err = device_error_word();
   AWQB_REQUIRE(err != nullptr, kCudaError, "cannot resolve the device error word");
   CUtensorMap tw, ts, tz, tx;
   st = make_gemv_maps(x, blob, M, K, N, gp, &tw, &ts, &tz, &tx);
@@ -663,7 +664,7 @@ int gemm_impl(const void* x, int64_t M, int64_t K, int64_t N, int64_t G, int dty
   AWQB_REQUIRE(workspace_bytes >= pl.cnt_bytes + pl.part_bytes, kInvalidArgument,
                "workspace too small: %lld < %lld bytes", (long long)workspace_bytes,
                (long long)(pl.cnt_bytes + pl.part_bytes));
-  uint32_t* err = device_err_ptr();
+  uint32_t* err = device_error_word();
   AWQB_REQUIRE(err != nullptr, kCudaError, "cannot resolve the device error word");
 
   CUtensorMap tm;
@@ -927,7 +928,7 @@ int grouped_impl(const void* x_sorted, int64_t rows_max, int64_t K, int64_t N,
   AWQB_REQUIRE(workspace_bytes >= pl.cnt_bytes + pl.part_bytes, kInvalidArgument,
                "workspace too small: %lld < %lld bytes", (long long)workspace_bytes,
                (long long)(pl.cnt_bytes + pl.part_bytes));
-  uint32_t* err = device_err_ptr();
+  uint32_t* err = device_error_word();
   AWQB_REQUIRE(err != nullptr, kCudaError, "cannot resolve the device error word");
   CUtensorMap tm;
   int is3d = 0;

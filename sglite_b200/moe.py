@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import re
 from dataclasses import dataclass
-from typing import Dict, Optional, Tuple
+from typing import Dict, Optional, Tuple, Union
 
 import torch
 
@@ -75,6 +75,42 @@ class AWQExpertWeights:
         return cls(blob, K, N8 * 8, G, scales.dtype, e_begin, num_global_experts, inter)
 
 
+@dataclass
+class DenseExpertWeights:
+    """A rank's 16-bit experts of one projection, as the reference's MoELayer holds
+    them (layers/moe_layer.py:36-47): gate_up [E, 2I, H] (the gate rows, then the
+    up rows), down [E, H, I]. For checkpoints that leave their experts
+    unquantised."""
+
+    w: torch.Tensor              # [E_local, N, K]
+    e_begin: int = 0             # first global expert id held here
+    num_global_experts: Optional[int] = None
+
+    def __post_init__(self):
+        if self.w.dim() != 3 or self.w.dtype not in ops.DTYPE_CODE:
+            raise ValueError("dense experts are a float16 or bfloat16 [E, N, K] tensor")
+
+    @property
+    def num_experts(self) -> int:
+        return self.w.shape[0]
+
+    @property
+    def N(self) -> int:
+        return self.w.shape[1]
+
+    @property
+    def K(self) -> int:
+        return self.w.shape[2]
+
+    @property
+    def act_dtype(self) -> torch.dtype:
+        return self.w.dtype
+
+    @property
+    def e_end(self) -> int:
+        return self.e_begin + self.num_experts
+
+
 def choose_block_m(num_tokens: int, topk: int, num_experts: int) -> int:
     """Rows per expert block (the grouped GEMM's token tile), from the mean
     number of rows per expert. Measured on B200 (Qwen3-30B-A3B experts): a
@@ -92,20 +128,27 @@ def choose_block_m(num_tokens: int, topk: int, num_experts: int) -> int:
     return 128
 
 
-class AWQB200MoeBackend(BaseMoeBackend):
-    """MoE backend over AWQ int4 experts (registered as "awq_b200")."""
+ExpertWeights = Union[AWQExpertWeights, DenseExpertWeights]
 
-    def forward(self, hidden_states: torch.Tensor, w1: AWQExpertWeights, w2: AWQExpertWeights,
+
+class AWQB200MoeBackend(BaseMoeBackend):
+    """MoE backend over AWQ int4 experts (registered as "awq_b200"). 16-bit experts
+    (``DenseExpertWeights``, or the plain [E, N, K] tensors that the reference's
+    backends take) run on the grouped 16-bit kernel."""
+
+    def forward(self, hidden_states: torch.Tensor, w1: ExpertWeights, w2: ExpertWeights,
                 gating_output: torch.Tensor, topk: int, renormalize: bool, activation: str = "silu",
                 apply_router_weight_on_input: bool = False) -> torch.Tensor:
         if activation != "silu":
             raise ValueError(f"activation {activation!r} not supported by the AWQ B200 MoE backend")
         if apply_router_weight_on_input:
             raise ValueError("router weights are applied to the down-projection output only")
+        if isinstance(w1, torch.Tensor) and isinstance(w2, torch.Tensor):
+            w1, w2 = DenseExpertWeights(w1), DenseExpertWeights(w2)
         topk_weights, topk_ids = ops.moe_topk_softmax(gating_output, topk, renormalize)
         return self.experts(hidden_states, w1, w2, topk_weights, topk_ids)
 
-    def experts(self, hidden_states: torch.Tensor, w1: AWQExpertWeights, w2: AWQExpertWeights,
+    def experts(self, hidden_states: torch.Tensor, w1: ExpertWeights, w2: ExpertWeights,
                 topk_weights: torch.Tensor, topk_ids: torch.Tensor) -> torch.Tensor:
         x = hidden_states
         if not x.is_contiguous():
@@ -120,6 +163,10 @@ class AWQB200MoeBackend(BaseMoeBackend):
             raise ValueError("w1 and w2 hold different experts")
         E_glob = w1.num_global_experts or w1.num_experts
         numel = M * topk
+        if isinstance(w1, DenseExpertWeights) != isinstance(w2, DenseExpertWeights):
+            raise ValueError("w1 and w2 must both be AWQ or both be 16-bit experts")
+        if isinstance(w1, DenseExpertWeights):
+            return self._dense_experts(x, w1, w2, topk_weights, topk_ids, E_glob)
         block_m = choose_block_m(M, topk, E_glob)
         sorted_ids, block_expert, npp = ops.moe_align(topk_ids, w1.e_begin, w1.e_end, block_m)
         rows = sorted_ids.numel()
@@ -139,6 +186,24 @@ class AWQB200MoeBackend(BaseMoeBackend):
         ids = topk_ids if (w1.e_begin != 0 or w1.e_end != E_glob) else None
         ops.moe_topk_sum(y3, M, topk, ids, w1.e_begin, w1.e_end, hidden_states)
         return hidden_states
+
+
+    def _dense_experts(self, x: torch.Tensor, w1: DenseExpertWeights, w2: DenseExpertWeights,
+                       topk_weights: torch.Tensor, topk_ids: torch.Tensor, E_glob: int) -> torch.Tensor:
+        """The same pipeline over 16-bit experts: the rows are grouped without
+        padding, and the kernel reads the groups' bounds on the device."""
+        M, H = x.shape
+        topk = topk_ids.shape[1]
+        numel = M * topk
+        if numel == 0:
+            return x
+        order, offsets = ops.group_rows(topk_ids.reshape(-1), w1.num_experts, w1.e_begin)
+        xs = ops.moe_gather_rows(x, order, offsets[-1:], topk, numel)
+        a = ops.grouped_gemm(xs, w1.w, offsets, silu_mul=True)
+        y3 = torch.empty((numel, H), dtype=x.dtype, device=x.device)
+        ops.grouped_gemm(a, w2.w, offsets, out=y3, row_map=order, row_scale=topk_weights.reshape(-1).contiguous())
+        ids = topk_ids if (w1.e_begin != 0 or w1.e_end != E_glob) else None
+        return ops.moe_topk_sum(y3, M, topk, ids, w1.e_begin, w1.e_end, x)
 
 
 def route(gating_output: torch.Tensor, topk: int, renormalize: bool) -> Tuple[torch.Tensor, torch.Tensor]:

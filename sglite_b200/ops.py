@@ -552,3 +552,284 @@ def moe_topk_sum(y3: torch.Tensor, M: int, topk: int, topk_ids: Optional[torch.T
         call("awqb_moe_topk_sum", _p(y3), M, topk, H, _p(topk_ids), e_begin, e_end, _dtype_code(y3.dtype),
              _p(out), _stream(dev))
     return out
+
+
+# ---------------------------------------------------------------- around the projections
+_FN: Dict[str, object] = {}
+
+
+def _launch(name: str, device_index: int, *args) -> None:
+    """Call a C-ABI entry point with ``device_index`` current and its stream last."""
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(lib(), name)
+    prev = _cur_device()
+    if prev == device_index:
+        check(fn(*args, _raw_stream(device_index)))
+        return
+    torch.cuda.set_device(device_index)
+    try:
+        check(fn(*args, _raw_stream(device_index)))
+    finally:
+        torch.cuda.set_device(prev)
+
+
+def _on(device_index: int, **tensors: Optional[torch.Tensor]) -> None:
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or t.get_device() != device_index):
+            raise ValueError(f"{name} must live on the same CUDA device as the other tensors (there is no CPU path)")
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+GATE_ACTIVATIONS = {"none": 0, "sigmoid": 1, "tanh": 2, "silu": 3}
+
+
+def gated_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor], eps: float, *,
+                      post_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                      gate_act: str = "none", scale: float = 1.0, weight_offset: float = 0.0,
+                      out: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None
+                      ) -> Tuple[Optional[torch.Tensor], torch.Tensor]:
+    """The norms around a block with its gate and residual scale:
+    ``b = rmsnorm(x) * (weight_offset + post_weight)`` (or x without post_weight),
+    ``h = residual + scale * gate_act(gate) * b`` and
+    ``y = rmsnorm(h) * (weight_offset + weight)``, fp32 inside, the second norm over
+    the unrounded h. Returns (y, h); y is None without ``weight``.
+
+    gate broadcasts over x: the shape of x, [N] or [1, N] (per channel), [.., 1]
+    (per row) or one value. residual is of x's dtype or float32. ``out`` may be x
+    and ``residual_out`` may be residual (in place)."""
+    code = _dtype_code(x.dtype)
+    if not x.is_cuda:
+        raise ValueError("tensors must live on a CUDA device (there is no CPU path)")
+    N = x.shape[-1]
+    di = x.get_device()
+    if residual.shape != x.shape or (residual.dtype != x.dtype and residual.dtype != torch.float32):
+        raise ValueError("residual must have the shape of x and its dtype or float32")
+    for w in (weight, post_weight):
+        if w is not None and (w.numel() != N or w.dtype != x.dtype or not w.is_contiguous()):
+            raise ValueError("norm weights must be contiguous [N] tensors in the activation dtype")
+    act = GATE_ACTIVATIONS.get(gate_act)
+    if act is None:
+        raise ValueError(f"gate activation {gate_act!r}: one of {tuple(GATE_ACTIVATIONS)}")
+    x2, ldx = _rows_2d(x, N)
+    r2, ldr = _rows_2d(residual, N)
+    M = x2.shape[0]
+    gate_row = gate_col = 0
+    if gate is not None:
+        if gate.dtype != x.dtype:
+            raise ValueError("gate must have the activation dtype")
+        wide = gate.dim() > 0 and gate.shape[-1] == N
+        if not wide and gate.dim() > 0 and gate.shape[-1] != 1:
+            raise ValueError(f"gate {tuple(gate.shape)} does not broadcast over x {tuple(x.shape)}")
+        rows = gate.numel() // N if wide else gate.numel()
+        if rows != 1 and (rows != M or gate.shape[:-1] != x.shape[:-1]):
+            raise ValueError(f"gate {tuple(gate.shape)} does not broadcast over x {tuple(x.shape)}")
+        if gate.dim() > 2 and rows > 1 and not gate.is_contiguous():
+            raise ValueError("tensors with more than 2 dimensions must be contiguous")
+        if wide and gate.stride(-1) != 1:
+            raise ValueError("the last dimension must be the contiguous feature dimension")
+        gate_col = 1 if wide else 0
+        if rows > 1:
+            gate_row = gate.stride(-2)
+    if weight is None:
+        if out is not None:
+            raise ValueError("out is the second norm's result: it needs weight")
+        ldo = 0
+    else:
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        elif out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError("out must have the shape and dtype of x")
+        _, ldo = _rows_2d(out, N)
+    if residual_out is None:
+        residual_out = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+    elif residual_out.shape != x.shape or residual_out.dtype != residual.dtype:
+        raise ValueError("residual_out must have the shape and dtype of residual")
+    _, ldro = _rows_2d(residual_out, N)
+    _on(di, residual=residual, weight=weight, post_weight=post_weight, gate=gate, out=out, residual_out=residual_out)
+    _launch("awqb_gated_add_rmsnorm", di, x2.data_ptr(), ldx, r2.data_ptr(), ldr, residual.dtype == torch.float32,
+            _ptr(post_weight), _ptr(gate), gate_row, gate_col, act, scale, _ptr(weight), weight_offset, _ptr(out), ldo,
+            residual_out.data_ptr(), ldro, M, N, eps, code)
+    return out, residual_out
+
+
+def _token_head_strides(t: torch.Tensor) -> Tuple[int, int]:
+    """Strides of the token and head dimensions; a dimension of one has none."""
+    s0, s1, _ = t.stride()
+    return (s0 if t.shape[0] > 1 else 0), (s1 if t.shape[1] > 1 else 0)
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, *,
+           interleaved: bool = False, scale: float = 1.0, q_weight: Optional[torch.Tensor] = None,
+           k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, q_out: Optional[torch.Tensor] = None,
+           k_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Rotary positions of q [M, Hq, D] and k [M, Hk, D] (slices of the merged QKV
+    output will do: any token and head strides), after the per-head RMSNorm when
+    q_weight / k_weight [D] are given. positions [M] int32 or int64; inv_freq
+    float64 [rot_dim / 2] (``rotary.RotaryEmbedding`` makes it, long-context
+    scalings included); the first rot_dim elements of a head turn, in pairs
+    (j, j + rot_dim / 2) or, interleaved, (2j, 2j + 1). ``scale`` multiplies the
+    turned elements. Tokens with a negative position are padding: their
+    outputs are left as they were. ``q_out`` / ``k_out`` may be q / k (in place)."""
+    code = _dtype_code(q.dtype)
+    if q.dim() != 3 or not q.is_cuda:
+        raise ValueError("q must be a [tokens, heads, head_dim] tensor on a CUDA device (there is no CPU path)")
+    di = q.get_device()
+    M, Hq, D = q.shape
+    if q.stride(2) != 1:
+        raise ValueError("the head dimension must be contiguous")
+    if positions.numel() != M or positions.dim() != 1 or positions.dtype not in (torch.int32, torch.int64) \
+            or not positions.is_contiguous():
+        raise ValueError("positions must be a contiguous int32 or int64 [tokens] tensor")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous float64 [rot_dim / 2] tensor")
+    if q_out is None:
+        q_out = torch.empty((M, Hq, D), dtype=q.dtype, device=q.device)
+    elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(2) != 1:
+        raise ValueError("q_out must have the shape and dtype of q and contiguous heads")
+    sq, so = _token_head_strides(q), _token_head_strides(q_out)
+    if k is None:
+        if k_out is not None or k_weight is not None:
+            raise ValueError("k_out and k_weight need k")
+        Hk, kp, kop, sk, sko = 0, None, None, (0, 0), (0, 0)
+    else:
+        if k.dim() != 3 or k.shape[0] != M or k.shape[2] != D or k.dtype != q.dtype or k.stride(2) != 1:
+            raise ValueError("k must be a [tokens, heads, head_dim] tensor with q's tokens, head_dim and dtype")
+        Hk = k.shape[1]
+        if k_out is None:
+            k_out = torch.empty((M, Hk, D), dtype=q.dtype, device=q.device)
+        elif k_out.shape != k.shape or k_out.dtype != k.dtype or k_out.stride(2) != 1:
+            raise ValueError("k_out must have the shape and dtype of k and contiguous heads")
+        kp, kop, sk, sko = k.data_ptr(), k_out.data_ptr(), _token_head_strides(k), _token_head_strides(k_out)
+    for w in (q_weight, k_weight):
+        if w is not None and (w.numel() != D or w.dtype != q.dtype or not w.is_contiguous()):
+            raise ValueError("the norm weights must be contiguous [head_dim] tensors in q's dtype")
+    _on(di, k=k, positions=positions, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight, q_out=q_out, k_out=k_out)
+    _launch("awqb_rotary", di, q.data_ptr(), sq[0], sq[1], Hq, kp, sk[0], sk[1], Hk, positions.data_ptr(),
+            positions.dtype == torch.int64, inv_freq.data_ptr(), 2 * inv_freq.numel(), D, M, interleaved, scale,
+            _ptr(q_weight), _ptr(k_weight), eps, q_out.data_ptr(), so[0], so[1], kop, sko[0], sko[1], code)
+    return q_out, k_out
+
+
+def group_rows(ids: torch.Tensor, num_groups: int, begin: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Stable grouping of rows by id: (order [n], offsets [num_groups + 1]), int32.
+    ``order[offsets[g]:offsets[g + 1]]`` are the indices whose id is begin + g, in
+    index order; indices whose id is in no group come last."""
+    if ids.dtype != torch.int32 or not ids.is_contiguous() or not ids.is_cuda:
+        raise ValueError("ids must be a contiguous int32 tensor on a CUDA device")
+    di, n = ids.get_device(), ids.numel()
+    order = torch.empty(n, dtype=torch.int32, device=ids.device)
+    offsets = torch.empty(max(num_groups, 0) + 1, dtype=torch.int32, device=ids.device)
+    nb = int(lib().awqb_group_rows_workspace_bytes(n, num_groups))
+    ws = torch.empty(nb, dtype=torch.uint8, device=ids.device) if nb > 0 else None
+    _launch("awqb_group_rows", di, ids.data_ptr(), n, begin, num_groups, order.data_ptr(), offsets.data_ptr(), _ptr(ws),
+            nb)
+    return order, offsets
+
+
+def _offsets_ok(offsets: torch.Tensor, groups: int, what: str) -> None:
+    if offsets.dtype != torch.int32 or offsets.numel() != groups + 1 or not offsets.is_contiguous():
+        raise ValueError(f"offsets must be a contiguous int32 [{what} + 1] tensor")
+
+
+def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out: Optional[torch.Tensor] = None,
+                 silu_mul: bool = False, row_map: Optional[torch.Tensor] = None,
+                 row_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Matrix products grouped by expert over 16-bit weights w [E, N, K]:
+    ``y[r] = x[r] @ w[e].T`` for ``offsets[e] <= r < offsets[e + 1]``, fp32
+    accumulation; with silu_mul, w holds the gate rows and then the up rows and
+    ``y = silu(gate) * up`` [.., N / 2]. offsets [E + 1] int32 stays on the device
+    and must not decrease.
+
+    y[r] goes to row r of ``out``, or to row row_map[r] (int32 [rows]; rows that
+    map outside ``out`` are dropped), times row_scale[its row of out] (fp32) if
+    given. Rows of ``out`` that nothing goes to are left as they were; without
+    ``out`` a new [rows, N] tensor is returned, in which those rows are undefined."""
+    code = _dtype_code(x.dtype)
+    if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[2]:
+        raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)} must be [rows, K] and [experts, N, K]")
+    if not x.is_cuda:
+        raise ValueError("tensors must live on a CUDA device (there is no CPU path)")
+    if w.dtype != x.dtype or not w.is_contiguous() or (x.stride(1) != 1 and x.shape[1] != 1):
+        raise ValueError("w must be contiguous and of x's dtype, and x's rows contiguous")
+    di = x.get_device()
+    rows, K = x.shape
+    E, N, _ = w.shape
+    _offsets_ok(offsets, E, "experts")
+    n_out = N // 2 if silu_mul else N
+    if out is None:
+        out = torch.empty((rows, n_out), dtype=x.dtype, device=x.device)
+    elif out.dim() != 2 or out.shape[1] != n_out or out.dtype != x.dtype or out.stride(1) != 1:
+        raise ValueError(f"out must be a [rows, {n_out}] tensor of x's dtype with contiguous rows")
+    if row_map is not None and (row_map.dtype != torch.int32 or row_map.numel() != rows or not row_map.is_contiguous()):
+        raise ValueError("row_map must be a contiguous int32 [rows] tensor")
+    if row_scale is not None and (row_scale.dtype != torch.float32 or row_scale.numel() != out.shape[0]
+                                  or not row_scale.is_contiguous()):
+        raise ValueError("row_scale must be a contiguous float32 tensor with one value for each row of out")
+    _on(di, w=w, offsets=offsets, out=out, row_map=row_map, row_scale=row_scale)
+    _launch("awqb_grouped_gemm", di, x.data_ptr(), rows, x.stride(0) if rows > 1 else K, w.data_ptr(), E, K, N,
+            offsets.data_ptr(), code, silu_mul, _ptr(row_map), _ptr(row_scale), out.data_ptr(), out.shape[0],
+            out.stride(0) if out.shape[0] > 1 else n_out)
+    return out
+
+
+_LORA_BYTES: Dict[Tuple[int, int, int, int, int], int] = {}
+_SLICES: Dict[Tuple[int, ...], object] = {}
+
+
+def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor,
+         base: torch.Tensor, *, slices: Optional[Tuple[int, ...]] = None, scales: Optional[torch.Tensor] = None,
+         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Low-rank adapters of many requests beside a shared projection:
+    ``out[t] = base[t] + scales[l] * (x[t] @ a[l].T) @ b[l].T`` for the rows t that
+    use adapter l, ``out[t] = base[t]`` for rows without one. x [M, K]; base [M, N]
+    is the projection's output; ``order``, ``offsets`` are ``group_rows`` of the
+    rows' adapter numbers (one call serves every projection of a step).
+
+    slices: widths of a merged projection's parts (QKV, gate_up), each with its own
+    pair; a [L, len(slices) * rank, K] stacks their first factors, b [L, N, rank] the
+    second ones. Sums are fp32. ``out`` may be base (in place)."""
+    code = _dtype_code(x.dtype)
+    if x.dim() != 2 or a.dim() != 3 or b.dim() != 3 or base.dim() != 2 or not x.is_cuda:
+        raise ValueError("x [M, K], a [L, slices * rank, K], b [L, N, rank] and base [M, N] must be CUDA tensors "
+                         "(there is no CPU path)")
+    M, K = x.shape
+    L, N, rank = b.shape
+    slices = (N,) if slices is None else tuple(slices)
+    if a.shape != (L, len(slices) * rank, K) or base.shape != (M, N):
+        raise ValueError(f"inconsistent shapes: x {tuple(x.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)}, "
+                         f"base {tuple(base.shape)}, {len(slices)} slices")
+    if a.dtype != x.dtype or b.dtype != x.dtype or base.dtype != x.dtype or not a.is_contiguous() \
+            or not b.is_contiguous():
+        raise ValueError("a, b and base must be of x's dtype, a and b contiguous")
+    if (x.stride(1) != 1 and K != 1) or (base.stride(1) != 1 and N != 1):
+        raise ValueError("the rows of x and base must be contiguous")
+    if order.dtype != torch.int32 or order.numel() != M or not order.is_contiguous():
+        raise ValueError("order must be a contiguous int32 [M] tensor")
+    _offsets_ok(offsets, L, "adapters")
+    if scales is not None and (scales.dtype != torch.float32 or scales.numel() != L or not scales.is_contiguous()):
+        raise ValueError("scales must be a contiguous float32 [adapters] tensor")
+    if out is None:
+        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    elif out.shape != base.shape or out.dtype != x.dtype or out.stride(1) != 1:
+        raise ValueError("out must be a [M, N] tensor of x's dtype with contiguous rows")
+    di = x.get_device()
+    _on(di, a=a, b=b, order=order, offsets=offsets, base=base, scales=scales, out=out)
+    key = (M, K, L, rank, len(slices))
+    nb = _LORA_BYTES.get(key)
+    if nb is None:
+        v = c_i64(0)
+        call("awqb_lora_workspace_bytes", M, K, L, rank, len(slices), ctypes.byref(v))
+        nb = _LORA_BYTES[key] = v.value
+    widths = _SLICES.get(slices)
+    if widths is None:
+        widths = _SLICES[slices] = (c_i64 * len(slices))(*slices)
+    # from the caching allocator: private to the stream, or to the graph being captured
+    ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=x.device)
+    _launch("awqb_lora", di, x.data_ptr(), M, x.stride(0) if M > 1 else K, K, a.data_ptr(), b.data_ptr(), L, rank, N,
+            widths, len(slices), order.data_ptr(), offsets.data_ptr(), _ptr(scales), base.data_ptr(),
+            base.stride(0) if M > 1 else N, out.data_ptr(), out.stride(0) if M > 1 else N, code, ws.data_ptr(), nb)
+    return out

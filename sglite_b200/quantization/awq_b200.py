@@ -16,6 +16,7 @@ import torch
 from torch.nn.parameter import Parameter
 
 from .. import ops
+from ..lora import LoraAdapters, LoraBatch
 from .base_config import LinearMethodBase, QuantizationConfig, set_weight_attrs
 
 SUPPORTED_GROUP_SIZES = (-1, 32, 64, 128)
@@ -155,7 +156,12 @@ class AWQB200LinearMethod(LinearMethodBase):
         }
 
     def apply_weights(self, weights: Dict[str, Any], x: torch.Tensor,
-                      bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                      bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                      adapters: Optional[LoraAdapters] = None, batch: Optional[LoraBatch] = None) -> torch.Tensor:
+        """x W (+ bias); with ``adapters``, plus each row's low-rank adapter
+        (``batch`` says which row uses which)."""
+        if adapters is not None and batch is None:
+            raise ValueError("adapters need the batch that says which row uses which adapter")
         if not weights.get("_weights_processed", False):
             raise RuntimeError("process_weights_after_loading must run before apply_weights")
         if x.dtype != weights["_act_dtype"]:
@@ -163,5 +169,6 @@ class AWQB200LinearMethod(LinearMethodBase):
                              f"{weights['_act_dtype']} the weights were loaded with")
         # out: optional preallocated [..., N] result (e.g. a slice of a buffer the
         # caller copies to the host in one piece)
-        return ops.gemm(x, weights["qweight"], weights["_input_size"], weights["_output_size"],
-                        weights["_group_size"], bias=bias, out=out)
+        y = ops.gemm(x, weights["qweight"], weights["_input_size"], weights["_output_size"],
+                     weights["_group_size"], bias=bias, out=out)
+        return y if adapters is None else adapters.add_to(y, x, batch)

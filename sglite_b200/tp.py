@@ -15,6 +15,7 @@ from typing import Dict, List, Optional
 
 import torch
 
+from .lora import LoraAdapters, LoraBatch
 from .quantization.awq_b200 import AWQB200LinearMethod
 
 AWQ_KEYS = ("qweight", "qzeros", "scales")
@@ -64,6 +65,7 @@ class _AWQLinear:
         self.local_input_size = local_in
         self.local_output_size = local_out
         self.bias = bias
+        self.adapters: Optional[LoraAdapters] = None  # this rank's part (LoraAdapters.shard)
 
     def load(self, shard: Dict[str, torch.Tensor]) -> None:
         for k in AWQ_KEYS:
@@ -72,8 +74,13 @@ class _AWQLinear:
             self.weights[k] = shard[k]
         self.weights = self.method.process_weights_after_loading(self.weights)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return self.method.apply_weights(self.weights, x, self.bias)
+    def forward(self, x: torch.Tensor, lora: Optional[LoraBatch] = None) -> torch.Tensor:
+        """``lora``: which row uses which of ``self.adapters`` (None: no row uses one)."""
+        if lora is None:
+            return self.method.apply_weights(self.weights, x, self.bias)
+        if self.adapters is None:
+            raise ValueError("this projection holds no adapters")
+        return self.method.apply_weights(self.weights, x, self.bias, adapters=self.adapters, batch=lora)
 
 
 class ColumnParallelAWQLinear(_AWQLinear):
@@ -91,7 +98,8 @@ class RowParallelAWQLinear(_AWQLinear):
     max_rows) run the GEMM fused with the all-reduce in one kernel over peer
     memory; otherwise the GEMM is followed by the NCCL all-reduce. (The
     reference adds the bias on every rank before reducing; that case keeps the
-    NCCL path so the semantics stay identical.)"""
+    NCCL path so the semantics stay identical.) Adapters add each rank's product
+    to its partial output before the reduction, on the NCCL path as well."""
 
     def __init__(self, method, input_size: int, output_size: int, tp_size: int, comm=None, bias=None,
                  exchange=None):
@@ -100,8 +108,8 @@ class RowParallelAWQLinear(_AWQLinear):
         self.comm = comm
         self.exchange = exchange
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if self.tp_size > 1 and self.exchange is not None and self.bias is None:
+    def forward(self, x: torch.Tensor, lora: Optional[LoraBatch] = None) -> torch.Tensor:
+        if self.tp_size > 1 and self.exchange is not None and self.bias is None and lora is None:
             M = x.numel() // self.local_input_size
             if M <= self.exchange.max_rows and self.local_output_size <= self.exchange.max_n:
                 w = self.weights
@@ -109,7 +117,7 @@ class RowParallelAWQLinear(_AWQLinear):
                     raise ValueError(f"activations are {x.dtype}, weights were loaded for {w['_act_dtype']}")
                 return self.exchange.gemm_allreduce(x, w["qweight"], self.local_input_size,
                                                     self.local_output_size, w["_group_size"])
-        y = super().forward(x)
+        y = super().forward(x, lora)
         if self.tp_size > 1:
             y = self.comm.all_reduce(y)
         return y
