@@ -26,6 +26,7 @@
 #include "awqb200.h"
 #include "awqb_common.h"
 #include "awqb_ptx.cuh"
+#include "awqb_tma.h"
 #include "awqb_vec.cuh"
 
 namespace awqb {
@@ -37,9 +38,9 @@ constexpr int kMaxSlices = 4;
 constexpr int kMaxParts = 8;      // parts of K
 constexpr int kFirstWarps = 8;
 constexpr int kSecondWarps = 4;
-// Rows from which the 64-row tiles are taken: below, 16-row tiles keep more CTAs
+// Rows from which the prompt kernels are taken: below, 16-row tiles keep more CTAs
 // in flight and pad the few rows of a decode batch's adapters less.
-constexpr int64_t kWideRows = 512;
+constexpr int64_t kPromptRows = 512;
 
 struct Args {
   const void *x, *a, *b, *base;
@@ -47,6 +48,7 @@ struct Args {
   const float* scales;
   void* out;
   float* h;  // [parts][M][R]
+  uint32_t* err;
   int64_t ldx, ld_base, ld_out;
   int M, K, L, rank, R, N, S, parts, k_part;
   int slice_end[kMaxSlices];
@@ -121,12 +123,11 @@ __device__ __forceinline__ void mma32(float (&d)[4], const uint4& lo_row, const 
   mma16816<T>(d, lo_row.z, hi_row.z, lo_row.w, hi_row.w, b.z, b.w);
 }
 
-// kM row tiles of 16, kN column tiles of 8.
-template <typename T, int kM, int kN>
+// Decode batches: 16 rows x 16 columns of A.
+template <typename T>
 __global__ void __launch_bounds__(kFirstWarps * 32) lora_first_kernel(const __grid_constant__ Args g) {
-  constexpr int kRows = kM * 16, kCols = kN * 8;
-  extern __shared__ float4 meet4[];
-  float* meet = reinterpret_cast<float*>(meet4);  // [kFirstWarps / 2][kM * kN * 4][32]
+  constexpr int kRows = 16, kN = 2, kCols = kN * 8;
+  __shared__ float meet[kFirstWarps / 2 * kN * 4 * 32];
   grid_dep_wait();
   grid_dep_launch();
   const int col_tiles = (g.R + kCols - 1) / kCols;
@@ -134,63 +135,161 @@ __global__ void __launch_bounds__(kFirstWarps * 32) lora_first_kernel(const __gr
   const Rows r = find_rows<kFirstWarps * 32, kRows>(g, blockIdx.x / (g.parts * col_tiles), true);
   if (r.n <= 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
-  const T* x[kM][2];
-#pragma unroll
-  for (int m = 0; m < kM; ++m)
+  const T* x[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int row = m * 16 + i * 8 + gr;
+      const int row = i * 8 + gr;
       const int tok = row < r.n ? g.order[r.p0 + row] : -1;
-      x[m][i] = tok >= 0 && tok < g.M ? static_cast<const T*>(g.x) + tok * g.ldx + t * 8 : nullptr;
+      x[i] = tok >= 0 && tok < g.M ? static_cast<const T*>(g.x) + tok * g.ldx + t * 8 : nullptr;
     }
   const T* w = static_cast<const T*>(g.a) + ((int64_t)r.adapter * g.R + ct * kCols + gr) * g.K + t * 8;
   const int cols_left = g.R - ct * kCols;
-  float d[kM][kN][4] = {};
+  float d[kN][4] = {};
   const int k_end = min(g.K, (part + 1) * g.k_part);
   const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll(kM == 1 ? 4 : 1)
-  for (int k = part * g.k_part + warp * 32; k < k_end; k += kFirstWarps * 32) {
-    const bool in = k + t * 8 < k_end;
-    uint4 xa[kM][2], wb[kN];
+  constexpr int kAhead = 4;  // steps whose loads are in flight together
+  for (int k0 = part * g.k_part + warp * 32; k0 < k_end; k0 += kAhead * kFirstWarps * 32) {
+    uint4 xa[kAhead][2], wb[kAhead][kN];
 #pragma unroll
-    for (int n = 0; n < kN; ++n)
-      wb[n] = in && n * 8 < cols_left ? __ldg(reinterpret_cast<const uint4*>(w + (int64_t)n * 8 * g.K + k)) : zero;
+    for (int j = 0; j < kAhead; ++j) {
+      const int k = k0 + j * kFirstWarps * 32;
+      const bool in = k + t * 8 < k_end;
 #pragma unroll
-    for (int m = 0; m < kM; ++m)
+      for (int n = 0; n < kN; ++n)
+        wb[j][n] = in && n * 8 < cols_left ? __ldg(reinterpret_cast<const uint4*>(w + (int64_t)n * 8 * g.K + k)) : zero;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        xa[m][i] = in && x[m][i] != nullptr ? __ldg(reinterpret_cast<const uint4*>(x[m][i] + k)) : zero;
+        for (int i = 0; i < 2; ++i)
+          xa[j][i] = in && x[i] != nullptr ? __ldg(reinterpret_cast<const uint4*>(x[i] + k)) : zero;
+    }
 #pragma unroll
-    for (int m = 0; m < kM; ++m)
+    for (int j = 0; j < kAhead; ++j)
 #pragma unroll
-      for (int n = 0; n < kN; ++n) mma32<T>(d[m][n], xa[m][0], xa[m][1], wb[n]);
+        for (int n = 0; n < kN; ++n) mma32<T>(d[n], xa[j][0], xa[j][1], wb[j][n]);
   }
   // the warps' sums, halving the number of warps each time
 #pragma unroll
   for (int half = kFirstWarps / 2; half > 0; half /= 2) {
     if (warp >= half && warp < 2 * half)
 #pragma unroll
-      for (int i = 0; i < kM * kN * 4; ++i)
-        meet[((warp - half) * kM * kN * 4 + i) * 32 + lane] = d[i / (kN * 4)][i / 4 % kN][i % 4];
+      for (int i = 0; i < kN * 4; ++i)
+        meet[((warp - half) * kN * 4 + i) * 32 + lane] = d[i / 4][i % 4];
     __syncthreads();
     if (warp < half)
 #pragma unroll
-      for (int i = 0; i < kM * kN * 4; ++i) d[i / (kN * 4)][i / 4 % kN][i % 4] += meet[(warp * kM * kN * 4 + i) * 32 + lane];
+      for (int i = 0; i < kN * 4; ++i) d[i / 4][i % 4] += meet[(warp * kN * 4 + i) * 32 + lane];
     __syncthreads();
   }
   if (warp != 0) return;
   float* h = g.h + (int64_t)part * g.M * g.R + ct * kCols + t * 2;
 #pragma unroll
-  for (int m = 0; m < kM; ++m)
-#pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int row = m * 16 + i * 8 + gr;
+      const int row = i * 8 + gr;
       if (row >= r.n) continue;
 #pragma unroll
       for (int n = 0; n < kN; ++n)
         if (n * 8 < cols_left)
-          *reinterpret_cast<float2*>(h + (int64_t)(r.p0 + row) * g.R + n * 8) = make_float2(d[m][n][2 * i], d[m][n][2 * i + 1]);
+          *reinterpret_cast<float2*>(h + (int64_t)(r.p0 + row) * g.R + n * 8) = make_float2(d[n][2 * i], d[n][2 * i + 1]);
     }
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+constexpr int kWideTile = 64;   // rows, columns and k of a stage
+constexpr int kWideStages = 4;
+constexpr int kWideBytes = 2 * kWideTile * kWideTile * 2;  // a stage: rows of x, rows of A
+
+// The same for prompts: 64 rows x 64 columns over a part of K through a ring of
+// shared-memory stages. Held in registers the 64 x 64 sums of every warp left no
+// room to load ahead (48 us for 4111 rows, K = 4096, 128 columns); here the
+// eight warps share the tile (16 x 32 each) and three stages are in flight.
+// 16-byte chunk c of row r sits at chunk c ^ (r & 7): no bank conflicts.
+template <typename T>
+__global__ void __launch_bounds__(kFirstWarps * 32) lora_first_wide_kernel(const __grid_constant__ Args g) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int col_tiles = (g.R + kWideTile - 1) / kWideTile;
+  const int part = blockIdx.x % g.parts, ct = blockIdx.x / g.parts % col_tiles;
+  const Rows r = find_rows<kFirstWarps * 32, kWideTile>(g, blockIdx.x / (g.parts * col_tiles), true);
+  if (r.n <= 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int chunk = threadIdx.x & 7, lrow = threadIdx.x >> 3;  // this thread loads rows lrow, lrow + 32
+  const T *src[2][2];
+  bool has[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = lrow + 32 * i;
+    const int tok = row < r.n ? g.order[r.p0 + row] : -1;
+    has[0][i] = tok >= 0 && tok < g.M;
+    src[0][i] = static_cast<const T*>(g.x) + (has[0][i] ? tok * g.ldx : 0) + chunk * 8;
+    const int col = ct * kWideTile + row;
+    has[1][i] = col < g.R;
+    src[1][i] = static_cast<const T*>(g.a) + ((int64_t)r.adapter * g.R + (has[1][i] ? col : 0)) * g.K + chunk * 8;
+  }
+  const uint32_t base = smem_u32(ring);
+  const int k_begin = part * g.k_part, k_end = min(g.K, k_begin + g.k_part);
+  const int steps = (k_end - k_begin + kWideTile - 1) / kWideTile;
+  const auto load = [&](int step) {
+    if (step < steps) {
+      const uint32_t stage = base + step % kWideStages * kWideBytes;
+      const int k = k_begin + step * kWideTile;
+      const bool in = k + chunk * 8 < k_end;
+#pragma unroll
+      for (int o = 0; o < 2; ++o)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = lrow + 32 * i;
+          const bool ok = in && has[o][i];
+          cp_async16(stage + o * (kWideBytes / 2) + row * 128 + ((chunk ^ (row & 7)) << 4), src[o][i] + (ok ? k : 0), ok);
+        }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kWideStages - 1; ++i) load(i);
+  const int m0 = (warp & 3) * 16, n0 = (warp >> 2) * 32;
+  // ldmatrix rows: x 16 rows x 2 chunks; A 16 columns x 2 chunks, twice
+  const int xr = m0 + (lane & 15), xc = lane >> 4;
+  const int ar = n0 + (lane & 7) + ((lane >> 4) << 3), ac = (lane >> 3) & 1;
+  float d[4][4] = {};
+  for (int step = 0; step < steps; ++step) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kWideStages - 2) : "memory");
+    __syncthreads();
+    load(step + kWideStages - 1);
+    const uint32_t xs = base + step % kWideStages * kWideBytes, as = xs + kWideBytes / 2;
+#pragma unroll
+    for (int kk = 0; kk < kWideTile / 16; ++kk) {
+      uint32_t xa[4], b0[4], b1[4];
+      ldmatrix4(xs + xr * 128 + (((2 * kk + xc) ^ (xr & 7)) << 4), xa);
+      ldmatrix4(as + ar * 128 + (((2 * kk + ac) ^ (ar & 7)) << 4), b0);
+      ldmatrix4(as + (ar + 16) * 128 + (((2 * kk + ac) ^ (ar & 7)) << 4), b1);
+      mma16816<T>(d[0], xa[0], xa[1], xa[2], xa[3], b0[0], b0[1]);
+      mma16816<T>(d[1], xa[0], xa[1], xa[2], xa[3], b0[2], b0[3]);
+      mma16816<T>(d[2], xa[0], xa[1], xa[2], xa[3], b1[0], b1[1]);
+      mma16816<T>(d[3], xa[0], xa[1], xa[2], xa[3], b1[2], b1[3]);
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  const int gr = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = m0 + i * 8 + gr;
+    if (row >= r.n) continue;
+    float* h = g.h + ((int64_t)part * g.M + r.p0 + row) * g.R;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int col = ct * kWideTile + n0 + n * 8 + t * 2;
+      if (col < g.R) *reinterpret_cast<float2*>(h + col) = make_float2(d[n][2 * i], d[n][2 * i + 1]);
+    }
+  }
 }
 
 // The two 16-bit halves of a value.
@@ -201,125 +300,142 @@ __device__ __forceinline__ void halves(float v, T* hi, T* lo) {
   *lo = (T)(fabsf((float)*hi) < INFINITY ? rest : 0.f);
 }
 
-constexpr int kBlock = 32;  // features of a warp's step
-constexpr int kHStride = kMaxRank + 32;  // halves per row of h in shared memory: 16-byte loads of 8 lanes hit all banks
+// The power of two that a row of h is divided by before it is split: fp16 gets the
+// row's largest value to 2^14 .. 2^15 (exact), bf16 has fp32's range. Whole warps.
+template <typename T>
+__device__ __forceinline__ int row_exponent(float top) {
+  if (!std::is_same<T, __half>::value) return 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  return top > 0.f && top < INFINITY ? min(max(ilogbf(top) - 14, -100), 100) : 0;
+}
 
-template <typename T, int kM>
-__global__ void __launch_bounds__(kSecondWarps * 32) lora_second_kernel(const __grid_constant__ Args g, int chunks, int chunk) {
-  constexpr int kRows = kM * 16;
-  __shared__ __align__(16) T hs[2][kRows][kHStride];
-  __shared__ float row_scale[kRows];
-  __shared__ int row_of[kRows];
-  const bool in_place = g.out == g.base;
-  const Rows r = find_rows<kSecondWarps * 32, kRows>(g, blockIdx.x / chunks, in_place);
-  if (r.n <= 0) {
-    grid_dep_wait();
-    return;
-  }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
-  // this CTA's features: chunk blockIdx.x % chunks of some slice
-  int c = blockIdx.x % chunks, s = 0, s0 = 0;
+constexpr int kBlock = 32;                      // features of a warp
+constexpr int kChunk = kSecondWarps * kBlock;   // features of a CTA
+
+// The chunk of features that CTA c of a tile takes: chunks of `chunk` features,
+// slice after slice, none of them over two slices.
+struct Feats {
+  int slice, begin, end;
+};
+__device__ __forceinline__ Feats find_feats(const Args& g, int c, int chunk) {
+  int s = 0, s0 = 0;
   for (;; ++s) {
     const int here = (g.slice_end[s] - s0 + chunk - 1) / chunk;
     if (c < here) break;
     c -= here;
     s0 = g.slice_end[s];
   }
-  const int f_begin = s0 + c * chunk, f_end = min(g.slice_end[s], f_begin + chunk);
-  for (int i = threadIdx.x; i < kRows; i += kSecondWarps * 32) {
-    const int tok = i < r.n ? g.order[r.p0 + i] : -1;
-    row_of[i] = tok >= 0 && tok < g.M ? tok : -1;
+  return {s, s0 + c * chunk, min(g.slice_end[s], s0 + (c + 1) * chunk)};
+}
+
+// Decode batches: 16 rows, 32 features per warp. kRank32: the rank in blocks of 32.
+template <typename T, int kRank32>
+__global__ void __launch_bounds__(kSecondWarps * 32) lora_second_kernel(const __grid_constant__ Args g, int chunks) {
+  constexpr int kRows = 16;
+  // 64 bytes past a multiple of 128: the 16-byte loads of 8 lanes hit all banks
+  constexpr int kHStride = (kRank32 + 1) / 2 * 64 + 32;
+  __shared__ __align__(16) T hs[2][kRows][kHStride];
+  __shared__ float row_scale[kRows];
+  const Rows r = find_rows<kSecondWarps * 32, kRows>(g, blockIdx.x / chunks, g.out == g.base);
+  if (r.n <= 0) {
+    grid_dep_wait();
+    return;
   }
-  const float scale = r.adapter >= 0 && g.scales ? g.scales[r.adapter] : 1.f;
-  const int blocks32 = (g.rank + 31) / 32;
-  grid_dep_wait();
-  if (r.adapter >= 0) {
-    for (int row = warp; row < kRows; row += kSecondWarps) {
-      float v[kMaxRank / 32];
-      float top = 0.f;
+  const bool adapted = r.adapter >= 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
+  const Feats feats = find_feats(g, blockIdx.x % chunks, kChunk);
+  const int f = feats.begin + warp * kBlock;
+  // What the first kernel does not write is loaded before it has ended: it let
+  // this kernel start only after everything in front of it was complete.
+  uint4 y[2], wb[kRank32][4];
+  int tok[2];
 #pragma unroll
-      for (int i = 0; i < kMaxRank / 32; ++i) {
-        const int j = i * 32 + lane;
-        v[i] = 0.f;
-        if (row < r.n && j < g.rank) {
-          const float* src = g.h + (int64_t)(r.p0 + row) * g.R + s * g.rank + j;
-          for (int q = 0; q < g.parts; ++q) v[i] += src[(int64_t)q * g.M * g.R];
-        }
+  for (int i = 0; i < 2; ++i) {
+    tok[i] = i * 8 + gr < r.n && f + t * 8 < feats.end ? g.order[r.p0 + i * 8 + gr] : -1;
+    if (tok[i] >= g.M) tok[i] = -1;
+    if (tok[i] >= 0)
+      y[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(g.base) + tok[i] * g.ld_base + f + t * 8);
+  }
+  // Columns of the four 8-column products are dealt so that lane t of a row ends
+  // with features 8t .. 8t + 7.
+  const int col = (gr >> 1) * 8 + (gr & 1);
+#pragma unroll
+  for (int k = 0; k < kRank32; ++k)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int feat = f + col + 2 * n;
+      wb[k][n] = adapted && feat < feats.end && k * 32 + t * 8 < g.rank
+                     ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(g.b) +
+                                                            ((int64_t)r.adapter * g.N + feat) * g.rank + k * 32 + t * 8))
+                     : make_uint4(0, 0, 0, 0);
+    }
+  const float scale = adapted && g.scales ? g.scales[r.adapter] : 1.f;
+  grid_dep_wait();
+  if (adapted) {
+    for (int row = warp; row < r.n; row += kSecondWarps) {
+      const float* src = g.h + (int64_t)(r.p0 + row) * g.R + feats.slice * g.rank + lane;
+      float u[kMaxParts][kRank32], v[kRank32] = {}, top = 0.f;
+#pragma unroll
+      for (int part = 0; part < kMaxParts; ++part)
+#pragma unroll
+        for (int i = 0; i < kRank32; ++i)
+          u[part][i] = part < g.parts && i * 32 + lane < g.rank ? src[(int64_t)part * g.M * g.R + i * 32] : 0.f;
+#pragma unroll
+      for (int i = 0; i < kRank32; ++i) {
+#pragma unroll
+        for (int part = 0; part < kMaxParts; ++part) v[i] += u[part][i];
         top = fmaxf(top, fabsf(v[i]));
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // fp16: bring the row's largest value to 2^14 (exact: a power of two)
-      const int e = std::is_same<T, __half>::value && top > 0.f && top < INFINITY ? min(max(ilogbf(top) - 14, -100), 100) : 0;
+      const int e = row_exponent<T>(top);
       const float down = ldexpf(1.f, -e);
 #pragma unroll
-      for (int i = 0; i < kMaxRank / 32; ++i)
-        if (i < blocks32) halves<T>(v[i] * down, &hs[0][row][i * 32 + lane], &hs[1][row][i * 32 + lane]);
+      for (int i = 0; i < kRank32; ++i)
+        halves<T>(v[i] * down, &hs[0][row][i * 32 + lane], &hs[1][row][i * 32 + lane]);
       if (lane == 0) row_scale[row] = scale * ldexpf(1.f, e);
     }
   }
   __syncthreads();
-  // Columns of the four 8-column products of a block are dealt so that lane t of
-  // a row ends with features 8t .. 8t + 7.
-  const int col = (gr >> 1) * 8 + (gr & 1);
-  const T* b = static_cast<const T*>(g.b) + (int64_t)(r.adapter >= 0 ? r.adapter : 0) * g.N * g.rank + t * 8;
-  for (int f = f_begin + warp * kBlock; f < f_end; f += kSecondWarps * kBlock) {
-    uint4 y[kM][2];
-    const bool mine = f + t * 8 < f_end;
+  float d[4][4] = {};
+  if (adapted) {
 #pragma unroll
-    for (int m = 0; m < kM; ++m)
+    for (int k = 0; k < kRank32; ++k)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int tok = row_of[m * 16 + i * 8 + gr];
-        if (tok >= 0 && mine)
-          y[m][i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(g.base) + tok * g.ld_base + f + t * 8);
+      for (int part = 0; part < 2; ++part) {
+        const uint4 lo = *reinterpret_cast<const uint4*>(&hs[part][gr][k * 32 + t * 8]);
+        const uint4 hi = *reinterpret_cast<const uint4*>(&hs[part][8 + gr][k * 32 + t * 8]);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) mma32<T>(d[n], lo, hi, wb[k][n]);
       }
-    float d[kM][4][4] = {};
-    if (r.adapter >= 0) {
-      for (int k = 0; k < blocks32; ++k) {
-        uint4 wb[4];
+  }
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const int feat = f + col + 2 * n;
-          wb[n] = feat < f_end && k * 32 + t * 8 < g.rank
-                      ? __ldg(reinterpret_cast<const uint4*>(b + (int64_t)feat * g.rank + k * 32))
-                      : make_uint4(0, 0, 0, 0);
-        }
+  for (int i = 0; i < 2; ++i) {
+    if (tok[i] < 0) continue;
+    uint4 o = y[i];
+    if (adapted) {
+      float v[8];
+      unpack_vec<T>(o, v);
+      const float w = row_scale[i * 8 + gr];
 #pragma unroll
-        for (int m = 0; m < kM; ++m)
-#pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            const uint4 lo = *reinterpret_cast<const uint4*>(&hs[part][m * 16 + gr][k * 32 + t * 8]);
-            const uint4 hi = *reinterpret_cast<const uint4*>(&hs[part][m * 16 + 8 + gr][k * 32 + t * 8]);
-#pragma unroll
-            for (int n = 0; n < 4; ++n) mma32<T>(d[m][n], lo, hi, wb[n]);
-          }
+      for (int n = 0; n < 4; ++n) {
+        v[2 * n] += w * d[n][2 * i];
+        v[2 * n + 1] += w * d[n][2 * i + 1];
       }
+      o = pack_vec<T>(v);
     }
-#pragma unroll
-    for (int m = 0; m < kM; ++m)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int tok = row_of[m * 16 + i * 8 + gr];
-        if (tok < 0 || !mine) continue;
-        uint4 o = y[m][i];
-        if (r.adapter >= 0) {
-          float v[8];
-          unpack_vec<T>(o, v);
-          const float w = row_scale[m * 16 + i * 8 + gr];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            v[2 * n] += w * d[m][n][2 * i];
-            v[2 * n + 1] += w * d[m][n][2 * i + 1];
-          }
-          o = pack_vec<T>(v);
-        }
-        *reinterpret_cast<uint4*>(static_cast<T*>(g.out) + tok * g.ld_out + f + t * 8) = o;
-      }
+    *reinterpret_cast<uint4*>(static_cast<T*>(g.out) + tok[i] * g.ld_out + f + t * 8) = o;
   }
 }
 
-bool wide_tiles(int64_t M) { return M >= kWideRows; }
+}  // namespace
+}  // namespace awqb
+
+#include "awqb_lora_wide.cuh"
+
+namespace awqb {
+namespace {
+
+bool wide_tiles(int64_t M) { return M >= kPromptRows; }
 
 // Parts of K: enough CTAs for about two per SM, each part at least 64 k per warp.
 int parts_of_k(int64_t M, int64_t K, int64_t R) {
@@ -331,9 +447,24 @@ int parts_of_k(int64_t M, int64_t K, int64_t R) {
 
 int64_t max_tiles(const Args& g, int rows) { return std::min<int64_t>(g.M, g.M / rows + g.L + 2); }
 
-template <typename T, int kM, int kN>
-int launch_tiles(const Args& g, cudaStream_t st) {
-  const int cols = kN * 8, col_tiles = (g.R + cols - 1) / cols;
+// B's rows (features of all adapters) in blocks of 128 x 64 k, zero past the rank.
+int make_b_map(CUtensorMap* tm, const Args& g) {
+  const auto enc = tensor_map_encoder();
+  AWQB_REQUIRE(enc != nullptr, kCudaError, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t dim[2] = {(cuuint64_t)g.rank, (cuuint64_t)g.L * g.N};
+  const cuuint64_t stride[1] = {(cuuint64_t)g.rank * 2};
+  const cuuint32_t box[2] = {64, kWideFeat}, one[2] = {1, 1};
+  const CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(g.b), dim, stride, box, one,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  AWQB_REQUIRE(r == CUDA_SUCCESS, kCudaError, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return kOk;
+}
+
+template <typename T>
+int launch(const Args& g, cudaStream_t st) {
+  const bool wide = wide_tiles(g.M);
+  const int rows = wide ? kWideTile : 16, cols = wide ? kWideTile : 16;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -341,27 +472,47 @@ int launch_tiles(const Args& g, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cfg.gridDim = dim3((unsigned)(max_tiles(g, kM * 16) * col_tiles * g.parts));
+  cfg.gridDim = dim3((unsigned)(max_tiles(g, rows) * ((g.R + cols - 1) / cols) * g.parts));
   cfg.blockDim = dim3(kFirstWarps * 32);
-  cfg.dynamicSmemBytes = kFirstWarps / 2 * kM * kN * 4 * 32 * 4;
-  const auto first = lora_first_kernel<T, kM, kN>;
-  if (cfg.dynamicSmemBytes > 32 * 1024)
-    AWQB_CUDA(cudaFuncSetAttribute(first, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes));
-  AWQB_CUDA(cudaLaunchKernelEx(&cfg, first, g));
-  // features per CTA: one block per warp for decode batches, four for prompts
-  const int chunk = kSecondWarps * kBlock * (kM == 1 ? 1 : 4);
-  int chunks = 0;
+  if (wide) {
+    cfg.dynamicSmemBytes = kWideStages * kWideBytes;
+    AWQB_CUDA(cudaFuncSetAttribute(lora_first_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   kWideStages * kWideBytes));
+    AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_first_wide_kernel<T>, g));
+  } else {
+    AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_first_kernel<T>, g));
+  }
+  // Features per CTA: one block per warp for decode batches; for prompts as many
+  // as leave eight CTAs per SM, since every CTA prepares its rows' halves anew.
+  const int rows2 = wide ? kWideRows2 : 16;
+  const int64_t step = wide ? kWideFeat : kChunk;
+  int64_t chunk = step;
+  if (wide) {
+    const int64_t share = (g.M + rows2 - 1) / rows2 * g.N / (8 * device_sm_count());
+    chunk = std::max<int64_t>(1, std::min<int64_t>(16, share / step)) * step;
+  }
+  int64_t chunks = 0;
   for (int s = 0, s0 = 0; s < g.S; s0 = g.slice_end[s++]) chunks += (g.slice_end[s] - s0 + chunk - 1) / chunk;
-  cfg.gridDim = dim3((unsigned)(max_tiles(g, kM * 16) * chunks));
+  cfg.gridDim = dim3((unsigned)(max_tiles(g, rows2) * chunks));
+  if (wide) {
+    const int atoms = (g.rank + 63) / 64;
+    CUtensorMap tm;
+    const int status = make_b_map(&tm, g);
+    if (status != kOk) return status;
+    cfg.blockDim = dim3(kWideThreads);
+    cfg.dynamicSmemBytes = wide_smem(atoms);
+    AWQB_CUDA(cudaFuncSetAttribute(lora_second_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   wide_smem(kMaxRank / 64)));
+    AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_second_wide_kernel<T>, tm, g, (int)chunks, (int)chunk, atoms));
+    return kOk;
+  }
   cfg.blockDim = dim3(kSecondWarps * 32);
   cfg.dynamicSmemBytes = 0;
-  AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_second_kernel<T, kM>, g, chunks, chunk));
+  const auto second = g.rank <= 32   ? lora_second_kernel<T, 1>
+                      : g.rank <= 64 ? lora_second_kernel<T, 2>
+                                     : lora_second_kernel<T, 4>;
+  AWQB_CUDA(cudaLaunchKernelEx(&cfg, second, g, (int)chunks));
   return kOk;
-}
-
-template <typename T>
-int launch(const Args& g, cudaStream_t st) {
-  return wide_tiles(g.M) ? launch_tiles<T, 4, 8>(g, st) : launch_tiles<T, 1, 2>(g, st);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -424,6 +575,8 @@ extern "C" int awqb_lora(const void* x, int64_t M, int64_t ldx, int64_t K, const
                kInvalidArgument, "tensors must be 16-byte aligned");
   AWQB_REQUIRE(workspace != nullptr && workspace_bytes >= need, kInvalidArgument,
                "workspace too small: %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
+  g.err = device_error_word();
+  AWQB_REQUIRE(g.err != nullptr, kCudaError, "cannot resolve the device error word");
   g.x = x, g.a = a, g.b = b, g.base = base, g.order = order, g.offsets = offsets, g.scales = scales, g.out = out;
   g.h = static_cast<float*>(workspace);
   g.ldx = ldx, g.ld_base = ld_base, g.ld_out = ld_out;
