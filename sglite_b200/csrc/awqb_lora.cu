@@ -47,7 +47,9 @@ struct Args {
   const int32_t *order, *offsets;
   const float* scales;
   void* out;
-  float* h;  // [parts][M][R]
+  float* h;      // [parts][M][R]
+  void* halves;  // prompts: [slices][2][M][rank], see the join kernel
+  float* up;     // prompts: [slices][M]
   uint32_t* err;
   int64_t ldx, ld_base, ld_out;
   int M, K, L, rank, R, N, S, parts, k_part;
@@ -137,11 +139,11 @@ __global__ void __launch_bounds__(kFirstWarps * 32) lora_first_kernel(const __gr
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
   const T* x[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = i * 8 + gr;
-      const int tok = row < r.n ? g.order[r.p0 + row] : -1;
-      x[i] = tok >= 0 && tok < g.M ? static_cast<const T*>(g.x) + tok * g.ldx + t * 8 : nullptr;
-    }
+  for (int i = 0; i < 2; ++i) {
+    const int row = i * 8 + gr;
+    const int tok = row < r.n ? g.order[r.p0 + row] : -1;
+    x[i] = tok >= 0 && tok < g.M ? static_cast<const T*>(g.x) + tok * g.ldx + t * 8 : nullptr;
+  }
   const T* w = static_cast<const T*>(g.a) + ((int64_t)r.adapter * g.R + ct * kCols + gr) * g.K + t * 8;
   const int cols_left = g.R - ct * kCols;
   float d[kN][4] = {};
@@ -158,21 +160,20 @@ __global__ void __launch_bounds__(kFirstWarps * 32) lora_first_kernel(const __gr
       for (int n = 0; n < kN; ++n)
         wb[j][n] = in && n * 8 < cols_left ? __ldg(reinterpret_cast<const uint4*>(w + (int64_t)n * 8 * g.K + k)) : zero;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          xa[j][i] = in && x[i] != nullptr ? __ldg(reinterpret_cast<const uint4*>(x[i] + k)) : zero;
+      for (int i = 0; i < 2; ++i)
+        xa[j][i] = in && x[i] != nullptr ? __ldg(reinterpret_cast<const uint4*>(x[i] + k)) : zero;
     }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
 #pragma unroll
-        for (int n = 0; n < kN; ++n) mma32<T>(d[n], xa[j][0], xa[j][1], wb[j][n]);
+      for (int n = 0; n < kN; ++n) mma32<T>(d[n], xa[j][0], xa[j][1], wb[j][n]);
   }
   // the warps' sums, halving the number of warps each time
 #pragma unroll
   for (int half = kFirstWarps / 2; half > 0; half /= 2) {
     if (warp >= half && warp < 2 * half)
 #pragma unroll
-      for (int i = 0; i < kN * 4; ++i)
-        meet[((warp - half) * kN * 4 + i) * 32 + lane] = d[i / 4][i % 4];
+      for (int i = 0; i < kN * 4; ++i) meet[((warp - half) * kN * 4 + i) * 32 + lane] = d[i / 4][i % 4];
     __syncthreads();
     if (warp < half)
 #pragma unroll
@@ -182,113 +183,13 @@ __global__ void __launch_bounds__(kFirstWarps * 32) lora_first_kernel(const __gr
   if (warp != 0) return;
   float* h = g.h + (int64_t)part * g.M * g.R + ct * kCols + t * 2;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = i * 8 + gr;
-      if (row >= r.n) continue;
-#pragma unroll
-      for (int n = 0; n < kN; ++n)
-        if (n * 8 < cols_left)
-          *reinterpret_cast<float2*>(h + (int64_t)(r.p0 + row) * g.R + n * 8) = make_float2(d[n][2 * i], d[n][2 * i + 1]);
-    }
-}
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-
-constexpr int kWideTile = 64;   // rows, columns and k of a stage
-constexpr int kWideStages = 4;
-constexpr int kWideBytes = 2 * kWideTile * kWideTile * 2;  // a stage: rows of x, rows of A
-
-// The same for prompts: 64 rows x 64 columns over a part of K through a ring of
-// shared-memory stages. Held in registers the 64 x 64 sums of every warp left no
-// room to load ahead (48 us for 4111 rows, K = 4096, 128 columns); here the
-// eight warps share the tile (16 x 32 each) and three stages are in flight.
-// 16-byte chunk c of row r sits at chunk c ^ (r & 7): no bank conflicts.
-template <typename T>
-__global__ void __launch_bounds__(kFirstWarps * 32) lora_first_wide_kernel(const __grid_constant__ Args g) {
-  extern __shared__ __align__(128) uint8_t ring[];
-  grid_dep_wait();
-  grid_dep_launch();
-  const int col_tiles = (g.R + kWideTile - 1) / kWideTile;
-  const int part = blockIdx.x % g.parts, ct = blockIdx.x / g.parts % col_tiles;
-  const Rows r = find_rows<kFirstWarps * 32, kWideTile>(g, blockIdx.x / (g.parts * col_tiles), true);
-  if (r.n <= 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int chunk = threadIdx.x & 7, lrow = threadIdx.x >> 3;  // this thread loads rows lrow, lrow + 32
-  const T *src[2][2];
-  bool has[2][2];
-#pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int row = lrow + 32 * i;
-    const int tok = row < r.n ? g.order[r.p0 + row] : -1;
-    has[0][i] = tok >= 0 && tok < g.M;
-    src[0][i] = static_cast<const T*>(g.x) + (has[0][i] ? tok * g.ldx : 0) + chunk * 8;
-    const int col = ct * kWideTile + row;
-    has[1][i] = col < g.R;
-    src[1][i] = static_cast<const T*>(g.a) + ((int64_t)r.adapter * g.R + (has[1][i] ? col : 0)) * g.K + chunk * 8;
-  }
-  const uint32_t base = smem_u32(ring);
-  const int k_begin = part * g.k_part, k_end = min(g.K, k_begin + g.k_part);
-  const int steps = (k_end - k_begin + kWideTile - 1) / kWideTile;
-  const auto load = [&](int step) {
-    if (step < steps) {
-      const uint32_t stage = base + step % kWideStages * kWideBytes;
-      const int k = k_begin + step * kWideTile;
-      const bool in = k + chunk * 8 < k_end;
-#pragma unroll
-      for (int o = 0; o < 2; ++o)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = lrow + 32 * i;
-          const bool ok = in && has[o][i];
-          cp_async16(stage + o * (kWideBytes / 2) + row * 128 + ((chunk ^ (row & 7)) << 4), src[o][i] + (ok ? k : 0), ok);
-        }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll
-  for (int i = 0; i < kWideStages - 1; ++i) load(i);
-  const int m0 = (warp & 3) * 16, n0 = (warp >> 2) * 32;
-  // ldmatrix rows: x 16 rows x 2 chunks; A 16 columns x 2 chunks, twice
-  const int xr = m0 + (lane & 15), xc = lane >> 4;
-  const int ar = n0 + (lane & 7) + ((lane >> 4) << 3), ac = (lane >> 3) & 1;
-  float d[4][4] = {};
-  for (int step = 0; step < steps; ++step) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kWideStages - 2) : "memory");
-    __syncthreads();
-    load(step + kWideStages - 1);
-    const uint32_t xs = base + step % kWideStages * kWideBytes, as = xs + kWideBytes / 2;
-#pragma unroll
-    for (int kk = 0; kk < kWideTile / 16; ++kk) {
-      uint32_t xa[4], b0[4], b1[4];
-      ldmatrix4(xs + xr * 128 + (((2 * kk + xc) ^ (xr & 7)) << 4), xa);
-      ldmatrix4(as + ar * 128 + (((2 * kk + ac) ^ (ar & 7)) << 4), b0);
-      ldmatrix4(as + (ar + 16) * 128 + (((2 * kk + ac) ^ (ar & 7)) << 4), b1);
-      mma16816<T>(d[0], xa[0], xa[1], xa[2], xa[3], b0[0], b0[1]);
-      mma16816<T>(d[1], xa[0], xa[1], xa[2], xa[3], b0[2], b0[3]);
-      mma16816<T>(d[2], xa[0], xa[1], xa[2], xa[3], b1[0], b1[1]);
-      mma16816<T>(d[3], xa[0], xa[1], xa[2], xa[3], b1[2], b1[3]);
-    }
-  }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  const int gr = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = m0 + i * 8 + gr;
+    const int row = i * 8 + gr;
     if (row >= r.n) continue;
-    float* h = g.h + ((int64_t)part * g.M + r.p0 + row) * g.R;
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int col = ct * kWideTile + n0 + n * 8 + t * 2;
-      if (col < g.R) *reinterpret_cast<float2*>(h + col) = make_float2(d[n][2 * i], d[n][2 * i + 1]);
-    }
+    for (int n = 0; n < kN; ++n)
+      if (n * 8 < cols_left)
+        *reinterpret_cast<float2*>(h + (int64_t)(r.p0 + row) * g.R + n * 8) = make_float2(d[n][2 * i], d[n][2 * i + 1]);
   }
 }
 
@@ -437,34 +338,100 @@ namespace {
 
 bool wide_tiles(int64_t M) { return M >= kPromptRows; }
 
-// Parts of K: enough CTAs for about two per SM, each part at least 64 k per warp.
+// Parts of K: enough CTAs to fill the GPU, each part long enough to be worth its
+// sums (64 k per warp of a decode batch's CTA, eight stages of a prompt's).
 int parts_of_k(int64_t M, int64_t K, int64_t R) {
-  const int rows = wide_tiles(M) ? 64 : 16, cols = wide_tiles(M) ? 64 : 16;
+  const bool wide = wide_tiles(M);
+  const int rows = wide ? kWideRows : 16, cols = wide ? 128 : 16;
   const int64_t tiles = (M + rows - 1) / rows * ((R + cols - 1) / cols);
-  const int64_t want = 296 / std::max<int64_t>(tiles, 1), most = K / (kFirstWarps * 64);
+  const int64_t want = (wide ? 222 : 296) / std::max<int64_t>(tiles, 1), most = K / 512;
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)kMaxParts}));
+}
+
+// The workspace: parts of h, then for prompts the halves and their powers of two.
+struct Layout {
+  int64_t halves, up, bytes;
+};
+Layout layout(int64_t M, int64_t K, int64_t R, int64_t S) {
+  const auto round = [](int64_t v) { return (v + 255) / 256 * 256; };
+  Layout l = {};
+  l.halves = round(M * R * 4 * parts_of_k(M, K, R));
+  l.up = l.halves + (wide_tiles(M) ? round(M * R * 4) : 0);
+  l.bytes = l.up + (wide_tiles(M) ? round(M * S * 4) : 0);
+  return l;
 }
 
 int64_t max_tiles(const Args& g, int rows) { return std::min<int64_t>(g.M, g.M / rows + g.L + 2); }
 
-// B's rows (features of all adapters) in blocks of 128 x 64 k, zero past the rank.
-int make_b_map(CUtensorMap* tm, const Args& g) {
+// rows x 64 k of a row-major matrix, 128-byte swizzle, zeros outside.
+int make_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t k, int64_t ld, int box_rows) {
   const auto enc = tensor_map_encoder();
   AWQB_REQUIRE(enc != nullptr, kCudaError, "cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint64_t dim[2] = {(cuuint64_t)g.rank, (cuuint64_t)g.L * g.N};
-  const cuuint64_t stride[1] = {(cuuint64_t)g.rank * 2};
-  const cuuint32_t box[2] = {64, kWideFeat}, one[2] = {1, 1};
-  const CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(g.b), dim, stride, box, one,
+  const cuuint64_t dim[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  const cuuint64_t stride[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, one[2] = {1, 1};
+  const CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dim, stride, box, one,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   AWQB_REQUIRE(r == CUDA_SUCCESS, kCudaError, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return kOk;
 }
 
+// Chunks of `chunk` features over all slices.
+int64_t count_chunks(const Args& g, int64_t chunk) {
+  int64_t chunks = 0;
+  for (int s = 0, s0 = 0; s < g.S; s0 = g.slice_end[s++]) chunks += (g.slice_end[s] - s0 + chunk - 1) / chunk;
+  return chunks;
+}
+
+template <typename T>
+int launch_decode(const Args& g, cudaLaunchConfig_t cfg) {
+  cfg.gridDim = dim3((unsigned)(max_tiles(g, 16) * ((g.R + 15) / 16) * g.parts));
+  cfg.blockDim = dim3(kFirstWarps * 32);
+  AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_first_kernel<T>, g));
+  const int64_t chunks = count_chunks(g, kChunk);
+  cfg.gridDim = dim3((unsigned)(max_tiles(g, 16) * chunks));
+  cfg.blockDim = dim3(kSecondWarps * 32);
+  const auto second = g.rank <= 32   ? lora_second_kernel<T, 1>
+                      : g.rank <= 64 ? lora_second_kernel<T, 2>
+                                     : lora_second_kernel<T, 4>;
+  AWQB_CUDA(cudaLaunchKernelEx(&cfg, second, g, (int)chunks));
+  return kOk;
+}
+
+template <typename T>
+int launch_prompt(const Args& g, cudaLaunchConfig_t cfg) {
+  const int col_box = std::min(128, g.R), atoms = (g.rank + 63) / 64;
+  CUtensorMap tx, ta, tb, th;
+  int st = make_map(&tx, g.x, g.M, g.K, g.ldx, 1);
+  if (st == kOk) st = make_map(&ta, g.a, (int64_t)g.L * g.R, g.K, g.K, col_box);
+  if (st == kOk) st = make_map(&tb, g.b, (int64_t)g.L * g.N, g.rank, g.rank, kWideFeat);
+  if (st == kOk) st = make_map(&th, g.halves, (int64_t)g.S * 2 * g.M, g.rank, g.rank, kWideRows);
+  if (st != kOk) return st;
+  cfg.gridDim = dim3((unsigned)(max_tiles(g, kWideRows) * ((g.R + 127) / 128) * g.parts));
+  cfg.blockDim = dim3(kFirstWideThreads);
+  cfg.dynamicSmemBytes = first_wide_smem();
+  AWQB_CUDA(cudaFuncSetAttribute(lora_first_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, first_wide_smem()));
+  AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_first_wide_kernel<T>, tx, ta, g, col_box));
+  cfg.gridDim = dim3((unsigned)((g.M + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_join_kernel<T>, g));
+  // features per CTA: as many as leave eight CTAs per SM
+  const int64_t share = (g.M + kWideRows - 1) / kWideRows * g.N / (8 * device_sm_count());
+  const int64_t chunk = std::max<int64_t>(1, std::min<int64_t>(16, share / kWideFeat)) * kWideFeat;
+  const int64_t chunks = count_chunks(g, chunk);
+  cfg.gridDim = dim3((unsigned)(max_tiles(g, kWideRows) * chunks));
+  cfg.blockDim = dim3(kSecondWideThreads);
+  cfg.dynamicSmemBytes = second_wide_smem(atoms);
+  AWQB_CUDA(cudaFuncSetAttribute(lora_second_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 second_wide_smem(kMaxRank / 64)));
+  AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_second_wide_kernel<T>, tb, th, g, (int)chunks, (int)chunk, atoms));
+  return kOk;
+}
+
 template <typename T>
 int launch(const Args& g, cudaStream_t st) {
-  const bool wide = wide_tiles(g.M);
-  const int rows = wide ? kWideTile : 16, cols = wide ? kWideTile : 16;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -472,47 +439,7 @@ int launch(const Args& g, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cfg.gridDim = dim3((unsigned)(max_tiles(g, rows) * ((g.R + cols - 1) / cols) * g.parts));
-  cfg.blockDim = dim3(kFirstWarps * 32);
-  if (wide) {
-    cfg.dynamicSmemBytes = kWideStages * kWideBytes;
-    AWQB_CUDA(cudaFuncSetAttribute(lora_first_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   kWideStages * kWideBytes));
-    AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_first_wide_kernel<T>, g));
-  } else {
-    AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_first_kernel<T>, g));
-  }
-  // Features per CTA: one block per warp for decode batches; for prompts as many
-  // as leave eight CTAs per SM, since every CTA prepares its rows' halves anew.
-  const int rows2 = wide ? kWideRows2 : 16;
-  const int64_t step = wide ? kWideFeat : kChunk;
-  int64_t chunk = step;
-  if (wide) {
-    const int64_t share = (g.M + rows2 - 1) / rows2 * g.N / (8 * device_sm_count());
-    chunk = std::max<int64_t>(1, std::min<int64_t>(16, share / step)) * step;
-  }
-  int64_t chunks = 0;
-  for (int s = 0, s0 = 0; s < g.S; s0 = g.slice_end[s++]) chunks += (g.slice_end[s] - s0 + chunk - 1) / chunk;
-  cfg.gridDim = dim3((unsigned)(max_tiles(g, rows2) * chunks));
-  if (wide) {
-    const int atoms = (g.rank + 63) / 64;
-    CUtensorMap tm;
-    const int status = make_b_map(&tm, g);
-    if (status != kOk) return status;
-    cfg.blockDim = dim3(kWideThreads);
-    cfg.dynamicSmemBytes = wide_smem(atoms);
-    AWQB_CUDA(cudaFuncSetAttribute(lora_second_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   wide_smem(kMaxRank / 64)));
-    AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_second_wide_kernel<T>, tm, g, (int)chunks, (int)chunk, atoms));
-    return kOk;
-  }
-  cfg.blockDim = dim3(kSecondWarps * 32);
-  cfg.dynamicSmemBytes = 0;
-  const auto second = g.rank <= 32   ? lora_second_kernel<T, 1>
-                      : g.rank <= 64 ? lora_second_kernel<T, 2>
-                                     : lora_second_kernel<T, 4>;
-  AWQB_CUDA(cudaLaunchKernelEx(&cfg, second, g, (int)chunks));
-  return kOk;
+  return wide_tiles(g.M) ? launch_prompt<T>(g, cfg) : launch_decode<T>(g, cfg);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -540,7 +467,7 @@ extern "C" int awqb_lora_workspace_bytes(int64_t M, int64_t K, int64_t L, int64_
   AWQB_REQUIRE(bytes != nullptr, kInvalidArgument, "bytes is null");
   const int st = check_sizes(M, K, L, rank, num_slices);
   if (st != kOk) return st;
-  *bytes = M * rank * num_slices * 4 * parts_of_k(M, K, rank * num_slices);
+  *bytes = layout(M, K, rank * num_slices, num_slices).bytes;
   return kOk;
 }
 
@@ -583,7 +510,10 @@ extern "C" int awqb_lora(const void* x, int64_t M, int64_t ldx, int64_t K, const
   g.M = (int)M, g.K = (int)K, g.L = (int)L, g.rank = (int)rank, g.R = (int)(rank * num_slices), g.N = (int)N;
   g.S = (int)num_slices;
   g.parts = parts_of_k(M, K, g.R);
-  g.k_part = (int)((K + g.parts - 1) / g.parts + 31) / 32 * 32;
+  g.k_part = (int)((K + g.parts - 1) / g.parts + 63) / 64 * 64;
+  const Layout at = layout(M, K, g.R, num_slices);
+  g.halves = static_cast<uint8_t*>(workspace) + at.halves;
+  g.up = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at.up);
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   return dtype == AWQB_DTYPE_F16 ? launch<__half>(g, cs) : launch<__nv_bfloat16>(g, cs);
 }

@@ -1,4 +1,5 @@
-// Conversions between 16-byte vectors of fp16 / bf16 and fp32 registers.
+// Conversions between 16-byte vectors of fp16 / bf16 and fp32 registers. Pairs at
+// a time: the packed conversions are one instruction for two values.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -9,19 +10,41 @@
 namespace awqb {
 
 template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {  // a bf16 is the upper half of its fp32
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+template <typename T>
 __device__ __forceinline__ void unpack_vec(const uint4& u, float (&f)[8]) {
-  const T* h = reinterpret_cast<const T*>(&u);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = (float)h[j];
+  for (int j = 0; j < 4; ++j) {
+    const float2 p = Pair<T>::unpack(w[j]);
+    f[2 * j] = p.x;
+    f[2 * j + 1] = p.y;
+  }
 }
 
 template <typename T>
 __device__ __forceinline__ uint4 pack_vec(const float (&f)[8]) {
-  uint4 u;
-  T* h = reinterpret_cast<T*>(&u);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) h[j] = (T)f[j];
-  return u;
+  return make_uint4(Pair<T>::pack(f[0], f[1]), Pair<T>::pack(f[2], f[3]), Pair<T>::pack(f[4], f[5]),
+                    Pair<T>::pack(f[6], f[7]));
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
