@@ -277,6 +277,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     const int per_row = feats / 8;                      // threads that write one token
     const int fl = (tid % per_row) * 8, tk = tid / per_row;
     const int tok_step = 128 / per_row;
+    // Feature c stands at c, its halves of eight swapped where bit 5 is set: the
+    // 16-byte reads of eight lanes then hit all banks.
+    const int put = tid ^ ((tid >> 3) & 4), get = fl + ((fl >> 3) & 4);
     int n_tile = 0;
     bool ok = true;
     for (int t = cta; t < total; t += ctas, ++n_tile) {
@@ -307,21 +310,20 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
           }
         }
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) turn[j * kFeat + tid] = __uint_as_float(v[j / 16][j % 16]);
+        for (int j = 0; j < kChunk; ++j) turn[j * kFeat + put] = __uint_as_float(v[j / 16][j % 16]);
         named_bar_sync(1, 128);
         const int m = min(kChunk, tile.rows - c);
         for (int j = tk; j < m; j += tok_step) {
           const int to = dst[b * C::kTok + c + j];
           if (to < 0 || f >= p.n_out) continue;
-          const float* src = turn + j * kFeat + fl;
+          const float* src = turn + j * kFeat;
           float y[8];
-#pragma unroll
-          for (int i = 0; i < 8; i += 4) *reinterpret_cast<float4*>(y + i) = *reinterpret_cast<const float4*>(src + i);
+          *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(src + get);
+          *reinterpret_cast<float4*>(y + 4) = *reinterpret_cast<const float4*>(src + (get ^ 4));
           if (p.silu) {
             float u[8];
-#pragma unroll
-            for (int i = 0; i < 8; i += 4)
-              *reinterpret_cast<float4*>(u + i) = *reinterpret_cast<const float4*>(src + kFeat / 2 + i);
+            *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(src + kFeat / 2 + get);
+            *reinterpret_cast<float4*>(u + 4) = *reinterpret_cast<const float4*>(src + kFeat / 2 + (get ^ 4));
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = y[i] / (1.f + __expf(-y[i])) * u[i];
           }

@@ -402,8 +402,9 @@ int launch_decode(const Args& g, cudaLaunchConfig_t cfg) {
 template <typename T>
 int launch_prompt(const Args& g, cudaLaunchConfig_t cfg) {
   const int col_box = std::min(128, g.R), atoms = (g.rank + 63) / 64;
-  CUtensorMap tx, ta, tb, th;
+  CUtensorMap tx, trun, ta, tb, th;
   int st = make_map(&tx, g.x, g.M, g.K, g.ldx, 1);
+  if (st == kOk) st = make_map(&trun, g.x, g.M, g.K, g.ldx, kWideRows);
   if (st == kOk) st = make_map(&ta, g.a, (int64_t)g.L * g.R, g.K, g.K, col_box);
   if (st == kOk) st = make_map(&tb, g.b, (int64_t)g.L * g.N, g.rank, g.rank, kWideFeat);
   if (st == kOk) st = make_map(&th, g.halves, (int64_t)g.S * 2 * g.M, g.rank, g.rank, kWideRows);
@@ -412,7 +413,7 @@ int launch_prompt(const Args& g, cudaLaunchConfig_t cfg) {
   cfg.blockDim = dim3(kFirstWideThreads);
   cfg.dynamicSmemBytes = first_wide_smem();
   AWQB_CUDA(cudaFuncSetAttribute(lora_first_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, first_wide_smem()));
-  AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_first_wide_kernel<T>, tx, ta, g, col_box));
+  AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_first_wide_kernel<T>, tx, trun, ta, g, col_box));
   cfg.gridDim = dim3((unsigned)((g.M + 7) / 8));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;

@@ -51,7 +51,7 @@ __device__ __forceinline__ void linger() {
 
 template <typename T>
 __global__ void __launch_bounds__(kFirstWideThreads, 2)
-lora_first_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_a,
+lora_first_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_run, const __grid_constant__ CUtensorMap tm_a,
                        const __grid_constant__ Args g, int col_box) {
   extern __shared__ uint8_t raw[];
   uint8_t* ring = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
@@ -97,6 +97,12 @@ lora_first_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       row[i] = tok >= 0 && tok < g.M ? tok : 0;  // no such place: some row, its column is not used
     }
     const int groups = (n + 3) / 4;
+    // a run of one request's tokens: neighbouring rows, one box
+    const int row0 = __shfl_sync(0xffffffffu, row[0], 0);
+    bool mine = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mine = mine && (lane * 4 + i >= r.n || row[i] == row0 + lane * 4 + i);
+    const bool run = __all_sync(0xffffffffu, mine);
     const uint64_t keep = policy_evict_last();
     for (int i = 0; i < stages && ok; ++i) {
       const int s = i % kFirstStages;
@@ -105,11 +111,12 @@ lora_first_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       const uint32_t base = smem_u32(ring + s * 2 * kAtomBytes), bar = smem_u32(&full[s]);
       const int k = k_begin + i * 64;
       if (elect_one()) {
-        mbar_arrive_expect_tx(bar, groups * 512 + col_box * 128);
+        mbar_arrive_expect_tx(bar, (run ? kAtomBytes : groups * 512) + col_box * 128);
+        if (run) tma_load_2d(base, &tm_run, k, row0, bar, keep);
         tma_load_2d(base + kAtomBytes, &tm_a, k, r.adapter * g.R + ct * 128, bar, keep);
       }
       __syncwarp();
-      if (lane < groups) tma_gather4(base + lane * 512, &tm_x, k, row[0], row[1], row[2], row[3], bar);
+      if (!run && lane < groups) tma_gather4(base + lane * 512, &tm_x, k, row[0], row[1], row[2], row[3], bar);
     }
   } else if (warp == 5) {
     const uint32_t idesc = make_idesc_f16(128, n, std::is_same<T, __nv_bfloat16>::value);
@@ -316,6 +323,9 @@ lora_second_wide_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_c
   } else {  // ---------------------------------------------------------- epilogue
     const int group = warp >> 2, tid = threadIdx.x & 127;
     const int fl = (tid & 15) * 8, tk = tid >> 4;
+    // Feature c stands at c, its halves of eight swapped where bit 5 is set: the
+    // 16-byte reads of eight lanes then hit all banks.
+    const int put = tid ^ ((tid >> 3) & 4), get = fl + ((fl >> 3) & 4);
     float* turn = turns + group * 32 * kWideFeat;
     uint4 y[4];
     const auto load_base = [&](int f, int first, uint4 (&v)[4]) {  // places first + tk + 8 j
@@ -349,7 +359,7 @@ lora_second_wide_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_c
           if (lane == 0) mbar_arrive(smem_u32(&acc_empty[b]));
         }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) turn[j * kWideFeat + tid] = __uint_as_float(v[j / 16][j % 16]);
+        for (int j = 0; j < 32; ++j) turn[j * kWideFeat + put] = __uint_as_float(v[j / 16][j % 16]);
         uint4 y_next[4];
         load_base(last ? f + kWideFeat : f, last ? group * 32 : first + 64, y_next);
         named_bar_sync(1 + group, 128);
@@ -359,8 +369,8 @@ lora_second_wide_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_c
           const int64_t to = row_out[i];
           if (to >= 0 && f < f_end) {
             const float w = row_scale[i];
-            const float4 p0 = *reinterpret_cast<const float4*>(turn + (tk + 8 * j) * kWideFeat + fl);
-            const float4 p1 = *reinterpret_cast<const float4*>(turn + (tk + 8 * j) * kWideFeat + fl + 4);
+            const float4 p0 = *reinterpret_cast<const float4*>(turn + (tk + 8 * j) * kWideFeat + get);
+            const float4 p1 = *reinterpret_cast<const float4*>(turn + (tk + 8 * j) * kWideFeat + (get ^ 4));
             float o[8];
             unpack_vec<T>(y[j], o);
             o[0] += w * p0.x, o[1] += w * p0.y, o[2] += w * p0.z, o[3] += w * p0.w;
