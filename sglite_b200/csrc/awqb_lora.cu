@@ -340,10 +340,11 @@ bool wide_tiles(int64_t M) { return M >= kPromptRows; }
 
 // Parts of K: enough CTAs to fill the GPU, each part long enough to be worth its
 // sums (64 k per warp of a decode batch's CTA, eight stages of a prompt's).
-int parts_of_k(int64_t M, int64_t K, int64_t R) {
+int parts_of_k(int64_t M, int64_t K, int64_t R, int64_t L) {
   const bool wide = wide_tiles(M);
-  const int rows = wide ? kWideRows : 16, cols = wide ? 128 : 16;
-  const int64_t tiles = (M + rows - 1) / rows * ((R + cols - 1) / cols);
+  // a decode batch may have a tile for every adapter, a prompt has few partial ones
+  const int64_t rows = wide ? (M + kWideRows - 1) / kWideRows : std::min(M, M / 16 + L);
+  const int64_t tiles = rows * (wide ? (R + 127) / 128 : (R + 15) / 16);
   const int64_t want = (wide ? 222 : 296) / std::max<int64_t>(tiles, 1), most = K / 512;
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)kMaxParts}));
 }
@@ -352,10 +353,10 @@ int parts_of_k(int64_t M, int64_t K, int64_t R) {
 struct Layout {
   int64_t halves, up, bytes;
 };
-Layout layout(int64_t M, int64_t K, int64_t R, int64_t S) {
+Layout layout(int64_t M, int64_t K, int64_t R, int64_t S, int64_t L) {
   const auto round = [](int64_t v) { return (v + 255) / 256 * 256; };
   Layout l = {};
-  l.halves = round(M * R * 4 * parts_of_k(M, K, R));
+  l.halves = round(M * R * 4 * parts_of_k(M, K, R, L));
   l.up = l.halves + (wide_tiles(M) ? round(M * R * 4) : 0);
   l.bytes = l.up + (wide_tiles(M) ? round(M * S * 4) : 0);
   return l;
@@ -420,7 +421,7 @@ int launch_prompt(const Args& g, cudaLaunchConfig_t cfg) {
   AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_join_kernel<T>, g));
   // features per CTA: as many as leave eight CTAs per SM
   const int64_t share = (g.M + kWideRows - 1) / kWideRows * g.N / (8 * device_sm_count());
-  const int64_t chunk = std::max<int64_t>(1, std::min<int64_t>(16, share / kWideFeat)) * kWideFeat;
+  const int64_t chunk = std::max<int64_t>(1, std::min<int64_t>(32, share / kWideFeat)) * kWideFeat;
   const int64_t chunks = count_chunks(g, chunk);
   cfg.gridDim = dim3((unsigned)(max_tiles(g, kWideRows) * chunks));
   cfg.blockDim = dim3(kSecondWideThreads);
@@ -468,7 +469,7 @@ extern "C" int awqb_lora_workspace_bytes(int64_t M, int64_t K, int64_t L, int64_
   AWQB_REQUIRE(bytes != nullptr, kInvalidArgument, "bytes is null");
   const int st = check_sizes(M, K, L, rank, num_slices);
   if (st != kOk) return st;
-  *bytes = layout(M, K, rank * num_slices, num_slices).bytes;
+  *bytes = layout(M, K, rank * num_slices, num_slices, L).bytes;
   return kOk;
 }
 
@@ -510,9 +511,9 @@ extern "C" int awqb_lora(const void* x, int64_t M, int64_t ldx, int64_t K, const
   g.ldx = ldx, g.ld_base = ld_base, g.ld_out = ld_out;
   g.M = (int)M, g.K = (int)K, g.L = (int)L, g.rank = (int)rank, g.R = (int)(rank * num_slices), g.N = (int)N;
   g.S = (int)num_slices;
-  g.parts = parts_of_k(M, K, g.R);
+  g.parts = parts_of_k(M, K, g.R, L);
   g.k_part = (int)((K + g.parts - 1) / g.parts + 63) / 64 * 64;
-  const Layout at = layout(M, K, g.R, num_slices);
+  const Layout at = layout(M, K, g.R, num_slices, L);
   g.halves = static_cast<uint8_t*>(workspace) + at.halves;
   g.up = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at.up);
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);

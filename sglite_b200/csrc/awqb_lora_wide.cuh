@@ -13,7 +13,10 @@
 //   second: a CTA takes 128 places and a chunk of one slice's features, keeps the
 //           places' halves in shared memory and walks the chunk in blocks of 128
 //           features (both halves times the same block of B, two accumulators);
-//           two groups of four warps take turns over 32 places at a time.
+//           two groups of four warps turn 16 places at a time. base comes through
+//           cp.async, three turns ahead: each thread reads what it copied itself. (In
+//           registers one turn ahead fit, 121 us; two were slower, 185 us, since
+//           waiting for the older loads also waited for the younger ones.)
 #pragma once
 #include "awqb_ptx.cuh"
 
@@ -29,8 +32,18 @@ constexpr int kSecondWideThreads = 320; // eight epilogue warps, producer, MMA i
 constexpr uint32_t kErrLoraWait = 256u; // a bounded wait gave up
 
 constexpr int first_wide_smem() { return 1024 + kFirstStages * 2 * kAtomBytes; }
-// atoms: ceil(rank / 64). The halves of h, two blocks of B, two turning buffers.
-constexpr int second_wide_smem(int atoms) { return 1024 + 4 * atoms * kAtomBytes + 2 * 32 * kWideFeat * 4; }
+constexpr int kTurn = 16;               // places that a group turns at a time
+constexpr int kAhead = 3;               // turns whose base is on its way
+
+// atoms: ceil(rank / 64). The halves of h, a block of B, for each group two turning
+// buffers and the base of kAhead turns: two CTAs per SM up to rank 64.
+constexpr int second_wide_smem(int atoms) {
+  return 1024 + 3 * atoms * kAtomBytes + 2 * 2 * kTurn * kWideFeat * 4 + 2 * kAhead * kTurn * kWideFeat * 2;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 
 // Four rows (y0..y3) x 64 k by their numbers; the tensor map's box is one row high.
 __device__ __forceinline__ void tma_gather4(uint32_t dst, const void* tmap, int32_t x, int32_t y0, int32_t y1, int32_t y2,
@@ -217,10 +230,11 @@ lora_second_wide_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_c
   extern __shared__ uint8_t raw[];
   uint8_t* h_smem = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
   uint8_t* b_smem = h_smem + 2 * atoms * kAtomBytes;
-  float* turns = reinterpret_cast<float*>(b_smem + 2 * atoms * kAtomBytes);  // [2][32][kWideFeat]
+  float* turns = reinterpret_cast<float*>(b_smem + atoms * kAtomBytes);  // [group][2][kTurn][kWideFeat]
+  uint8_t* bases = reinterpret_cast<uint8_t*>(turns + 4 * kTurn * kWideFeat);  // [group][kAhead][2][128] vectors
   __shared__ float row_scale[kWideRows];
   __shared__ int64_t row_in[kWideRows], row_out[kWideRows];  // where a place's row starts, or -1
-  __shared__ uint64_t h_full, b_full[2], b_empty[2], acc_full[2], acc_empty[2];
+  __shared__ uint64_t h_full, b_full, b_empty, acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
 
@@ -242,20 +256,27 @@ lora_second_wide_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_c
   if (r.adapter < 0) {  // rows without an adapter: out = base
     __syncthreads();
     grid_dep_wait();
-    const int vecs = (f_end - f_begin) / 8;
-    for (int i = threadIdx.x; i < r.n * vecs; i += kSecondWideThreads) {
-      const int row = i / vecs, f = f_begin + i % vecs * 8;
-      if (row_in[row] >= 0)
-        *reinterpret_cast<uint4*>(static_cast<T*>(g.out) + row_out[row] + f) =
-            *reinterpret_cast<const uint4*>(static_cast<const T*>(g.base) + row_in[row] + f);
+    for (int row = warp; row < r.n; row += kSecondWideThreads / 32) {
+      if (row_in[row] < 0) continue;
+      const T* src = static_cast<const T*>(g.base) + row_in[row];
+      T* dst = static_cast<T*>(g.out) + row_out[row];
+      for (int f = f_begin + lane * 8; f < f_end; f += 4 * 256) {
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (f + j * 256 < f_end) v[j] = *reinterpret_cast<const uint4*>(src + f + j * 256);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (f + j * 256 < f_end) *reinterpret_cast<uint4*>(dst + f + j * 256) = v[j];
+      }
     }
     return;
   }
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&h_full), 1);
+    mbar_init(smem_u32(&b_full), 1);
+    mbar_init(smem_u32(&b_empty), 1);
     for (int b = 0; b < 2; ++b) {
-      mbar_init(smem_u32(&b_full[b]), 1);
-      mbar_init(smem_u32(&b_empty[b]), 1);
       mbar_init(smem_u32(&acc_full[b]), 1);
       mbar_init(smem_u32(&acc_empty[b]), 8);
     }
@@ -287,13 +308,12 @@ lora_second_wide_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_c
     }
     __syncwarp();
     for (int fb = 0; fb < blocks && ok; ++fb) {
-      const int b = fb & 1;
-      ok = mbar_wait(smem_u32(&b_empty[b]), ((fb >> 1) & 1) ^ 1);
+      ok = mbar_wait(smem_u32(&b_empty), (fb & 1) ^ 1);
       if (ok && elect_one()) {
-        mbar_arrive_expect_tx(smem_u32(&b_full[b]), atoms * kAtomBytes);
+        mbar_arrive_expect_tx(smem_u32(&b_full), atoms * kAtomBytes);
         for (int a = 0; a < atoms; ++a)
-          tma_load_2d(smem_u32(b_smem + (b * atoms + a) * kAtomBytes), &tm_b, a * 64,
-                      r.adapter * g.N + f_begin + fb * kWideFeat, smem_u32(&b_full[b]), keep);
+          tma_load_2d(smem_u32(b_smem + a * kAtomBytes), &tm_b, a * 64, r.adapter * g.N + f_begin + fb * kWideFeat,
+                      smem_u32(&b_full), keep);
       }
       __syncwarp();
     }
@@ -304,18 +324,18 @@ lora_second_wide_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_c
     ok = mbar_wait(smem_u32(&h_full), 0);
     for (int fb = 0; fb < blocks && ok; ++fb) {
       const int b = fb & 1;
-      ok = mbar_wait(smem_u32(&acc_empty[b]), ((fb >> 1) & 1) ^ 1) && mbar_wait(smem_u32(&b_full[b]), (fb >> 1) & 1);
+      ok = mbar_wait(smem_u32(&acc_empty[b]), ((fb >> 1) & 1) ^ 1) && mbar_wait(smem_u32(&b_full), fb & 1);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t b_desc = make_sw128_kmajor_desc(smem_u32(b_smem + b * atoms * kAtomBytes));
+        const uint64_t b_desc = make_sw128_kmajor_desc(smem_u32(b_smem));
         for (int half = 0; half < 2; ++half)
           for (int k = 0; k < steps; ++k) {
             const uint32_t at = (k >> 2) * (kAtomBytes >> 4) + (k & 3) * 2;
             tc_mma_f16(tmem + b * kWideRows, b_desc + at, h_desc + half * atoms * (kAtomBytes >> 4) + at, idesc,
                        half + k > 0);
           }
-        tc_commit(smem_u32(&b_empty[b]));
+        tc_commit(smem_u32(&b_empty));
         tc_commit(smem_u32(&acc_full[b]));
       }
       __syncwarp();
@@ -326,62 +346,77 @@ lora_second_wide_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_c
     // Feature c stands at c, its halves of eight swapped where bit 5 is set: the
     // 16-byte reads of eight lanes then hit all banks.
     const int put = tid ^ ((tid >> 3) & 4), get = fl + ((fl >> 3) & 4);
-    float* turn = turns + group * 32 * kWideFeat;
-    uint4 y[4];
-    const auto load_base = [&](int f, int first, uint4 (&v)[4]) {  // places first + tk + 8 j
+    float* turn = turns + group * 2 * kTurn * kWideFeat;
+    const uint32_t mine = smem_u32(bases) + (group * kAhead * 2 * 128 + tid) * 16;
+    // This group's turns: every second 16 places of every block.
+    const int per_block = max(0, ((r.n + kTurn - 1) / kTurn - group + 1) / 2);
+    const int all = blocks * per_block;
+    int copy_block = 0, copy_turn = 0, copied = 0;  // the next turn to copy base for, and its number
+    const auto copy_base = [&]() {
+      if (copied < all) {
+        const int f = f_begin + copy_block * kWideFeat + fl, first = (group + 2 * copy_turn) * kTurn + tk;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t at = row_in[(first + tk + 8 * j) & (kWideRows - 1)];  // -1 past r.n
-        if (at >= 0 && f < f_end) v[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(g.base) + at + f);
+        for (int j = 0; j < 2; ++j) {
+          const int64_t at = row_in[first + 8 * j];  // -1 past r.n
+          if (at >= 0 && f < f_end)
+            cp_async16(mine + (copied % kAhead * 2 + j) * 128 * 16, static_cast<const T*>(g.base) + at + f);
+        }
+        if (++copy_turn == per_block) copy_turn = 0, ++copy_block;
+        ++copied;
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (group * 32 < r.n) load_base(f_begin + fl, group * 32, y);
-    for (int fb = 0; fb < blocks; ++fb) {
+    for (int i = 0; i < kAhead; ++i) copy_base();
+    int q = 0;
+    for (int fb = 0; fb < blocks && per_block > 0; ++fb) {
       const int b = fb & 1, f = f_begin + fb * kWideFeat + fl;
-      ok = mbar_wait(smem_u32(&acc_full[b]), (fb >> 1) & 1);
-      if (!named_bar_and(1 + group, 128, ok)) break;
+      ok = named_bar_and(1 + group, 128, mbar_wait(smem_u32(&acc_full[b]), (fb >> 1) & 1));
+      if (!ok) break;
       tc_fence_after();
-      if (group * 32 >= r.n) {  // nothing for this group
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&acc_empty[b]));
-        continue;
-      }
-      for (int first = group * 32; first < r.n; first += 64) {
-        uint32_t v[2][16];
-        const uint32_t at = tmem + b * kWideRows + first + ((uint32_t)(warp & 3) << 21);
-        tmem_ld16(at, v[0]);
-        tmem_ld16(at + 16, v[1]);
+      for (int i = 0; i < per_block; ++i, ++q) {
+        const int first = (group + 2 * i) * kTurn;
+        uint32_t v[16];
+        tmem_ld16(tmem + b * kWideRows + first + ((uint32_t)(warp & 3) << 21), v);
         tmem_ld_wait();
-        const bool last = first + 64 >= r.n;
-        if (last) {
+        if (i == per_block - 1) {  // the accumulator is read
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&acc_empty[b]));
         }
+        float* here = turn + (q & 1) * kTurn * kWideFeat;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) turn[j * kWideFeat + put] = __uint_as_float(v[j / 16][j % 16]);
-        uint4 y_next[4];
-        load_base(last ? f + kWideFeat : f, last ? group * 32 : first + 64, y_next);
-        named_bar_sync(1 + group, 128);
+        for (int j = 0; j < kTurn; ++j) here[j * kWideFeat + put] = __uint_as_float(v[j]);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        named_bar_sync(1 + group, 128);  // two buffers: the next turn's writes need no second one
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = first + tk + 8 * j;
-          const int64_t to = row_out[i];
+        for (int j = 0; j < 2; ++j) {
+          const int64_t to = row_out[first + tk + 8 * j];
           if (to >= 0 && f < f_end) {
-            const float w = row_scale[i];
-            const float4 p0 = *reinterpret_cast<const float4*>(turn + (tk + 8 * j) * kWideFeat + get);
-            const float4 p1 = *reinterpret_cast<const float4*>(turn + (tk + 8 * j) * kWideFeat + (get ^ 4));
+            const float w = row_scale[first + tk + 8 * j];
+            const float4 p0 = *reinterpret_cast<const float4*>(here + (tk + 8 * j) * kWideFeat + get);
+            const float4 p1 = *reinterpret_cast<const float4*>(here + (tk + 8 * j) * kWideFeat + (get ^ 4));
+            uint4 y;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                         : "r"(mine + (q % kAhead * 2 + j) * 128 * 16)
+                         : "memory");
             float o[8];
-            unpack_vec<T>(y[j], o);
+            unpack_vec<T>(y, o);
             o[0] += w * p0.x, o[1] += w * p0.y, o[2] += w * p0.z, o[3] += w * p0.w;
             o[4] += w * p1.x, o[5] += w * p1.y, o[6] += w * p1.z, o[7] += w * p1.w;
             *reinterpret_cast<uint4*>(static_cast<T*>(g.out) + to + f) = pack_vec<T>(o);
           }
-          y[j] = y_next[j];
         }
-        named_bar_sync(1 + group, 128);
+        copy_base();
       }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (per_block == 0)  // no places for this group: it only lets the accumulators go
+      for (int fb = 0; fb < blocks && ok; ++fb) {
+        ok = mbar_wait(smem_u32(&acc_full[fb & 1]), (fb >> 1) & 1);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&acc_empty[fb & 1]));
+      }
   }
   if (!ok && lane == 0) {
     failed = 1;
