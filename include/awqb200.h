@@ -219,6 +219,8 @@ int awqb_rmsnorm(const void* input, const void* weight, void* out, int64_t M, in
 int awqb_fused_add_rmsnorm(void* input, void* residual, const void* weight, int64_t M, int64_t N,
                            int64_t ld_in, int64_t ld_res, float eps, int dtype, void* stream);
 
+/* The entry points of this section that take a structure read it during the call
+ * only; it may be reused or freed afterwards. */
 /* The norms around a block, fused with its gate and residual scale: the step
  * between one block's projection output x and the next block's input. Per row,
  * in fp32:
@@ -239,11 +241,30 @@ int awqb_fused_add_rmsnorm(void* input, void* residual, const void* weight, int6
  * pointers 16-byte aligned. out may equal x and residual_out may equal
  * residual; other overlaps are not allowed. Extends RMSNormFused,
  * srt/model_executor/layers/norm.py:28-47. */
-int awqb_gated_add_rmsnorm(const void* x, int64_t ld_x, const void* residual, int64_t ld_res, int residual_f32,
-                           const void* post_weight, const void* gate, int64_t gate_row, int64_t gate_col,
-                           int gate_act, float scale, const void* weight, float weight_offset, void* out,
-                           int64_t ld_out, void* residual_out, int64_t ld_res_out, int64_t M, int64_t N,
-                           float eps, int dtype, void* stream);
+typedef struct {
+  const void* x;
+  int64_t ld_x;
+  const void* residual;
+  int64_t ld_res;
+  int residual_f32;
+  const void* post_weight;
+  const void* gate;
+  int64_t gate_row;
+  int64_t gate_col;
+  int gate_act;
+  float scale;
+  const void* weight;
+  float weight_offset;
+  void* out;
+  int64_t ld_out;
+  void* residual_out;
+  int64_t ld_res_out;
+  int64_t M;
+  int64_t N;
+  float eps;
+  int dtype;
+} awqb_gated_norm_args;
+int awqb_gated_add_rmsnorm(const awqb_gated_norm_args* args, void* stream);
 
 /* ------------------------------------------------------------------------
  * Rotary positions of q and k between the QKV projection and attention, with
@@ -264,12 +285,27 @@ int awqb_gated_add_rmsnorm(const void* x, int64_t ld_x, const void* residual, in
  * and pointers of q, k, the weights and outputs 16-byte aligned. Hk may be 0
  * (no k). Replaces the rotary call of RopeAttn, models/blocks.py:134-139 and
  * layers/rotary.py. */
-int awqb_rotary(const void* q, int64_t q_row, int64_t q_head, int64_t Hq, const void* k, int64_t k_row,
-                int64_t k_head, int64_t Hk, const void* positions, int positions_i64, const double* inv_freq,
-                int64_t rot_dim, int64_t head_dim, int64_t M, int interleaved, float scale,
-                const void* q_weight, const void* k_weight, float eps, void* q_out, int64_t q_out_row,
-                int64_t q_out_head, void* k_out, int64_t k_out_row, int64_t k_out_head, int dtype,
-                void* stream);
+typedef struct {
+  const void* q;
+  int64_t q_row, q_head, Hq;
+  const void* k;
+  int64_t k_row, k_head, Hk;
+  const void* positions;
+  int positions_i64;
+  const double* inv_freq;
+  int64_t rot_dim, head_dim, M;
+  int interleaved;
+  float scale;
+  const void* q_weight;
+  const void* k_weight;
+  float eps;
+  void* q_out;
+  int64_t q_out_row, q_out_head;
+  void* k_out;
+  int64_t k_out_row, k_out_head;
+  int dtype;
+} awqb_rotary_args;
+int awqb_rotary(const awqb_rotary_args* args, void* stream);
 
 /* ------------------------------------------------------------------------
  * Work on rows that belong to groups (experts, adapters).
@@ -296,15 +332,26 @@ int awqb_group_rows(const int32_t* ids, int64_t n, int64_t begin, int64_t groups
  * N of 8 (16 with silu_mul); ldx and ldo are in elements, multiples of 8;
  * x, w and out 16-byte aligned. out must not overlap the inputs. E <= 1024.
  * Replaces fused_moe_kernel over dense experts, kernels/triton/fused_moe.py:155-285. */
-int awqb_grouped_gemm(const void* x, int64_t rows, int64_t ldx, const void* w, int64_t E, int64_t K, int64_t N,
-                      const int32_t* offsets, int dtype, int silu_mul, const int32_t* row_map,
-                      const float* row_scale, void* out, int64_t out_rows, int64_t ldo, void* stream);
+typedef struct {
+  const void* x;
+  int64_t rows, ldx;
+  const void* w;
+  int64_t E, K, N;
+  const int32_t* offsets;
+  int dtype;
+  int silu_mul;
+  const int32_t* row_map;
+  const float* row_scale;
+  void* out;
+  int64_t out_rows, ldo;
+} awqb_grouped_gemm_args;
+int awqb_grouped_gemm(const awqb_grouped_gemm_args* args, void* stream);
 /* Low-rank adapters of many requests beside a shared projection:
  *   out[t] = base[t] + scales[a] * (x[t] a[a]^T) b[a]^T
  * for the rows t = order[offsets[a] .. offsets[a + 1]) of adapter a; rows in no
  * adapter (the rest of order) get out = base. A merged projection (QKV,
- * gate_up) has num_slices > 1 slices of its N outputs (slices: their widths, on
- * the host, adding up to N; null with num_slices 1), each with its own pair: a
+ * gate_up) has num_slices > 1 slices of its N outputs (slices: their widths,
+ * adding up to N), each with its own pair: a
  * [L][num_slices * rank][K] stacks the slices' first factors, b [L][N][rank]
  * their second ones. Sums are fp32; the product of the first factor is kept in
  * fp32 (as two 16-bit halves in the tensor cores). scales [L] fp32 or null (1).
@@ -314,10 +361,26 @@ int awqb_grouped_gemm(const void* x, int64_t rows, int64_t ldx, const void* w, i
  * most 128, num_slices at most 4, L at most 1024; row strides are in elements,
  * multiples of 8; pointers 16-byte aligned. No counterpart in the reference. */
 int awqb_lora_workspace_bytes(int64_t M, int64_t K, int64_t L, int64_t rank, int64_t num_slices, int64_t* bytes);
-int awqb_lora(const void* x, int64_t M, int64_t ldx, int64_t K, const void* a, const void* b, int64_t L,
-              int64_t rank, int64_t N, const int64_t* slices, int64_t num_slices, const int32_t* order,
-              const int32_t* offsets, const float* scales, const void* base, int64_t ld_base, void* out,
-              int64_t ld_out, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+typedef struct {
+  const void* x;
+  int64_t M, ldx, K;
+  const void* a;
+  const void* b;
+  int64_t L, rank, N;
+  int64_t num_slices;
+  int64_t slices[4];
+  const int32_t* order;
+  const int32_t* offsets;
+  const float* scales;
+  const void* base;
+  int64_t ld_base;
+  void* out;
+  int64_t ld_out;
+  int dtype;
+  void* workspace;
+  int64_t workspace_bytes;
+} awqb_lora_args;
+int awqb_lora(const awqb_lora_args* args, void* stream);
 
 /* ------------------------------------------------------------------------
  * Tensor-parallel all-reduce. Replaces NCCLWrapper (create_nccl_uid, ctor,

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libawqb200.so")
@@ -63,21 +64,13 @@ _SIGNATURES = {
     "awqb_rmsnorm": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, ctypes.c_float, c_int, c_vp]),
     "awqb_fused_add_rmsnorm": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, ctypes.c_float, c_int,
                                        c_vp]),
-    "awqb_gated_add_rmsnorm": (
-        c_int, [c_vp, c_i64, c_vp, c_i64, c_int, c_vp, c_vp, c_i64, c_i64, c_int, ctypes.c_float, c_vp, ctypes.c_float,
-                c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, ctypes.c_float, c_int, c_vp]),
-    "awqb_rotary": (
-        c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_i64, c_i64, c_i64, c_int,
-                ctypes.c_float, c_vp, c_vp, ctypes.c_float, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_vp]),
+    "awqb_gated_add_rmsnorm": (c_int, [ctypes.c_char_p, c_vp]),
+    "awqb_rotary": (c_int, [ctypes.c_char_p, c_vp]),
     "awqb_group_rows_workspace_bytes": (c_i64, [c_i64, c_i64]),
     "awqb_group_rows": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp]),
-    "awqb_grouped_gemm": (
-        c_int, [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_int, c_vp, c_vp, c_vp, c_i64, c_i64,
-                c_vp]),
+    "awqb_grouped_gemm": (c_int, [ctypes.c_char_p, c_vp]),
     "awqb_lora_workspace_bytes": (c_int, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64p]),
-    "awqb_lora": (
-        c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64,
-                c_vp, c_i64, c_int, c_vp, c_i64, c_vp]),
+    "awqb_lora": (c_int, [ctypes.c_char_p, c_vp]),
     "awqb_moe_topk_sum": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_vp, c_vp]),
     "awqb_nccl_unique_id_bytes": (c_int, []),
     "awqb_nccl_get_unique_id": (c_int, [c_vp]),
@@ -98,6 +91,16 @@ _SIGNATURES = {
 }
 
 EXPORTED = tuple(_SIGNATURES)
+
+# Layouts (native alignment) of the structures that some entry points take, field by
+# field as in include/awqb200.h. Packing one is several times cheaper than
+# converting twenty arguments one by one; null pointers are 0.
+ARGS = {
+    "awqb_gated_add_rmsnorm": struct.Struct("@PqPqiPPqqifPfPqPqqqfi"),
+    "awqb_rotary": struct.Struct("@PqqqPqqqPiPqqqifPPfPqqPqqi"),
+    "awqb_grouped_gemm": struct.Struct("@PqqPqqqPiiPPPqq"),
+    "awqb_lora": struct.Struct("@PqqqPPqqqqqqqqPPPPqPqiPq"),
+}
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

@@ -2,20 +2,28 @@
 //   b = post ? x * rsqrt(mean(x^2) + eps) * (offset + post) : x
 //   h = residual + scale * act(gate) * b            (stored rounded)
 //   y = h * rsqrt(mean(h^2) + eps) * (offset + pre)
-// A row stays in registers from its loads to its last store, so x, residual and
-// gate are read once and h, y written once; both sums are over fp32 values.
+//
+// Bound by HBM: x, residual and gate are read once, h and y written once. A CTA
+// takes a row and holds it in registers from its loads to its last store; all of
+// a row's loads are issued before the first sum, the weights' (L1 and L2 hits)
+// before the sum that they follow, so a row waits for memory once. Both sums are
+// over fp32 values, in a fixed order. Launched with programmatic dependent
+// launch, like the other norms.
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "awqb200.h"
 #include "awqb_common.h"
+#include "awqb_ptx.cuh"
 #include "awqb_vec.cuh"
 
 namespace awqb {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kMaxThreads = 512;
 constexpr int kMaxVec = 4;  // 16-byte vectors per thread
-constexpr int kMaxN = kThreads * 8 * kMaxVec;
+constexpr int kMaxN = kMaxThreads * 8 * kMaxVec;
 
 struct Args {
   const void *x, *residual, *post, *gate, *pre;
@@ -25,108 +33,141 @@ struct Args {
   float scale, offset, eps;
 };
 
-// Sum over the CTA; every thread gets the same value.
+// Sum over the CTA; every thread gets the same value. `red` is used once per call site.
 __device__ __forceinline__ float block_sum(float v, float* red) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   v = warp_sum(v);
-  __syncthreads();  // an earlier sum may still be read
   if (lane == 0) red[warp] = v;
   __syncthreads();
-  return warp_sum(lane < kThreads / 32 ? red[lane] : 0.f);
+  return warp_sum(lane < (int)blockDim.x / 32 ? red[lane] : 0.f);
 }
 
+// exp2 and reciprocal approximations (relative error about 1e-6) for the
+// sigmoid: exact division would make this copy-like kernel issue-bound.
 __device__ __forceinline__ float activate(float g, int act) {
-  if (act == 1) return 1.f / (1.f + expf(-g));
+  if (act == 1) return __fdividef(1.f, 1.f + __expf(-g));
   if (act == 2) return tanhf(g);
-  if (act == 3) return g / (1.f + expf(-g));
+  if (act == 3) return __fdividef(g, 1.f + __expf(-g));
   return g;
 }
 
-template <typename T, bool kResF32>
-__global__ void __launch_bounds__(kThreads) gated_norm_kernel(const Args a) {
-  __shared__ float red[kThreads / 32];
+template <typename T, bool kResF32, int kVec>
+__global__ void __launch_bounds__(kMaxThreads) gated_norm_kernel(const __grid_constant__ Args a) {
+  __shared__ float red[2][kMaxThreads / 32];
+  grid_dep_wait();
+  grid_dep_launch();
   const int64_t row = blockIdx.x;
   const int nvec = a.N / 8;
-  float b[kMaxVec][8], h[kMaxVec][8];
-  float ss = 0.f;
+  const uint4* xp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ld_x);
+  const uint4* rp = reinterpret_cast<const uint4*>(static_cast<const char*>(a.residual) + row * a.ld_res * (kResF32 ? 4 : 2));
+  const T* gp = static_cast<const T*>(a.gate) + row * a.gate_row;
+  constexpr int kRes = kResF32 ? 2 : 1;  // vectors of residual per vector of x
+  uint4 x[kVec], r[kVec][kRes], g[kVec], w[kVec];
 #pragma unroll
-  for (int i = 0; i < kMaxVec; ++i) {
-    const int v = i * kThreads + threadIdx.x;
+  for (int i = 0; i < kVec; ++i) {
+    const int v = i * blockDim.x + threadIdx.x;
     if (v < nvec) {
-      unpack_vec<T>(reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ld_x)[v], b[i]);
-      if (kResF32) {
-        const float4* r = reinterpret_cast<const float4*>(static_cast<const float*>(a.residual) + row * a.ld_res);
-        const float4 lo = r[2 * v], hi = r[2 * v + 1];
-        h[i][0] = lo.x, h[i][1] = lo.y, h[i][2] = lo.z, h[i][3] = lo.w;
-        h[i][4] = hi.x, h[i][5] = hi.y, h[i][6] = hi.z, h[i][7] = hi.w;
-      } else {
-        unpack_vec<T>(reinterpret_cast<const uint4*>(static_cast<const T*>(a.residual) + row * a.ld_res)[v], h[i]);
-      }
+      x[i] = xp[v];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss += b[i][j] * b[i][j];
+      for (int j = 0; j < kRes; ++j) r[i][j] = rp[kRes * v + j];
+      if (a.gate != nullptr && a.gate_col) g[i] = reinterpret_cast<const uint4*>(gp)[v];
     }
   }
+  float one_gate = a.scale;
+  if (a.gate != nullptr && !a.gate_col) one_gate *= activate((float)gp[0], a.act);
   float rms = 1.f;
-  if (a.post != nullptr) rms = rsqrtf(block_sum(ss, red) / (float)a.N + a.eps);
-  ss = 0.f;
+  if (a.post != nullptr) {
+    float ss = 0.f;
 #pragma unroll
-  for (int i = 0; i < kMaxVec; ++i) {
-    const int v = i * kThreads + threadIdx.x;
-    if (v < nvec) {
-      if (a.post != nullptr) {
-        float w[8];
-        unpack_vec<T>(static_cast<const uint4*>(a.post)[v], w);
+    for (int i = 0; i < kVec; ++i) {
+      const int v = i * blockDim.x + threadIdx.x;
+      if (v < nvec) {
+        w[i] = static_cast<const uint4*>(a.post)[v];
+        float b[8];
+        unpack_vec<T>(x[i], b);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) b[i][j] *= rms * (a.offset + w[j]);
+        for (int j = 0; j < 8; ++j) ss += b[j] * b[j];
       }
-      if (a.gate != nullptr) {
-        const T* gp = static_cast<const T*>(a.gate) + row * a.gate_row;
-        float g[8];
-        if (a.gate_col) {
-          unpack_vec<T>(reinterpret_cast<const uint4*>(gp)[v], g);
-        } else {
+    }
+    rms = rsqrtf(block_sum(ss, red[0]) / (float)a.N + a.eps);
+  }
+  float h[kVec][8], ss = 0.f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) g[j] = (float)gp[0];
+  for (int i = 0; i < kVec; ++i) {
+    const int v = i * blockDim.x + threadIdx.x;
+    if (v < nvec) {
+      float b[8];
+      unpack_vec<T>(x[i], b);
+      if (a.post != nullptr) {
+        float p[8];
+        unpack_vec<T>(w[i], p);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] *= rms * (a.offset + p[j]);
+      }
+      if (a.pre != nullptr) w[i] = static_cast<const uint4*>(a.pre)[v];
+      if (a.gate != nullptr && a.gate_col) {
+        float t[8];
+        unpack_vec<T>(g[i], t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] *= activate(t[j], a.act);
+      }
+      if (kResF32) {
+#pragma unroll
+        for (int j = 0; j < kRes; ++j) {
+          h[i][4 * j] = __uint_as_float(r[i][j].x), h[i][4 * j + 1] = __uint_as_float(r[i][j].y);
+          h[i][4 * j + 2] = __uint_as_float(r[i][j].z), h[i][4 * j + 3] = __uint_as_float(r[i][j].w);
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) b[i][j] *= activate(g[j], a.act);
+      } else {
+        unpack_vec<T>(r[i][0], h[i]);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        h[i][j] += a.scale * b[i][j];
+        h[i][j] += one_gate * b[j];
         ss += h[i][j] * h[i][j];
       }
+      uint4* to = reinterpret_cast<uint4*>(static_cast<char*>(a.residual_out) + row * a.ld_res_out * (kResF32 ? 4 : 2));
       if (kResF32) {
-        float4* r = reinterpret_cast<float4*>(static_cast<float*>(a.residual_out) + row * a.ld_res_out);
-        r[2 * v] = make_float4(h[i][0], h[i][1], h[i][2], h[i][3]);
-        r[2 * v + 1] = make_float4(h[i][4], h[i][5], h[i][6], h[i][7]);
+#pragma unroll
+        for (int j = 0; j < kRes; ++j)
+          to[kRes * v + j] = make_uint4(__float_as_uint(h[i][4 * j]), __float_as_uint(h[i][4 * j + 1]),
+                                        __float_as_uint(h[i][4 * j + 2]), __float_as_uint(h[i][4 * j + 3]));
       } else {
-        reinterpret_cast<uint4*>(static_cast<T*>(a.residual_out) + row * a.ld_res_out)[v] = pack_vec<T>(h[i]);
+        to[v] = pack_vec<T>(h[i]);
       }
     }
   }
   if (a.pre == nullptr) return;
-  rms = rsqrtf(block_sum(ss, red) / (float)a.N + a.eps);
+  rms = rsqrtf(block_sum(ss, red[1]) / (float)a.N + a.eps);
 #pragma unroll
-  for (int i = 0; i < kMaxVec; ++i) {
-    const int v = i * kThreads + threadIdx.x;
+  for (int i = 0; i < kVec; ++i) {
+    const int v = i * blockDim.x + threadIdx.x;
     if (v < nvec) {
-      float w[8];
-      unpack_vec<T>(static_cast<const uint4*>(a.pre)[v], w);
+      float p[8];
+      unpack_vec<T>(w[i], p);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] *= rms * (a.offset + w[j]);
+      for (int j = 0; j < 8; ++j) h[i][j] *= rms * (a.offset + p[j]);
       reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.ld_out)[v] = pack_vec<T>(h[i]);
     }
   }
 }
 
-template <typename T>
-int launch(const Args& a, int64_t M, bool res_f32, cudaStream_t stream) {
-  if (res_f32)
-    gated_norm_kernel<T, true><<<(unsigned)M, kThreads, 0, stream>>>(a);
-  else
-    gated_norm_kernel<T, false><<<(unsigned)M, kThreads, 0, stream>>>(a);
-  AWQB_LAUNCH_CHECK();
+template <typename T, bool kResF32>
+int launch(const Args& a, int64_t M, cudaStream_t stream) {
+  // one vector per thread up to 4096 features, then two, then four
+  const int nvec = a.N / 8, vecs = nvec <= kMaxThreads ? 1 : nvec <= 2 * kMaxThreads ? 2 : 4;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)M);
+  cfg.blockDim = dim3((unsigned)(((nvec + vecs - 1) / vecs + 31) / 32 * 32));
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const auto kernel = vecs == 1   ? gated_norm_kernel<T, kResF32, 1>
+                      : vecs == 2 ? gated_norm_kernel<T, kResF32, 2>
+                                  : gated_norm_kernel<T, kResF32, 4>;
+  AWQB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
   return kOk;
 }
 
@@ -137,7 +178,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 using namespace awqb;
 
-extern "C" int awqb_gated_add_rmsnorm(const void* x, int64_t ld_x, const void* residual, int64_t ld_res,
+static int awqb_gated_add_rmsnorm_impl(const void* x, int64_t ld_x, const void* residual, int64_t ld_res,
                                       int residual_f32, const void* post_weight, const void* gate, int64_t gate_row,
                                       int64_t gate_col, int gate_act, float scale, const void* weight,
                                       float weight_offset, void* out, int64_t ld_out, void* residual_out,
@@ -164,6 +205,13 @@ extern "C" int awqb_gated_add_rmsnorm(const void* x, int64_t ld_x, const void* r
   Args a = {x,      residual, post_weight, gate,   weight, out,    residual_out, ld_x,         ld_res, gate_row,
             gate_col, ld_out, ld_res_out,  (int)N, gate_act, scale, weight_offset, eps};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == AWQB_DTYPE_F16 ? launch<__half>(a, M, residual_f32 != 0, st)
-                                 : launch<__nv_bfloat16>(a, M, residual_f32 != 0, st);
+  if (dtype == AWQB_DTYPE_F16) return residual_f32 ? launch<__half, true>(a, M, st) : launch<__half, false>(a, M, st);
+  return residual_f32 ? launch<__nv_bfloat16, true>(a, M, st) : launch<__nv_bfloat16, false>(a, M, st);
+}
+
+extern "C" int awqb_gated_add_rmsnorm(const awqb_gated_norm_args* a, void* stream) {
+  AWQB_REQUIRE(a != nullptr, kInvalidArgument, "args is null");
+  return awqb_gated_add_rmsnorm_impl(a->x, a->ld_x, a->residual, a->ld_res, a->residual_f32, a->post_weight, a->gate, a->gate_row,
+                                     a->gate_col, a->gate_act, a->scale, a->weight, a->weight_offset, a->out, a->ld_out,
+                                     a->residual_out, a->ld_res_out, a->M, a->N, a->eps, a->dtype, stream);
 }

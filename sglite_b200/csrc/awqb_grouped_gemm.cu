@@ -432,7 +432,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 using namespace awqb;
 
-extern "C" int awqb_grouped_gemm(const void* x, int64_t rows, int64_t ldx, const void* w, int64_t E, int64_t K,
+static int awqb_grouped_gemm_impl(const void* x, int64_t rows, int64_t ldx, const void* w, int64_t E, int64_t K,
                                  int64_t N, const int32_t* offsets, int dtype, int silu_mul, const int32_t* row_map,
                                  const float* row_scale, void* out, int64_t out_rows, int64_t ldo, void* stream) {
   AWQB_REQUIRE(dtype == AWQB_DTYPE_F16 || dtype == AWQB_DTYPE_BF16, kInvalidArgument, "bad dtype %d", dtype);
@@ -464,4 +464,10 @@ extern "C" int awqb_grouped_gemm(const void* x, int64_t rows, int64_t ldx, const
   if (dtype == AWQB_DTYPE_F16)
     return pair ? launch<__half, 2>(x, ldx, w, p, st) : launch<__half, 1>(x, ldx, w, p, st);
   return pair ? launch<__nv_bfloat16, 2>(x, ldx, w, p, st) : launch<__nv_bfloat16, 1>(x, ldx, w, p, st);
+}
+
+extern "C" int awqb_grouped_gemm(const awqb_grouped_gemm_args* a, void* stream) {
+  AWQB_REQUIRE(a != nullptr, kInvalidArgument, "args is null");
+  return awqb_grouped_gemm_impl(a->x, a->rows, a->ldx, a->w, a->E, a->K, a->N, a->offsets, a->dtype, a->silu_mul, a->row_map,
+                                a->row_scale, a->out, a->out_rows, a->ldo, stream);
 }

@@ -473,7 +473,7 @@ extern "C" int awqb_lora_workspace_bytes(int64_t M, int64_t K, int64_t L, int64_
   return kOk;
 }
 
-extern "C" int awqb_lora(const void* x, int64_t M, int64_t ldx, int64_t K, const void* a, const void* b, int64_t L,
+static int awqb_lora_impl(const void* x, int64_t M, int64_t ldx, int64_t K, const void* a, const void* b, int64_t L,
                          int64_t rank, int64_t N, const int64_t* slices, int64_t num_slices, const int32_t* order,
                          const int32_t* offsets, const float* scales, const void* base, int64_t ld_base, void* out,
                          int64_t ld_out, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -483,11 +483,10 @@ extern "C" int awqb_lora(const void* x, int64_t M, int64_t ldx, int64_t K, const
   if (st != kOk) return st;
   AWQB_REQUIRE(N > 0 && N % 8 == 0 && N <= (1 << 20), kInvalidArgument, "N=%lld must be a positive multiple of 8",
                (long long)N);
-  AWQB_REQUIRE(slices != nullptr || num_slices == 1, kInvalidArgument, "the slices' widths are missing");
   Args g = {};
   int64_t end = 0;
   for (int s = 0; s < num_slices; ++s) {
-    const int64_t w = slices ? slices[s] : N;
+    const int64_t w = slices[s];
     AWQB_REQUIRE(w > 0 && w % 8 == 0 && w <= N, kInvalidArgument, "slice width %lld must be a positive multiple of 8",
                  (long long)w);
     end += w;
@@ -518,4 +517,11 @@ extern "C" int awqb_lora(const void* x, int64_t M, int64_t ldx, int64_t K, const
   g.up = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at.up);
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   return dtype == AWQB_DTYPE_F16 ? launch<__half>(g, cs) : launch<__nv_bfloat16>(g, cs);
+}
+
+extern "C" int awqb_lora(const awqb_lora_args* a, void* stream) {
+  AWQB_REQUIRE(a != nullptr, kInvalidArgument, "args is null");
+  return awqb_lora_impl(a->x, a->M, a->ldx, a->K, a->a, a->b, a->L, a->rank, a->N, a->slices, a->num_slices, a->order,
+                        a->offsets, a->scales, a->base, a->ld_base, a->out, a->ld_out, a->dtype, a->workspace,
+                        a->workspace_bytes, stream);
 }

@@ -13,7 +13,7 @@ from typing import Dict, Optional, Tuple
 
 import torch
 
-from ._lib import c_i64, call, check, lib
+from ._lib import ARGS, c_i64, call, check, lib
 
 DTYPE_CODE = {torch.float16: 0, torch.bfloat16: 1}
 
@@ -555,36 +555,72 @@ def moe_topk_sum(y3: torch.Tensor, M: int, topk: int, topk_ids: Optional[torch.T
 
 
 # ---------------------------------------------------------------- around the projections
+# These run once per block and token, for single tokens too, so their host side is
+# kept short: one look at each tensor, one packed structure, one call.
 _FN: Dict[str, object] = {}
 
 
-def _launch(name: str, device_index: int, *args) -> None:
-    """Call a C-ABI entry point with ``device_index`` current and its stream last."""
+def _entry(name: str):
+    """(C function, packer of its argument structure)."""
     fn = _FN.get(name)
     if fn is None:
-        fn = _FN[name] = getattr(lib(), name)
+        fn = _FN[name] = (getattr(lib(), name), ARGS[name].pack if name in ARGS else None)
+    return fn
+
+
+def _run(fn, device_index: int, *args) -> None:
+    """Call ``fn`` with ``device_index`` current and that device's stream last."""
     prev = _cur_device()
     if prev == device_index:
-        check(fn(*args, _raw_stream(device_index)))
-        return
-    torch.cuda.set_device(device_index)
-    try:
-        check(fn(*args, _raw_stream(device_index)))
-    finally:
-        torch.cuda.set_device(prev)
+        status = fn(*args, _raw_stream(device_index))
+    else:
+        torch.cuda.set_device(device_index)
+        try:
+            status = fn(*args, _raw_stream(device_index))
+        finally:
+            torch.cuda.set_device(prev)
+    if status:
+        check(status)
 
 
-def _on(device_index: int, **tensors: Optional[torch.Tensor]) -> None:
-    for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.get_device() != device_index):
-            raise ValueError(f"{name} must live on the same CUDA device as the other tensors (there is no CPU path)")
+def _device_of(t: torch.Tensor) -> int:
+    di = t.get_device()
+    if di < 0:
+        raise ValueError("tensors must live on a CUDA device (there is no CPU path)")
+    return di
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _wrong_device(name: str):
+    return ValueError(f"{name} must live on the same CUDA device as the other tensors")
+
+
+def _row_stride(t: torch.Tensor, n: int, name: str) -> int:
+    """Stride between the rows of t [.., n] seen as [rows, n] (elements)."""
+    if t.is_contiguous():
+        return n
+    s = t.stride()
+    if s[-1] != 1 or t.dim() != 2:
+        raise ValueError(f"{name} must have contiguous rows, and be contiguous with more than 2 dimensions")
+    return s[0] if t.shape[0] > 1 else n
 
 
 GATE_ACTIVATIONS = {"none": 0, "sigmoid": 1, "tanh": 2, "silu": 3}
+
+
+def _gate_strides(gate: torch.Tensor, x: torch.Tensor, n: int) -> Tuple[int, int]:
+    """(row, feature) strides of a gate that broadcasts over x [.., n]."""
+    shape = gate.shape
+    wide = len(shape) > 0 and shape[-1] == n
+    if not wide and len(shape) > 0 and shape[-1] != 1:
+        raise ValueError(f"gate {tuple(shape)} does not broadcast over x {tuple(x.shape)}")
+    rows = gate.numel() // n if wide else gate.numel()
+    if rows != 1 and shape[:-1] != x.shape[:-1]:
+        raise ValueError(f"gate {tuple(shape)} does not broadcast over x {tuple(x.shape)}")
+    if wide and gate.stride(-1) != 1:
+        raise ValueError("the gate's last dimension must be the contiguous feature dimension")
+    if len(shape) > 2 and rows > 1 and not gate.is_contiguous():
+        raise ValueError("a gate with more than 2 dimensions must be contiguous")
+    return (gate.stride(-2) if rows > 1 else 0), (1 if wide else 0)
 
 
 def gated_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor], eps: float, *,
@@ -601,65 +637,65 @@ def gated_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[
     gate broadcasts over x: the shape of x, [N] or [1, N] (per channel), [.., 1]
     (per row) or one value. residual is of x's dtype or float32. ``out`` may be x
     and ``residual_out`` may be residual (in place)."""
-    code = _dtype_code(x.dtype)
-    if not x.is_cuda:
-        raise ValueError("tensors must live on a CUDA device (there is no CPU path)")
-    N = x.shape[-1]
-    di = x.get_device()
-    if residual.shape != x.shape or (residual.dtype != x.dtype and residual.dtype != torch.float32):
+    dtype, shape = x.dtype, x.shape
+    code = _dtype_code(dtype)
+    di = _device_of(x)
+    N = shape[-1]
+    wide = residual.dtype == torch.float32
+    if residual.shape != shape or (not wide and residual.dtype != dtype):
         raise ValueError("residual must have the shape of x and its dtype or float32")
-    for w in (weight, post_weight):
-        if w is not None and (w.numel() != N or w.dtype != x.dtype or not w.is_contiguous()):
-            raise ValueError("norm weights must be contiguous [N] tensors in the activation dtype")
+    if residual.get_device() != di:
+        raise _wrong_device("residual")
+    pw = pp = pg = po = ldo = gate_row = gate_col = 0
+    if weight is not None:
+        if weight.numel() != N or weight.dtype != dtype or not weight.is_contiguous():
+            raise ValueError("weight must be a contiguous [N] tensor in the activation dtype")
+        if weight.get_device() != di:
+            raise _wrong_device("weight")
+        pw = weight.data_ptr()
+    if post_weight is not None:
+        if post_weight.numel() != N or post_weight.dtype != dtype or not post_weight.is_contiguous():
+            raise ValueError("post_weight must be a contiguous [N] tensor in the activation dtype")
+        if post_weight.get_device() != di:
+            raise _wrong_device("post_weight")
+        pp = post_weight.data_ptr()
     act = GATE_ACTIVATIONS.get(gate_act)
     if act is None:
         raise ValueError(f"gate activation {gate_act!r}: one of {tuple(GATE_ACTIVATIONS)}")
-    x2, ldx = _rows_2d(x, N)
-    r2, ldr = _rows_2d(residual, N)
-    M = x2.shape[0]
-    gate_row = gate_col = 0
     if gate is not None:
-        if gate.dtype != x.dtype:
+        if gate.dtype != dtype:
             raise ValueError("gate must have the activation dtype")
-        wide = gate.dim() > 0 and gate.shape[-1] == N
-        if not wide and gate.dim() > 0 and gate.shape[-1] != 1:
-            raise ValueError(f"gate {tuple(gate.shape)} does not broadcast over x {tuple(x.shape)}")
-        rows = gate.numel() // N if wide else gate.numel()
-        if rows != 1 and (rows != M or gate.shape[:-1] != x.shape[:-1]):
-            raise ValueError(f"gate {tuple(gate.shape)} does not broadcast over x {tuple(x.shape)}")
-        if gate.dim() > 2 and rows > 1 and not gate.is_contiguous():
-            raise ValueError("tensors with more than 2 dimensions must be contiguous")
-        if wide and gate.stride(-1) != 1:
-            raise ValueError("the last dimension must be the contiguous feature dimension")
-        gate_col = 1 if wide else 0
-        if rows > 1:
-            gate_row = gate.stride(-2)
-    if weight is None:
-        if out is not None:
-            raise ValueError("out is the second norm's result: it needs weight")
-        ldo = 0
-    else:
+        if gate.get_device() != di:
+            raise _wrong_device("gate")
+        gate_row, gate_col = _gate_strides(gate, x, N)
+        pg = gate.data_ptr()
+    ldx, ldr = _row_stride(x, N, "x"), _row_stride(residual, N, "residual")
+    if weight is not None:
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        elif out.shape != x.shape or out.dtype != x.dtype:
-            raise ValueError("out must have the shape and dtype of x")
-        _, ldo = _rows_2d(out, N)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        elif out.shape != shape or out.dtype != dtype or out.get_device() != di:
+            raise ValueError("out must have the shape, dtype and device of x")
+        po, ldo = out.data_ptr(), _row_stride(out, N, "out")
+    elif out is not None:
+        raise ValueError("out is the second norm's result: it needs weight")
     if residual_out is None:
-        residual_out = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-    elif residual_out.shape != x.shape or residual_out.dtype != residual.dtype:
-        raise ValueError("residual_out must have the shape and dtype of residual")
-    _, ldro = _rows_2d(residual_out, N)
-    _on(di, residual=residual, weight=weight, post_weight=post_weight, gate=gate, out=out, residual_out=residual_out)
-    _launch("awqb_gated_add_rmsnorm", di, x2.data_ptr(), ldx, r2.data_ptr(), ldr, residual.dtype == torch.float32,
-            _ptr(post_weight), _ptr(gate), gate_row, gate_col, act, scale, _ptr(weight), weight_offset, _ptr(out), ldo,
-            residual_out.data_ptr(), ldro, M, N, eps, code)
+        residual_out = torch.empty_like(residual, memory_format=torch.contiguous_format)
+    elif residual_out.shape != shape or residual_out.dtype != residual.dtype or residual_out.get_device() != di:
+        raise ValueError("residual_out must have the shape, dtype and device of residual")
+    fn, pack = _entry("awqb_gated_add_rmsnorm")
+    _run(fn, di, pack(x.data_ptr(), ldx, residual.data_ptr(), ldr, wide, pp, pg, gate_row, gate_col, act, scale, pw,
+                      weight_offset, po, ldo, residual_out.data_ptr(), _row_stride(residual_out, N, "residual_out"),
+                      x.numel() // N if N else 0, N, eps, code))
     return out, residual_out
 
 
 def _token_head_strides(t: torch.Tensor) -> Tuple[int, int]:
     """Strides of the token and head dimensions; a dimension of one has none."""
-    s0, s1, _ = t.stride()
-    return (s0 if t.shape[0] > 1 else 0), (s1 if t.shape[1] > 1 else 0)
+    s0, s1, s2 = t.stride()
+    n0, n1, n2 = t.shape
+    if s2 != 1 and n2 > 1:
+        raise ValueError("the head dimension must be contiguous")
+    return (s0 if n0 > 1 else 0), (s1 if n1 > 1 else 0)
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, *,
@@ -674,43 +710,53 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     (j, j + rot_dim / 2) or, interleaved, (2j, 2j + 1). ``scale`` multiplies the
     turned elements. Tokens with a negative position are padding: their
     outputs are left as they were. ``q_out`` / ``k_out`` may be q / k (in place)."""
-    code = _dtype_code(q.dtype)
-    if q.dim() != 3 or not q.is_cuda:
-        raise ValueError("q must be a [tokens, heads, head_dim] tensor on a CUDA device (there is no CPU path)")
-    di = q.get_device()
+    dtype = q.dtype
+    code = _dtype_code(dtype)
+    di = _device_of(q)
+    if q.dim() != 3:
+        raise ValueError("q must be a [tokens, heads, head_dim] tensor")
     M, Hq, D = q.shape
-    if q.stride(2) != 1:
-        raise ValueError("the head dimension must be contiguous")
-    if positions.numel() != M or positions.dim() != 1 or positions.dtype not in (torch.int32, torch.int64) \
-            or not positions.is_contiguous():
+    long = positions.dtype == torch.int64
+    if positions.shape != (M,) or not (long or positions.dtype == torch.int32) or not positions.is_contiguous():
         raise ValueError("positions must be a contiguous int32 or int64 [tokens] tensor")
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous float64 [rot_dim / 2] tensor")
+    if positions.get_device() != di or inv_freq.get_device() != di:
+        raise _wrong_device("positions and inv_freq")
     if q_out is None:
-        q_out = torch.empty((M, Hq, D), dtype=q.dtype, device=q.device)
-    elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(2) != 1:
-        raise ValueError("q_out must have the shape and dtype of q and contiguous heads")
-    sq, so = _token_head_strides(q), _token_head_strides(q_out)
-    if k is None:
-        if k_out is not None or k_weight is not None:
-            raise ValueError("k_out and k_weight need k")
-        Hk, kp, kop, sk, sko = 0, None, None, (0, 0), (0, 0)
-    else:
-        if k.dim() != 3 or k.shape[0] != M or k.shape[2] != D or k.dtype != q.dtype or k.stride(2) != 1:
-            raise ValueError("k must be a [tokens, heads, head_dim] tensor with q's tokens, head_dim and dtype")
+        q_out = torch.empty((M, Hq, D), dtype=dtype, device=q.device)
+    elif q_out.shape != q.shape or q_out.dtype != dtype or q_out.get_device() != di:
+        raise ValueError("q_out must have the shape, dtype and device of q")
+    q0, q1 = _token_head_strides(q)
+    o0, o1 = _token_head_strides(q_out)
+    Hk = kp = ko = k0 = k1 = ko0 = ko1 = wq = wk = 0
+    if k is not None:
+        if k.dim() != 3 or k.shape[0] != M or k.shape[2] != D or k.dtype != dtype or k.get_device() != di:
+            raise ValueError("k must be a [tokens, heads, head_dim] tensor with q's tokens, head_dim, dtype and device")
         Hk = k.shape[1]
         if k_out is None:
-            k_out = torch.empty((M, Hk, D), dtype=q.dtype, device=q.device)
-        elif k_out.shape != k.shape or k_out.dtype != k.dtype or k_out.stride(2) != 1:
-            raise ValueError("k_out must have the shape and dtype of k and contiguous heads")
-        kp, kop, sk, sko = k.data_ptr(), k_out.data_ptr(), _token_head_strides(k), _token_head_strides(k_out)
-    for w in (q_weight, k_weight):
-        if w is not None and (w.numel() != D or w.dtype != q.dtype or not w.is_contiguous()):
-            raise ValueError("the norm weights must be contiguous [head_dim] tensors in q's dtype")
-    _on(di, k=k, positions=positions, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight, q_out=q_out, k_out=k_out)
-    _launch("awqb_rotary", di, q.data_ptr(), sq[0], sq[1], Hq, kp, sk[0], sk[1], Hk, positions.data_ptr(),
-            positions.dtype == torch.int64, inv_freq.data_ptr(), 2 * inv_freq.numel(), D, M, interleaved, scale,
-            _ptr(q_weight), _ptr(k_weight), eps, q_out.data_ptr(), so[0], so[1], kop, sko[0], sko[1], code)
+            k_out = torch.empty((M, Hk, D), dtype=dtype, device=q.device)
+        elif k_out.shape != k.shape or k_out.dtype != dtype or k_out.get_device() != di:
+            raise ValueError("k_out must have the shape, dtype and device of k")
+        kp, ko = k.data_ptr(), k_out.data_ptr()
+        k0, k1 = _token_head_strides(k)
+        ko0, ko1 = _token_head_strides(k_out)
+    elif k_out is not None or k_weight is not None:
+        raise ValueError("k_out and k_weight need k")
+    if q_weight is not None:
+        if q_weight.numel() != D or q_weight.dtype != dtype or not q_weight.is_contiguous() \
+                or q_weight.get_device() != di:
+            raise ValueError("q_weight must be a contiguous [head_dim] tensor in q's dtype on its device")
+        wq = q_weight.data_ptr()
+    if k_weight is not None:
+        if k_weight.numel() != D or k_weight.dtype != dtype or not k_weight.is_contiguous() \
+                or k_weight.get_device() != di:
+            raise ValueError("k_weight must be a contiguous [head_dim] tensor in q's dtype on its device")
+        wk = k_weight.data_ptr()
+    fn, pack = _entry("awqb_rotary")
+    _run(fn, di, pack(q.data_ptr(), q0, q1, Hq, kp, k0, k1, Hk, positions.data_ptr(), long, inv_freq.data_ptr(),
+                      2 * inv_freq.numel(), D, M, interleaved, scale, wq, wk, eps, q_out.data_ptr(), o0, o1, ko, ko0,
+                      ko1, code))
     return q_out, k_out
 
 
@@ -718,21 +764,17 @@ def group_rows(ids: torch.Tensor, num_groups: int, begin: int = 0) -> Tuple[torc
     """Stable grouping of rows by id: (order [n], offsets [num_groups + 1]), int32.
     ``order[offsets[g]:offsets[g + 1]]`` are the indices whose id is begin + g, in
     index order; indices whose id is in no group come last."""
-    if ids.dtype != torch.int32 or not ids.is_contiguous() or not ids.is_cuda:
-        raise ValueError("ids must be a contiguous int32 tensor on a CUDA device")
-    di, n = ids.get_device(), ids.numel()
+    di = _device_of(ids)
+    if ids.dtype != torch.int32 or not ids.is_contiguous():
+        raise ValueError("ids must be a contiguous int32 tensor")
+    n = ids.numel()
     order = torch.empty(n, dtype=torch.int32, device=ids.device)
     offsets = torch.empty(max(num_groups, 0) + 1, dtype=torch.int32, device=ids.device)
     nb = int(lib().awqb_group_rows_workspace_bytes(n, num_groups))
     ws = torch.empty(nb, dtype=torch.uint8, device=ids.device) if nb > 0 else None
-    _launch("awqb_group_rows", di, ids.data_ptr(), n, begin, num_groups, order.data_ptr(), offsets.data_ptr(), _ptr(ws),
-            nb)
+    _run(_entry("awqb_group_rows")[0], di, ids.data_ptr(), n, begin, num_groups, order.data_ptr(), offsets.data_ptr(),
+         None if ws is None else ws.data_ptr(), nb)
     return order, offsets
-
-
-def _offsets_ok(offsets: torch.Tensor, groups: int, what: str) -> None:
-    if offsets.dtype != torch.int32 or offsets.numel() != groups + 1 or not offsets.is_contiguous():
-        raise ValueError(f"offsets must be a contiguous int32 [{what} + 1] tensor")
 
 
 def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out: Optional[torch.Tensor] = None,
@@ -748,36 +790,42 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out
     map outside ``out`` are dropped), times row_scale[its row of out] (fp32) if
     given. Rows of ``out`` that nothing goes to are left as they were; without
     ``out`` a new [rows, N] tensor is returned, in which those rows are undefined."""
-    code = _dtype_code(x.dtype)
+    dtype = x.dtype
+    code = _dtype_code(dtype)
+    di = _device_of(x)
     if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[2]:
         raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)} must be [rows, K] and [experts, N, K]")
-    if not x.is_cuda:
-        raise ValueError("tensors must live on a CUDA device (there is no CPU path)")
-    if w.dtype != x.dtype or not w.is_contiguous() or (x.stride(1) != 1 and x.shape[1] != 1):
-        raise ValueError("w must be contiguous and of x's dtype, and x's rows contiguous")
-    di = x.get_device()
+    if w.dtype != dtype or not w.is_contiguous() or w.get_device() != di:
+        raise ValueError("w must be contiguous, of x's dtype and on its device")
     rows, K = x.shape
     E, N, _ = w.shape
-    _offsets_ok(offsets, E, "experts")
+    if offsets.dtype != torch.int32 or offsets.numel() != E + 1 or not offsets.is_contiguous() \
+            or offsets.get_device() != di:
+        raise ValueError("offsets must be a contiguous int32 [experts + 1] tensor on x's device")
     n_out = N // 2 if silu_mul else N
     if out is None:
-        out = torch.empty((rows, n_out), dtype=x.dtype, device=x.device)
-    elif out.dim() != 2 or out.shape[1] != n_out or out.dtype != x.dtype or out.stride(1) != 1:
-        raise ValueError(f"out must be a [rows, {n_out}] tensor of x's dtype with contiguous rows")
-    if row_map is not None and (row_map.dtype != torch.int32 or row_map.numel() != rows or not row_map.is_contiguous()):
-        raise ValueError("row_map must be a contiguous int32 [rows] tensor")
-    if row_scale is not None and (row_scale.dtype != torch.float32 or row_scale.numel() != out.shape[0]
-                                  or not row_scale.is_contiguous()):
-        raise ValueError("row_scale must be a contiguous float32 tensor with one value for each row of out")
-    _on(di, w=w, offsets=offsets, out=out, row_map=row_map, row_scale=row_scale)
-    _launch("awqb_grouped_gemm", di, x.data_ptr(), rows, x.stride(0) if rows > 1 else K, w.data_ptr(), E, K, N,
-            offsets.data_ptr(), code, silu_mul, _ptr(row_map), _ptr(row_scale), out.data_ptr(), out.shape[0],
-            out.stride(0) if out.shape[0] > 1 else n_out)
+        out = torch.empty((rows, n_out), dtype=dtype, device=x.device)
+    elif out.dim() != 2 or out.shape[1] != n_out or out.dtype != dtype or out.get_device() != di:
+        raise ValueError(f"out must be a [rows, {n_out}] tensor of x's dtype on its device")
+    out_rows = out.shape[0]
+    pm = ps = 0
+    if row_map is not None:
+        if row_map.dtype != torch.int32 or row_map.numel() != rows or not row_map.is_contiguous() \
+                or row_map.get_device() != di:
+            raise ValueError("row_map must be a contiguous int32 [rows] tensor on x's device")
+        pm = row_map.data_ptr()
+    if row_scale is not None:
+        if row_scale.dtype != torch.float32 or row_scale.numel() != out_rows or not row_scale.is_contiguous() \
+                or row_scale.get_device() != di:
+            raise ValueError("row_scale must be a contiguous float32 tensor on x's device, one value per row of out")
+        ps = row_scale.data_ptr()
+    fn, pack = _entry("awqb_grouped_gemm")
+    _run(fn, di, pack(x.data_ptr(), rows, _row_stride(x, K, "x"), w.data_ptr(), E, K, N, offsets.data_ptr(), code,
+                      silu_mul, pm, ps, out.data_ptr(), out_rows, _row_stride(out, n_out, "out")))
     return out
 
 
 _LORA_BYTES: Dict[Tuple[int, int, int, int, int], int] = {}
-_SLICES: Dict[Tuple[int, ...], object] = {}
 
 
 def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor,
@@ -789,47 +837,52 @@ def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, order: torch.Tensor,
     is the projection's output; ``order``, ``offsets`` are ``group_rows`` of the
     rows' adapter numbers (one call serves every projection of a step).
 
-    slices: widths of a merged projection's parts (QKV, gate_up), each with its own
-    pair; a [L, len(slices) * rank, K] stacks their first factors, b [L, N, rank] the
-    second ones. Sums are fp32. ``out`` may be base (in place)."""
-    code = _dtype_code(x.dtype)
-    if x.dim() != 2 or a.dim() != 3 or b.dim() != 3 or base.dim() != 2 or not x.is_cuda:
-        raise ValueError("x [M, K], a [L, slices * rank, K], b [L, N, rank] and base [M, N] must be CUDA tensors "
-                         "(there is no CPU path)")
+    slices: widths of a merged projection's parts (QKV, gate_up; at most 4), each with
+    its own pair; a [L, len(slices) * rank, K] stacks their first factors, b
+    [L, N, rank] the second ones. Sums are fp32. ``out`` may be base (in place)."""
+    dtype = x.dtype
+    code = _dtype_code(dtype)
+    di = _device_of(x)
+    if x.dim() != 2 or a.dim() != 3 or b.dim() != 3 or base.dim() != 2:
+        raise ValueError("x [M, K], a [L, slices * rank, K], b [L, N, rank] and base [M, N] are wanted")
     M, K = x.shape
     L, N, rank = b.shape
-    slices = (N,) if slices is None else tuple(slices)
-    if a.shape != (L, len(slices) * rank, K) or base.shape != (M, N):
+    parts = 1 if slices is None else len(slices)
+    if not 1 <= parts <= 4:
+        raise ValueError(f"{parts} slices: 1..4 are supported")
+    if a.shape != (L, parts * rank, K) or base.shape != (M, N):
         raise ValueError(f"inconsistent shapes: x {tuple(x.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)}, "
-                         f"base {tuple(base.shape)}, {len(slices)} slices")
-    if a.dtype != x.dtype or b.dtype != x.dtype or base.dtype != x.dtype or not a.is_contiguous() \
-            or not b.is_contiguous():
+                         f"base {tuple(base.shape)}, {parts} slices")
+    if a.dtype != dtype or b.dtype != dtype or base.dtype != dtype or not a.is_contiguous() or not b.is_contiguous():
         raise ValueError("a, b and base must be of x's dtype, a and b contiguous")
-    if (x.stride(1) != 1 and K != 1) or (base.stride(1) != 1 and N != 1):
-        raise ValueError("the rows of x and base must be contiguous")
+    if a.get_device() != di or b.get_device() != di or base.get_device() != di or order.get_device() != di \
+            or offsets.get_device() != di:
+        raise _wrong_device("a, b, base, order and offsets")
     if order.dtype != torch.int32 or order.numel() != M or not order.is_contiguous():
         raise ValueError("order must be a contiguous int32 [M] tensor")
-    _offsets_ok(offsets, L, "adapters")
-    if scales is not None and (scales.dtype != torch.float32 or scales.numel() != L or not scales.is_contiguous()):
-        raise ValueError("scales must be a contiguous float32 [adapters] tensor")
+    if offsets.dtype != torch.int32 or offsets.numel() != L + 1 or not offsets.is_contiguous():
+        raise ValueError("offsets must be a contiguous int32 [adapters + 1] tensor")
+    ps = 0
+    if scales is not None:
+        if scales.dtype != torch.float32 or scales.numel() != L or not scales.is_contiguous() \
+                or scales.get_device() != di:
+            raise ValueError("scales must be a contiguous float32 [adapters] tensor on x's device")
+        ps = scales.data_ptr()
     if out is None:
-        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    elif out.shape != base.shape or out.dtype != x.dtype or out.stride(1) != 1:
-        raise ValueError("out must be a [M, N] tensor of x's dtype with contiguous rows")
-    di = x.get_device()
-    _on(di, a=a, b=b, order=order, offsets=offsets, base=base, scales=scales, out=out)
-    key = (M, K, L, rank, len(slices))
+        out = torch.empty((M, N), dtype=dtype, device=x.device)
+    elif out.shape != (M, N) or out.dtype != dtype or out.get_device() != di:
+        raise ValueError("out must have the shape, dtype and device of base")
+    key = (M, K, L, rank, parts)
     nb = _LORA_BYTES.get(key)
     if nb is None:
         v = c_i64(0)
-        call("awqb_lora_workspace_bytes", M, K, L, rank, len(slices), ctypes.byref(v))
+        call("awqb_lora_workspace_bytes", M, K, L, rank, parts, ctypes.byref(v))
         nb = _LORA_BYTES[key] = v.value
-    widths = _SLICES.get(slices)
-    if widths is None:
-        widths = _SLICES[slices] = (c_i64 * len(slices))(*slices)
     # from the caching allocator: private to the stream, or to the graph being captured
-    ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=x.device)
-    _launch("awqb_lora", di, x.data_ptr(), M, x.stride(0) if M > 1 else K, K, a.data_ptr(), b.data_ptr(), L, rank, N,
-            widths, len(slices), order.data_ptr(), offsets.data_ptr(), _ptr(scales), base.data_ptr(),
-            base.stride(0) if M > 1 else N, out.data_ptr(), out.stride(0) if M > 1 else N, code, ws.data_ptr(), nb)
+    ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+    w = ((N,) if slices is None else tuple(slices)) + (0, 0, 0, 0)
+    fn, pack = _entry("awqb_lora")
+    _run(fn, di, pack(x.data_ptr(), M, _row_stride(x, K, "x"), K, a.data_ptr(), b.data_ptr(), L, rank, N, parts, w[0], w[1],
+                      w[2], w[3], order.data_ptr(), offsets.data_ptr(), ps, base.data_ptr(),
+                      _row_stride(base, N, "base"), out.data_ptr(), _row_stride(out, N, "out"), code, ws.data_ptr(), nb))
     return out

@@ -1,7 +1,6 @@
 """Refusals and host logic of the operators around the projections; no GPU. Every
 C-ABI refusal comes before any GPU work, so made-up addresses are never read."""
 
-import ctypes
 import math
 
 import pytest
@@ -15,10 +14,17 @@ from sglite_b200.rotary import RotaryEmbedding, rotary_frequencies
 P = 256  # an aligned address that nothing reads
 
 
+def _call(name, args):
+    """args as in include/awqb200.h, packed where the entry point takes a structure."""
+    fn = getattr(_lib.lib(), name)
+    if name not in _lib.ARGS:
+        return fn(*args)
+    return fn(_lib.ARGS[name].pack(*(0 if v is None else v for v in args[:-1])), args[-1])
+
+
 def _refused(name, args, status, text):
-    lib = _lib.lib()
-    assert getattr(lib, name)(*args) == status
-    assert text in lib.awqb_last_error()
+    assert _call(name, args) == status
+    assert text in _lib.lib().awqb_last_error()
 
 
 def _replace(args, **at):
@@ -75,28 +81,31 @@ def test_grouped_gemm_refusals(change, text):
     _refused("awqb_grouped_gemm", _replace(GG, **change), 1, text)
 
 
-LORA = [P, 16, 256, 256, P, P, 4, 16, 512, None, 1, P, P, None, P, 512, P, 512, 1, P, 1 << 30, None]
+LORA = [P, 16, 256, 256, P, P, 4, 16, 512, 1, 512, 0, 0, 0, P, P, None, P, 512, P, 512, 1, P, 1 << 30, None]
 
 
 @pytest.mark.parametrize("change,text", [
     ({"_3": 100}, b"K="), ({"_7": 12}, b"rank"), ({"_7": 136}, b"rank"), ({"_7": 0}, b"rank"), ({"_6": 0}, b"adapters"),
-    ({"_6": 2000}, b"adapters"), ({"_10": 5}, b"slices"), ({"_10": 2}, b"missing"), ({"_8": 500}, b"N="),
-    ({"_2": 248}, b"row strides"), ({"_15": 500}, b"row strides"), ({"_20": 16}, b"workspace"), ({"_19": None}, b"workspace"),
-    ({"_0": None}, b"null"), ({"_11": None}, b"null"), ({"_16": 8}, b"16-byte"), ({"_18": 3}, b"dtype")])
+    ({"_6": 2000}, b"adapters"), ({"_9": 5}, b"slices"), ({"_9": 0}, b"slices"), ({"_8": 500}, b"N="),
+    ({"_9": 2, "_10": 256, "_11": 128}, b"add up"), ({"_9": 2, "_10": 508, "_11": 4}, b"slice width"),
+    ({"_10": 0}, b"slice width"), ({"_2": 248}, b"row strides"), ({"_18": 500}, b"row strides"),
+    ({"_20": 508}, b"row strides"), ({"_23": 16}, b"workspace"), ({"_22": None}, b"workspace"), ({"_0": None}, b"null"),
+    ({"_14": None}, b"null"), ({"_19": 8}, b"16-byte"), ({"_21": 3}, b"dtype")])
 def test_lora_refusals(change, text):
     _refused("awqb_lora", _replace(LORA, **change), 1, text)
-    widths = (ctypes.c_int64 * 2)(256, 128)
-    _refused("awqb_lora", _replace(LORA, _9=widths, _10=2), 1, b"add up")
-    widths = (ctypes.c_int64 * 2)(508, 4)
-    _refused("awqb_lora", _replace(LORA, _9=widths, _10=2), 1, b"slice width")
+
+
+def test_a_missing_structure_is_refused():
+    for name in _lib.ARGS:
+        assert getattr(_lib.lib(), name)(None, None) == 1
+        assert b"args" in _lib.lib().awqb_last_error()
 
 
 def test_nothing_to_do_is_ok():
-    lib = _lib.lib()
-    assert lib.awqb_gated_add_rmsnorm(*_replace(NORM, _0=None, _17=0)) == 0
-    assert lib.awqb_rotary(*_replace(ROT, _0=None, _13=0)) == 0
-    assert lib.awqb_grouped_gemm(*_replace(GG, _0=None, _1=0)) == 0
-    assert lib.awqb_lora(*_replace(LORA, _0=None, _1=0)) == 0
+    assert _call("awqb_gated_add_rmsnorm", _replace(NORM, _0=None, _17=0)) == 0
+    assert _call("awqb_rotary", _replace(ROT, _0=None, _13=0)) == 0
+    assert _call("awqb_grouped_gemm", _replace(GG, _0=None, _1=0)) == 0
+    assert _call("awqb_lora", _replace(LORA, _0=None, _1=0)) == 0
 
 
 def test_wrappers_refuse_cpu_tensors_and_bad_shapes():
