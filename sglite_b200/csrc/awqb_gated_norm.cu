@@ -52,7 +52,7 @@ __device__ __forceinline__ float activate(float g, int act) {
 }
 
 template <typename T, bool kResF32, int kVec>
-__global__ void __launch_bounds__(kMaxThreads) gated_norm_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kMaxThreads, kVec <= 2 ? 2 : 1) gated_norm_kernel(const __grid_constant__ Args a) {
   __shared__ float red[2][kMaxThreads / 32];
   grid_dep_wait();
   grid_dep_launch();

@@ -1,15 +1,20 @@
 // Rotary positions of q and k, with their per-head RMSNorm folded in.
 //
-// Pair j of a head turns by the angle positions[m] * inv_freq[j]. The angle is
-// taken in turns (inv_freq / 2 pi, fp64) and reduced to a fraction of a turn in
-// fp64, so a position of millions loses nothing before the fp32 sine. Nothing is
-// tabulated: a token's sines are made once and serve all its heads.
+// Pair j of a head turns by the angle positions[m] * inv_freq[j]. Whole turns do not
+// matter, so the angle is kept as a 64-bit fraction of a turn: inv_freq / 2 pi
+// modulo 1, from fp64, times the position modulo 2^64, one integer product that
+// loses nothing at positions of millions. Its upper 32 bits go to the fp32 sine.
+// Nothing is tabulated by position: a token's sines are made once and serve all
+// its heads.
 //
-// Bound by HBM (q and k in and out). A CTA takes a token. A thread keeps one piece
-// of a head for all the heads it serves, with the sines in registers: the vectors
-// of eight at d and d + rot_dim / 2 (or one vector of four neighbouring pairs);
-// its first head's loads are issued before the sines are made. The lanes of a
-// head (a power of two) add up its squares by shuffles.
+// Bound by HBM (q and k in and out), and by instruction issue next to it. Warps work
+// by themselves: one takes a token (or, where tokens are few, a batch of its
+// heads), makes its sines, and turns batches of heads in packed fp32 arithmetic
+// (two values per instruction), a piece of a head per lane: the vectors of eight at
+// d and d + rot_dim / 2, or one vector of four neighbouring pairs. A batch's
+// loads are issued together. The lanes of a head (a power of two) add up its squares
+// by shuffles. With CTAs that shared a token's sines, their barriers and starts
+// left memory idle (8192 tokens of 32 + 8 heads of 128 with q/k norm: 37 us).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -22,8 +27,7 @@
 namespace awqb {
 namespace {
 
-constexpr int kThreads = 256;      // of the general kernel
-constexpr int kVecThreads = 320;   // at most, of the vector kernel
+constexpr int kThreads = 256;
 constexpr int kMaxD = 256;
 
 struct Side {  // q or k
@@ -37,114 +41,181 @@ struct Args {
   const void* positions;
   const double* inv_freq;
   int Hq, H, D, rot, pos64, interleaved;
-  float scale, eps;
+  float scale, eps, inv_d;
 };
 
-// scale * (cos, sin) of the token's pairs into shared memory, cos at [pair], sin at
-// [kMaxD / 2 + pair]; `place` is where a pair stands.
-template <typename Place>
-__device__ __forceinline__ void make_sines(const Args& a, int64_t pos, float* cs, Place place) {
-  for (int j = threadIdx.x; j < a.rot / 2; j += blockDim.x) {
-    const double turns = (double)pos * (a.inv_freq[j] * 0.15915494309189533577);  // 1 / (2 pi)
-    float s, c;
-    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-    cs[place(j)] = a.scale * c;
-    cs[kMaxD / 2 + place(j)] = a.scale * s;
-  }
+// The 64-bit fraction of a turn that a pair advances per position.
+__device__ __forceinline__ uint64_t turn_fraction(double inv_freq) {
+  const double turns = inv_freq * 0.15915494309189533577;  // 1 / (2 pi)
+  return (uint64_t)((turns - floor(turns)) * 18446744073709551616.0);  // 2^64
+}
+
+// scale * cos of the angle fraction * pos into *at, scale * sin kMaxD / 2 further.
+__device__ __forceinline__ void make_sine(const Args& a, uint64_t fraction, int64_t pos, float* at) {
+  const int upper = (int)((fraction * (uint64_t)pos) >> 32);  // in 2^-32 turns, -1/2 .. 1/2
+  float s, c;
+  sincospif((float)upper * 4.656612873077392578125e-10f, &s, &c);  // 2^-31
+  at[0] = a.scale * c;
+  at[kMaxD / 2] = a.scale * s;
 }
 
 __device__ __forceinline__ int64_t position_of(const Args& a, int64_t m) {
   return a.pos64 ? static_cast<const int64_t*>(a.positions)[m] : (int64_t) static_cast<const int32_t*>(a.positions)[m];
 }
 
-// kInterleaved: piece u is the vector at 8u. Otherwise pieces below rot / 16 are the
-// vectors at 8u and 8u + rot / 2, the others the vectors past rot. `lanes` lanes
-// (a power of two) per head, the last ones idle if a head has fewer pieces.
-template <typename T, bool kInterleaved>
-__global__ void __launch_bounds__(kVecThreads) rotary_vec_kernel(const __grid_constant__ Args a, int lanes, int pieces) {
-  __shared__ __align__(16) float cs[kMaxD];
+// Two fp32 values per instruction.
+__device__ __forceinline__ uint64_t bits(float2 v) { return *reinterpret_cast<const uint64_t*>(&v); }
+__device__ __forceinline__ float2 floats(uint64_t v) { return *reinterpret_cast<const float2*>(&v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return floats(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+  return floats(d);
+}
+// (x, y) turned by the angles of cosine c and sine s.
+__device__ __forceinline__ void turn2(float2& x, float2& y, float2 c, float2 s) {
+  const float2 minus = make_float2(-s.x, -s.y), p = x;
+  x = fma2(y, minus, mul2(x, c));
+  y = fma2(p, s, mul2(y, c));
+}
+template <typename T>
+__device__ __forceinline__ void unpack_pairs(const uint4& v, float2 (&f)[4]) {
+  f[0] = Pair<T>::unpack(v.x), f[1] = Pair<T>::unpack(v.y), f[2] = Pair<T>::unpack(v.z), f[3] = Pair<T>::unpack(v.w);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack_pairs(const float2 (&f)[4]) {
+  return make_uint4(Pair<T>::pack(f[0].x, f[0].y), Pair<T>::pack(f[1].x, f[1].y), Pair<T>::pack(f[2].x, f[2].y),
+                    Pair<T>::pack(f[3].x, f[3].y));
+}
+
+// Which elements a piece u of a head holds: kWhole, the vectors at 8u and
+// 8u + rot / 2 (the whole head turns); kPart, the same below rot / 16, then the
+// vectors past rot; kNext, the vector at 8u (interleaved).
+enum Pieces { kWhole, kPart, kNext };
+
+// `lanes` lanes (a power of two) per head, the last ones idle if a head has fewer
+// pieces.
+// kBatch: steps (32 / lanes heads each) whose loads are in flight together.
+template <typename T, Pieces kKind, bool kNorm, int kBatch>
+__global__ void __launch_bounds__(kThreads, 2)
+rotary_vec_kernel(const __grid_constant__ Args a, int64_t M, int lanes, int pieces, int q_batches, int k_batches, int per_unit) {
+  constexpr bool kInterleaved = kKind == kNext;
+  __shared__ __align__(16) float cs[kThreads / 32][kMaxD];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int u = lane & (lanes - 1), per_step = 32 / lanes, half = a.rot / 2;
+  const bool turns = kKind == kWhole || (kInterleaved ? u * 8 < a.rot : u * 16 < a.rot);
+  const bool two = kKind == kWhole || (kKind == kPart && turns);
+  const int at0 = kInterleaved || two ? u * 8 : a.rot + (u - a.rot / 16) * 8, at1 = u * 8 + half;
+  const int first = kInterleaved ? u * 4 : u * 8, get = kInterleaved ? first : first + ((first >> 3) & 4);
   grid_dep_wait();
   grid_dep_launch();
-  const int64_t m = blockIdx.x;
-  const int64_t pos = position_of(a, m);
-  if (pos < 0) return;  // padding
-  const int u = threadIdx.x & (lanes - 1), per_pass = blockDim.x / lanes, half = a.rot / 2;
-  const bool turns = kInterleaved ? u * 8 < a.rot : u * 16 < a.rot;
-  const bool two = !kInterleaved && turns;
-  const int at0 = kInterleaved || two ? u * 8 : a.rot + (u - a.rot / 16) * 8, at1 = u * 8 + half;
-  const auto side_of = [&](int hh) -> const Side& { return a.side[hh >= a.Hq]; };
-  const auto load = [&](int hh, uint4& v0, uint4& v1) {
-    if (hh >= a.H || u >= pieces) return;
-    const Side& s = side_of(hh);
-    const T* in = static_cast<const T*>(s.in) + m * s.row + (hh >= a.Hq ? hh - a.Hq : hh) * s.head;
-    v0 = *reinterpret_cast<const uint4*>(in + at0);
-    if (two) v1 = *reinterpret_cast<const uint4*>(in + at1);
-  };
-  int hh = threadIdx.x / lanes;
-  uint4 v0 = {}, v1 = {};
-  load(hh, v0, v1);
-  // Pair j stands at j, its halves of eight swapped where bit 5 is set: the
-  // 16-byte reads of eight lanes then hit all banks.
-  make_sines(a, pos, cs, [](int j) { return kInterleaved ? j : j ^ ((j >> 3) & 4); });
-  __syncthreads();
-  constexpr int kPairs = kInterleaved ? 4 : 8;
-  float c[kPairs], sn[kPairs];
-  if (turns) {
-    const int first = kInterleaved ? u * 4 : u * 8, get = kInterleaved ? first : first + ((first >> 3) & 4);
+  // this lane's pairs for the sines: lane, lane + 32, ...; the loads' latency passes
+  // while the first token is fetched
+  uint64_t fraction[kMaxD / 64];  // the bits of inv_freq until they are first used
+  bool fractions = false;
 #pragma unroll
-    for (int i = 0; i < kPairs; i += 4) {
-      *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(cs + (get ^ i));
-      *reinterpret_cast<float4*>(sn + i) = *reinterpret_cast<const float4*>(cs + kMaxD / 2 + (get ^ i));
-    }
-  }
-  for (int h0 = 0; h0 < a.H; h0 += per_pass, hh += per_pass) {
-    uint4 n0 = {}, n1 = {};
-    load(hh + per_pass, n0, n1);
-    const bool live = hh < a.H && u < pieces;
-    const Side& s = side_of(min(hh, a.H - 1));
-    float x[8], y[8];
-    unpack_vec<T>(v0, x);
-    unpack_vec<T>(v1, y);
-    if (a.side[0].weight != nullptr || a.side[1].weight != nullptr) {  // uniform: all lanes shuffle
-      float ss = 0.f;
+  for (int i = 0; i < kMaxD / 64; ++i)
+    fraction[i] = lane + 32 * i < half ? (uint64_t)__double_as_longlong(a.inv_freq[lane + 32 * i]) : 0;
+  const int batches = q_batches + k_batches, splits = (batches + per_unit - 1) / per_unit;
+  const int64_t units = M * splits;
+  float* sines = cs[warp];
+  for (int64_t unit = (int64_t)blockIdx.x * (kThreads / 32) + warp; unit < units; unit += (int64_t)gridDim.x * (kThreads / 32)) {
+    const int64_t m = splits == 1 ? unit : unit / splits;
+    const int b0 = splits == 1 ? 0 : (int)(unit - m * splits) * per_unit, b1 = min(batches, b0 + per_unit);
+    const int64_t pos = position_of(a, m);
+    float2 c[4], sn[4];  // interleaved: four pairs in the first two
+    for (int b = b0; b < b1; ++b) {
+      const bool is_k = b >= q_batches;
+      const Side& s = a.side[is_k];
+      const int heads = is_k ? a.H - a.Hq : a.Hq;
+      const int h0 = (is_k ? b - q_batches : b) * kBatch * per_step + lane / lanes;
+      const T* in = static_cast<const T*>(s.in) + m * s.row + h0 * s.head;
+      uint4 v0[kBatch] = {}, v1[kBatch] = {};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + (two ? y[i] * y[i] : 0.f);
-      for (int o = lanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (live && s.weight != nullptr) {
-        const float rms = rsqrtf(ss / (float)a.D + a.eps);
-        float w[8];
-        unpack_vec<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(s.weight) + at0), w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= rms * w[i];
-        if (two) {
-          unpack_vec<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(s.weight) + at1), w);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] *= rms * w[i];
+      for (int i = 0; i < kBatch; ++i)
+        if (h0 + i * per_step < heads && u < pieces) {
+          const T* at = in + i * per_step * s.head;
+          v0[i] = *reinterpret_cast<const uint4*>(at + at0);
+          if (two) v1[i] = *reinterpret_cast<const uint4*>(at + at1);
         }
-      }
-    }
-    if (live) {
-      T* out = static_cast<T*>(s.out) + m * s.out_row + (hh >= a.Hq ? hh - a.Hq : hh) * s.out_head;
-      if (kInterleaved) {
+      if (pos < 0) break;  // padding (the same for the whole warp)
+      if (b == b0) {
+        // Pair j stands at j, its halves of eight swapped where bit 5 is set: the
+        // 16-byte reads of eight lanes then hit all banks.
+        if (!fractions) {
+          fractions = true;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (u * 4 + i < half) {
-            const float p = x[2 * i], q = x[2 * i + 1];
-            x[2 * i] = p * c[i] - q * sn[i];
-            x[2 * i + 1] = p * sn[i] + q * c[i];
+          for (int i = 0; i < kMaxD / 64; ++i) fraction[i] = turn_fraction(__longlong_as_double((long long)fraction[i]));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kMaxD / 64; ++i) {
+          const int j = lane + 32 * i;
+          if (32 * i < half && j < half)
+            make_sine(a, fraction[i], pos, sines + (kInterleaved ? j : j ^ ((j >> 3) & 4)));
+        }
+        __syncwarp();
+        if (turns) {
+#pragma unroll
+          for (int i = 0; i < (kInterleaved ? 2 : 4); i += 2) {
+            const float4 p = *reinterpret_cast<const float4*>(sines + (get ^ (2 * i)));
+            const float4 q = *reinterpret_cast<const float4*>(sines + kMaxD / 2 + (get ^ (2 * i)));
+            c[i] = make_float2(p.x, p.y), c[i + 1] = make_float2(p.z, p.w);
+            sn[i] = make_float2(q.x, q.y), sn[i + 1] = make_float2(q.z, q.w);
           }
-      } else if (two) {
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          const float p = x[i], q = y[i];
-          x[i] = p * c[i] - q * sn[i];
-          y[i] = p * sn[i] + q * c[i];
         }
-        *reinterpret_cast<uint4*>(out + at1) = pack_vec<T>(y);
       }
-      *reinterpret_cast<uint4*>(out + at0) = pack_vec<T>(x);
+      float2 w0[4], w1[4];  // this piece's norm weights
+      const bool normed = kNorm && s.weight != nullptr;
+      if (normed && u < pieces) {
+        const T* w = static_cast<const T*>(s.weight);
+        unpack_pairs<T>(*reinterpret_cast<const uint4*>(w + at0), w0);
+        if (two) unpack_pairs<T>(*reinterpret_cast<const uint4*>(w + at1), w1);
+      }
+      T* out = static_cast<T*>(s.out) + m * s.out_row + h0 * s.out_head;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (h0 - lane / lanes + i * per_step >= heads) break;  // no lane has a head
+        float2 x[4], y[4];
+        unpack_pairs<T>(v0[i], x);
+        unpack_pairs<T>(v1[i], y);
+        if (normed) {  // all lanes shuffle; those without a piece hold zeros
+          float2 sq = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sq = fma2(x[j], x[j], sq);
+          if (two)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sq = fma2(y[j], y[j], sq);
+          float ss = sq.x + sq.y;
+          for (int o = lanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float rms = rsqrtf(ss * a.inv_d + a.eps);
+          const float2 both = make_float2(rms, rms);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = mul2(mul2(x[j], both), w0[j]);
+          if (two)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = mul2(mul2(y[j], both), w1[j]);
+        }
+        if (h0 + i * per_step >= heads || u >= pieces) continue;
+        T* to = out + i * per_step * s.out_head;
+        if (kInterleaved) {
+          const float cc[4] = {c[0].x, c[0].y, c[1].x, c[1].y}, ss[4] = {sn[0].x, sn[0].y, sn[1].x, sn[1].y};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (u * 4 + j < half)
+              x[j] = make_float2(x[j].x * cc[j] - x[j].y * ss[j], x[j].x * ss[j] + x[j].y * cc[j]);
+        } else if (two) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) turn2(x[j], y[j], c[j], sn[j]);
+          *reinterpret_cast<uint4*>(to + at1) = pack_pairs<T>(y);
+        }
+        *reinterpret_cast<uint4*>(to + at0) = pack_pairs<T>(x);
+      }
     }
-    v0 = n0, v1 = n1;
   }
 }
 
@@ -159,7 +230,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   const int64_t pos = position_of(a, m);
   if (pos < 0) return;  // padding
   const int half = a.rot / 2;
-  make_sines(a, pos, cs, [](int j) { return j; });
+  for (int j = threadIdx.x; j < half; j += kThreads) make_sine(a, turn_fraction(a.inv_freq[j]), pos, &cs[j]);
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int hh = warp; hh < a.H; hh += kThreads / 32) {
@@ -172,7 +243,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     if (w != nullptr) {
       float ss = 0.f;
       for (int d = lane; d < a.D; d += 32) ss += (float)in[d] * (float)in[d];
-      rms = rsqrtf(warp_sum(ss) / (float)a.D + a.eps);
+      rms = rsqrtf(warp_sum(ss) * a.inv_d + a.eps);
     }
     for (int j = lane; j < half; j += 32) {
       const int i0 = a.interleaved ? 2 * j : j, i1 = a.interleaved ? 2 * j + 1 : j + half;
@@ -190,6 +261,12 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   }
 }
 
+template <typename T, Pieces kKind>
+auto pick(bool norm, bool few) {
+  return norm ? (few ? rotary_vec_kernel<T, kKind, true, 1> : rotary_vec_kernel<T, kKind, true, 4>)
+              : (few ? rotary_vec_kernel<T, kKind, false, 1> : rotary_vec_kernel<T, kKind, false, 4>);
+}
+
 template <typename T>
 int launch(const Args& a, int64_t M, cudaStream_t st) {
   cudaLaunchAttribute attr[1];
@@ -197,22 +274,32 @@ int launch(const Args& a, int64_t M, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)M);
+  cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (!a.interleaved && a.rot % 16 != 0) {
-    cfg.blockDim = dim3(kThreads);
     AWQB_CUDA(cudaLaunchKernelEx(&cfg, rotary_kernel<T>, a));
     return kOk;
   }
   const int pieces = a.interleaved ? a.D / 8 : a.rot / 16 + (a.D - a.rot) / 8;
   int lanes = 1;
   while (lanes < pieces) lanes *= 2;
-  // equal passes over the heads, whole warps
-  const int most = kVecThreads / lanes, passes = (a.H + most - 1) / most, heads = (a.H + passes - 1) / passes;
-  cfg.blockDim = dim3((unsigned)((heads * lanes + 31) / 32 * 32));
-  AWQB_CUDA(a.interleaved ? cudaLaunchKernelEx(&cfg, rotary_vec_kernel<T, true>, a, lanes, pieces)
-                          : cudaLaunchKernelEx(&cfg, rotary_vec_kernel<T, false>, a, lanes, pieces));
+  // Few tokens: a warp per step, all at once. Else batches of four steps, and whole
+  // tokens once they give every warp of a full GPU one.
+  const int64_t warps = (int64_t)device_sm_count() * 2 * (kThreads / 32);
+  const int steps = (a.Hq * lanes + 31) / 32 + ((a.H - a.Hq) * lanes + 31) / 32;
+  const bool few = M * steps <= warps;
+  const int per_batch = (few ? 1 : 4) * 32 / lanes;
+  const int q_batches = (a.Hq + per_batch - 1) / per_batch, k_batches = (a.H - a.Hq + per_batch - 1) / per_batch;
+  const int per_unit = M >= warps ? q_batches + k_batches : 1;
+  const int64_t units = M * ((q_batches + k_batches + per_unit - 1) / per_unit);
+  cfg.gridDim = dim3((unsigned)((std::min(units, warps) + kThreads / 32 - 1) / (kThreads / 32)));
+  const bool norm = a.side[0].weight != nullptr || a.side[1].weight != nullptr;
+  const auto kernel = a.interleaved  ? pick<T, kNext>(norm, few)
+                      : a.rot == a.D ? pick<T, kWhole>(norm, few)
+                                     : pick<T, kPart>(norm, few);
+  AWQB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, M, lanes, pieces, q_batches, k_batches, per_unit));
   return kOk;
 }
 
@@ -234,7 +321,7 @@ static int awqb_rotary_impl(const void* q, int64_t q_row, int64_t q_head, int64_
                "head_dim=%lld must be a positive multiple of 8, at most %d", (long long)head_dim, kMaxD);
   AWQB_REQUIRE(rot_dim >= 2 && rot_dim % 2 == 0 && rot_dim <= head_dim, kInvalidArgument,
                "rot_dim=%lld must be even, 2..head_dim", (long long)rot_dim);
-  AWQB_REQUIRE(M >= 0 && M <= 0x7fffffff && Hq >= 1 && Hq <= 65536 && Hk >= 0 && Hk <= 65536, kInvalidArgument,
+  AWQB_REQUIRE(M >= 0 && M < (1 << 30) && Hq >= 1 && Hq <= 65536 && Hk >= 0 && Hk <= 65536, kInvalidArgument,
                "bad sizes: %lld tokens, %lld q heads, %lld k heads", (long long)M, (long long)Hq, (long long)Hk);
   AWQB_REQUIRE((q_row | q_head | q_out_row | q_out_head) % 8 == 0 &&
                    (Hk == 0 || (k_row | k_head | k_out_row | k_out_head) % 8 == 0),
@@ -258,6 +345,7 @@ static int awqb_rotary_impl(const void* q, int64_t q_row, int64_t q_head, int64_
   a.interleaved = interleaved != 0;
   a.scale = scale;
   a.eps = eps;
+  a.inv_d = 1.f / (float)head_dim;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == AWQB_DTYPE_F16 ? launch<__half>(a, M, st) : launch<__nv_bfloat16>(a, M, st);
 }
