@@ -672,14 +672,14 @@ def gated_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[
     ldx, ldr = _row_stride(x, N, "x"), _row_stride(residual, N, "residual")
     if weight is not None:
         if out is None:
-            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+            out = torch.empty_like(x)  # (padded rows give a contiguous result)
         elif out.shape != shape or out.dtype != dtype or out.get_device() != di:
             raise ValueError("out must have the shape, dtype and device of x")
         po, ldo = out.data_ptr(), _row_stride(out, N, "out")
     elif out is not None:
         raise ValueError("out is the second norm's result: it needs weight")
     if residual_out is None:
-        residual_out = torch.empty_like(residual, memory_format=torch.contiguous_format)
+        residual_out = torch.empty_like(residual)
     elif residual_out.shape != shape or residual_out.dtype != residual.dtype or residual_out.get_device() != di:
         raise ValueError("residual_out must have the shape, dtype and device of residual")
     fn, pack = _entry("awqb_gated_add_rmsnorm")
@@ -689,13 +689,7 @@ def gated_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[
     return out, residual_out
 
 
-def _token_head_strides(t: torch.Tensor) -> Tuple[int, int]:
-    """Strides of the token and head dimensions; a dimension of one has none."""
-    s0, s1, s2 = t.stride()
-    n0, n1, n2 = t.shape
-    if s2 != 1 and n2 > 1:
-        raise ValueError("the head dimension must be contiguous")
-    return (s0 if n0 > 1 else 0), (s1 if n1 > 1 else 0)
+_HEADS_NOT_CONTIGUOUS = "the head dimension must be contiguous"
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, *,
@@ -723,26 +717,40 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         raise ValueError("inv_freq must be a contiguous float64 [rot_dim / 2] tensor")
     if positions.get_device() != di or inv_freq.get_device() != di:
         raise _wrong_device("positions and inv_freq")
+    q0, q1, q2 = q.stride()
     if q_out is None:
-        q_out = torch.empty((M, Hq, D), dtype=dtype, device=q.device)
+        q_out = q.new_empty((M, Hq, D))
+        o0, o1, o2 = Hq * D, D, 1
     elif q_out.shape != q.shape or q_out.dtype != dtype or q_out.get_device() != di:
         raise ValueError("q_out must have the shape, dtype and device of q")
-    q0, q1 = _token_head_strides(q)
-    o0, o1 = _token_head_strides(q_out)
+    else:
+        o0, o1, o2 = q_out.stride()
+    if q2 != 1 or o2 != 1:
+        raise ValueError(_HEADS_NOT_CONTIGUOUS)
     Hk = kp = ko = k0 = k1 = ko0 = ko1 = wq = wk = 0
     if k is not None:
         if k.dim() != 3 or k.shape[0] != M or k.shape[2] != D or k.dtype != dtype or k.get_device() != di:
             raise ValueError("k must be a [tokens, heads, head_dim] tensor with q's tokens, head_dim, dtype and device")
         Hk = k.shape[1]
+        k0, k1, k2 = k.stride()
         if k_out is None:
-            k_out = torch.empty((M, Hk, D), dtype=dtype, device=q.device)
+            k_out = q.new_empty((M, Hk, D))
+            ko0, ko1, ko2 = Hk * D, D, 1
         elif k_out.shape != k.shape or k_out.dtype != dtype or k_out.get_device() != di:
             raise ValueError("k_out must have the shape, dtype and device of k")
+        else:
+            ko0, ko1, ko2 = k_out.stride()
+        if k2 != 1 or ko2 != 1:
+            raise ValueError(_HEADS_NOT_CONTIGUOUS)
         kp, ko = k.data_ptr(), k_out.data_ptr()
-        k0, k1 = _token_head_strides(k)
-        ko0, ko1 = _token_head_strides(k_out)
+        if Hk == 1:
+            k1 = ko1 = 0
     elif k_out is not None or k_weight is not None:
         raise ValueError("k_out and k_weight need k")
+    if M == 1:  # a dimension of one has no stride
+        q0 = o0 = k0 = ko0 = 0
+    if Hq == 1:
+        q1 = o1 = 0
     if q_weight is not None:
         if q_weight.numel() != D or q_weight.dtype != dtype or not q_weight.is_contiguous() \
                 or q_weight.get_device() != di:
@@ -804,7 +812,7 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out
         raise ValueError("offsets must be a contiguous int32 [experts + 1] tensor on x's device")
     n_out = N // 2 if silu_mul else N
     if out is None:
-        out = torch.empty((rows, n_out), dtype=dtype, device=x.device)
+        out = x.new_empty((rows, n_out))
     elif out.dim() != 2 or out.shape[1] != n_out or out.dtype != dtype or out.get_device() != di:
         raise ValueError(f"out must be a [rows, {n_out}] tensor of x's dtype on its device")
     out_rows = out.shape[0]
@@ -869,7 +877,7 @@ def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, order: torch.Tensor,
             raise ValueError("scales must be a contiguous float32 [adapters] tensor on x's device")
         ps = scales.data_ptr()
     if out is None:
-        out = torch.empty((M, N), dtype=dtype, device=x.device)
+        out = x.new_empty((M, N))
     elif out.shape != (M, N) or out.dtype != dtype or out.get_device() != di:
         raise ValueError("out must have the shape, dtype and device of base")
     key = (M, K, L, rank, parts)
