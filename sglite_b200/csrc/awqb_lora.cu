@@ -62,9 +62,10 @@ struct Rows {
 
 // The rows of tile `tile` of kRows places: the groups are [0, offsets[0]) without an
 // adapter, the adapters', and the rest without one. With adapters_only the first
-// and last kind have no tiles. All threads of the CTA take part.
+// and last kind have no tiles. *total gets the number of tiles, if asked for. All
+// threads of the CTA take part.
 template <int kThreads, int kRows>
-__device__ __forceinline__ Rows find_rows(const Args& g, int tile, bool adapters_only) {
+__device__ __forceinline__ Rows find_rows(const Args& g, int tile, bool adapters_only, int* total) {
   __shared__ int warp_tot[kThreads / 32];
   __shared__ Rows found;
   const int groups = g.L + 2;
@@ -99,8 +100,14 @@ __device__ __forceinline__ Rows find_rows(const Args& g, int tile, bool adapters
     found.p0 = p0;
     found.n = min(kRows, bound(e + 1) - p0);
   }
+  if (total != nullptr) {
+    *total = 0;
+    for (int w = 0; w < kThreads / 32; ++w) *total += warp_tot[w];
+  }
   __syncthreads();
-  return found;
+  const Rows r = found;
+  __syncthreads();  // found may be written again
+  return r;
 }
 
 template <typename T>
@@ -134,7 +141,7 @@ __global__ void __launch_bounds__(kFirstWarps * 32) lora_first_kernel(const __gr
   grid_dep_launch();
   const int col_tiles = (g.R + kCols - 1) / kCols;
   const int part = blockIdx.x % g.parts, ct = blockIdx.x / g.parts % col_tiles;
-  const Rows r = find_rows<kFirstWarps * 32, kRows>(g, blockIdx.x / (g.parts * col_tiles), true);
+  const Rows r = find_rows<kFirstWarps * 32, kRows>(g, blockIdx.x / (g.parts * col_tiles), true, nullptr);
   if (r.n <= 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
   const T* x[2];
@@ -238,7 +245,7 @@ __global__ void __launch_bounds__(kSecondWarps * 32) lora_second_kernel(const __
   constexpr int kHStride = (kRank32 + 1) / 2 * 64 + 32;
   __shared__ __align__(16) T hs[2][kRows][kHStride];
   __shared__ float row_scale[kRows];
-  const Rows r = find_rows<kSecondWarps * 32, kRows>(g, blockIdx.x / chunks, g.out == g.base);
+  const Rows r = find_rows<kSecondWarps * 32, kRows>(g, blockIdx.x / chunks, g.out == g.base, nullptr);
   if (r.n <= 0) {
     grid_dep_wait();
     return;
@@ -419,16 +426,13 @@ int launch_prompt(const Args& g, cudaLaunchConfig_t cfg) {
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
   AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_join_kernel<T>, g));
-  // features per CTA: as many as leave eight CTAs per SM
-  const int64_t share = (g.M + kWideRows - 1) / kWideRows * g.N / (8 * device_sm_count());
-  const int64_t chunk = std::max<int64_t>(1, std::min<int64_t>(32, share / kWideFeat)) * kWideFeat;
-  const int64_t chunks = count_chunks(g, chunk);
-  cfg.gridDim = dim3((unsigned)(max_tiles(g, kWideRows) * chunks));
+  const int64_t blocks_per_tile = count_chunks(g, kWideFeat);
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(max_tiles(g, kWideRows) * blocks_per_tile, device_sm_count()));
   cfg.blockDim = dim3(kSecondWideThreads);
   cfg.dynamicSmemBytes = second_wide_smem(atoms);
   AWQB_CUDA(cudaFuncSetAttribute(lora_second_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 second_wide_smem(kMaxRank / 64)));
-  AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_second_wide_kernel<T>, tb, th, g, (int)chunks, (int)chunk, atoms));
+                                 std::max(second_wide_smem(1), second_wide_smem(2))));
+  AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_second_wide_kernel<T>, tb, th, g, (int)blocks_per_tile, atoms));
   return kOk;
 }
 

@@ -10,13 +10,17 @@
 //           by their numbers per stage. Columns on the accumulator's lanes, so
 //           that a warp writes 32 neighbouring columns of a place.
 //   join:   a warp per place adds the parts in order and splits the sums in halves.
-//   second: a CTA takes 128 places and a chunk of one slice's features, keeps the
-//           places' halves in shared memory and walks the chunk in blocks of 128
-//           features (both halves times the same block of B, two accumulators);
-//           two groups of four warps turn 16 places at a time. base comes through
-//           cp.async, three turns ahead: each thread reads what it copied itself. (In
-//           registers one turn ahead fit, 121 us; two were slower, 185 us, since
-//           waiting for the older loads also waited for the younger ones.)
+//   second: persistent CTAs take equal runs of units (128 places x 128 features) and
+//           walk them in segments of one tile of places and one slice, whose halves of
+//           h stay in shared memory. Places on the accumulator's lanes: a thread adds
+//           its products to its place's row of base in shared memory, where its warp
+//           copied 32 rows of 128 features (256 bytes each) one block ahead and from
+//           where it writes them out the same way; no warp waits for another. Two
+//           groups of four warps work on alternate blocks. (Features on the lanes, the
+//           accumulator turned through shared memory in fp32 and base through the
+//           threads: bound by their instructions, 115 us for 4111 rows, rank 64, 28672
+//           features. Rows by bulk copies, one per row and block: 124 us, 16 clocks
+//           for each copy.)
 #pragma once
 #include "awqb_ptx.cuh"
 
@@ -32,15 +36,23 @@ constexpr int kSecondWideThreads = 320; // eight epilogue warps, producer, MMA i
 constexpr uint32_t kErrLoraWait = 256u; // a bounded wait gave up
 
 constexpr int first_wide_smem() { return 1024 + kFirstStages * 2 * kAtomBytes; }
-constexpr int kTurn = 16;               // places that a group turns at a time
-constexpr int kAhead = 3;               // turns whose base is on its way
+// A row of a block in shared memory: 16 bytes past a multiple of 128, so that the
+// 16-byte accesses of eight rows hit all banks.
+constexpr int kRowBytes = kWideFeat * 2 + 16;
+constexpr int kTileBytes = kWideRows * kRowBytes;
+// atoms: ceil(rank / 64). The halves of h, two blocks of B, and for each group two
+// tiles of base, or one where the factors leave no room.
+__host__ __device__ constexpr int base_tiles(int atoms) { return atoms == 1 ? 2 : 1; }
+__host__ __device__ constexpr int second_wide_smem(int atoms) { return 1024 + 4 * atoms * kAtomBytes + 2 * base_tiles(atoms) * kTileBytes; }
 
-// atoms: ceil(rank / 64). The halves of h, a block of B, for each group two turning
-// buffers and the base of kAhead turns: two CTAs per SM up to rank 64.
-constexpr int second_wide_smem(int atoms) {
-  return 1024 + 3 * atoms * kAtomBytes + 2 * 2 * kTurn * kWideFeat * 4 + 2 * kAhead * kTurn * kWideFeat * 2;
+__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
 }
-
+__device__ __forceinline__ void st_shared(uint32_t at, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -76,7 +88,7 @@ lora_first_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
   grid_dep_launch();
   const int col_tiles = (g.R + 127) / 128;
   const int part = blockIdx.x % g.parts, ct = blockIdx.x / g.parts % col_tiles;
-  const Rows r = find_rows<kFirstWideThreads, kWideRows>(g, blockIdx.x / (g.parts * col_tiles), true);
+  const Rows r = find_rows<kFirstWideThreads, kWideRows>(g, blockIdx.x / (g.parts * col_tiles), true, nullptr);
   if (r.n <= 0) return;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kFirstStages; ++s) {
@@ -224,61 +236,27 @@ __global__ void __launch_bounds__(256) lora_join_kernel(const __grid_constant__ 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kSecondWideThreads, 2)
+__global__ void __launch_bounds__(kSecondWideThreads, 1)
 lora_second_wide_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_h,
-                        const __grid_constant__ Args g, int chunks, int chunk, int atoms) {
+                        const __grid_constant__ Args g, int blocks_per_tile, int atoms) {
   extern __shared__ uint8_t raw[];
   uint8_t* h_smem = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
   uint8_t* b_smem = h_smem + 2 * atoms * kAtomBytes;
-  float* turns = reinterpret_cast<float*>(b_smem + atoms * kAtomBytes);  // [group][2][kTurn][kWideFeat]
-  uint8_t* bases = reinterpret_cast<uint8_t*>(turns + 4 * kTurn * kWideFeat);  // [group][kAhead][2][128] vectors
-  __shared__ float row_scale[kWideRows];
+  uint8_t* tiles_smem = b_smem + 2 * atoms * kAtomBytes;  // [group][base_tiles][kTileBytes]
   __shared__ int64_t row_in[kWideRows], row_out[kWideRows];  // where a place's row starts, or -1
-  __shared__ uint64_t h_full, b_full, b_empty, acc_full[2], acc_empty[2];
+  __shared__ uint64_t h_full, b_full[2], b_empty[2], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Rows r = find_rows<kSecondWideThreads, kWideRows>(g, blockIdx.x / chunks, g.out == g.base);
-  if (r.n <= 0) {
-    grid_dep_wait();
-    return;
-  }
-  const Feats feats = find_feats(g, blockIdx.x % chunks, chunk);
-  const int s = feats.slice, f_begin = feats.begin, f_end = feats.end;
-  const int blocks = (f_end - f_begin + kWideFeat - 1) / kWideFeat;
-  for (int i = threadIdx.x; i < kWideRows; i += kSecondWideThreads) {
-    const int tok = i < r.n ? g.order[r.p0 + i] : -1;
-    const bool in = tok >= 0 && tok < g.M;
-    row_in[i] = in ? tok * g.ld_base : -1;
-    row_out[i] = in ? tok * g.ld_out : -1;
-  }
-  if (r.adapter < 0) {  // rows without an adapter: out = base
-    __syncthreads();
-    grid_dep_wait();
-    for (int row = warp; row < r.n; row += kSecondWideThreads / 32) {
-      if (row_in[row] < 0) continue;
-      const T* src = static_cast<const T*>(g.base) + row_in[row];
-      T* dst = static_cast<T*>(g.out) + row_out[row];
-      for (int f = f_begin + lane * 8; f < f_end; f += 4 * 256) {
-        uint4 v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (f + j * 256 < f_end) v[j] = *reinterpret_cast<const uint4*>(src + f + j * 256);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (f + j * 256 < f_end) *reinterpret_cast<uint4*>(dst + f + j * 256) = v[j];
-      }
-    }
-    return;
-  }
+  const int bufs = base_tiles(atoms);
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&h_full), 1);
-    mbar_init(smem_u32(&b_full), 1);
-    mbar_init(smem_u32(&b_empty), 1);
     for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&b_full[b]), 1);
+      mbar_init(smem_u32(&b_empty[b]), 1);
       mbar_init(smem_u32(&acc_full[b]), 1);
-      mbar_init(smem_u32(&acc_empty[b]), 8);
+      mbar_init(smem_u32(&acc_empty[b]), 4);
     }
     failed = 0;
     fence_barrier_init();
@@ -286,150 +264,184 @@ lora_second_wide_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_c
     prefetch_tmap(&tm_h);
   }
   if (warp == 9) {
-    tmem_alloc(smem_u32(&tmem_slot), 2 * kWideRows);
+    tmem_alloc(smem_u32(&tmem_slot), 2 * kWideFeat);
     tmem_relinquish();
   }
-  grid_dep_wait();
-  const float scale = g.scales ? g.scales[r.adapter] : 1.f;
-  for (int i = threadIdx.x; i < r.n; i += kSecondWideThreads) row_scale[i] = scale * g.up[(int64_t)s * g.M + r.p0 + i];
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  const bool in_place = g.out == g.base;
+  int tiles = 0;
+  find_rows<kSecondWideThreads, kWideRows>(g, -1, in_place, &tiles);
+  const int64_t units = (int64_t)tiles * blocks_per_tile;
+  const int64_t u1 = units * (blockIdx.x + 1) / gridDim.x;
+  int done = 0, segments = 0;  // blocks and segments of products so far: the barriers' phases
   bool ok = true;
-  if (warp == 8) {  // ------------------------------------------------- h, B
-    const uint64_t keep = policy_evict_last();
-    if (elect_one()) {
-      mbar_arrive_expect_tx(smem_u32(&h_full), 2 * atoms * kAtomBytes);
-      for (int half = 0; half < 2; ++half)
-        for (int a = 0; a < atoms; ++a)
-          tma_load_2d(smem_u32(h_smem + (half * atoms + a) * kAtomBytes), &tm_h, a * 64, (2 * s + half) * g.M + r.p0,
-                      smem_u32(&h_full), keep);
+  grid_dep_wait();
+  for (int64_t u = units * blockIdx.x / gridDim.x; u < u1;) {
+    const Rows r = find_rows<kSecondWideThreads, kWideRows>(g, (int)(u / blocks_per_tile), in_place, nullptr);
+    const Feats feats = find_feats(g, (int)(u % blocks_per_tile), kWideFeat);
+    const int s = feats.slice, f_begin = feats.begin;
+    const int left = (g.slice_end[s] - f_begin + kWideFeat - 1) / kWideFeat;
+    const int blocks = (int)min((int64_t)left, u1 - u);
+    const int f_end = min(g.slice_end[s], f_begin + blocks * kWideFeat);
+    u += blocks;
+    if (r.adapter < 0) {  // rows without an adapter: out = base, a row per warp
+      for (int row = warp; row < r.n; row += kSecondWideThreads / 32) {
+        const int tok = g.order[r.p0 + row];
+        if (tok < 0 || tok >= g.M) continue;
+        const T* src = static_cast<const T*>(g.base) + tok * g.ld_base;
+        T* dst = static_cast<T*>(g.out) + tok * g.ld_out;
+        for (int f = f_begin + lane * 8; f < f_end; f += 4 * 256) {
+          uint4 v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (f + j * 256 < f_end) v[j] = *reinterpret_cast<const uint4*>(src + f + j * 256);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (f + j * 256 < f_end) *reinterpret_cast<uint4*>(dst + f + j * 256) = v[j];
+        }
+      }
+      continue;
+    }
+    if (warp == 8) {  // ----------------------------------------------- h, B
+      const uint64_t keep = policy_evict_last();
+      if (elect_one()) {
+        mbar_arrive_expect_tx(smem_u32(&h_full), 2 * atoms * kAtomBytes);
+        for (int half = 0; half < 2; ++half)
+          for (int a = 0; a < atoms; ++a)
+            tma_load_2d(smem_u32(h_smem + (half * atoms + a) * kAtomBytes), &tm_h, a * 64, (2 * s + half) * g.M + r.p0,
+                        smem_u32(&h_full), keep);
+      }
+      __syncwarp();
+      for (int i = 0; i < blocks && ok; ++i) {
+        const int b = (done + i) & 1;
+        ok = mbar_wait(smem_u32(&b_empty[b]), (((done + i) >> 1) & 1) ^ 1);
+        if (ok && elect_one()) {
+          mbar_arrive_expect_tx(smem_u32(&b_full[b]), atoms * kAtomBytes);
+          for (int a = 0; a < atoms; ++a)
+            tma_load_2d(smem_u32(b_smem + (b * atoms + a) * kAtomBytes), &tm_b, a * 64,
+                        r.adapter * g.N + f_begin + i * kWideFeat, smem_u32(&b_full[b]), keep);
+        }
+        __syncwarp();
+      }
+    } else if (warp == 9) {  // ---------------------------------------- products
+      const uint32_t idesc = make_idesc_f16(kWideRows, kWideFeat, std::is_same<T, __nv_bfloat16>::value);
+      const uint64_t h_desc = make_sw128_kmajor_desc(smem_u32(h_smem));
+      const int steps = (g.rank + 15) / 16;
+      ok = mbar_wait(smem_u32(&h_full), segments & 1);
+      for (int i = 0; i < blocks && ok; ++i) {
+        const int b = (done + i) & 1, phase = ((done + i) >> 1) & 1;
+        ok = mbar_wait(smem_u32(&acc_empty[b]), phase ^ 1) && mbar_wait(smem_u32(&b_full[b]), phase);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t b_desc = make_sw128_kmajor_desc(smem_u32(b_smem + b * atoms * kAtomBytes));
+          for (int half = 0; half < 2; ++half)
+            for (int k = 0; k < steps; ++k) {
+              const uint32_t at = (k >> 2) * (kAtomBytes >> 4) + (k & 3) * 2;
+              tc_mma_f16(tmem + b * kWideFeat, h_desc + half * atoms * (kAtomBytes >> 4) + at, b_desc + at, idesc,
+                         half + k > 0);
+            }
+          tc_commit(smem_u32(&b_empty[b]));
+          tc_commit(smem_u32(&acc_full[b]));
+        }
+        __syncwarp();
+      }
+    } else {  // -------------------------------------------------------- epilogue
+      const int group = warp >> 2, row = threadIdx.x & 127;
+      int tok = row < r.n ? g.order[r.p0 + row] : -1;
+      if (tok >= g.M) tok = -1;
+      const float scale = tok >= 0 ? (g.scales ? g.scales[r.adapter] : 1.f) * g.up[(int64_t)s * g.M + r.p0 + row] : 0.f;
+      if (group == 0) {
+        row_in[row] = tok >= 0 ? tok * g.ld_base : -1;
+        row_out[row] = tok >= 0 ? tok * g.ld_out : -1;
+      }
+      named_bar_sync(1, 256);
+      // the warp's rows of a block: lane l moves vector l % 16 of rows l / 16 + 2 j
+      const int row0 = (warp & 3) * 32 + (lane >> 4), rows = min(32, r.n - (warp & 3) * 32), fl = (lane & 15) * 8;
+      const uint32_t tile = smem_u32(tiles_smem) + (group * bufs * 4 + (warp & 3)) * 32 * kRowBytes;
+      const uint32_t mine = tile + (row & 31) * kRowBytes, moved = tile + (lane >> 4) * kRowBytes + (lane & 15) * 16;
+      const auto fetch = [&](int i, int buf) {  // base of block i of the segment, if there is one
+        const int f = f_begin + i * kWideFeat + fl;
+        if (i < blocks && f < f_end)
+          for (int j = 0; j < rows; j += 2) {
+            const int64_t at = row_in[row0 + j];  // -1 past r.n
+            if (at >= 0) cp_async16(moved + buf * kTileBytes + j * kRowBytes, static_cast<const T*>(g.base) + at + f);
+          }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      const int first = (group ^ done) & 1;  // the group's blocks are those of its accumulator
+      int buf = 0;
+      fetch(first, 0);
+      for (int i = first; i < blocks && ok; i += 2) {
+        const int f = f_begin + i * kWideFeat, width = min(kWideFeat, f_end - f);
+        if (bufs == 2) {
+          fetch(i + 2, buf ^ 1);
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
+        ok = mbar_wait(smem_u32(&acc_full[group]), ((done + i) >> 1) & 1);
+        if (!__all_sync(0xffffffffu, ok)) {  // (and the lanes' copies are seen by all)
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t at = mine + buf * kTileBytes, acc = tmem + group * kWideFeat + ((uint32_t)(warp & 3) << 21);
+        for (int c = 0; c < kWideFeat; c += 32) {
+          uint32_t v[2][16];
+          tmem_ld16(acc + c, v[0]);
+          tmem_ld16(acc + c + 16, v[1]);
+          uint4 y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j] = ld_shared(at + c * 2 + j * 16);
+          tmem_ld_wait();
+          if (c == kWideFeat - 32) {  // the accumulator is read
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&acc_empty[group]));
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float o[8];
+            unpack_vec<T>(y[j], o);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) o[q] += scale * __uint_as_float(v[j / 2][j % 2 * 8 + q]);
+            st_shared(at + c * 2 + j * 16, pack_vec<T>(o));
+          }
+        }
+        __syncwarp();
+        if (fl < width) {
+#pragma unroll 4
+          for (int j = 0; j < rows; j += 2) {
+            const int64_t to = row_out[row0 + j];
+            if (to >= 0)
+              *reinterpret_cast<uint4*>(static_cast<T*>(g.out) + to + f + fl) = ld_shared(moved + buf * kTileBytes + j * kRowBytes);
+          }
+        }
+        __syncwarp();
+        if (bufs == 2) buf ^= 1; else fetch(i + 2, 0);
+      }
+    }
+    done += blocks;
+    ++segments;
+    if (!ok && lane == 0) {
+      failed = 1;
+      atomicOr(g.err, kErrLoraWait);
     }
     __syncwarp();
-    for (int fb = 0; fb < blocks && ok; ++fb) {
-      ok = mbar_wait(smem_u32(&b_empty), (fb & 1) ^ 1);
-      if (ok && elect_one()) {
-        mbar_arrive_expect_tx(smem_u32(&b_full), atoms * kAtomBytes);
-        for (int a = 0; a < atoms; ++a)
-          tma_load_2d(smem_u32(b_smem + a * kAtomBytes), &tm_b, a * 64, r.adapter * g.N + f_begin + fb * kWideFeat,
-                      smem_u32(&b_full), keep);
-      }
-      __syncwarp();
-    }
-  } else if (warp == 9) {  // ------------------------------------------ products
-    const uint32_t idesc = make_idesc_f16(kWideFeat, (r.n + 15) / 16 * 16, std::is_same<T, __nv_bfloat16>::value);
-    const uint64_t h_desc = make_sw128_kmajor_desc(smem_u32(h_smem));
-    const int steps = (g.rank + 15) / 16;
-    ok = mbar_wait(smem_u32(&h_full), 0);
-    for (int fb = 0; fb < blocks && ok; ++fb) {
-      const int b = fb & 1;
-      ok = mbar_wait(smem_u32(&acc_empty[b]), ((fb >> 1) & 1) ^ 1) && mbar_wait(smem_u32(&b_full), fb & 1);
-      if (!ok) break;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t b_desc = make_sw128_kmajor_desc(smem_u32(b_smem));
-        for (int half = 0; half < 2; ++half)
-          for (int k = 0; k < steps; ++k) {
-            const uint32_t at = (k >> 2) * (kAtomBytes >> 4) + (k & 3) * 2;
-            tc_mma_f16(tmem + b * kWideRows, b_desc + at, h_desc + half * atoms * (kAtomBytes >> 4) + at, idesc,
-                       half + k > 0);
-          }
-        tc_commit(smem_u32(&b_empty));
-        tc_commit(smem_u32(&acc_full[b]));
-      }
-      __syncwarp();
-    }
-  } else {  // ---------------------------------------------------------- epilogue
-    const int group = warp >> 2, tid = threadIdx.x & 127;
-    const int fl = (tid & 15) * 8, tk = tid >> 4;
-    // Feature c stands at c, its halves of eight swapped where bit 5 is set: the
-    // 16-byte reads of eight lanes then hit all banks.
-    const int put = tid ^ ((tid >> 3) & 4), get = fl + ((fl >> 3) & 4);
-    float* turn = turns + group * 2 * kTurn * kWideFeat;
-    const uint32_t mine = smem_u32(bases) + (group * kAhead * 2 * 128 + tid) * 16;
-    // This group's turns: every second 16 places of every block.
-    const int per_block = max(0, ((r.n + kTurn - 1) / kTurn - group + 1) / 2);
-    const int all = blocks * per_block;
-    int copy_block = 0, copy_turn = 0, copied = 0;  // the next turn to copy base for, and its number
-    const auto copy_base = [&]() {
-      if (copied < all) {
-        const int f = f_begin + copy_block * kWideFeat + fl, first = (group + 2 * copy_turn) * kTurn + tk;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int64_t at = row_in[first + 8 * j];  // -1 past r.n
-          if (at >= 0 && f < f_end)
-            cp_async16(mine + (copied % kAhead * 2 + j) * 128 * 16, static_cast<const T*>(g.base) + at + f);
-        }
-        if (++copy_turn == per_block) copy_turn = 0, ++copy_block;
-        ++copied;
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    for (int i = 0; i < kAhead; ++i) copy_base();
-    int q = 0;
-    for (int fb = 0; fb < blocks && per_block > 0; ++fb) {
-      const int b = fb & 1, f = f_begin + fb * kWideFeat + fl;
-      ok = named_bar_and(1 + group, 128, mbar_wait(smem_u32(&acc_full[b]), (fb >> 1) & 1));
-      if (!ok) break;
-      tc_fence_after();
-      for (int i = 0; i < per_block; ++i, ++q) {
-        const int first = (group + 2 * i) * kTurn;
-        uint32_t v[16];
-        tmem_ld16(tmem + b * kWideRows + first + ((uint32_t)(warp & 3) << 21), v);
-        tmem_ld_wait();
-        if (i == per_block - 1) {  // the accumulator is read
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&acc_empty[b]));
-        }
-        float* here = turn + (q & 1) * kTurn * kWideFeat;
-#pragma unroll
-        for (int j = 0; j < kTurn; ++j) here[j * kWideFeat + put] = __uint_as_float(v[j]);
-        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
-        named_bar_sync(1 + group, 128);  // two buffers: the next turn's writes need no second one
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int64_t to = row_out[first + tk + 8 * j];
-          if (to >= 0 && f < f_end) {
-            const float w = row_scale[first + tk + 8 * j];
-            const float4 p0 = *reinterpret_cast<const float4*>(here + (tk + 8 * j) * kWideFeat + get);
-            const float4 p1 = *reinterpret_cast<const float4*>(here + (tk + 8 * j) * kWideFeat + (get ^ 4));
-            uint4 y;
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
-                         : "r"(mine + (q % kAhead * 2 + j) * 128 * 16)
-                         : "memory");
-            float o[8];
-            unpack_vec<T>(y, o);
-            o[0] += w * p0.x, o[1] += w * p0.y, o[2] += w * p0.z, o[3] += w * p0.w;
-            o[4] += w * p1.x, o[5] += w * p1.y, o[6] += w * p1.z, o[7] += w * p1.w;
-            *reinterpret_cast<uint4*>(static_cast<T*>(g.out) + to + f) = pack_vec<T>(o);
-          }
-        }
-        copy_base();
-      }
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (per_block == 0)  // no places for this group: it only lets the accumulators go
-      for (int fb = 0; fb < blocks && ok; ++fb) {
-        ok = mbar_wait(smem_u32(&acc_full[fb & 1]), (fb >> 1) & 1);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&acc_empty[fb & 1]));
-      }
+    __syncthreads();  // the halves are read
+    if (failed) break;
   }
-  if (!ok && lane == 0) {
-    failed = 1;
-    atomicOr(g.err, kErrLoraWait);
-  }
-  __syncwarp();
-  __syncthreads();
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (failed) linger();
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * kWideRows);
+    tmem_dealloc(tmem, 2 * kWideFeat);
   }
 }
 
