@@ -352,7 +352,7 @@ int parts_of_k(int64_t M, int64_t K, int64_t R, int64_t L) {
   // a decode batch may have a tile for every adapter, a prompt has few partial ones
   const int64_t rows = wide ? (M + kWideRows - 1) / kWideRows : std::min(M, M / 16 + L);
   const int64_t tiles = rows * (wide ? (R + 127) / 128 : (R + 15) / 16);
-  const int64_t want = (wide ? 222 : 296) / std::max<int64_t>(tiles, 1), most = K / 512;
+  const int64_t want = 296 / std::max<int64_t>(tiles, 1), most = K / 512;
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)kMaxParts}));
 }
 
@@ -410,9 +410,8 @@ int launch_decode(const Args& g, cudaLaunchConfig_t cfg) {
 template <typename T>
 int launch_prompt(const Args& g, cudaLaunchConfig_t cfg) {
   const int col_box = std::min(128, g.R), atoms = (g.rank + 63) / 64;
-  CUtensorMap tx, trun, ta, tb, th;
-  int st = make_map(&tx, g.x, g.M, g.K, g.ldx, 1);
-  if (st == kOk) st = make_map(&trun, g.x, g.M, g.K, g.ldx, kWideRows);
+  CUtensorMap tx, ta, tb, th;
+  int st = make_map(&tx, g.x, g.M, g.K, g.ldx, kWideRows);
   if (st == kOk) st = make_map(&ta, g.a, (int64_t)g.L * g.R, g.K, g.K, col_box);
   if (st == kOk) st = make_map(&tb, g.b, (int64_t)g.L * g.N, g.rank, g.rank, kWideFeat);
   if (st == kOk) st = make_map(&th, g.halves, (int64_t)g.S * 2 * g.M, g.rank, g.rank, kWideRows);
@@ -421,7 +420,7 @@ int launch_prompt(const Args& g, cudaLaunchConfig_t cfg) {
   cfg.blockDim = dim3(kFirstWideThreads);
   cfg.dynamicSmemBytes = first_wide_smem();
   AWQB_CUDA(cudaFuncSetAttribute(lora_first_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, first_wide_smem()));
-  AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_first_wide_kernel<T>, tx, trun, ta, g, col_box));
+  AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_first_wide_kernel<T>, tx, ta, g, col_box));
   cfg.gridDim = dim3((unsigned)((g.M + 7) / 8));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;

@@ -6,9 +6,12 @@
 // out). Here the tensor core fetches its operands from shared memory, TMA brings
 // them, and the warps only turn the accumulator and stream base and out.
 //   first:  a CTA takes 128 places of one adapter x up to 128 columns over a part of
-//           K. The rows of x are scattered: each lane of the producer warp gathers four
-//           by their numbers per stage. Columns on the accumulator's lanes, so
-//           that a warp writes 32 neighbouring columns of a place.
+//           K. A run of neighbouring rows of x (one request's tokens) comes by one TMA box
+//           a stage; scattered rows by cp.async of the four warps that wait for
+//           the accumulator. (Gathering copies, four rows each, took about 60 clocks
+//           apiece: 22 us for 4111 rows, K = 4096, 128 columns.) Columns on the
+//           accumulator's lanes, so that a warp writes 32 neighbouring columns of
+//           a place.
 //   join:   a warp per place adds the parts in order and splits the sums in halves.
 //   second: persistent CTAs take equal runs of units (128 places x 128 features) and
 //           walk them in segments of one tile of places and one slice, whose halves of
@@ -53,18 +56,8 @@ __device__ __forceinline__ uint4 ld_shared(uint32_t at) {
 __device__ __forceinline__ void st_shared(uint32_t at, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-
-// Four rows (y0..y3) x 64 k by their numbers; the tensor map's box is one row high.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const void* tmap, int32_t x, int32_t y0, int32_t y1, int32_t y2,
-                                            int32_t y3, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(tmap), "r"(x), "r"(y0), "r"(y1), "r"(y2), "r"(y3), "r"(bar)
-      : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in = true) {  // zeros if not in
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 
 // After a wait gave up: copies and products in flight get time to end.
@@ -76,7 +69,7 @@ __device__ __forceinline__ void linger() {
 
 template <typename T>
 __global__ void __launch_bounds__(kFirstWideThreads, 2)
-lora_first_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_run, const __grid_constant__ CUtensorMap tm_a,
+lora_first_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_a,
                        const __grid_constant__ Args g, int col_box) {
   extern __shared__ uint8_t raw[];
   uint8_t* ring = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
@@ -90,9 +83,12 @@ lora_first_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
   const int part = blockIdx.x % g.parts, ct = blockIdx.x / g.parts % col_tiles;
   const Rows r = find_rows<kFirstWideThreads, kWideRows>(g, blockIdx.x / (g.parts * col_tiles), true, nullptr);
   if (r.n <= 0) return;
+  const int row0 = g.order[r.p0];
+  const bool run = __syncthreads_and((int)threadIdx.x >= r.n || g.order[r.p0 + threadIdx.x] == row0 + (int)threadIdx.x) &&
+                   row0 >= 0 && row0 + r.n <= g.M;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kFirstStages; ++s) {
-      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&full[s]), run ? 1 : 1 + 128);
       mbar_init(smem_u32(&empty[s]), 1);
     }
     mbar_init(smem_u32(&acc_full), 1);
@@ -114,20 +110,6 @@ lora_first_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
   const int n = (r.n + 15) / 16 * 16;
   bool ok = true;
   if (warp == 4) {
-    int row[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int place = lane * 4 + i;
-      const int tok = place < r.n ? g.order[r.p0 + place] : 0;
-      row[i] = tok >= 0 && tok < g.M ? tok : 0;  // no such place: some row, its column is not used
-    }
-    const int groups = (n + 3) / 4;
-    // a run of one request's tokens: neighbouring rows, one box
-    const int row0 = __shfl_sync(0xffffffffu, row[0], 0);
-    bool mine = true;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) mine = mine && (lane * 4 + i >= r.n || row[i] == row0 + lane * 4 + i);
-    const bool run = __all_sync(0xffffffffu, mine);
     const uint64_t keep = policy_evict_last();
     for (int i = 0; i < stages && ok; ++i) {
       const int s = i % kFirstStages;
@@ -136,12 +118,11 @@ lora_first_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       const uint32_t base = smem_u32(ring + s * 2 * kAtomBytes), bar = smem_u32(&full[s]);
       const int k = k_begin + i * 64;
       if (elect_one()) {
-        mbar_arrive_expect_tx(bar, (run ? kAtomBytes : groups * 512) + col_box * 128);
-        if (run) tma_load_2d(base, &tm_run, k, row0, bar, keep);
+        mbar_arrive_expect_tx(bar, (run ? kAtomBytes : 0) + col_box * 128);
+        if (run) tma_load_2d(base, &tm_x, k, row0, bar, keep);
         tma_load_2d(base + kAtomBytes, &tm_a, k, r.adapter * g.R + ct * 128, bar, keep);
       }
       __syncwarp();
-      if (!run && lane < groups) tma_gather4(base + lane * 512, &tm_x, k, row[0], row[1], row[2], row[3], bar);
     }
   } else if (warp == 5) {
     const uint32_t idesc = make_idesc_f16(128, n, std::is_same<T, __nv_bfloat16>::value);
@@ -161,7 +142,38 @@ lora_first_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
       __syncwarp();
     }
   } else {
-    ok = mbar_wait(smem_u32(&acc_full), 0);
+    if (!run) {  // these warps copy x: 8 lanes a row, 16 bytes each
+      const int chunk = threadIdx.x & 7, line = threadIdx.x >> 3;
+      int row[8];  // rows line + 16 j; no such place: its column is not used
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int place = line + 16 * j;
+        row[j] = place < r.n ? g.order[r.p0 + place] : -1;
+        if (row[j] >= g.M) row[j] = -1;
+      }
+      const auto landed = [&](int i) {  // stage i's copies of this thread are complete
+        fence_proxy_async_smem();
+        mbar_arrive(smem_u32(&full[i % kFirstStages]));
+      };
+      for (int i = 0; i < stages && ok; ++i) {
+        const int s = i % kFirstStages, k = k_begin + i * 64 + chunk * 8;
+        ok = mbar_wait(smem_u32(&empty[s]), ((i / kFirstStages) & 1) ^ 1);
+        if (!ok) break;
+        const uint32_t base = smem_u32(ring + s * 2 * kAtomBytes) + line * 128 + ((chunk ^ (line & 7)) << 4);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (row[j] >= 0)
+            cp_async16(base + j * 16 * 128, static_cast<const T*>(g.x) + row[j] * g.ldx + (k < g.K ? k : 0), k < g.K);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        if (i > 1) landed(i - 2);
+      }
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      if (ok && stages > 1) landed(stages - 2);
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if (ok) landed(stages - 1);
+    }
+    ok = ok && mbar_wait(smem_u32(&acc_full), 0);
     if (named_bar_and(1, 128, ok)) {
       tc_fence_after();
       const int col = ct * 128 + threadIdx.x;
