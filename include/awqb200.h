@@ -328,7 +328,8 @@ int awqb_group_rows(const int32_t* ids, int64_t n, int64_t begin, int64_t groups
  * [offsets[0], offsets[E]) are not computed. With row_map, y[r] goes to row
  * row_map[r] of out (rows that map outside 0..out_rows - 1 are dropped), else
  * to row r; with row_scale (fp32) it is multiplied by row_scale[its out row].
- * Rows of out that nothing maps to are left as they were. K is a multiple of 8,
+ * No two rows may map to one. Rows of out that nothing maps to are left as they
+ * were. K is a multiple of 8,
  * N of 8 (16 with silu_mul); ldx and ldo are in elements, multiples of 8;
  * x, w and out 16-byte aligned. out must not overlap the inputs. E <= 1024.
  * Replaces fused_moe_kernel over dense experts, kernels/triton/fused_moe.py:155-285. */
@@ -357,10 +358,11 @@ int awqb_grouped_gemm(const awqb_grouped_gemm_args* args, void* stream);
  * fp32 (as two 16-bit halves in the tensor cores). scales [L] fp32 or null (1).
  * order [M] and offsets [L + 1] as awqb_group_rows gives them: order is a
  * permutation of the rows (an entry outside 0..M - 1 is skipped). out may
- * equal base. K is a multiple of 8, the slice widths of 8, rank of 8 and at
+ * equal base (with the same row stride); other overlaps are not allowed. K is a multiple of 8, the slice widths of 8, rank of 8 and at
  * most 128, num_slices at most 4, L at most 1024; row strides are in elements,
  * multiples of 8; pointers 16-byte aligned. No counterpart in the reference. */
-int awqb_lora_workspace_bytes(int64_t M, int64_t K, int64_t L, int64_t rank, int64_t num_slices, int64_t* bytes);
+int awqb_lora_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t L, int64_t rank, int64_t num_slices,
+                              int64_t* bytes);
 typedef struct {
   const void* x;
   int64_t M, ldx, K;

@@ -69,7 +69,7 @@ _SIGNATURES = {
     "awqb_group_rows_workspace_bytes": (c_i64, [c_i64, c_i64]),
     "awqb_group_rows": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp]),
     "awqb_grouped_gemm": (c_int, [ctypes.c_char_p, c_vp]),
-    "awqb_lora_workspace_bytes": (c_int, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64p]),
+    "awqb_lora_workspace_bytes": (c_int, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64p]),
     "awqb_lora": (c_int, [ctypes.c_char_p, c_vp]),
     "awqb_moe_topk_sum": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_vp, c_vp]),
     "awqb_nccl_unique_id_bytes": (c_int, []),

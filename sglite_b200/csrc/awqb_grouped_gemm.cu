@@ -13,7 +13,7 @@
 // warp, an MMA warp (tcgen05, fp32 accumulators in tensor memory) and epilogue warps
 // work side by side.
 //
-// Two kernels. Up to 64 rows per expert on average the weights' bytes bound the work:
+// Two kernels. Up to 24 rows per expert on average the weights' bytes bound the work:
 // one CTA per tile of 128 features x up to 64 tokens, eight stages in flight. Above,
 // the tensor cores and their power do: a CTA pair takes 256 features x up to 256
 // tokens with two accumulators, so that a tile is stored while the next one is
@@ -653,7 +653,10 @@ static int awqb_grouped_gemm_impl(const void* x, int64_t rows, int64_t ldx, cons
   AWQB_REQUIRE(p.err != nullptr, kCudaError, "cannot resolve the device error word");
   p.ldo = ldo, p.out_rows = out_rows;
   p.rows = (int)rows, p.E = (int)E, p.K = (int)K, p.N = (int)N, p.n_out = (int)n_out, p.silu = silu_mul != 0;
-  const bool many = rows > 64 * E;
+  // Measured, few / many in us: 128 experts 2048 -> 1536 at 16, 32, 64 rows per expert
+  // 126 / 129, 141 / 130, 178 / 138; 768 -> 2048 65 / 66, 78 / 67, 100 / 76; eight experts
+  // 4096 -> 14336 161 / 167, 158 / 168, 207 / 168.
+  const bool many = rows > 24 * E;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == AWQB_DTYPE_F16)
     return many ? launch<__half, true>(x, ldx, w, p, st) : launch<__half, false>(x, ldx, w, p, st);

@@ -38,9 +38,13 @@ constexpr int kMaxSlices = 4;
 constexpr int kMaxParts = 8;      // parts of K
 constexpr int kFirstWarps = 8;
 constexpr int kSecondWarps = 4;
-// Rows from which the prompt kernels are taken: below, 16-row tiles keep more CTAs
-// in flight and pad the few rows of a decode batch's adapters less.
-constexpr int64_t kPromptRows = 512;
+// The prompt kernels cost about 14 us more at the start (three launches, tcgen05
+// tiles of 128 rows) and then move base and out at HBM speed; the decode kernels
+// cost about 2.4e-8 us per unit of M * (N * (50 + rank) + K * columns). Measured,
+// decode / prompt in us at K = 4096, N = 28672, rank 16: M = 256 23 / 27, 512 39 / 30,
+// 2048 137 / 65; K = 14336, N = 4096, rank 64: 512 25 / 25, 1024 37 / 27; K = N = 4096,
+// rank 16: 512 11 / 22, 2048 26 / 28.
+constexpr double kPromptWork = 8e8;
 
 struct Args {
   const void *x, *a, *b, *base;
@@ -343,16 +347,22 @@ __global__ void __launch_bounds__(kSecondWarps * 32) lora_second_kernel(const __
 namespace awqb {
 namespace {
 
-bool wide_tiles(int64_t M) { return M >= kPromptRows; }
+struct Sizes {
+  int64_t M, K, N, L, rank, S, R;
+};
+
+bool for_prompt(const Sizes& z) {
+  return (double)z.M * ((double)z.N * (50 + z.rank) + (double)z.K * z.R) > kPromptWork;
+}
 
 // Parts of K: enough CTAs to fill the GPU, each part long enough to be worth its
 // sums (64 k per warp of a decode batch's CTA, eight stages of a prompt's).
-int parts_of_k(int64_t M, int64_t K, int64_t R, int64_t L) {
-  const bool wide = wide_tiles(M);
+int parts_of_k(const Sizes& z) {
+  const bool wide = for_prompt(z);
   // a decode batch may have a tile for every adapter, a prompt has few partial ones
-  const int64_t rows = wide ? (M + kWideRows - 1) / kWideRows : std::min(M, M / 16 + L);
-  const int64_t tiles = rows * (wide ? (R + 127) / 128 : (R + 15) / 16);
-  const int64_t want = 296 / std::max<int64_t>(tiles, 1), most = K / 512;
+  const int64_t rows = wide ? (z.M + kWideRows - 1) / kWideRows : std::min(z.M, z.M / 16 + z.L);
+  const int64_t tiles = rows * (wide ? (z.R + 127) / 128 : (z.R + 15) / 16);
+  const int64_t want = 296 / std::max<int64_t>(tiles, 1), most = z.K / 512;
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)kMaxParts}));
 }
 
@@ -360,12 +370,13 @@ int parts_of_k(int64_t M, int64_t K, int64_t R, int64_t L) {
 struct Layout {
   int64_t halves, up, bytes;
 };
-Layout layout(int64_t M, int64_t K, int64_t R, int64_t S, int64_t L) {
+Layout layout(const Sizes& z) {
   const auto round = [](int64_t v) { return (v + 255) / 256 * 256; };
+  const bool wide = for_prompt(z);
   Layout l = {};
-  l.halves = round(M * R * 4 * parts_of_k(M, K, R, L));
-  l.up = l.halves + (wide_tiles(M) ? round(M * R * 4) : 0);
-  l.bytes = l.up + (wide_tiles(M) ? round(M * S * 4) : 0);
+  l.halves = round(z.M * z.R * 4 * parts_of_k(z));
+  l.up = l.halves + (wide ? round(z.M * z.R * 4) : 0);
+  l.bytes = l.up + (wide ? round(z.M * z.S * 4) : 0);
   return l;
 }
 
@@ -436,7 +447,7 @@ int launch_prompt(const Args& g, cudaLaunchConfig_t cfg) {
 }
 
 template <typename T>
-int launch(const Args& g, cudaStream_t st) {
+int launch(const Args& g, bool prompt, cudaStream_t st) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -444,15 +455,17 @@ int launch(const Args& g, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return wide_tiles(g.M) ? launch_prompt<T>(g, cfg) : launch_decode<T>(g, cfg);
+  return prompt ? launch_prompt<T>(g, cfg) : launch_decode<T>(g, cfg);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-int check_sizes(int64_t M, int64_t K, int64_t L, int64_t rank, int64_t S) {
+int check_sizes(int64_t M, int64_t K, int64_t N, int64_t L, int64_t rank, int64_t S) {
   AWQB_REQUIRE(M >= 0 && M < (1ll << 24), kInvalidArgument, "bad number of rows %lld", (long long)M);
   AWQB_REQUIRE(K > 0 && K % 8 == 0 && K <= (1 << 20), kInvalidArgument, "K=%lld must be a positive multiple of 8",
                (long long)K);
+  AWQB_REQUIRE(N > 0 && N % 8 == 0 && N <= (1 << 20), kInvalidArgument, "N=%lld must be a positive multiple of 8",
+               (long long)N);
   AWQB_REQUIRE(L >= 1 && L <= kMaxAdapters, kInvalidArgument, "%lld adapters: 1..%d are supported", (long long)L,
                kMaxAdapters);
   AWQB_REQUIRE(rank >= 8 && rank % 8 == 0 && rank <= kMaxRank, kInvalidArgument,
@@ -467,12 +480,12 @@ int check_sizes(int64_t M, int64_t K, int64_t L, int64_t rank, int64_t S) {
 
 using namespace awqb;
 
-extern "C" int awqb_lora_workspace_bytes(int64_t M, int64_t K, int64_t L, int64_t rank, int64_t num_slices,
+extern "C" int awqb_lora_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t L, int64_t rank, int64_t num_slices,
                                          int64_t* bytes) {
   AWQB_REQUIRE(bytes != nullptr, kInvalidArgument, "bytes is null");
-  const int st = check_sizes(M, K, L, rank, num_slices);
+  const int st = check_sizes(M, K, N, L, rank, num_slices);
   if (st != kOk) return st;
-  *bytes = layout(M, K, rank * num_slices, num_slices, L).bytes;
+  *bytes = layout({M, K, N, L, rank, num_slices, rank * num_slices}).bytes;
   return kOk;
 }
 
@@ -482,10 +495,8 @@ static int awqb_lora_impl(const void* x, int64_t M, int64_t ldx, int64_t K, cons
                          int64_t ld_out, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   AWQB_REQUIRE(dtype == AWQB_DTYPE_F16 || dtype == AWQB_DTYPE_BF16, kInvalidArgument, "bad dtype %d", dtype);
   int64_t need = 0;
-  const int st = awqb_lora_workspace_bytes(M, K, L, rank, num_slices, &need);
+  const int st = awqb_lora_workspace_bytes(M, K, N, L, rank, num_slices, &need);
   if (st != kOk) return st;
-  AWQB_REQUIRE(N > 0 && N % 8 == 0 && N <= (1 << 20), kInvalidArgument, "N=%lld must be a positive multiple of 8",
-               (long long)N);
   Args g = {};
   int64_t end = 0;
   for (int s = 0; s < num_slices; ++s) {
@@ -501,6 +512,8 @@ static int awqb_lora_impl(const void* x, int64_t M, int64_t ldx, int64_t K, cons
                kInvalidArgument, "row strides must be at least the row's length and multiples of 8");
   if (M == 0) return kOk;
   AWQB_REQUIRE(x && a && b && order && offsets && base && out, kInvalidArgument, "null pointer");
+  AWQB_REQUIRE(out != base || ld_out == ld_base, kInvalidArgument,
+               "out is base with another row stride: in place, the strides must agree");
   AWQB_REQUIRE(aligned16(x) && aligned16(a) && aligned16(b) && aligned16(base) && aligned16(out) &&
                    aligned16(workspace),
                kInvalidArgument, "tensors must be 16-byte aligned");
@@ -513,13 +526,14 @@ static int awqb_lora_impl(const void* x, int64_t M, int64_t ldx, int64_t K, cons
   g.ldx = ldx, g.ld_base = ld_base, g.ld_out = ld_out;
   g.M = (int)M, g.K = (int)K, g.L = (int)L, g.rank = (int)rank, g.R = (int)(rank * num_slices), g.N = (int)N;
   g.S = (int)num_slices;
-  g.parts = parts_of_k(M, K, g.R, L);
+  const Sizes z = {M, K, N, L, rank, num_slices, g.R};
+  g.parts = parts_of_k(z);
   g.k_part = (int)((K + g.parts - 1) / g.parts + 63) / 64 * 64;
-  const Layout at = layout(M, K, g.R, num_slices, L);
+  const Layout at = layout(z);
   g.halves = static_cast<uint8_t*>(workspace) + at.halves;
   g.up = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at.up);
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  return dtype == AWQB_DTYPE_F16 ? launch<__half>(g, cs) : launch<__nv_bfloat16>(g, cs);
+  return dtype == AWQB_DTYPE_F16 ? launch<__half>(g, for_prompt(z), cs) : launch<__nv_bfloat16>(g, for_prompt(z), cs);
 }
 
 extern "C" int awqb_lora(const awqb_lora_args* a, void* stream) {

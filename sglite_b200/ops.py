@@ -794,8 +794,8 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out
     ``y = silu(gate) * up`` [.., N / 2]. offsets [E + 1] int32 stays on the device
     and must not decrease.
 
-    y[r] goes to row r of ``out``, or to row row_map[r] (int32 [rows]; rows that
-    map outside ``out`` are dropped), times row_scale[its row of out] (fp32) if
+    y[r] goes to row r of ``out``, or to row row_map[r] (int32 [rows]; no two rows to
+    one; rows that map outside ``out`` are dropped), times row_scale[its row of out] (fp32) if
     given. Rows of ``out`` that nothing goes to are left as they were; without
     ``out`` a new [rows, N] tensor is returned, in which those rows are undefined."""
     dtype = x.dtype
@@ -833,7 +833,7 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out
     return out
 
 
-_LORA_BYTES: Dict[Tuple[int, int, int, int, int], int] = {}
+_LORA_BYTES: Dict[Tuple[int, int, int, int, int, int], int] = {}
 
 
 def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor,
@@ -847,7 +847,8 @@ def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, order: torch.Tensor,
 
     slices: widths of a merged projection's parts (QKV, gate_up; at most 4), each with
     its own pair; a [L, len(slices) * rank, K] stacks their first factors, b
-    [L, N, rank] the second ones. Sums are fp32. ``out`` may be base (in place)."""
+    [L, N, rank] the second ones. Sums are fp32. ``out`` may be base (in place); it must
+    not overlap the inputs otherwise."""
     dtype = x.dtype
     code = _dtype_code(dtype)
     di = _device_of(x)
@@ -880,11 +881,11 @@ def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, order: torch.Tensor,
         out = x.new_empty((M, N))
     elif out.shape != (M, N) or out.dtype != dtype or out.get_device() != di:
         raise ValueError("out must have the shape, dtype and device of base")
-    key = (M, K, L, rank, parts)
+    key = (M, K, N, L, rank, parts)
     nb = _LORA_BYTES.get(key)
     if nb is None:
         v = c_i64(0)
-        call("awqb_lora_workspace_bytes", M, K, L, rank, parts, ctypes.byref(v))
+        call("awqb_lora_workspace_bytes", M, K, N, L, rank, parts, ctypes.byref(v))
         nb = _LORA_BYTES[key] = v.value
     # from the caching allocator: private to the stream, or to the graph being captured
     ws = torch.empty(nb, dtype=torch.uint8, device=x.device)

@@ -90,7 +90,7 @@ LORA = [P, 16, 256, 256, P, P, 4, 16, 512, 1, 512, 0, 0, 0, P, P, None, P, 512, 
     ({"_9": 2, "_10": 256, "_11": 128}, b"add up"), ({"_9": 2, "_10": 508, "_11": 4}, b"slice width"),
     ({"_10": 0}, b"slice width"), ({"_2": 248}, b"row strides"), ({"_18": 500}, b"row strides"),
     ({"_20": 508}, b"row strides"), ({"_23": 16}, b"workspace"), ({"_22": None}, b"workspace"), ({"_0": None}, b"null"),
-    ({"_14": None}, b"null"), ({"_19": 8}, b"16-byte"), ({"_21": 3}, b"dtype")])
+    ({"_14": None}, b"null"), ({"_19": 8}, b"16-byte"), ({"_21": 3}, b"dtype"), ({"_20": 520}, b"in place")])
 def test_lora_refusals(change, text):
     _refused("awqb_lora", _replace(LORA, **change), 1, text)
 

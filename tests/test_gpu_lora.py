@@ -54,6 +54,103 @@ def test_sizes(cuda, M, K, slices, rank, dtype):
     assert torch.equal(y, got)
 
 
+def _prompt(M, K, slices, rank):
+    """Whether these sizes go to the prompt kernels (the rule of awqb_lora.cu): what
+    follows is meant to."""
+    return M * (sum(slices) * (50 + rank) + K * rank * len(slices)) > 8e8
+
+
+@pytest.mark.parametrize("M,K,slices,rank", [(600, 72, (24584, 8, 1032), 8), (1300, 200, (8200, 136), 24),
+                                             (300, 1000, (16008, 3000), 128), (700, 2560, (9728, 9728), 64),
+                                             (2100, 1024, (4096, 1024, 1024), 32), (130, 8, (40000,), 128),
+                                             (900, 14336, (4096,), 64), (1025, 4096, (1536, 512, 512, 1032), 96)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sort", [False, True])
+def test_prompt_sizes(cuda, M, K, slices, rank, dtype, sort):
+    """Rows in random order (copied one by one) and in order (runs), in and out of place."""
+    assert _prompt(M, K, slices, rank)
+    L = 6
+    x, a, b, base, ids, scales = _case(cuda, M, K, slices, rank, L, dtype, sort=sort)
+    order, offsets = ops.group_rows(ids, L)
+    base0 = base.clone()
+    got = ops.lora(x, a, b, order, offsets, base, slices=slices, scales=scales)
+    assert torch.equal(base, base0)
+    _check(got, x, a, b, ids, base, slices, scales)
+    y = base.clone()
+    ops.lora(x, a, b, order, offsets, y, slices=slices, scales=scales, out=y)
+    assert torch.equal(y, got)
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("kind", ["one", "none", "first", "last", "many", "tiles"])
+def test_prompt_who_uses_which(cuda, kind):
+    M, K, N, L = 1500, 256, 8192, 1024 if kind == "many" else 9
+    assert _prompt(M, K, (N,), 64)
+    x, a, b, base, ids, scales = _case(cuda, M, K, (N,), 64, L, torch.bfloat16)
+    if kind == "tiles":  # groups of exactly one tile, one row more and one less
+        ids = torch.repeat_interleave(torch.arange(9, device=cuda), torch.tensor([128, 129, 127, 0, 1, 256, 384, 0, 400], device=cuda))
+        ids = torch.cat([ids, torch.full((M - ids.numel(),), -1, device=cuda)]).to(torch.int32)
+    elif kind != "many":
+        ids = torch.full_like(ids, {"one": 4, "none": -1, "first": 0, "last": L - 1}[kind])
+    order, offsets = ops.group_rows(ids, L)
+    _check(ops.lora(x, a, b, order, offsets, base, scales=scales), x, a, b, ids, base, (N,), scales)
+    assert ops.device_error() == 0
+
+
+def test_prompt_strides_extremes_and_graphs(cuda):
+    M, K, N, r, L, dtype = 1200, 512, 8192, 64, 4, torch.float16
+    assert _prompt(M, K, (N,), r)
+    x, a, b, base, ids, scales = _case(cuda, M, K, (N,), r, L, dtype)
+    wide_x = torch.full((M, K + 8), float("nan"), dtype=dtype, device=cuda)
+    wide_x[:, :K] = x
+    wide = torch.full((M, N + 16), 5.0, dtype=dtype, device=cuda)
+    wide[:, :N] = base
+    order, offsets = ops.group_rows(ids, L)
+    y = wide[:, :N]
+    ops.lora(wide_x[:, :K], a, b, order, offsets, y, scales=scales, out=y)
+    _check(y, x, a, b, ids, base, (N,), scales)
+    assert bool((wide[:, N:] == 5).all())
+    # a first product past fp16's range
+    big = ops.lora(x * 64, a * 2048, b * 2.0 ** -12, order, offsets, base)
+    _check(big, x * 64, a * 2048, b * 2.0 ** -12, ids, base, (N,), None)
+    # infinities and NaN stay in their rows
+    x2 = x.clone()
+    x2[7, 3], x2[600, 9] = float("nan"), float("inf")
+    ids2 = ids.clamp_min(0)
+    bad = ~torch.isfinite(ops.lora(x2, a, b, *ops.group_rows(ids2, L), base))
+    assert bool(bad[7].all()) and bool(bad[600].any())
+    bad[7] = bad[600] = False
+    assert not bool(bad.any())
+    # a graph that groups and adds, replayed with another mix of adapters
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o2, f2 = ops.group_rows(ids, L)
+        out = ops.lora(x, a, b, o2, f2, base, scales=scales)
+    for shift in (0, 1):
+        ids.add_(shift).remainder_(L + 1)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(out, x, a, b, ids, base, (N,), scales)
+    assert ops.device_error() == 0
+
+
+def test_two_streams_at_once(cuda):
+    """Calls that run side by side have workspaces of their own."""
+    cases = [_case(cuda, M, 1024, (N,), 32, 5, torch.bfloat16, seed=i) for i, (M, N) in enumerate(((40, 512), (900, 16384)))]
+    groups = [ops.group_rows(c[4], 5) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = [[], []]
+    for _ in range(4):
+        for i, (s, c, g) in enumerate(zip(streams, cases, groups)):
+            with torch.cuda.stream(s):
+                outs[i].append(ops.lora(c[0], c[1], c[2], g[0], g[1], c[3], scales=c[5]))
+    torch.cuda.synchronize()
+    for c, os in zip(cases, outs):
+        for o in os:
+            _check(o, c[0], c[1], c[2], c[4], c[3], (c[3].shape[1],), c[5])
+
+
 @pytest.mark.parametrize("kind", ["one", "none", "first", "last", "many"])
 @pytest.mark.parametrize("M", [33, 2000])
 def test_who_uses_which(cuda, M, kind):

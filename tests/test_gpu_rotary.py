@@ -52,6 +52,26 @@ def test_layouts(cuda, D, rot, interleaved, norm, dtype):
             assert torch.equal(q1[..., rot:], q[..., rot:]) and torch.equal(k1[..., rot:], k[..., rot:])
 
 
+@pytest.mark.parametrize("M,Hq,Hk,D,rot,interleaved,norm", [
+    (2600, 40, 8, 128, 128, False, True), (2401, 33, 1, 128, 64, True, True), (5000, 7, 3, 80, 80, False, False),
+    (700, 64, 8, 64, 32, False, True), (2500, 1, 1, 256, 256, False, True), (2369, 128, 16, 16, 16, True, False)])
+def test_many_tokens(cuda, M, Hq, Hk, D, rot, interleaved, norm):
+    """Whole tokens and batches of heads per warp, heads that do not fill a batch,
+    padding among them."""
+    g = torch.Generator(device=cuda).manual_seed(M)
+    dtype = torch.bfloat16
+    q = torch.randn((M, Hq, D), generator=g, device=cuda).to(dtype)
+    k = torch.randn((M, Hk, D), generator=g, device=cuda).to(dtype)
+    pos = torch.randint(-200, 100000, (M,), generator=g, device=cuda)
+    qw = (torch.rand(D, generator=g, device=cuda) + 0.5).to(dtype) if norm else None
+    inv = _inv(rot, cuda)
+    q_out, k_out = torch.full_like(q, 3.0), torch.full_like(k, 3.0)
+    ops.rotary(q, k, pos, inv, interleaved=interleaved, scale=0.75, q_weight=qw, q_out=q_out, k_out=k_out)
+    _ok(q_out, q, pos, inv, interleaved, 0.75, qw)
+    _ok(k_out, k, pos, inv, interleaved, 0.75)  # q alone is normed
+    assert bool((q_out[pos < 0] == 3).all()) and bool((k_out[pos < 0] == 3).all())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_merged_projection_in_place_padding_and_position_types(cuda, dtype):
     M, Hq, Hk, D = 65, 16, 2, 128
