@@ -432,7 +432,7 @@ int launch_prompt(const Args& g, cudaLaunchConfig_t cfg) {
   cfg.dynamicSmemBytes = first_wide_smem();
   AWQB_CUDA(cudaFuncSetAttribute(lora_first_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, first_wide_smem()));
   AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_first_wide_kernel<T>, tx, ta, g, col_box));
-  cfg.gridDim = dim3((unsigned)((g.M + 7) / 8));
+  cfg.gridDim = dim3((unsigned)(((int64_t)g.M * g.S + 7) / 8));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
   AWQB_CUDA(cudaLaunchKernelEx(&cfg, lora_join_kernel<T>, g));

@@ -12,7 +12,7 @@
 //           apiece: 22 us for 4111 rows, K = 4096, 128 columns.) Columns on the
 //           accumulator's lanes, so that a warp writes 32 neighbouring columns of
 //           a place.
-//   join:   a warp per place adds the parts in order and splits the sums in halves.
+//   join:   a warp per place and slice adds the parts in order and splits the sums in halves.
 //   second: persistent CTAs take equal runs of units (128 places x 128 features) and
 //           walk them in segments of one tile of places and one slice, whose halves of
 //           h stay in shared memory. Places on the accumulator's lanes: a thread adds
@@ -203,48 +203,45 @@ lora_first_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_co
   }
 }
 
-// halves[slice][hi, lo][place][rank], down[slice][place]: the power of two that a
+// halves[slice][hi, lo][place][rank], up[slice][place]: the power of two that a
 // place's halves were divided by.
 template <typename T>
 __global__ void __launch_bounds__(256) lora_join_kernel(const __grid_constant__ Args g) {
-  const int place = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int unit = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int place = unit / g.S, s = unit - place * g.S;
   grid_dep_wait();
   grid_dep_launch();
   if (place >= g.M || place < g.offsets[0] || place >= g.offsets[g.L]) return;
-  for (int s = 0; s < g.S; ++s) {
-    float2 v[kMaxRank / 64] = {};
-    const float* src = g.h + (int64_t)place * g.R + s * g.rank + lane * 2;
-    for (int p0 = 0; p0 < g.parts; p0 += 4) {
-      float2 u[4][kMaxRank / 64];
+  constexpr int kPairs = kMaxRank / 64;
+  const float* src = g.h + (int64_t)place * g.R + s * g.rank + lane * 2;
+  float2 u[kMaxParts][kPairs], v[kPairs] = {};
 #pragma unroll
-      for (int p = 0; p < 4; ++p)
+  for (int p = 0; p < kMaxParts; ++p)
 #pragma unroll
-        for (int i = 0; i < kMaxRank / 64; ++i)
-          u[p][i] = p0 + p < g.parts && i * 64 + lane * 2 < g.rank
-                        ? *reinterpret_cast<const float2*>(src + (int64_t)(p0 + p) * g.M * g.R + i * 64)
-                        : make_float2(0.f, 0.f);
+    for (int i = 0; i < kPairs; ++i)
+      u[p][i] = p < g.parts && i * 64 + lane * 2 < g.rank
+                    ? *reinterpret_cast<const float2*>(src + (int64_t)p * g.M * g.R + i * 64)
+                    : make_float2(0.f, 0.f);
+  float top = 0.f;
 #pragma unroll
-      for (int p = 0; p < 4; ++p)
+  for (int i = 0; i < kPairs; ++i) {
 #pragma unroll
-        for (int i = 0; i < kMaxRank / 64; ++i) v[i].x += u[p][i].x, v[i].y += u[p][i].y;
-    }
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < kMaxRank / 64; ++i) top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
-    const int e = row_exponent<T>(top);
-    const float down = ldexpf(1.f, -e);
-    T* to = static_cast<T*>(g.halves) + ((int64_t)s * 2 * g.M + place) * g.rank + lane * 2;
-#pragma unroll
-    for (int i = 0; i < kMaxRank / 64; ++i) {
-      if (i * 64 + lane * 2 >= g.rank) continue;
-      T hi[2], lo[2];
-      halves<T>(v[i].x * down, &hi[0], &lo[0]);
-      halves<T>(v[i].y * down, &hi[1], &lo[1]);
-      *reinterpret_cast<uint32_t*>(to + i * 64) = *reinterpret_cast<uint32_t*>(hi);
-      *reinterpret_cast<uint32_t*>(to + (int64_t)g.M * g.rank + i * 64) = *reinterpret_cast<uint32_t*>(lo);
-    }
-    if (lane == 0) g.up[(int64_t)s * g.M + place] = ldexpf(1.f, e);
+    for (int p = 0; p < kMaxParts; ++p) v[i].x += u[p][i].x, v[i].y += u[p][i].y;
+    top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
   }
+  const int e = row_exponent<T>(top);
+  const float down = ldexpf(1.f, -e);
+  T* to = static_cast<T*>(g.halves) + ((int64_t)s * 2 * g.M + place) * g.rank + lane * 2;
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    if (i * 64 + lane * 2 >= g.rank) continue;
+    T hi[2], lo[2];
+    halves<T>(v[i].x * down, &hi[0], &lo[0]);
+    halves<T>(v[i].y * down, &hi[1], &lo[1]);
+    *reinterpret_cast<uint32_t*>(to + i * 64) = *reinterpret_cast<uint32_t*>(hi);
+    *reinterpret_cast<uint32_t*>(to + (int64_t)g.M * g.rank + i * 64) = *reinterpret_cast<uint32_t*>(lo);
+  }
+  if (lane == 0) g.up[(int64_t)s * g.M + place] = ldexpf(1.f, e);
 }
 
 template <typename T>

@@ -64,7 +64,7 @@ GROUP = [P, 100, 0, 8, P, P, None, 0, None]
 
 @pytest.mark.parametrize("change,text", [
     ({"_3": 0}, b"groups"), ({"_3": 1025}, b"groups"), ({"_1": -1}, b"number of ids"), ({"_0": None}, b"null"),
-    ({"_5": None}, b"null"), ({"_1": 9000}, b"workspace"), ({"_2": 1 << 40}, b"first id")])
+    ({"_5": None}, b"null"), ({"_1": 20000}, b"workspace"), ({"_2": 1 << 40}, b"first id")])
 def test_group_rows_refusals(change, text):
     _refused("awqb_group_rows", _replace(GROUP, **change), 1, text)
 

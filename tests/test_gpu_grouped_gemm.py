@@ -13,7 +13,7 @@ from sglite_b200.moe import AWQB200MoeBackend, DenseExpertWeights
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("n", [0, 1, 31, 1000, 8191, 8192, 40001])
+@pytest.mark.parametrize("n", [0, 1, 31, 1000, 8192, 10239, 10240, 40001])
 @pytest.mark.parametrize("groups,begin", [(1, 0), (7, 2), (128, 0), (1024, 0), (1000, -3)])
 def test_group_rows(cuda, n, groups, begin):
     g = torch.Generator().manual_seed(n + groups)
