@@ -167,8 +167,10 @@ extern "C" int awqb_group_rows(const int32_t* ids, int64_t n, int64_t begin, int
   const int B = (int)groups + 1;
   if (n < kMultiMin) {
     const int smem = 32 * B * 4;
+    // (the most that any call wants: another thread's call may set it before this launch)
     if (smem > 48 * 1024 - 256)
-      AWQB_CUDA(cudaFuncSetAttribute(group_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      AWQB_CUDA(cudaFuncSetAttribute(group_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     32 * (kMaxGroups + 1) * 4));
     group_small_kernel<<<1, 1024, smem, st>>>(ids, (int)n, (int)begin, (int)groups, order, offsets);
     AWQB_LAUNCH_CHECK();
     return kOk;

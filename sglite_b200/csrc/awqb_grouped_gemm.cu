@@ -592,8 +592,12 @@ int launch(const void* x, int64_t ldx, const void* w, Params p, cudaStream_t str
                            : make_map(&tw, w, (int64_t)p.E * p.N, p.K, p.K, p.silu ? kFeat / 2 : kFeat);
   for (int i = 0; i < 3 && st == kOk; ++i) st = make_map(&tx.box[i], x, p.rows, p.K, ldx, kTokCta >> (2 - i));
   if (st != kOk) return st;
-  const int smem = 1024 + C::kStages * C::kStageBytes + (kMany ? 0 : Few::kChunk * kFeat * 4) + 4 * C::kTok * 4 + (3 * p.E + 1) * 4;
-  AWQB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const auto smem_for = [](int E) {
+    return 1024 + C::kStages * C::kStageBytes + (kMany ? 0 : Few::kChunk * kFeat * 4) + 4 * C::kTok * 4 + (3 * E + 1) * 4;
+  };
+  const int smem = smem_for(p.E);
+  // (the most that any call wants: another thread's call may set it before this launch)
+  AWQB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_for(kMaxExperts)));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(kCluster);
   cfg.blockDim = dim3(C::kThreads);

@@ -166,7 +166,7 @@ class AWQB200MoeBackend(BaseMoeBackend):
         if isinstance(w1, DenseExpertWeights) != isinstance(w2, DenseExpertWeights):
             raise ValueError("w1 and w2 must both be AWQ or both be 16-bit experts")
         if isinstance(w1, DenseExpertWeights):
-            return self._dense_experts(x, w1, w2, topk_weights, topk_ids, E_glob)
+            return self._dense_experts(x, w1, w2, topk_weights, topk_ids)
         block_m = choose_block_m(M, topk, E_glob)
         sorted_ids, block_expert, npp = ops.moe_align(topk_ids, w1.e_begin, w1.e_end, block_m)
         rows = sorted_ids.numel()
@@ -189,7 +189,7 @@ class AWQB200MoeBackend(BaseMoeBackend):
 
 
     def _dense_experts(self, x: torch.Tensor, w1: DenseExpertWeights, w2: DenseExpertWeights,
-                       topk_weights: torch.Tensor, topk_ids: torch.Tensor, E_glob: int) -> torch.Tensor:
+                       topk_weights: torch.Tensor, topk_ids: torch.Tensor) -> torch.Tensor:
         """The same pipeline over 16-bit experts: the rows are grouped without
         padding, and the kernel reads the groups' bounds on the device."""
         M, H = x.shape
@@ -202,8 +202,8 @@ class AWQB200MoeBackend(BaseMoeBackend):
         a = ops.grouped_gemm(xs, w1.w, offsets, silu_mul=True)
         y3 = torch.empty((numel, H), dtype=x.dtype, device=x.device)
         ops.grouped_gemm(a, w2.w, offsets, out=y3, row_map=order, row_scale=topk_weights.reshape(-1).contiguous())
-        ids = topk_ids if (w1.e_begin != 0 or w1.e_end != E_glob) else None
-        return ops.moe_topk_sum(y3, M, topk, ids, w1.e_begin, w1.e_end, x)
+        # always by the ids: an id that no expert here has (another rank's, padding) wrote no row of y3
+        return ops.moe_topk_sum(y3, M, topk, topk_ids, w1.e_begin, w1.e_end, x)
 
 
 def route(gating_output: torch.Tensor, topk: int, renormalize: bool) -> Tuple[torch.Tensor, torch.Tensor]:

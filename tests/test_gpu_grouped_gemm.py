@@ -188,3 +188,56 @@ def test_moe_backend_over_dense_experts(cuda, M, dtype):
         p2 = DenseExpertWeights(w2[lo:lo + E // 2], lo, E)
         parts += backend.forward(x.clone(), p1, p2, logits, topk, True).float()
     assert rel_err(parts, ref.cpu()) <= 1e-2
+
+
+def test_ids_of_no_expert_here_add_nothing(cuda):
+    """The first half of the experts, with nothing said about how many there are in
+    all, and padding: their choices are worth exactly those with weight zero."""
+    M, E, H, I, topk, dtype = 40, 8, 128, 64, 3, torch.bfloat16
+    g = torch.Generator(device=cuda).manual_seed(9)
+    x = torch.randn((M, H), generator=g, device=cuda).to(dtype)
+    w1 = DenseExpertWeights((torch.randn((E, 2 * I, H), generator=g, device=cuda) / 11).to(dtype))
+    w2 = DenseExpertWeights((torch.randn((E, H, I), generator=g, device=cuda) / 8).to(dtype))
+    ids = torch.randint(-1, 2 * E, (M, topk), generator=g, device=cuda).to(torch.int32)
+    tw = torch.rand((M, topk), generator=g, device=cuda)
+    here = (ids >= 0) & (ids < E)
+    assert bool((~here).any()) and bool(here.any())
+    backend = AWQB200MoeBackend()
+    poison = torch.full((M * topk, H), float("nan"), dtype=dtype, device=cuda)
+    del poison  # what the allocator hands out next is not zero
+    y = backend.experts(x.clone(), w1, w2, tw, ids)
+    want = backend.experts(x.clone(), w1, w2, tw * here, torch.where(here, ids, 0))
+    assert torch.equal(y, want)
+
+
+def test_calls_of_two_threads(cuda):
+    """Both threads' launches want different amounts of shared memory of the same kernels."""
+    import threading
+
+    g = torch.Generator(device=cuda).manual_seed(3)
+    jobs, failures = [], []
+    for groups in (500, 1000):
+        ids = torch.randint(0, groups, (4000,), generator=g, device=cuda).to(torch.int32)
+        x = torch.randn((4000, 64), generator=g, device=cuda).to(torch.bfloat16)
+        w = torch.randn((groups, 32, 64), generator=g, device=cuda).to(torch.bfloat16)
+        order, offsets = ops.group_rows(ids, groups)
+        jobs.append((ids, groups, x, w, order, offsets, ops.grouped_gemm(x, w, offsets)))
+    torch.cuda.synchronize()
+
+    def work(ids, groups, x, w, order, offsets, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(300):
+                    o, f = ops.group_rows(ids, groups)
+                    y = ops.grouped_gemm(x, w, f)
+                    assert torch.equal(o, order) and torch.equal(f, offsets) and torch.equal(y, want)
+        except BaseException as e:  # reported by the test itself
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
+    assert ops.device_error() == 0
