@@ -305,6 +305,13 @@ int launch(const Args& a, int64_t M, cudaStream_t st) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+// No element of [rows, heads, D] stands where another does.
+bool apart(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t D) {
+  if (rows <= 1) return heads <= 1 || head >= D;
+  if (heads <= 1) return row >= D;
+  return (head >= D && row >= (heads - 1) * head + D) || (row >= D && head >= (rows - 1) * row + D);
+}
+
 }  // namespace
 }  // namespace awqb
 
@@ -327,6 +334,8 @@ static int awqb_rotary_impl(const void* q, int64_t q_row, int64_t q_head, int64_
                    (Hk == 0 || (k_row | k_head | k_out_row | k_out_head) % 8 == 0),
                kInvalidArgument, "strides must be multiples of 8");
   AWQB_REQUIRE(eps >= 0.f, kInvalidArgument, "eps must be >= 0");
+  AWQB_REQUIRE(apart(M, q_out_row, Hq, q_out_head, head_dim) && (Hk == 0 || apart(M, k_out_row, Hk, k_out_head, head_dim)),
+               kInvalidArgument, "the outputs' tokens or heads overlap");
   if (M == 0) return kOk;
   AWQB_REQUIRE(q && q_out && positions && inv_freq && (Hk == 0 || (k && k_out)), kInvalidArgument, "null pointer");
   AWQB_REQUIRE(aligned16(q) && aligned16(q_out) && aligned16(q_weight) &&

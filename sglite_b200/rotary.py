@@ -18,9 +18,10 @@ from . import ops
 def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[Dict[str, Any]] = None
                        ) -> Tuple[torch.Tensor, float]:
     """(inv_freq float64 [rot_dim / 2], factor on the turned elements) for a
-    checkpoint's ``rope_scaling`` entry: None or "default", "linear", "dynamic" (the
-    base stretched for a context ``factor`` times the original one), "llama3",
-    "yarn", "longrope" (one factor per pair)."""
+    checkpoint's ``rope_scaling`` entry: None or "default", "linear", "llama3", "yarn",
+    "longrope" (one factor per pair: ``long_factor``, with what its factor on the
+    elements follows from, or ``factors`` with an ``attention_factor``, else 1).
+    "dynamic" is refused: its speeds change with the length that a sequence has."""
     if rot_dim < 2 or rot_dim % 2:
         raise ValueError(f"rot_dim {rot_dim} must be even and positive")
     half = rot_dim // 2
@@ -41,10 +42,11 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[Di
             raise ValueError(f"longrope needs {half} factors, got {len(factors)}")
         inv = inv / torch.tensor([float(f) for f in factors], dtype=torch.float64)
         attention = scaling.get("attention_factor")
-        if attention is None:
-            factor, original = scaling.get("factor"), scaling.get("original_max_position_embeddings")
-            attention = math.sqrt(1.0 + math.log(factor) / math.log(original)) if factor and original and factor > 1 \
-                else 1.0
+        if attention is None and scaling.get("factors") and scaling.get("factor") is None:
+            attention = 1.0
+        elif attention is None:
+            factor, original = need("factor"), need("original_max_position_embeddings")
+            attention = math.sqrt(1.0 + math.log(factor) / math.log(original)) if factor > 1.0 else 1.0
         return inv, float(attention)
     factor = need("factor")
     if factor < 1.0:
@@ -52,10 +54,7 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[Di
     if kind == "linear":
         return inv / factor, 1.0
     if kind == "dynamic":
-        if rot_dim == 2:
-            return inv, 1.0
-        stretched = float(base) * factor ** (rot_dim / (rot_dim - 2))
-        return torch.as_tensor(stretched, dtype=torch.float64) ** (-2.0 * pair / rot_dim), 1.0
+        raise ValueError("rope_scaling of type 'dynamic' changes with the sequence's length: not supported")
     original = need("original_max_position_embeddings")
     if kind == "llama3":
         low, high = need("low_freq_factor"), need("high_freq_factor")
@@ -70,11 +69,15 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[Di
         def pair_of(turns: float) -> float:  # the pair that makes so many turns over the original context
             return rot_dim * math.log(original / (turns * 2.0 * math.pi)) / (2.0 * math.log(float(base)))
 
-        lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rot_dim - 1)
+        lo, hi = pair_of(fast), pair_of(slow)
+        if scaling.get("truncate", True):
+            lo, hi = math.floor(lo), math.ceil(hi)
+        lo, hi = max(lo, 0), min(hi, rot_dim - 1)
         ramp = ((pair - lo) / max(hi - lo, 0.001)).clamp(0.0, 1.0)
         mscale = scaling.get("attention_factor")
-        if mscale is None:
-            mscale = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+        if mscale is None:  # with "mscale" and "mscale_all_dim", the ratio of both
+            up, down = float(scaling.get("mscale") or 1.0), float(scaling.get("mscale_all_dim") or 0.0)
+            mscale = (0.1 * up * math.log(factor) + 1.0) / (0.1 * down * math.log(factor) + 1.0)
         return inv * (1.0 - ramp) + inv / factor * ramp, float(mscale)
     raise ValueError(f"unknown rope_scaling type {kind!r}")
 

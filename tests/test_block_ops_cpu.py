@@ -54,7 +54,8 @@ ROT = [P, 4096, 128, 32, P, 1024, 128, 8, P, 1, P, 128, 128, 4, 0, 1.0, P, P, 1e
     ({"_12": 100}, b"head_dim"), ({"_12": 264}, b"head_dim"), ({"_11": 130}, b"rot_dim"), ({"_11": 3}, b"rot_dim"),
     ({"_11": 0}, b"rot_dim"), ({"_3": 0}, b"sizes"), ({"_7": -1}, b"sizes"), ({"_1": 4100}, b"strides"),
     ({"_24": 4}, b"strides"), ({"_8": None}, b"null"), ({"_4": None}, b"null"), ({"_19": 8}, b"16-byte"),
-    ({"_25": 9}, b"dtype"), ({"_18": -1.0}, b"eps")])
+    ({"_25": 9}, b"dtype"), ({"_18": -1.0}, b"eps"), ({"_21": 0}, b"overlap"), ({"_20": 0}, b"overlap"),
+    ({"_20": 4088}, b"overlap"), ({"_23": 1016}, b"overlap"), ({"_24": 120}, b"overlap")])
 def test_rotary_refusals(change, text):
     _refused("awqb_rotary", _replace(ROT, **change), 1, text)
 
@@ -145,9 +146,6 @@ def test_frequencies_follow_their_formulas():
     assert f == 1.0 and inv.dtype == torch.float64
     assert torch.allclose(inv, torch.tensor([10000.0 ** (-2 * j / 128) for j in range(64)], dtype=torch.float64), rtol=1e-14)
     assert torch.allclose(rotary_frequencies(128, 10000.0, {"type": "linear", "factor": 8})[0], inv / 8, rtol=1e-14)
-    dyn = rotary_frequencies(128, 10000.0, {"rope_type": "dynamic", "factor": 4})[0]
-    # the fastest pair keeps its speed, the slowest one is stretched by the factor
-    assert abs(float(dyn[0]) - 1) < 1e-15 and math.isclose(float(dyn[-1]), float(inv[-1]) / 4, rel_tol=1e-12)
     sc = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
           "original_max_position_embeddings": 8192}
     l3 = rotary_frequencies(128, 500000.0, sc)[0]
@@ -169,12 +167,30 @@ def test_frequencies_follow_their_formulas():
 
 @pytest.mark.parametrize("rot,scaling", [(7, None), (0, None), (8, {"type": "linear"}), (8, {"type": "linear", "factor": 0.5}),
                                          (8, {"type": "spiral", "factor": 2}), (8, {"type": "longrope", "factors": [1]}),
-                                         (8, {"type": "yarn", "factor": 2}),
+                                         (8, {"type": "yarn", "factor": 2}), (8, {"type": "dynamic", "factor": 2}),
+                                         (8, {"type": "longrope", "long_factor": [1, 2, 3, 4]}),
                                          (8, {"type": "llama3", "factor": 2, "original_max_position_embeddings": 10,
                                               "low_freq_factor": 4, "high_freq_factor": 4})])
 def test_frequency_refusals(rot, scaling):
     with pytest.raises(ValueError):
         rotary_frequencies(rot, 10000.0, scaling)
+
+
+def test_factors_on_the_turned_elements():
+    yarn = {"type": "yarn", "factor": 40, "original_max_position_embeddings": 4096}
+    m = 0.1 * math.log(40)
+    assert math.isclose(rotary_frequencies(64, 1e4, yarn)[1], m + 1)
+    assert math.isclose(rotary_frequencies(64, 1e4, {**yarn, "mscale": 0.707, "mscale_all_dim": 0.707})[1], 1.0)
+    assert math.isclose(rotary_frequencies(64, 1e4, {**yarn, "mscale": 0.5, "mscale_all_dim": 0.25})[1],
+                        (0.5 * m + 1) / (0.25 * m + 1))
+    long = {"type": "longrope", "long_factor": [1, 2, 3, 4], "factor": 32, "original_max_position_embeddings": 4096}
+    assert math.isclose(rotary_frequencies(8, 1e4, long)[1], math.sqrt(1 + math.log(32) / math.log(4096)))
+    # without rounding the ramp's ends to whole pairs, it runs from one exact pair to the other
+    exact = rotary_frequencies(64, 1e4, {**yarn, "truncate": False})[0] / rotary_frequencies(64, 1e4)[0]
+    lo, hi = (64 * math.log(4096 / (t * 2 * math.pi)) / (2 * math.log(1e4)) for t in (32, 1))
+    for j in range(32):
+        r = min(max((j - lo) / (hi - lo), 0), 1)
+        assert math.isclose(float(exact[j]), 1 - r + r / 40, rel_tol=1e-12)
 
 
 def test_rotary_layer_refuses_other_widths():
