@@ -2,9 +2,10 @@
 //   out[t] = base[t] + scale_a * (x[t] A_a^T) B_a^T,  a the row's adapter.
 //
 // Rows come grouped by adapter (order, offsets), so both products run on tiles
-// of rows of one adapter, on mma.sync: the ranks are so small that the bytes of
-// x, base and out (prompts) or A and B (decoding) bound the work, not the
-// products. Two kernels, the second launched as a programmatic dependent:
+// of rows of one adapter: the ranks are so small that the bytes of x, base and out
+// (prompts) or A and B (decoding) bound the work, not the products. Decode batches
+// take the two kernels of this file, on mma.sync, the second launched as a
+// programmatic dependent; prompts those of awqb_lora_wide.cuh.
 //   first:  h = x A^T, fp32. A CTA takes a tile of rows x columns of A over a
 //           part of K; its warps split that part, so that every byte of x and A is
 //           loaded once per CTA, straight into operand registers (16 bytes per
@@ -98,7 +99,7 @@ __device__ __forceinline__ Rows find_rows(const Args& g, int tile, bool adapters
   for (int w = 0; w < warp; ++w) before += warp_tot[w];
   if (tile >= before && tile < before + sum) {
     int t = tile - before, e = e0;
-    while (t >= tiles_of(e)) t -= tiles_of(e++);
+    while (e + 1 < e1 && t >= tiles_of(e)) t -= tiles_of(e++);
     const int p0 = bound(e) + t * kRows;
     found.adapter = e == 0 || e == g.L + 1 ? -1 : e - 1;
     found.p0 = p0;
@@ -216,10 +217,13 @@ __device__ __forceinline__ void halves(float v, T* hi, T* lo) {
 // row's largest value to 2^14 .. 2^15 (exact), bf16 has fp32's range. Whole warps.
 template <typename T>
 __device__ __forceinline__ int row_exponent(float top) {
-  if (!std::is_same<T, __half>::value) return 0;
+  if constexpr (std::is_same<T, __half>::value) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  return top > 0.f && top < INFINITY ? min(max(ilogbf(top) - 14, -100), 100) : 0;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    return top > 0.f && top < INFINITY ? min(max(ilogbf(top) - 14, -100), 100) : 0;
+  } else {
+    return 0;
+  }
 }
 
 constexpr int kBlock = 32;                      // features of a warp

@@ -888,7 +888,7 @@ def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, order: torch.Tensor,
         call("awqb_lora_workspace_bytes", M, K, N, L, rank, parts, ctypes.byref(v))
         nb = _LORA_BYTES[key] = v.value
     # from the caching allocator: private to the stream, or to the graph being captured
-    ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+    ws = x.new_empty((nb + 1) // 2)  # (x's values have two bytes)
     w = ((N,) if slices is None else tuple(slices)) + (0, 0, 0, 0)
     fn, pack = _entry("awqb_lora")
     _run(fn, di, pack(x.data_ptr(), M, _row_stride(x, K, "x"), K, a.data_ptr(), b.data_ptr(), L, rank, N, parts, w[0], w[1],
