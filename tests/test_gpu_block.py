@@ -98,3 +98,52 @@ def test_block(cuda, M, dtype):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(held, block(x, residual)))
     assert ops.device_error() == 0
+
+
+def test_offsets_past_32_bits(cuda):
+    """Rows 16 MB apart, the last ones more than 2^32 elements behind the first: the
+    bits are those of contiguous rows."""
+    M, apart, dtype = 600, (1 << 23) + 64, torch.bfloat16
+    room = torch.empty(M * apart, dtype=dtype, device=cuda).view(M, apart)
+    g = torch.Generator(device=cuda).manual_seed(7)
+
+    def normal(*shape, std=1.0):
+        return (torch.randn(shape, generator=g, device=cuda) * std).to(dtype)
+
+    def far(t, at):
+        v = room[:, at:at + t.shape[1]]
+        v.copy_(t)
+        return v
+
+    x = normal(M, 1024)
+    fx = far(x, 0)
+    for E, silu in ((2, False), (2, True), (32, False), (32, True)):  # many and few rows per expert
+        w = normal(E, 256, 1024, std=1 / 32)
+        order, offsets = ops.group_rows(torch.randint(0, E, (M,), generator=g, device=cuda).to(torch.int32), E)
+        want = ops.grouped_gemm(x, w, offsets, silu_mul=silu, row_map=order)
+        out = far(torch.zeros_like(want), 4096)
+        ops.grouped_gemm(fx, w, offsets, silu_mul=silu, row_map=order, out=out)
+        assert torch.equal(out, want)
+    ids = torch.randint(-1, 3, (M,), generator=g, device=cuda).to(torch.int32)
+    order, offsets = ops.group_rows(ids, 3)
+    for N in (512, 16384):  # decode and prompt kernels
+        a, b, base = normal(3, 64, 1024, std=1 / 32), normal(3, N, 64, std=1 / 8), normal(M, N)
+        want = ops.lora(x, a, b, order, offsets, base)
+        held = far(base, 4096)
+        ops.lora(fx, a, b, order, offsets, held, out=held)
+        assert torch.equal(held, want)
+    r, gate, w = normal(M, 1024), normal(M, 1024), normal(1024)
+    y, h = ops.gated_add_rmsnorm(x, r, w, 1e-6, post_weight=w, gate=gate, gate_act="silu")
+    fr = far(r, 2048)
+    out = ops.gated_add_rmsnorm(fx, fr, w, 1e-6, post_weight=w, gate=far(gate, 4096), gate_act="silu", out=fx,
+                                residual_out=fr)
+    assert torch.equal(out[0], y) and torch.equal(out[1], h)
+    pos = torch.randint(0, 100000, (M,), generator=g, device=cuda)
+    for rot in (128, 64, 20):  # vectors, part of the head, element by element
+        inv = RotaryEmbedding(8, 2, 128, rot_dim=rot).inv_freq(cuda)
+        q = normal(M, 1024)
+        want, _ = ops.rotary(q.view(M, 8, 128), None, pos, inv)
+        fq = far(q, 0).unflatten(1, (8, 128))
+        ops.rotary(fq, None, pos, inv, q_out=fq)
+        assert torch.equal(fq, want)
+    assert ops.device_error() == 0
