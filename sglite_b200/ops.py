@@ -618,9 +618,14 @@ def _gate_strides(gate: torch.Tensor, x: torch.Tensor, n: int) -> Tuple[int, int
         raise ValueError(f"gate {tuple(shape)} does not broadcast over x {tuple(x.shape)}")
     if wide and gate.stride(-1) != 1:
         raise ValueError("the gate's last dimension must be the contiguous feature dimension")
-    if len(shape) > 2 and rows > 1 and not gate.is_contiguous():
+    if rows <= 1:
+        return 0, int(wide)
+    if len(shape) == 2:
+        return gate.stride(0), int(wide)
+    if not gate.is_contiguous():
         raise ValueError("a gate with more than 2 dimensions must be contiguous")
-    return (gate.stride(-2) if rows > 1 else 0), (1 if wide else 0)
+    # from the shape: a contiguous tensor's dimensions of one may have any stride
+    return shape[-1], int(wide)
 
 
 def gated_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor], eps: float, *,

@@ -1,0 +1,31 @@
+"""The operators around the projections on the GPU, at the edges of what their
+documentation allows: layouts, streams, sizes and values that the operators' own
+files do not reach. Bounds are those of ``oracle/block_ref.py`` unless a test derives its own."""
+
+import pytest
+import torch
+
+from oracle.block_ref import gated_add_rmsnorm_ref, half_step
+from sglite_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("wide", [True, False])
+@pytest.mark.parametrize("B", [4, 33])
+def test_gate_with_a_dimension_of_one(cuda, wide, B):
+    """A decode step's [B, 1, N]: a gate made by turning [1, B, N] is contiguous, and its
+    middle stride says nothing. The bits are those of the gate's own copy."""
+    N, dtype = 512, torch.bfloat16
+    g = torch.Generator(device=cuda).manual_seed(B)
+    x, r = (torch.randn((B, 1, N), generator=g, device=cuda).to(dtype) for _ in range(2))
+    w = torch.rand(N, generator=g, device=cuda).to(dtype)
+    gate = torch.randn((1, B, N if wide else 1), generator=g, device=cuda).to(dtype).transpose(0, 1)
+    assert gate.is_contiguous() and gate.stride(1) == B * (N if wide else 1)
+    y, h = ops.gated_add_rmsnorm(x, r, w, 1e-6, gate=gate, gate_act="sigmoid")
+    y2, h2 = ops.gated_add_rmsnorm(x.view(B, N), r.view(B, N), w, 1e-6, gate=gate.clone().view(B, -1), gate_act="sigmoid")
+    assert torch.equal(y.view(B, N), y2) and torch.equal(h.view(B, N), h2)
+    ey, eh, b = gated_add_rmsnorm_ref(x, r, w, 1e-6, gate=gate, gate_act="sigmoid")
+    # one rounding, and fp32's on the way (each of a few operations at most 2^-16 of a term)
+    off = 2.0 ** -16 * (b.abs() + eh.abs())
+    assert bool(((h.double() - eh).abs() <= off + half_step(dtype) * (eh.abs() + off)).all())
