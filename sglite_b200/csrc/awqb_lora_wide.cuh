@@ -392,8 +392,9 @@ lora_second_wide_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_c
         } else {
           asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
+        __syncwarp();  // a lane waits for its own copies, and reads a row that the others copied
         ok = mbar_wait(smem_u32(&acc_full[group]), ((done + i) >> 1) & 1);
-        if (!__all_sync(0xffffffffu, ok)) {  // (and the lanes' copies are seen by all)
+        if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }

@@ -29,3 +29,29 @@ def test_gate_with_a_dimension_of_one(cuda, wide, B):
     # one rounding, and fp32's on the way (each of a few operations at most 2^-16 of a term)
     off = 2.0 ** -16 * (b.abs() + eh.abs())
     assert bool(((h.double() - eh).abs() <= off + half_step(dtype) * (eh.abs() + off)).all())
+
+
+@pytest.mark.parametrize("rank", [64, 128])  # two tiles of base per group of warps, or one
+@pytest.mark.parametrize("in_place", [False, True])
+def test_prompt_adapters_add_to_the_base_of_this_call(cuda, rank, in_place):
+    """Every element of base is its own and differs from call to call, and the adapters'
+    products are known to the bit (powers of two), so a base read before it has
+    arrived, from an earlier block or call, shows."""
+    M, K, N, L, dtype = 1500, 64, 9000, 3, torch.bfloat16
+    assert M * (N * (50 + rank) + K * rank) > 8e8  # the prompt kernels
+    g = torch.Generator(device=cuda).manual_seed(rank)
+    x = torch.zeros((M, K), dtype=dtype, device=cuda)
+    x[:, 0] = 1
+    a = torch.zeros((L, rank, K), dtype=dtype, device=cuda)
+    a[:, 0, 0] = torch.tensor([1.0, 2.0, 4.0], device=cuda)
+    b = torch.zeros((L, N, rank), dtype=dtype, device=cuda)
+    b[:, :, 0] = 1
+    ids = torch.randint(0, L, (M,), generator=g, device=cuda).to(torch.int32)
+    order, offsets = ops.group_rows(ids, L)
+    add = 2.0 ** ids[:, None].float()
+    for _ in range(20):
+        base = torch.randint(-100, 101, (M, N), generator=g, device=cuda).to(dtype)  # exact, also with 4 more
+        want = (base.float() + add).to(dtype)
+        got = ops.lora(x, a, b, order, offsets, base, out=base if in_place else None)
+        assert torch.equal(got, want)
+    assert ops.device_error() == 0
