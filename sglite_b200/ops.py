@@ -546,10 +546,15 @@ def fused_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
 
 def moe_topk_sum(y3: torch.Tensor, M: int, topk: int, topk_ids: Optional[torch.Tensor], e_begin: int,
                  e_end: int, out: torch.Tensor) -> torch.Tensor:
-    dev = _check_cuda(y3, out)
+    """out[m] = the sum of y3's rows m * topk .. m * topk + topk - 1; with topk_ids (int32
+    [M, topk]) only of those whose expert is in [e_begin, e_end)."""
+    ids = None if topk_ids is None else topk_ids.contiguous()
+    if ids is not None and (ids.dtype != torch.int32 or ids.numel() != M * topk):
+        raise ValueError(f"topk_ids must be an int32 [{M}, {topk}] tensor")
+    dev = _check_cuda(y3, out, ids)
     H = y3.shape[-1]
     with _DeviceGuard(dev):
-        call("awqb_moe_topk_sum", _p(y3), M, topk, H, _p(topk_ids), e_begin, e_end, _dtype_code(y3.dtype),
+        call("awqb_moe_topk_sum", _p(y3), M, topk, H, _p(ids), e_begin, e_end, _dtype_code(y3.dtype),
              _p(out), _stream(dev))
     return out
 

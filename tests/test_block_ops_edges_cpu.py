@@ -1,6 +1,9 @@
 """Host logic of the operators around the projections at the edges of what their
 documentation allows; no GPU."""
 
+import contextlib
+import ctypes
+
 import pytest
 import torch
 
@@ -53,3 +56,39 @@ def test_gates_that_do_not_broadcast_are_refused():
                  torch.zeros(64, 4, 1).permute(1, 2, 0), torch.zeros(2, 64).expand(4, 2, 64)):
         with pytest.raises(ValueError):
             ops._gate_strides(gate, x, 64)
+
+
+@pytest.mark.parametrize("ids", [
+    torch.zeros((3, 8), dtype=torch.int32)[:, :2], torch.zeros((1, 2), dtype=torch.int32).expand(3, 2),
+    torch.zeros((3, 1), dtype=torch.int32).expand(3, 2), torch.zeros((2, 3), dtype=torch.int32).T])
+def test_topk_sum_reads_ids_by_their_rows(monkeypatch, ids):
+    """The kernel reads M * topk ids one after the other: what it gets has to hold them."""
+    seen = {}
+
+    def record(name, *args):
+        ptr, n = args[4].value, ids.numel()
+        seen["ids"] = torch.frombuffer((ctypes.c_int32 * n).from_address(ptr), dtype=torch.int32).clone().view(ids.shape)
+
+    ids = ids.clone() if ids.is_contiguous() else ids
+    if ids.untyped_storage().nbytes() >= 4 * ids.numel():
+        ids.copy_(torch.arange(ids.numel()).view(ids.shape))
+    monkeypatch.setattr(ops, "call", record)
+    monkeypatch.setattr(ops, "_check_cuda", lambda *ts: ts[0].device)
+    monkeypatch.setattr(ops, "_DeviceGuard", contextlib.nullcontext)
+    monkeypatch.setattr(ops, "_stream", lambda dev: None)
+    y3, out = torch.zeros((6, 8), dtype=torch.bfloat16), torch.zeros((3, 8), dtype=torch.bfloat16)
+    try:
+        ops.moe_topk_sum(y3, 3, 2, ids, 0, 4, out)
+    except ValueError:
+        return  # refusing the layout is right as well
+    assert torch.equal(seen["ids"], ids)
+
+
+@pytest.mark.parametrize("ids", [torch.zeros((3, 2), dtype=torch.int64), torch.zeros((3, 1), dtype=torch.int32),
+                                 torch.zeros((2, 2), dtype=torch.int32)])
+def test_topk_sum_refuses_other_ids(monkeypatch, ids):
+    monkeypatch.setattr(ops, "call", lambda *a: pytest.fail("reached the kernel"))
+    monkeypatch.setattr(ops, "_check_cuda", lambda *ts: ts[0].device)
+    y3, out = torch.zeros((6, 8), dtype=torch.bfloat16), torch.zeros((3, 8), dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        ops.moe_topk_sum(y3, 3, 2, ids, 0, 4, out)

@@ -7,6 +7,7 @@ import torch
 
 from oracle.block_ref import gated_add_rmsnorm_ref, half_step
 from sglite_b200 import ops
+from sglite_b200.moe import AWQB200MoeBackend, DenseExpertWeights
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +56,26 @@ def test_prompt_adapters_add_to_the_base_of_this_call(cuda, rank, in_place):
         got = ops.lora(x, a, b, order, offsets, base, out=base if in_place else None)
         assert torch.equal(got, want)
     assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("layout", ["columns", "broadcast"])
+def test_dense_experts_take_ids_and_weights_of_any_layout(cuda, layout):
+    """Ids and weights that are the first columns of a wider ranking, or one row for all
+    tokens: the bits are those of their contiguous copies."""
+    M, E, H, I, topk, dtype = 37, 8, 128, 64, 3, torch.bfloat16
+    g = torch.Generator(device=cuda).manual_seed(2)
+    x = torch.randn((M, H), generator=g, device=cuda).to(dtype)
+    w1 = DenseExpertWeights((torch.randn((E // 2, 2 * I, H), generator=g, device=cuda) / 11).to(dtype), 2, E)
+    w2 = DenseExpertWeights((torch.randn((E // 2, H, I), generator=g, device=cuda) / 8).to(dtype), 2, E)
+    tw = torch.rand((M, E), generator=g, device=cuda)
+    if layout == "columns":
+        tw, ids = (t[:, :topk] for t in tw.sort(dim=1, descending=True))
+        ids = ids.to(torch.int32)
+        ids = torch.cat([ids, torch.full_like(ids, 7)], dim=1)[:, :topk]
+    else:
+        ids = torch.tensor([[5, 0, 3]], dtype=torch.int32, device=cuda).expand(M, topk)
+        tw = tw[:1, :topk].expand(M, topk)
+    assert not ids.is_contiguous() and not tw.is_contiguous()
+    backend = AWQB200MoeBackend()
+    got = backend.experts(x.clone(), w1, w2, tw, ids)
+    assert torch.equal(got, backend.experts(x.clone(), w1, w2, tw.contiguous(), ids.contiguous()))
