@@ -15,12 +15,31 @@ import torch
 from . import ops
 
 
-def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[Dict[str, Any]] = None
-                       ) -> Tuple[torch.Tensor, float]:
+def _longrope_factors(scaling: Dict[str, Any], max_length: Optional[int]) -> Sequence[float]:
+    """The list of an entry that applies to sequences of up to ``max_length`` tokens."""
+    if scaling.get("factors"):
+        return scaling["factors"]
+    short, long = list(scaling.get("short_factor") or ()), list(scaling.get("long_factor") or ())
+    if not short or short == long:
+        return long
+    if max_length is None:
+        raise ValueError("longrope with a short_factor changes with the sequences' length: say the longest one as "
+                         "max_length (or name the list as 'factors')")
+    original = scaling.get("original_max_position_embeddings")
+    if original is None:
+        raise ValueError("longrope with a short_factor needs 'original_max_position_embeddings'")
+    return short if max_length <= int(original) else long
+
+
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[Dict[str, Any]] = None,
+                       max_length: Optional[int] = None) -> Tuple[torch.Tensor, float]:
     """(inv_freq float64 [rot_dim / 2], factor on the turned elements) for a
     checkpoint's ``rope_scaling`` entry: None or "default", "linear", "llama3", "yarn",
     "longrope" (one factor per pair: ``long_factor``, with what its factor on the
     elements follows from, or ``factors`` with an ``attention_factor``, else 1).
+    Where a longrope entry has a ``short_factor`` as well, ``max_length`` says how long
+    sequences get: up to ``original_max_position_embeddings`` tokens take the short
+    list, longer ones the long one; without it the entry is refused.
     "dynamic" is refused: its speeds change with the length that a sequence has."""
     if rot_dim < 2 or rot_dim % 2:
         raise ValueError(f"rot_dim {rot_dim} must be even and positive")
@@ -37,7 +56,7 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: Optional[Di
         return float(scaling[key])
 
     if kind == "longrope":
-        factors: Sequence[float] = scaling.get("factors") or scaling.get("long_factor") or ()
+        factors = _longrope_factors(scaling, max_length)
         if len(factors) != half:
             raise ValueError(f"longrope needs {half} factors, got {len(factors)}")
         inv = inv / torch.tensor([float(f) for f in factors], dtype=torch.float64)
@@ -86,14 +105,15 @@ class RotaryEmbedding:
     """Rotary positions of a merged QKV projection's q and k, in place.
 
     With ``qk_norm`` the per-head RMSNorm of Qwen3's q and k runs in the same
-    kernel; its weights are ``q_weight`` and ``k_weight`` [head_dim]."""
+    kernel; its weights are ``q_weight`` and ``k_weight`` [head_dim]. ``max_length``:
+    the longest sequence, for scalings that depend on it (``rotary_frequencies``)."""
 
     def __init__(self, num_q_heads: int, num_kv_heads: int, head_dim: int, rot_dim: Optional[int] = None,
                  base: float = 10000.0, scaling: Optional[Dict[str, Any]] = None, interleaved: bool = False,
-                 qk_norm: bool = False, eps: float = 1e-6) -> None:
+                 qk_norm: bool = False, eps: float = 1e-6, max_length: Optional[int] = None) -> None:
         self.num_q_heads, self.num_kv_heads, self.head_dim = num_q_heads, num_kv_heads, head_dim
         self.interleaved, self.eps = interleaved, eps
-        self._inv_freq, self.scale = rotary_frequencies(rot_dim or head_dim, base, scaling)
+        self._inv_freq, self.scale = rotary_frequencies(rot_dim or head_dim, base, scaling, max_length)
         self._on_device: Dict[torch.device, torch.Tensor] = {}
         self.q_weight = torch.empty(head_dim) if qk_norm else None
         self.k_weight = torch.empty(head_dim) if qk_norm else None

@@ -3,11 +3,13 @@ documentation allows; no GPU."""
 
 import contextlib
 import ctypes
+import math
 
 import pytest
 import torch
 
 from sglite_b200 import ops
+from sglite_b200.rotary import RotaryEmbedding, rotary_frequencies
 
 
 def _gate_as_kernel_reads(gate, x, n):
@@ -92,3 +94,45 @@ def test_topk_sum_refuses_other_ids(monkeypatch, ids):
     y3, out = torch.zeros((6, 8), dtype=torch.bfloat16), torch.zeros((3, 8), dtype=torch.bfloat16)
     with pytest.raises(ValueError):
         ops.moe_topk_sum(y3, 3, 2, ids, 0, 4, out)
+
+
+LONG = {"rope_type": "longrope", "short_factor": [1.0, 1.5, 2.0, 2.5], "long_factor": [4.0, 8.0, 16.0, 32.0], "factor": 32.0,
+        "original_max_position_embeddings": 4096}
+
+
+def test_longrope_with_two_lists_needs_the_length_it_is_for():
+    """A checkpoint's entry with both lists: the short one up to the original length,
+    the long one beyond, and no guess."""
+    plain = rotary_frequencies(8, 1e4)[0]
+    with pytest.raises(ValueError, match="max_length"):
+        rotary_frequencies(8, 1e4, LONG)
+    with pytest.raises(ValueError, match="max_length"):
+        RotaryEmbedding(2, 1, 8, scaling=LONG)
+    for length, key in ((1, "short_factor"), (4096, "short_factor"), (4097, "long_factor"), (131072, "long_factor")):
+        inv, f = rotary_frequencies(8, 1e4, LONG, max_length=length)
+        assert torch.allclose(inv, plain / torch.tensor(LONG[key], dtype=torch.float64), rtol=1e-15)
+        assert math.isclose(f, math.sqrt(1 + math.log(32) / math.log(4096)))  # of the model, not of the length
+        layer = RotaryEmbedding(2, 1, 8, scaling=LONG, max_length=length)
+        assert torch.equal(layer.inv_freq(torch.device("cpu")), inv) and layer.scale == f
+    with pytest.raises(ValueError):
+        rotary_frequencies(8, 1e4, {**LONG, "original_max_position_embeddings": None, "attention_factor": 1.0},
+                           max_length=100)
+    with pytest.raises(ValueError):  # the list that applies has another length
+        rotary_frequencies(8, 1e4, {**LONG, "short_factor": [1.0]}, max_length=100)
+
+
+def test_longrope_without_a_choice_to_make():
+    plain = rotary_frequencies(8, 1e4)[0]
+    long = plain / torch.tensor(LONG["long_factor"], dtype=torch.float64)
+    one = {k: v for k, v in LONG.items() if k != "short_factor"}
+    for entry, length in ((one, None), (one, 100), ({**LONG, "short_factor": LONG["long_factor"]}, None)):
+        assert torch.allclose(rotary_frequencies(8, 1e4, entry, max_length=length)[0], long, rtol=1e-15)
+    named = {**LONG, "factors": LONG["short_factor"]}  # said outright
+    assert torch.allclose(rotary_frequencies(8, 1e4, named)[0], plain / torch.tensor(LONG["short_factor"], dtype=torch.float64))
+    short = {k: v for k, v in LONG.items() if k != "long_factor"}
+    with pytest.raises(ValueError):  # nothing for lengths beyond the original one
+        rotary_frequencies(8, 1e4, short)
+    with pytest.raises(ValueError):
+        rotary_frequencies(8, 1e4, short, max_length=5000)
+    assert torch.allclose(rotary_frequencies(8, 1e4, short, max_length=4096)[0],
+                          plain / torch.tensor(LONG["short_factor"], dtype=torch.float64))
