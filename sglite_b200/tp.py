@@ -75,11 +75,10 @@ class _AWQLinear:
         self.weights = self.method.process_weights_after_loading(self.weights)
 
     def forward(self, x: torch.Tensor, lora: Optional[LoraBatch] = None) -> torch.Tensor:
-        """``lora``: which row uses which of ``self.adapters`` (None: no row uses one)."""
-        if lora is None:
+        """``lora``: which row uses which of ``self.adapters`` (None: no row uses one). A
+        projection without adapters takes a step's batch too, and adds nothing."""
+        if lora is None or self.adapters is None:
             return self.method.apply_weights(self.weights, x, self.bias)
-        if self.adapters is None:
-            raise ValueError("this projection holds no adapters")
         return self.method.apply_weights(self.weights, x, self.bias, adapters=self.adapters, batch=lora)
 
 
@@ -109,7 +108,8 @@ class RowParallelAWQLinear(_AWQLinear):
         self.exchange = exchange
 
     def forward(self, x: torch.Tensor, lora: Optional[LoraBatch] = None) -> torch.Tensor:
-        if self.tp_size > 1 and self.exchange is not None and self.bias is None and lora is None:
+        adapted = lora is not None and self.adapters is not None
+        if self.tp_size > 1 and self.exchange is not None and self.bias is None and not adapted:
             M = x.numel() // self.local_input_size
             if M <= self.exchange.max_rows and self.local_output_size <= self.exchange.max_n:
                 w = self.weights
