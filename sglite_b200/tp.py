@@ -117,6 +117,8 @@ class RowParallelAWQLinear(_AWQLinear):
                     raise ValueError(f"activations are {x.dtype}, weights were loaded for {w['_act_dtype']}")
                 return self.exchange.gemm_allreduce(x, w["qweight"], self.local_input_size,
                                                     self.local_output_size, w["_group_size"])
+        if self.tp_size > 1 and self.comm is None:
+            raise ValueError("this call needs comm: the exchange serves batches without adapters and bias, up to its size")
         y = super().forward(x, lora)
         if self.tp_size > 1:
             y = self.comm.all_reduce(y)

@@ -55,3 +55,14 @@ def test_a_layer_with_adapters_uses_them_before_the_all_reduce():
         assert torch.equal(layer.forward(X, batch), torch.full((3, 8), want))
         assert layer.method.calls == [(adapters, batch)]
     assert torch.equal(layer.forward(X), torch.full((3, 8), 10.0))  # a batch without adapters
+
+
+def test_rows_that_need_the_communicator_say_so_before_any_work():
+    """An exchange alone serves batches without adapters and bias up to its size."""
+    row = RowParallelAWQLinear(_Method(), 32, 8, 2, exchange=_Exchange())
+    assert torch.equal(row.forward(X), torch.full((3, 8), 10.0))
+    row.adapters = object()
+    for x, lora in ((X, object()), (torch.zeros((65, 16), dtype=torch.bfloat16), None)):
+        with pytest.raises(ValueError, match="comm"):
+            row.forward(x, lora)
+    assert not row.method.calls
