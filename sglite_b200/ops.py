@@ -8,6 +8,7 @@ current CUDA stream (the reference launches on the engine stream,
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from typing import Dict, Optional, Tuple
 
@@ -843,7 +844,11 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out
     return out
 
 
-_LORA_BYTES: Dict[Tuple[int, int, int, int, int, int], int] = {}
+@functools.lru_cache(maxsize=1024)  # a call asks for the same few sizes in every step
+def _lora_workspace_bytes(M: int, K: int, N: int, L: int, rank: int, parts: int) -> int:
+    v = c_i64(0)
+    call("awqb_lora_workspace_bytes", M, K, N, L, rank, parts, ctypes.byref(v))
+    return v.value
 
 
 def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor,
@@ -891,12 +896,7 @@ def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, order: torch.Tensor,
         out = x.new_empty((M, N))
     elif out.shape != (M, N) or out.dtype != dtype or out.get_device() != di:
         raise ValueError("out must have the shape, dtype and device of base")
-    key = (M, K, N, L, rank, parts)
-    nb = _LORA_BYTES.get(key)
-    if nb is None:
-        v = c_i64(0)
-        call("awqb_lora_workspace_bytes", M, K, N, L, rank, parts, ctypes.byref(v))
-        nb = _LORA_BYTES[key] = v.value
+    nb = _lora_workspace_bytes(M, K, N, L, rank, parts)
     # from the caching allocator: private to the stream, or to the graph being captured
     ws = x.new_empty((nb + 1) // 2)  # (x's values have two bytes)
     w = ((N,) if slices is None else tuple(slices)) + (0, 0, 0, 0)

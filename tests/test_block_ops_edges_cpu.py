@@ -136,3 +136,18 @@ def test_longrope_without_a_choice_to_make():
         rotary_frequencies(8, 1e4, short, max_length=5000)
     assert torch.allclose(rotary_frequencies(8, 1e4, short, max_length=4096)[0],
                           plain / torch.tensor(LONG["short_factor"], dtype=torch.float64))
+
+
+def test_what_lora_keeps_between_calls_is_bounded(monkeypatch):
+    """Prompts come with any number of rows: nothing may be kept for each of them."""
+    monkeypatch.setattr(ops, "_device_of", lambda t: -1)  # the other tensors' device here
+    monkeypatch.setattr(ops, "_run", lambda *a: None)
+    monkeypatch.setattr(ops, "_LORA_BYTES", {}, raising=False)
+    a, b = torch.zeros((2, 8, 16), dtype=torch.bfloat16), torch.zeros((2, 8, 8), dtype=torch.bfloat16)
+    offsets = torch.zeros(3, dtype=torch.int32)
+    for M in range(1, 3001):
+        x, base = torch.empty((M, 16), dtype=torch.bfloat16), torch.empty((M, 8), dtype=torch.bfloat16)
+        ops.lora(x, a, b, torch.empty(M, dtype=torch.int32), offsets, base)
+    kept = sum(len(v) for v in vars(ops).values() if isinstance(v, dict) and v is not vars(ops).get("__builtins__"))
+    kept += sum(v.cache_info().currsize for v in vars(ops).values() if hasattr(v, "cache_info"))
+    assert kept < 1500
