@@ -219,8 +219,9 @@ rotary_vec_kernel(const __grid_constant__ Args a, int64_t M, int lanes, int piec
   }
 }
 
-// Any layout: a CTA per token, a warp per head, element by element. Taken where the
-// two halves of the turned part do not split into whole vectors.
+// A CTA per token, a warp per head, element by element: where the two halves of the
+// turned part do not split into whole vectors (never interleaved pairs, whose vectors
+// hold whole pairs).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Args a) {
   __shared__ float cs[kMaxD];
@@ -246,12 +247,11 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
       rms = rsqrtf(warp_sum(ss) * a.inv_d + a.eps);
     }
     for (int j = lane; j < half; j += 32) {
-      const int i0 = a.interleaved ? 2 * j : j, i1 = a.interleaved ? 2 * j + 1 : j + half;
-      float x = (float)in[i0], y = (float)in[i1];
-      if (w != nullptr) x *= rms * (float)w[i0], y *= rms * (float)w[i1];
+      float x = (float)in[j], y = (float)in[j + half];
+      if (w != nullptr) x *= rms * (float)w[j], y *= rms * (float)w[j + half];
       const float c = cs[j], sn = cs[kMaxD / 2 + j];
-      out[i0] = (T)(x * c - y * sn);
-      out[i1] = (T)(x * sn + y * c);
+      out[j] = (T)(x * c - y * sn);
+      out[j + half] = (T)(x * sn + y * c);
     }
     for (int d = a.rot + lane; d < a.D; d += 32) {
       float x = (float)in[d];
