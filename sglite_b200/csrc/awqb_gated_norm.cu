@@ -42,8 +42,9 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return warp_sum(lane < (int)blockDim.x / 32 ? red[lane] : 0.f);
 }
 
-// exp2 and reciprocal approximations (relative error about 1e-6) for the
-// sigmoid: exact division would make this copy-like kernel issue-bound.
+// The sigmoid by the approximate exponential and division (exact division would make
+// this copy-like kernel issue-bound): right to (6 + 1.173 |g|) 2^-23 of the value, 1.2e-5
+// at g = -80 and 9e-7 at |g| = 1, and 0 below g = -87.3, where it is under 2^-125.
 __device__ __forceinline__ float activate(float g, int act) {
   if (act == 1) return __fdividef(1.f, 1.f + __expf(-g));
   if (act == 2) return tanhf(g);

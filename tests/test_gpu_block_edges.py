@@ -79,3 +79,55 @@ def test_dense_experts_take_ids_and_weights_of_any_layout(cuda, layout):
     backend = AWQB200MoeBackend()
     got = backend.experts(x.clone(), w1, w2, tw, ids)
     assert torch.equal(got, backend.experts(x.clone(), w1, w2, tw.contiguous(), ids.contiguous()))
+
+
+# CUDA documents __expf(-g) to within 2 + floor(1.173 |g|) units (2^-23 relative) and
+# __fdividef to within 2 for denominators up to 2^126, above which it gives 0. With the
+# rounded sum 1 + e^-g and a last product that makes silu(g) * u and sigmoid(g) relatively
+# right to (6 + 1.173 |g|) 2^-23, and 0 for g below -87.3, where they are below |g| 2^-126.
+GATES = [0.0, 1e-3, 0.5, 3.0, 10.0, 19.875, 20.0, 40.0, 63.75, 79.5, 80.0, 86.0, 87.0, 87.5, 88.0, 89.0, 100.0, 120.0]
+
+
+def _act_error(g):
+    return (6 + 1.173 * g.abs()) * 2.0 ** -23, torch.where(g < -87.3, g.abs() + 1, 0.0) * 2.0 ** -126
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [5, 90])  # few and many rows per expert
+def test_silu_mul_of_large_gates(cuda, dtype, rows):
+    """One weight per feature, so that gate and up are known to the bit."""
+    gates = torch.tensor([s * v for v in GATES for s in (1, -1)] * 4, device=cuda)  # 144 features
+    I, K = gates.numel(), 64
+    w = torch.zeros((2, 2 * I, K), dtype=dtype, device=cuda)
+    w[:, :I, 0] = gates.to(dtype)
+    w[:, I:, 0] = (torch.arange(I, device=cuda) % 7 - 3).to(dtype) * 4
+    x = torch.zeros((rows, K), dtype=dtype, device=cuda)
+    x[:, 0] = 1
+    offsets = torch.tensor([0, rows // 2, rows], dtype=torch.int32, device=cuda)
+    got = ops.grouped_gemm(x, w, offsets, silu_mul=True).double()
+    g, u = w[0, :I, 0].double(), w[0, I:, 0].double()
+    want = g / (1 + torch.exp(-g)) * u
+    rel, flushed = _act_error(g)
+    tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2  # half of the type's smallest step
+    off = rel * want.abs() + flushed * u.abs()
+    assert bool(((got - want).abs() <= off + half_step(dtype) * (want.abs() + off) + tiny).all())
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "silu", "tanh"])
+def test_norm_with_large_gates(cuda, act):
+    """A zero fp32 residual shows the gated branch to 24 bits."""
+    N, dtype = 4096, torch.bfloat16
+    vals = torch.tensor([s * v for v in GATES for s in (1, -1)])
+    gate = vals.repeat(N // vals.numel() + 1)[:N].to(dtype).to(cuda)
+    x = (torch.arange(3 * N, device=cuda) % 13 - 6).to(dtype).view(3, N)
+    r = torch.zeros((3, N), device=cuda)
+    y, h = ops.gated_add_rmsnorm(x, r, torch.ones(N, dtype=dtype, device=cuda), 1e-6, gate=gate, gate_act=act)
+    g = gate.double()
+    a = {"sigmoid": 1 / (1 + torch.exp(-g)), "silu": g / (1 + torch.exp(-g)), "tanh": torch.tanh(g)}[act]
+    want = x.double() * a
+    rel, flushed = _act_error(g)
+    if act == "tanh":
+        flushed = flushed * 0
+    # the activation, two products and a sum with zero, each rounded once in fp32
+    off = (rel + 3 * 2.0 ** -24) * want.abs() + flushed * x.double().abs() + 2.0 ** -149
+    assert bool(((h.double() - want).abs() <= off).all())
