@@ -354,8 +354,9 @@ int awqb_grouped_gemm(const awqb_grouped_gemm_args* args, void* stream);
  * gate_up) has num_slices > 1 slices of its N outputs (slices: their widths,
  * adding up to N), each with its own pair: a
  * [L][num_slices * rank][K] stacks the slices' first factors, b [L][N][rank]
- * their second ones. Sums are fp32; the product of the first factor is kept in
- * fp32 (as two 16-bit halves in the tensor cores). scales [L] fp32 or null (1).
+ * their second ones. Sums are fp32; the product of the first factor enters the
+ * second one as two 16-bit halves: bf16 loses 2^-16 of each value, fp16 2^-22 or
+ * 2^-39 of the row's largest value in the slice. scales [L] fp32 or null (1).
  * order [M] and offsets [L + 1] as awqb_group_rows gives them: order is a
  * permutation of the rows (an entry outside 0..M - 1 is skipped). out may
  * equal base (with the same row stride); other overlaps are not allowed. K is a multiple of 8, the slice widths of 8, rank of 8 and at

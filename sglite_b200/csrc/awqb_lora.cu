@@ -14,9 +14,12 @@
 //           K are kept apart and added in order by the second kernel: no atomics,
 //           the same bits every time.
 //   second: out = base + scale * h B^T. h enters as two 16-bit halves
-//           (h = hi + lo, each rounded to nearest, after a power-of-two scale per
-//           row that keeps fp16 in range), so what is lost is 2^-16 (bf16) or
-//           2^-22 (fp16) of h, not 2^-8. Features are dealt to the product's
+//           (h = hi + lo, each rounded to nearest), so what is lost is 2^-16 of each
+//           value for bf16, not 2^-8. fp16 gets a power-of-two scale per row and slice
+//           that brings the largest value to 2^14 .. 2^15: 2^-22 of each value is lost,
+//           or 2^-39 of the largest where that is more (values under 2^-17 of it). A
+//           third half would be half as many products again for bits that the result's
+//           own rounding drops. Features are dealt to the product's
 //           columns so that a lane ends with 8 neighbouring ones: base and out move
 //           as 16-byte vectors.
 #include <cuda_runtime.h>

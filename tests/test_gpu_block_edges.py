@@ -131,3 +131,45 @@ def test_norm_with_large_gates(cuda, act):
     # the activation, two products and a sum with zero, each rounded once in fp32
     off = (rel + 3 * 2.0 ** -24) * want.abs() + flushed * x.double().abs() + 2.0 ** -149
     assert bool(((h.double() - want).abs() <= off).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N", [(5, 64), (1000, 16384)])  # decode and prompt kernels
+def test_ranks_of_very_different_size(cuda, dtype, M, N):
+    """h enters the second product as two 16-bit halves. bf16: 2^-16 of each value. fp16: a
+    place's largest value (per slice) is brought to 2^14 .. 2^15, so halves are off by
+    2^-22 of the value, or by half of fp16's smallest step, 2^-25, where that is more:
+    2^-39 of the largest. x is one, so that h is A's column to the bit; the largest rank's
+    B is 0 in half of the features, so that the small ranks stand alone there."""
+    K, L = 64, 2
+    assert (M * (N * 58 + K * 8) > 8e8) == (M == 1000)
+    sizes = torch.tensor([60000.0, 1.3, 2.0 ** -5 * 1.7, 2.0 ** -10 * 1.1, 2.0 ** -13 * 1.9, 2.0 ** -15 * 1.37, 2.0 ** -18, 0.0])
+    a = torch.zeros((L, 8, K), dtype=dtype, device=cuda)
+    a[0, :, 0] = sizes.to(dtype)
+    a[1, :, 0] = sizes.flip(0).to(dtype) * 0.5
+    g = torch.Generator(device=cuda).manual_seed(N)
+    b = (torch.rand((L, N, 8), generator=g, device=cuda) + 0.5).to(dtype)
+    b[0, :, 1:] *= 256
+    b[0, ::2, :3] = 0  # the large ranks leave these features alone
+    b[1, ::2, 5:] = 0
+    x = torch.zeros((M, K), dtype=dtype, device=cuda)
+    x[:, 0] = 1
+    base = torch.zeros((M, N), dtype=dtype, device=cuda)
+    base[:, 1::2] = 1
+    ids = (torch.arange(M, device=cuda) % 3 - 1).to(torch.int32)
+    scales = torch.tensor([2.0 ** -10, 0.75 * 2.0 ** -10], device=cuda)
+    got = ops.lora(x, a, b, *ops.group_rows(ids, L), base, scales=scales).double()
+    for l in range(L):
+        h, bl, s = a[l, :, 0].double(), b[l].double(), float(scales[l])
+        off_h = half_step(dtype) ** 2 * h.abs()
+        if dtype == torch.float16:
+            off_h = torch.maximum(off_h, 2.0 ** -39 * h.abs().max())
+        rows = (ids == l).nonzero()[:, 0]
+        d = s * (bl @ h)
+        want = base[rows].double() + d
+        # both halves' products (16 additions), two products and the last sum, each off by 2^-23
+        off = abs(s) * (bl.abs() @ (off_h + 18 * 2.0 ** -23 * h.abs())) + 2.0 ** -23 * want.abs()
+        step = 2.0 ** -25 if dtype == torch.float16 else 0.0
+        assert bool(((got[rows] - want).abs() <= off + half_step(dtype) * (want.abs() + off) + step).all())
+    assert torch.equal(got[ids < 0], base[ids < 0].double())
+    assert ops.device_error() == 0
