@@ -5,9 +5,14 @@ files do not reach. Bounds are those of ``oracle/block_ref.py`` unless a test de
 import pytest
 import torch
 
-from oracle.block_ref import gated_add_rmsnorm_ref, half_step
+from oracle.awq_ref import rel_err
+from oracle.block_ref import gated_add_rmsnorm_ref, half_step, lora_ref, within
 from sglite_b200 import ops
+from sglite_b200.lora import LoraAdapters, LoraBatch
 from sglite_b200.moe import AWQB200MoeBackend, DenseExpertWeights
+from sglite_b200.quantization import AWQB200Config
+from sglite_b200.synthetic import make_awq_weights
+from sglite_b200.tp import RowParallelAWQLinear, shard_awq
 
 pytestmark = pytest.mark.gpu
 
@@ -172,4 +177,77 @@ def test_ranks_of_very_different_size(cuda, dtype, M, N):
         step = 2.0 ** -25 if dtype == torch.float16 else 0.0
         assert bool(((got[rows] - want).abs() <= off + half_step(dtype) * (want.abs() + off) + step).all())
     assert torch.equal(got[ids < 0], base[ids < 0].double())
+    assert ops.device_error() == 0
+
+
+def test_rows_that_no_expert_wrote_are_not_summed(cuda, monkeypatch):
+    """Every buffer that the experts allocate starts as NaN, and the rows of choices that
+    are held nowhere here are seen to be NaN still when the sum runs."""
+    M, E, H, I, topk, dtype = 40, 8, 128, 64, 3, torch.bfloat16
+    g = torch.Generator(device=cuda).manual_seed(9)
+    x = torch.randn((M, H), generator=g, device=cuda).to(dtype)
+    w1 = DenseExpertWeights((torch.randn((E, 2 * I, H), generator=g, device=cuda) / 11).to(dtype))
+    w2 = DenseExpertWeights((torch.randn((E, H, I), generator=g, device=cuda) / 8).to(dtype))
+    ids = torch.randint(-1, 2 * E, (M, topk), generator=g, device=cuda).to(torch.int32)
+    ids[3] = -1  # a token with no expert here at all
+    tw = torch.rand((M, topk), generator=g, device=cuda)
+    here = (ids >= 0) & (ids < E)
+    backend = AWQB200MoeBackend()
+    want = backend.experts(x.clone(), w1, w2, tw * here, torch.where(here, ids, 0))
+    empty, topk_sum, seen = torch.empty, ops.moe_topk_sum, []
+
+    def poisoned(*args, **kw):
+        t = empty(*args, **kw)
+        return t.fill_(float("nan")) if t.is_floating_point() else t
+
+    def spy(y3, *args):
+        seen.append(y3.clone())
+        return topk_sum(y3, *args)
+
+    monkeypatch.setattr(torch, "empty", poisoned)
+    monkeypatch.setattr(ops, "moe_topk_sum", spy)
+    got = backend.experts(x.clone(), w1, w2, tw, ids)
+    monkeypatch.undo()
+    bare = torch.isnan(seen[0]).all(dim=1)
+    assert torch.equal(bare.view(M, topk), ~here)
+    assert torch.equal(got, want) and bool((got[3] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [3, 900])  # decode and prompt kernels
+def test_row_parallel_shards_with_adapters_add_up(cuda, dtype, M):
+    """The two ranks of a row-parallel projection one after the other, the all-reduce a sum
+    by hand: each shard is its projection's output plus its part of the adapters
+    (64-bit formula), and the sum of both is the whole layer's output."""
+    K, N, L, r = 512, 16384 if M == 900 else 256, 3, 32
+    wq = make_awq_weights(K, N, 128, dtype, seed=5)
+    method = AWQB200Config(4, 128, True).get_linear_method()
+    g = torch.Generator(device=cuda).manual_seed(M)
+    x = torch.randn((M, K), generator=g, device=cuda).to(dtype)
+    adapters = LoraAdapters((torch.randn((L, r, K), generator=g, device=cuda) * K ** -0.5).to(dtype),
+                            (torch.randn((L, N, r), generator=g, device=cuda)).to(dtype),
+                            torch.rand(L, generator=g, device=cuda) + 0.5)
+    ids = torch.randint(-1, L, (M,), generator=g, device=cuda).to(torch.int32)
+    batch = LoraBatch.from_ids(ids, L)
+
+    class Comm:  # takes this rank's part
+        def all_reduce(self, y):
+            return y
+
+    parts = []
+    for rank in range(2):
+        layer = RowParallelAWQLinear(method, K, N, 2, Comm())
+        layer.load({k: v.to(cuda) for k, v in shard_awq(wq, "row", rank, 2).items()})
+        layer.adapters = adapters.shard("row", rank, 2)
+        xs = x.chunk(2, dim=1)[rank].contiguous()
+        plain, y = layer.forward(xs), layer.forward(xs, batch)
+        want, bound = lora_ref(xs, layer.adapters.a, layer.adapters.b, ids, plain, (N,), adapters.scales,
+                               halves_eps=half_step(dtype) ** 2)
+        assert within(y, want, bound, dtype) <= 0
+        assert torch.equal(y[ids < 0], plain[ids < 0])
+        parts.append(y.double())
+    whole = RowParallelAWQLinear(method, K, N, 1)
+    whole.load({k: v.to(cuda) for k, v in wq.items() if k in ("qweight", "qzeros", "scales")})
+    whole.adapters = adapters
+    assert rel_err((parts[0] + parts[1]).float(), whole.forward(x, batch).float().cpu()) <= 1e-2  # that of the GEMM tests
     assert ops.device_error() == 0
