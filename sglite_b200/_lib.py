@@ -93,13 +93,14 @@ _SIGNATURES = {
 EXPORTED = tuple(_SIGNATURES)
 
 # Layouts (native alignment) of the structures that some entry points take, field by
-# field as in include/awqb200.h. Packing one is several times cheaper than
-# converting twenty arguments one by one; null pointers are 0.
+# field as in include/awqb200.h, with "0q" for the padding at their ends. Packing one
+# is several times cheaper than converting twenty arguments one by one; null pointers
+# are 0.
 ARGS = {
-    "awqb_gated_add_rmsnorm": struct.Struct("@PqPqiPPqqifPfPqPqqqfi"),
-    "awqb_rotary": struct.Struct("@PqqqPqqqPiPqqqifPPfPqqPqqi"),
-    "awqb_grouped_gemm": struct.Struct("@PqqPqqqPiiPPPqq"),
-    "awqb_lora": struct.Struct("@PqqqPPqqqqqqqqPPPPqPqiPq"),
+    "awqb_gated_add_rmsnorm": struct.Struct("@PqPqiPPqqifPfPqPqqqfi0q"),
+    "awqb_rotary": struct.Struct("@PqqqPqqqPiPqqqifPPfPqqPqqi0q"),
+    "awqb_grouped_gemm": struct.Struct("@PqqPqqqPiiPPPqq0q"),
+    "awqb_lora": struct.Struct("@PqqqPPqqqqqqqqPPPPqPqiPq0q"),
 }
 
 _lock = threading.Lock()

@@ -4,11 +4,14 @@ documentation allows; no GPU."""
 import contextlib
 import ctypes
 import math
+import os
+import struct
+import subprocess
 
 import pytest
 import torch
 
-from sglite_b200 import ops
+from sglite_b200 import _lib, ops
 from sglite_b200.rotary import RotaryEmbedding, rotary_frequencies
 
 
@@ -151,3 +154,22 @@ def test_what_lora_keeps_between_calls_is_bounded(monkeypatch):
     kept = sum(len(v) for v in vars(ops).values() if isinstance(v, dict) and v is not vars(ops).get("__builtins__"))
     kept += sum(v.cache_info().currsize for v in vars(ops).values() if hasattr(v, "cache_info"))
     assert kept < 1500
+
+
+def test_packed_structures_have_the_size_that_c_reads(tmp_path):
+    """Field offsets and sizes as a C compiler lays the structures out."""
+    names = {"awqb_gated_add_rmsnorm": ("awqb_gated_norm_args", "dtype"), "awqb_rotary": ("awqb_rotary_args", "dtype"),
+             "awqb_grouped_gemm": ("awqb_grouped_gemm_args", "ldo"), "awqb_lora": ("awqb_lora_args", "workspace_bytes")}
+    assert set(names) == set(_lib.ARGS)
+    lines = [f'printf("{k} %zu %zu\\n", sizeof({t}), offsetof({t}, {last}));' for k, (t, last) in names.items()]
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "awqb200.h"\nint main(void) {\n' + "\n".join(lines)
+                   + "\nreturn 0;\n}\n")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-I", include, str(src), "-o", str(tmp_path / "sizes")], check=True)
+    for line in subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout.splitlines():
+        name, size, last = line.split()
+        form = _lib.ARGS[name].format
+        fields = form.removesuffix("0q")
+        assert _lib.ARGS[name].size == int(size), name
+        assert struct.calcsize(fields) - struct.calcsize("@" + fields[-1]) == int(last), name
