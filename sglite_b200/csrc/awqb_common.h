@@ -28,6 +28,8 @@ int device_sm_count();  // of the current device, cached per device
 // bits into it when a bounded wait gives up); nullptr if it cannot be found.
 uint32_t* device_error_word();
 
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 }  // namespace awqb
 
 #define AWQB_REQUIRE(cond, code, ...)                        \

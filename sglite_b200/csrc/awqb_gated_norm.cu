@@ -172,18 +172,15 @@ int launch(const Args& a, int64_t M, cudaStream_t stream) {
   return kOk;
 }
 
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
 }  // namespace
 }  // namespace awqb
 
 using namespace awqb;
 
-static int awqb_gated_add_rmsnorm_impl(const void* x, int64_t ld_x, const void* residual, int64_t ld_res,
-                                      int residual_f32, const void* post_weight, const void* gate, int64_t gate_row,
-                                      int64_t gate_col, int gate_act, float scale, const void* weight,
-                                      float weight_offset, void* out, int64_t ld_out, void* residual_out,
-                                      int64_t ld_res_out, int64_t M, int64_t N, float eps, int dtype, void* stream) {
+extern "C" int awqb_gated_add_rmsnorm(const awqb_gated_norm_args* args, void* stream) {
+  AWQB_REQUIRE(args != nullptr, kInvalidArgument, "args is null");
+  const auto [x, ld_x, residual, ld_res, residual_f32, post_weight, gate, gate_row, gate_col, gate_act, scale,
+              weight, weight_offset, out, ld_out, residual_out, ld_res_out, M, N, eps, dtype] = *args;
   AWQB_REQUIRE(dtype == AWQB_DTYPE_F16 || dtype == AWQB_DTYPE_BF16, kInvalidArgument, "bad dtype %d", dtype);
   AWQB_REQUIRE(M >= 0 && M <= 0x7fffffff && N > 0 && N % 8 == 0 && N <= kMaxN, kInvalidArgument,
                "N=%lld must be a positive multiple of 8, at most %d", (long long)N, kMaxN);
@@ -208,11 +205,4 @@ static int awqb_gated_add_rmsnorm_impl(const void* x, int64_t ld_x, const void* 
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == AWQB_DTYPE_F16) return residual_f32 ? launch<__half, true>(a, M, st) : launch<__half, false>(a, M, st);
   return residual_f32 ? launch<__nv_bfloat16, true>(a, M, st) : launch<__nv_bfloat16, false>(a, M, st);
-}
-
-extern "C" int awqb_gated_add_rmsnorm(const awqb_gated_norm_args* a, void* stream) {
-  AWQB_REQUIRE(a != nullptr, kInvalidArgument, "args is null");
-  return awqb_gated_add_rmsnorm_impl(a->x, a->ld_x, a->residual, a->ld_res, a->residual_f32, a->post_weight, a->gate, a->gate_row,
-                                     a->gate_col, a->gate_act, a->scale, a->weight, a->weight_offset, a->out, a->ld_out,
-                                     a->residual_out, a->ld_res_out, a->M, a->N, a->eps, a->dtype, stream);
 }

@@ -146,13 +146,6 @@ __device__ __forceinline__ void load_rows(const Params& p, const Tile& tile, int
   }
 }
 
-// After a wait gave up: copies and products in flight get time to end.
-__device__ __forceinline__ void linger() {
-  const uint64_t t0 = globaltimer_ns();
-  while (globaltimer_ns() - t0 < 10000000ull) {
-  }
-}
-
 // silu(g) * u with the approximate exponential and division: right to
 // (6 + 1.173 |g|) 2^-23 of the value (1.2e-5 at g = -80; 16-bit results keep 2^-11 at
 // best), and 0 below g = -87.3, where |silu(g)| < 88 * 2^-126.
@@ -536,19 +529,6 @@ grouped_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
   }
 }
 
-int make_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t K, int64_t ld, int box_rows) {
-  const auto enc = tensor_map_encoder();
-  AWQB_REQUIRE(enc != nullptr, kCudaError, "cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint64_t dim[2] = {(cuuint64_t)K, (cuuint64_t)rows};
-  const cuuint64_t stride[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {kK, (cuuint32_t)box_rows}, step[2] = {1, 1};
-  const CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dim, stride, box, step,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  AWQB_REQUIRE(r == CUDA_SUCCESS, kCudaError, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return kOk;
-}
-
 // w as [expert][feature][gate, up][k]: a box of 64 features brings gate and up rows
 // by turns. Features past the last one read as zero.
 int make_gate_up_map(CUtensorMap* tm, const void* w, const Params& p) {
@@ -591,8 +571,8 @@ int launch(const void* x, int64_t ldx, const void* w, Params p, cudaStream_t str
   CUtensorMap tw;
   TokenMaps tx;
   int st = kMany && p.silu ? make_gate_up_map(&tw, w, p)
-                           : make_map(&tw, w, (int64_t)p.E * p.N, p.K, p.K, p.silu ? kFeat / 2 : kFeat);
-  for (int i = 0; i < 3 && st == kOk; ++i) st = make_map(&tx.box[i], x, p.rows, p.K, ldx, kTokCta >> (2 - i));
+                           : make_rows_map(&tw, w, (int64_t)p.E * p.N, p.K, p.K, p.silu ? kFeat / 2 : kFeat);
+  for (int i = 0; i < 3 && st == kOk; ++i) st = make_rows_map(&tx.box[i], x, p.rows, p.K, ldx, kTokCta >> (2 - i));
   if (st != kOk) return st;
   const auto smem_for = [](int E) {
     return 1024 + C::kStages * C::kStageBytes + (kMany ? 0 : Few::kChunk * kFeat * 4) + 4 * C::kTok * 4 + (3 * E + 1) * 4;
@@ -626,16 +606,14 @@ int launch(const void* x, int64_t ldx, const void* w, Params p, cudaStream_t str
   return kOk;
 }
 
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
 }  // namespace
 }  // namespace awqb
 
 using namespace awqb;
 
-static int awqb_grouped_gemm_impl(const void* x, int64_t rows, int64_t ldx, const void* w, int64_t E, int64_t K,
-                                 int64_t N, const int32_t* offsets, int dtype, int silu_mul, const int32_t* row_map,
-                                 const float* row_scale, void* out, int64_t out_rows, int64_t ldo, void* stream) {
+extern "C" int awqb_grouped_gemm(const awqb_grouped_gemm_args* args, void* stream) {
+  AWQB_REQUIRE(args != nullptr, kInvalidArgument, "args is null");
+  const auto [x, rows, ldx, w, E, K, N, offsets, dtype, silu_mul, row_map, row_scale, out, out_rows, ldo] = *args;
   AWQB_REQUIRE(dtype == AWQB_DTYPE_F16 || dtype == AWQB_DTYPE_BF16, kInvalidArgument, "bad dtype %d", dtype);
   AWQB_REQUIRE(E >= 1 && E <= kMaxExperts, kInvalidArgument, "%lld experts: 1..%d are supported", (long long)E,
                kMaxExperts);
@@ -667,10 +645,4 @@ static int awqb_grouped_gemm_impl(const void* x, int64_t rows, int64_t ldx, cons
   if (dtype == AWQB_DTYPE_F16)
     return many ? launch<__half, true>(x, ldx, w, p, st) : launch<__half, false>(x, ldx, w, p, st);
   return many ? launch<__nv_bfloat16, true>(x, ldx, w, p, st) : launch<__nv_bfloat16, false>(x, ldx, w, p, st);
-}
-
-extern "C" int awqb_grouped_gemm(const awqb_grouped_gemm_args* a, void* stream) {
-  AWQB_REQUIRE(a != nullptr, kInvalidArgument, "args is null");
-  return awqb_grouped_gemm_impl(a->x, a->rows, a->ldx, a->w, a->E, a->K, a->N, a->offsets, a->dtype, a->silu_mul, a->row_map,
-                                a->row_scale, a->out, a->out_rows, a->ldo, stream);
 }

@@ -389,20 +389,6 @@ Layout layout(const Sizes& z) {
 
 int64_t max_tiles(const Args& g, int rows) { return std::min<int64_t>(g.M, g.M / rows + g.L + 2); }
 
-// rows x 64 k of a row-major matrix, 128-byte swizzle, zeros outside.
-int make_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t k, int64_t ld, int box_rows) {
-  const auto enc = tensor_map_encoder();
-  AWQB_REQUIRE(enc != nullptr, kCudaError, "cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint64_t dim[2] = {(cuuint64_t)k, (cuuint64_t)rows};
-  const cuuint64_t stride[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, one[2] = {1, 1};
-  const CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dim, stride, box, one,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  AWQB_REQUIRE(r == CUDA_SUCCESS, kCudaError, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return kOk;
-}
-
 // Chunks of `chunk` features over all slices.
 int64_t count_chunks(const Args& g, int64_t chunk) {
   int64_t chunks = 0;
@@ -429,10 +415,10 @@ template <typename T>
 int launch_prompt(const Args& g, cudaLaunchConfig_t cfg) {
   const int col_box = std::min(128, g.R), atoms = (g.rank + 63) / 64;
   CUtensorMap tx, ta, tb, th;
-  int st = make_map(&tx, g.x, g.M, g.K, g.ldx, kWideRows);
-  if (st == kOk) st = make_map(&ta, g.a, (int64_t)g.L * g.R, g.K, g.K, col_box);
-  if (st == kOk) st = make_map(&tb, g.b, (int64_t)g.L * g.N, g.rank, g.rank, kWideFeat);
-  if (st == kOk) st = make_map(&th, g.halves, (int64_t)g.S * 2 * g.M, g.rank, g.rank, kWideRows);
+  int st = make_rows_map(&tx, g.x, g.M, g.K, g.ldx, kWideRows);
+  if (st == kOk) st = make_rows_map(&ta, g.a, (int64_t)g.L * g.R, g.K, g.K, col_box);
+  if (st == kOk) st = make_rows_map(&tb, g.b, (int64_t)g.L * g.N, g.rank, g.rank, kWideFeat);
+  if (st == kOk) st = make_rows_map(&th, g.halves, (int64_t)g.S * 2 * g.M, g.rank, g.rank, kWideRows);
   if (st != kOk) return st;
   cfg.gridDim = dim3((unsigned)(max_tiles(g, kWideRows) * ((g.R + 127) / 128) * g.parts));
   cfg.blockDim = dim3(kFirstWideThreads);
@@ -465,8 +451,6 @@ int launch(const Args& g, bool prompt, cudaStream_t st) {
   return prompt ? launch_prompt<T>(g, cfg) : launch_decode<T>(g, cfg);
 }
 
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
 int check_sizes(int64_t M, int64_t K, int64_t N, int64_t L, int64_t rank, int64_t S) {
   AWQB_REQUIRE(M >= 0 && M < (1ll << 24), kInvalidArgument, "bad number of rows %lld", (long long)M);
   AWQB_REQUIRE(K > 0 && K % 8 == 0 && K <= (1 << 20), kInvalidArgument, "K=%lld must be a positive multiple of 8",
@@ -496,10 +480,10 @@ extern "C" int awqb_lora_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_
   return kOk;
 }
 
-static int awqb_lora_impl(const void* x, int64_t M, int64_t ldx, int64_t K, const void* a, const void* b, int64_t L,
-                         int64_t rank, int64_t N, const int64_t* slices, int64_t num_slices, const int32_t* order,
-                         const int32_t* offsets, const float* scales, const void* base, int64_t ld_base, void* out,
-                         int64_t ld_out, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int awqb_lora(const awqb_lora_args* args, void* stream) {
+  AWQB_REQUIRE(args != nullptr, kInvalidArgument, "args is null");
+  const auto [x, M, ldx, K, a, b, L, rank, N, num_slices, slices, order, offsets, scales, base, ld_base, out, ld_out,
+              dtype, workspace, workspace_bytes] = *args;
   AWQB_REQUIRE(dtype == AWQB_DTYPE_F16 || dtype == AWQB_DTYPE_BF16, kInvalidArgument, "bad dtype %d", dtype);
   int64_t need = 0;
   const int st = awqb_lora_workspace_bytes(M, K, N, L, rank, num_slices, &need);
@@ -541,11 +525,4 @@ static int awqb_lora_impl(const void* x, int64_t M, int64_t ldx, int64_t K, cons
   g.up = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at.up);
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   return dtype == AWQB_DTYPE_F16 ? launch<__half>(g, for_prompt(z), cs) : launch<__nv_bfloat16>(g, for_prompt(z), cs);
-}
-
-extern "C" int awqb_lora(const awqb_lora_args* a, void* stream) {
-  AWQB_REQUIRE(a != nullptr, kInvalidArgument, "args is null");
-  return awqb_lora_impl(a->x, a->M, a->ldx, a->K, a->a, a->b, a->L, a->rank, a->N, a->slices, a->num_slices, a->order,
-                        a->offsets, a->scales, a->base, a->ld_base, a->out, a->ld_out, a->dtype, a->workspace,
-                        a->workspace_bytes, stream);
 }

@@ -60,13 +60,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool i
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 
-// After a wait gave up: copies and products in flight get time to end.
-__device__ __forceinline__ void linger() {
-  const uint64_t t0 = globaltimer_ns();
-  while (globaltimer_ns() - t0 < 10000000ull) {
-  }
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kFirstWideThreads, 2)
 lora_first_wide_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_a,

@@ -91,6 +91,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
   }
 }
 
+// After a wait gave up: copies and products in flight get time to end.
+__device__ __forceinline__ void linger() {
+  const uint64_t t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < 10000000ull) {
+  }
+}
+
 __device__ __forceinline__ void fence_barrier_init() {
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }

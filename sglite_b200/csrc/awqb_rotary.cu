@@ -303,8 +303,6 @@ int launch(const Args& a, int64_t M, cudaStream_t st) {
   return kOk;
 }
 
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
 // No element of [rows, heads, D] stands where another does.
 bool apart(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t D) {
   if (rows <= 1) return heads <= 1 || head >= D;
@@ -317,12 +315,11 @@ bool apart(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t D) {
 
 using namespace awqb;
 
-static int awqb_rotary_impl(const void* q, int64_t q_row, int64_t q_head, int64_t Hq, const void* k, int64_t k_row,
-                           int64_t k_head, int64_t Hk, const void* positions, int positions_i64,
-                           const double* inv_freq, int64_t rot_dim, int64_t head_dim, int64_t M, int interleaved,
-                           float scale, const void* q_weight, const void* k_weight, float eps, void* q_out,
-                           int64_t q_out_row, int64_t q_out_head, void* k_out, int64_t k_out_row, int64_t k_out_head,
-                           int dtype, void* stream) {
+extern "C" int awqb_rotary(const awqb_rotary_args* args, void* stream) {
+  AWQB_REQUIRE(args != nullptr, kInvalidArgument, "args is null");
+  const auto [q, q_row, q_head, Hq, k, k_row, k_head, Hk, positions, positions_i64, inv_freq, rot_dim, head_dim, M,
+              interleaved, scale, q_weight, k_weight, eps, q_out, q_out_row, q_out_head, k_out, k_out_row,
+              k_out_head, dtype] = *args;
   AWQB_REQUIRE(dtype == AWQB_DTYPE_F16 || dtype == AWQB_DTYPE_BF16, kInvalidArgument, "bad dtype %d", dtype);
   AWQB_REQUIRE(head_dim > 0 && head_dim % 8 == 0 && head_dim <= kMaxD, kInvalidArgument,
                "head_dim=%lld must be a positive multiple of 8, at most %d", (long long)head_dim, kMaxD);
@@ -357,12 +354,4 @@ static int awqb_rotary_impl(const void* q, int64_t q_row, int64_t q_head, int64_
   a.inv_d = 1.f / (float)head_dim;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == AWQB_DTYPE_F16 ? launch<__half>(a, M, st) : launch<__nv_bfloat16>(a, M, st);
-}
-
-extern "C" int awqb_rotary(const awqb_rotary_args* a, void* stream) {
-  AWQB_REQUIRE(a != nullptr, kInvalidArgument, "args is null");
-  return awqb_rotary_impl(a->q, a->q_row, a->q_head, a->Hq, a->k, a->k_row, a->k_head, a->Hk, a->positions,
-                          a->positions_i64, a->inv_freq, a->rot_dim, a->head_dim, a->M, a->interleaved, a->scale, a->q_weight,
-                          a->k_weight, a->eps, a->q_out, a->q_out_row, a->q_out_head, a->k_out, a->k_out_row,
-                          a->k_out_head, a->dtype, stream);
 }
