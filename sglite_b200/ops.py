@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import threading
 from typing import Dict, Optional, Tuple
 
@@ -619,7 +620,7 @@ def _gate_strides(gate: torch.Tensor, x: torch.Tensor, n: int) -> Tuple[int, int
     wide = len(shape) > 0 and shape[-1] == n
     if not wide and len(shape) > 0 and shape[-1] != 1:
         raise ValueError(f"gate {tuple(shape)} does not broadcast over x {tuple(x.shape)}")
-    rows = gate.numel() // n if wide else gate.numel()
+    rows = math.prod(shape[:-1])
     if rows != 1 and shape[:-1] != x.shape[:-1]:
         raise ValueError(f"gate {tuple(shape)} does not broadcast over x {tuple(x.shape)}")
     if wide and gate.stride(-1) != 1:

@@ -173,3 +173,14 @@ def test_packed_structures_have_the_size_that_c_reads(tmp_path):
         fields = form.removesuffix("0q")
         assert _lib.ARGS[name].size == int(size), name
         assert struct.calcsize(fields) - struct.calcsize("@" + fields[-1]) == int(last), name
+
+
+def test_empty_features_are_refused_as_such(monkeypatch):
+    """No features: a ValueError that says so, whatever the gate."""
+    monkeypatch.setattr(ops, "_device_of", lambda t: -1)
+    monkeypatch.setattr(ops, "_raw_stream", lambda i: 0)
+    monkeypatch.setattr(ops, "_cur_device", lambda: -1)
+    x, w = torch.zeros((3, 0), dtype=torch.bfloat16), torch.zeros(0, dtype=torch.bfloat16)
+    for gate in (None, torch.zeros((3, 0), dtype=torch.bfloat16), w, torch.zeros((3, 1), dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="N=0"):
+            ops.gated_add_rmsnorm(x, x, w, 1e-6, gate=gate)
