@@ -128,7 +128,7 @@ def choose_block_m(num_tokens: int, topk: int, num_experts: int) -> int:
     return 128
 
 
-ExpertWeights = Union[AWQExpertWeights, DenseExpertWeights]
+ExpertWeights = Union[AWQExpertWeights, DenseExpertWeights, torch.Tensor]
 
 
 class AWQB200MoeBackend(BaseMoeBackend):
@@ -143,14 +143,13 @@ class AWQB200MoeBackend(BaseMoeBackend):
             raise ValueError(f"activation {activation!r} not supported by the AWQ B200 MoE backend")
         if apply_router_weight_on_input:
             raise ValueError("router weights are applied to the down-projection output only")
-        if isinstance(w1, torch.Tensor) and isinstance(w2, torch.Tensor):
-            w1, w2 = DenseExpertWeights(w1), DenseExpertWeights(w2)
         topk_weights, topk_ids = ops.moe_topk_softmax(gating_output, topk, renormalize)
         return self.experts(hidden_states, w1, w2, topk_weights, topk_ids)
 
     def experts(self, hidden_states: torch.Tensor, w1: ExpertWeights, w2: ExpertWeights,
                 topk_weights: torch.Tensor, topk_ids: torch.Tensor) -> torch.Tensor:
         x = hidden_states
+        w1, w2 = (DenseExpertWeights(w) if isinstance(w, torch.Tensor) else w for w in (w1, w2))
         if not x.is_contiguous():
             raise ValueError("hidden_states must be contiguous")
         if x.dtype != w1.act_dtype or x.dtype != w2.act_dtype:

@@ -12,6 +12,7 @@ import pytest
 import torch
 
 from sglite_b200 import _lib, ops
+from sglite_b200.moe import AWQB200MoeBackend, AWQExpertWeights, DenseExpertWeights
 from sglite_b200.rotary import RotaryEmbedding, rotary_frequencies
 
 
@@ -184,3 +185,24 @@ def test_empty_features_are_refused_as_such(monkeypatch):
     for gate in (None, torch.zeros((3, 0), dtype=torch.bfloat16), w, torch.zeros((3, 1), dtype=torch.bfloat16)):
         with pytest.raises(ValueError, match="N=0"):
             ops.gated_add_rmsnorm(x, x, w, 1e-6, gate=gate)
+
+
+def test_experts_take_plain_tensors_one_by_one(monkeypatch):
+    """Plain [E, N, K] tensors stand for 16-bit experts in both calls, beside
+    DenseExpertWeights too; a plain tensor beside AWQ experts is refused."""
+    seen = []
+    backend = AWQB200MoeBackend()
+    monkeypatch.setattr(backend, "_dense_experts", lambda x, w1, w2, tw, ids: seen.append((w1, w2)) or x)
+    monkeypatch.setattr(ops, "moe_topk_softmax", lambda g, k, r: (torch.zeros(3, k), torch.zeros((3, k), dtype=torch.int32)))
+    x, w1, w2 = (torch.zeros(s, dtype=torch.float16) for s in ((3, 64), (4, 32, 64), (4, 64, 16)))
+    ids = torch.zeros((3, 2), dtype=torch.int32)
+    for a, b in ((w1, w2), (DenseExpertWeights(w1), w2), (w1, DenseExpertWeights(w2))):
+        backend.forward(x, a, b, torch.zeros(3, 4), 2, True)
+        backend.experts(x, a, b, torch.zeros(3, 2), ids)
+    assert len(seen) == 6
+    assert all(isinstance(w, DenseExpertWeights) and w.num_experts == 4 for pair in seen for w in pair)
+    with pytest.raises(ValueError, match="different experts"):  # the plain ones are experts 0 .. 3
+        backend.forward(x, DenseExpertWeights(w1, 4, 8), w2, torch.zeros(3, 8), 2, True)
+    awq = AWQExpertWeights(torch.zeros((1, 16), dtype=torch.uint8), 16, 64, 16, torch.float16)
+    with pytest.raises(ValueError, match="both"):
+        backend.experts(x, w1[:1], awq, torch.zeros(3, 2), ids)
