@@ -276,8 +276,9 @@ int awqb_gated_add_rmsnorm(const awqb_gated_norm_args* args, void* stream);
  *   pair j < rot_dim / 2 of v (elements j and j + rot_dim / 2, or 2j and 2j + 1
  *   if interleaved) turns by the angle positions[m] * inv_freq[j]: (a, b) ->
  *   scale * (a cos - b sin, a sin + b cos); elements from rot_dim on stay.
- * inv_freq is fp64 and the angle is reduced in fp64, so far positions keep
- * their accuracy; a long-context scaling enters through inv_freq and scale.
+ * inv_freq is fp64. The angle is the position times a 64-bit fraction of a turn,
+ * modulo whole turns, so far positions keep their accuracy (2^-24 of a turn at
+ * position 2^29); a long-context scaling enters through inv_freq and scale.
  * positions are int32, or int64 if positions_i64 != 0. A token with a negative
  * position is padding: its outputs are left as they were. Outputs may be the
  * inputs (in place); other overlaps are not allowed. head_dim is a multiple of

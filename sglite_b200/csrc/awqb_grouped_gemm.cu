@@ -19,7 +19,7 @@
 // tokens with two accumulators, so that a tile is stored while the next one is
 // multiplied. (512 features with one accumulator fetch a quarter less from L2, but
 // all pairs then store at the same time and wait for it: 16 % of their time, 806 us
-// against 731 for eight experts of 4096 -> 14336 over 8111 rows.)
+// against 752 in turn for eight experts of 4096 -> 14336 over 8111 rows.)
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -637,7 +637,9 @@ extern "C" int awqb_grouped_gemm(const awqb_grouped_gemm_args* args, void* strea
   AWQB_REQUIRE(p.err != nullptr, kCudaError, "cannot resolve the device error word");
   p.ldo = ldo, p.out_rows = out_rows;
   p.rows = (int)rows, p.E = (int)E, p.K = (int)K, p.N = (int)N, p.n_out = (int)n_out, p.silu = silu_mul != 0;
-  // Measured, few / many in us: 128 experts 2048 -> 1536 at 16, 32, 64 rows per expert
+  // By the rows of the buffer, the only count that the host has: padding and rows of
+  // no group count too, so a buffer with few live rows may take the many-rows kernel
+  // (at most the differences below). Measured, few / many in us: 128 experts 2048 -> 1536 at 16, 32, 64 rows per expert
   // 126 / 129, 141 / 130, 178 / 138; 768 -> 2048 65 / 66, 78 / 67, 100 / 76; eight experts
   // 4096 -> 14336 161 / 167, 158 / 168, 207 / 168.
   const bool many = rows > 24 * E;

@@ -2,8 +2,9 @@
 //
 // Pair j of a head turns by the angle positions[m] * inv_freq[j]. Whole turns do not
 // matter, so the angle is kept as a 64-bit fraction of a turn: inv_freq / 2 pi
-// modulo 1, from fp64, times the position modulo 2^64, one integer product that
-// loses nothing at positions of millions. Its upper 32 bits go to the fp32 sine.
+// modulo 1, times the position modulo 2^64. That integer product is exact; the
+// fraction comes from fp64 and is off by 2^-53 of inv_freq / 2 pi, which the position
+// multiplies (2^-24 of a turn at 2^29). Its upper 32 bits go to the fp32 sine.
 // Nothing is tabulated by position: a token's sines are made once and serve all
 // its heads.
 //
@@ -221,7 +222,8 @@ rotary_vec_kernel(const __grid_constant__ Args a, int64_t M, int lanes, int piec
 
 // A CTA per token, a warp per head, element by element: where the two halves of the
 // turned part do not split into whole vectors (never interleaved pairs, whose vectors
-// hold whole pairs).
+// hold whole pairs). Two bytes per access: 8192 tokens of 32 + 8 heads of 128, 20 of
+// them turned, in place: 135 us, 1.2 TB/s (64 turned, by whole vectors: 44 us).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Args a) {
   __shared__ float cs[kMaxD];

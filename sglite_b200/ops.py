@@ -709,7 +709,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
            k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, q_out: Optional[torch.Tensor] = None,
            k_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Rotary positions of q [M, Hq, D] and k [M, Hk, D] (slices of the merged QKV
-    output will do: any token and head strides), after the per-head RMSNorm when
+    output will do: token and head strides are multiples of 8), after the per-head RMSNorm when
     q_weight / k_weight [D] are given. positions [M] int32 or int64; inv_freq
     float64 [rot_dim / 2] (``rotary.RotaryEmbedding`` makes it, long-context
     scalings included); the first rot_dim elements of a head turn, in pairs
