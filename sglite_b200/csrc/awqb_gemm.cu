@@ -47,6 +47,13 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
         q == cudaDriverEntryPointSuccess)
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
   });
+  // The encoder is a driver call and wants a current context. A host thread that has
+  // made no runtime call yet has none; setting its device to itself binds one.
+  static thread_local bool bound = false;
+  if (!bound) {
+    int dev = 0;
+    bound = cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+  }
   return fn;
 }
 

@@ -7,7 +7,9 @@
 
 namespace awqb {
 
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();  // nullptr if the driver lacks it
+// nullptr if the driver lacks it. Binds the current device's context to the calling
+// thread if it is the thread's first call.
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
 // A row-major matrix of 16-bit values in boxes of box_rows x 64 k, 128-byte swizzle,
 // zeros outside; ld in elements.

@@ -251,3 +251,108 @@ def test_row_parallel_shards_with_adapters_add_up(cuda, dtype, M):
     whole.adapters = adapters
     assert rel_err((parts[0] + parts[1]).float(), whole.forward(x, batch).float().cpu()) <= 1e-2  # that of the GEMM tests
     assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("op", ["gemm 1", "gemm 64", "gemm 600", "grouped few", "grouped many", "lora decode", "lora prompt",
+                                "norm", "rotary", "group_rows", "experts"])
+def test_first_call_of_a_host_thread(cuda, op):
+    """A thread that has made no CUDA call yet has no current context."""
+    import threading
+
+    g = torch.Generator(device=cuda).manual_seed(4)
+    dtype = torch.bfloat16
+
+    def normal(*shape, std=1.0):
+        return (torch.randn(shape, generator=g, device=cuda) * std).to(dtype)
+
+    if op.startswith("gemm"):
+        wq = make_awq_weights(512, 256, 128, dtype, seed=6)
+        layer = RowParallelAWQLinear(AWQB200Config(4, 128, True).get_linear_method(), 512, 256, 1)
+        layer.load({k: v.to(cuda) for k, v in wq.items() if k in ("qweight", "qzeros", "scales")})
+        x = normal(int(op[5:]), 512)
+        call = lambda: layer.forward(x)  # noqa: E731
+    elif op.startswith("grouped"):
+        rows = 9 if op.endswith("few") else 200
+        x, w = normal(rows, 64), normal(2, 64, 64)
+        offsets = torch.tensor([0, rows // 2, rows], dtype=torch.int32, device=cuda)
+        call = lambda: ops.grouped_gemm(x, w, offsets)  # noqa: E731
+    elif op.startswith("lora"):
+        M, N = (9, 64) if op.endswith("decode") else (1200, 16384)
+        x, a, b, base = normal(M, 64), normal(2, 8, 64), normal(2, N, 8), normal(M, N)
+        order, offsets = ops.group_rows(torch.arange(M, device=cuda, dtype=torch.int32) % 2, 2)
+        call = lambda: ops.lora(x, a, b, order, offsets, base)  # noqa: E731
+    elif op == "norm":
+        x, r, w = normal(3, 64), normal(3, 64), normal(64)
+        call = lambda: ops.gated_add_rmsnorm(x, r, w, 1e-6)[0]  # noqa: E731
+    elif op == "rotary":
+        q, pos, inv = normal(3, 2, 64), torch.arange(3, device=cuda), torch.ones(32, dtype=torch.float64, device=cuda)
+        call = lambda: ops.rotary(q, None, pos, inv)[0]  # noqa: E731
+    elif op == "group_rows":
+        ids = torch.arange(30, device=cuda, dtype=torch.int32) % 4
+        call = lambda: ops.group_rows(ids, 4)[0]  # noqa: E731
+    else:
+        x, w1, w2, logits = normal(5, 64), normal(4, 64, 64), normal(4, 64, 32), torch.randn((5, 4), device=cuda)
+        call = lambda: AWQB200MoeBackend().forward(x.clone(), w1, w2, logits, 2, True)  # noqa: E731
+    want, got = call(), []
+    torch.cuda.synchronize()
+
+    def work():
+        try:
+            got.append(call())
+        except BaseException as e:  # compared below
+            got.append(e)
+
+    thread = threading.Thread(target=work)
+    thread.start()
+    thread.join()
+    assert isinstance(got[0], torch.Tensor), got
+    assert torch.equal(got[0], want)
+
+
+def test_two_threads_on_one_stream(cuda):
+    """Each call is several launches that start before the one in front has ended: launches of
+    another thread's call may fall between them, and change nothing."""
+    import threading
+
+    g = torch.Generator(device=cuda).manual_seed(4)
+    dtype = torch.bfloat16
+
+    def normal(*shape, std=1.0):
+        return (torch.randn(shape, generator=g, device=cuda) * std).to(dtype)
+
+    K, N = 512, 256
+    wq = make_awq_weights(K, N, 128, dtype, seed=6)
+    layer = RowParallelAWQLinear(AWQB200Config(4, 128, True).get_linear_method(), K, N, 1)
+    layer.load({k: v.to(cuda) for k, v in wq.items() if k in ("qweight", "qzeros", "scales")})
+    xs, w, offsets = normal(200, K), normal(3, 64, K, std=K ** -0.5), torch.tensor([0, 70, 90, 200], dtype=torch.int32, device=cuda)
+    few, res, weight = normal(9, K), normal(200, K), normal(K)
+
+    def others():
+        return (layer.forward(xs), ops.grouped_gemm(xs, w, offsets), ops.grouped_gemm(few, w, offsets.clamp_max(9)),
+                *ops.gated_add_rmsnorm(xs, res, weight, 1e-6))
+
+    adapted = []
+    for M, n in ((24, 256), (1200, 16384)):  # decode and prompt kernels
+        ids = torch.randint(-1, 4, (M,), generator=g, device=cuda).to(torch.int32)
+        adapted.append((normal(M, K), normal(4, 32, K, std=K ** -0.5), normal(4, n, 32), *ops.group_rows(ids, 4), normal(M, n)))
+
+    def adapters():
+        return tuple(ops.lora(x, a, b, order, off, base) for x, a, b, order, off, base in adapted)
+
+    jobs, failures = [(others, others()), (adapters, adapters())], []
+    torch.cuda.synchronize()
+
+    def work(f, want):
+        try:
+            for _ in range(60):
+                assert all(torch.equal(a, b) for a, b in zip(f(), want))
+        except BaseException as e:  # reported by the test itself
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
+    assert ops.device_error() == 0
