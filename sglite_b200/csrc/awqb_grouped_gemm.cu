@@ -637,9 +637,10 @@ extern "C" int awqb_grouped_gemm(const awqb_grouped_gemm_args* args, void* strea
   AWQB_REQUIRE(p.err != nullptr, kCudaError, "cannot resolve the device error word");
   p.ldo = ldo, p.out_rows = out_rows;
   p.rows = (int)rows, p.E = (int)E, p.K = (int)K, p.N = (int)N, p.n_out = (int)n_out, p.silu = silu_mul != 0;
-  // By the rows of the buffer, the only count that the host has: padding and rows of
-  // no group count too, so a buffer with few live rows may take the many-rows kernel
-  // (at most the differences below). Measured, few / many in us: 128 experts 2048 -> 1536 at 16, 32, 64 rows per expert
+  // By the rows of the buffer, the only count that the host has: padding and rows of no
+  // group count too. A large buffer with few live rows so takes the many-rows kernel,
+  // which costs it 1 to 5 % (128 experts 2048 -> 1536, one row each: 123 / 126 us; eight
+  // 4096 -> 14336: 156 / 161). Measured, few / many in us: 128 experts 2048 -> 1536 at 16, 32, 64 rows per expert
   // 126 / 129, 141 / 130, 178 / 138; 768 -> 2048 65 / 66, 78 / 67, 100 / 76; eight experts
   // 4096 -> 14336 161 / 167, 158 / 168, 207 / 168.
   const bool many = rows > 24 * E;
