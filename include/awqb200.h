@@ -387,6 +387,103 @@ typedef struct {
 int awqb_lora(const awqb_lora_args* args, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Microscaled 4-bit floating point (no counterpart in the reference, whose 4-bit
+ * weights are AWQ int4). e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives) in blocks along K:
+ *   AWQB_FP4_NV: 16 values share an e4m3 scale, a tensor one fp32 scale (null: 1).
+ *     u = x * (1 / scale); block scale s = e4m3(min(max |u| / 6, 448));
+ *     code = e2m1(u / s), 0 where s = 0; the code stands for code * s * scale;
+ *   AWQB_FP4_MX: 32 values share a power of two (e8m0), s = 2^(floor(log2 max |x|)
+ *     - 2), at least 2^-127; code = e2m1(x / s). There is no other scale: scale is null.
+ * Roundings to nearest, ties to even; larger values saturate; a block that holds an
+ * infinity or a NaN gets the scale NaN. K is a multiple of 32.
+ *
+ * Quantised rows: codes [rows][K / 2] bytes, the value with the even k in the lower
+ * four bits; scales [granules][rows][16] bytes, 16 consecutive scales of a row side
+ * by side (granules = ceil(K / 256) for NV, ceil(K / 512) for MX), zero past K.
+ * Pointers are 16-byte aligned, row strides in elements and multiples of 8.
+ */
+enum { AWQB_FP4_NV = 0, AWQB_FP4_MX = 1 };
+/* Row r of the result is x's row r, or with an index (int32 [rows]) x's row
+ * index[r] / per_row; rows whose index is outside x are left as they were, and so are
+ * rows from *count (int32, null: rows) on. dtype is x's. */
+typedef struct {
+  const void* x;
+  int64_t rows_in, ldx, K;
+  int format, dtype;
+  const float* scale;
+  const int32_t* index;
+  int64_t per_row;
+  const int32_t* count;
+  int64_t rows;
+  void* codes;
+  uint8_t* scales;
+} awqb_fp4_quantize_args;
+int awqb_fp4_quantize(const awqb_fp4_quantize_args* args, void* stream);
+/* out[r][k] = code * block scale * scale, rounded to dtype. */
+typedef struct {
+  const void* codes;
+  const uint8_t* scales;
+  int64_t rows, K;
+  int format, dtype;
+  const float* scale;
+  void* out;
+  int64_t ldo;
+} awqb_fp4_dequantize_args;
+int awqb_fp4_dequantize(const awqb_fp4_dequantize_args* args, void* stream);
+/* h = x + residual (stored to residual_out, rounded; residual null: h = x, and
+ * nothing is stored), quantised h * rsqrt(mean(h^2) + eps) * weight, the norm over the
+ * unrounded h and not rounded before its quantisation. residual_out may be residual.
+ * K <= 16384. */
+typedef struct {
+  const void* x;
+  int64_t ldx;
+  const void* residual;
+  int64_t ldr;
+  const void* weight;
+  void* residual_out;
+  int64_t ldro, rows, K;
+  float eps;
+  int format, dtype;
+  const float* scale;
+  void* codes;
+  uint8_t* scales;
+} awqb_fp4_add_rmsnorm_args;
+int awqb_fp4_add_rmsnorm(const awqb_fp4_add_rmsnorm_args* args, void* stream);
+/* y[r] = x_scale * w_scale[e] * x[r] w[e]^T (+ bias) for the rows r of group e, over
+ * quantised rows and weights of one format, fp32 sums. offsets (int32 [E + 1] on the
+ * device, not decreasing) bound the groups; without them (E = 1) all rows are one
+ * group. w [E][N][K / 2] bytes as codes are in rows; w_scales hold tiles of 128
+ * weight rows by four scales, zero past N and K:
+ * [E][ceil(N / 128)][ceil(K / 256)][k tile][32][4][4] bytes, where k tile is 0..3 (NV: 64 k) or 0..1
+ * (MX: 128 k) and rows r, r + 32, r + 64 and r + 96 of a tile stand side by side.
+ * x_scale fp32 [1], w_scale fp32 [E], or null. bias [N] in dtype, E = 1 only.
+ * silu_mul: w's rows are gate and up by turns; y = silu(gate) * up, [.., N / 2].
+ * y[r] goes to row r of out, or to row_map[r] (rows that map outside 0..out_rows - 1
+ * are dropped, no two to one), times row_scale[its row of out] if given; rows of out
+ * that nothing maps to are left as they were. N is a multiple of 8 (16 with
+ * silu_mul), ldo of 8. E <= 1024. out must not overlap the inputs. */
+typedef struct {
+  const void* codes;
+  const uint8_t* scales;
+  int64_t rows, K;
+  const void* w;
+  const uint8_t* w_scales;
+  int64_t E, N;
+  const int32_t* offsets;
+  int format, dtype;
+  const float* x_scale;
+  const float* w_scale;
+  const void* bias;
+  int silu_mul;
+  const int32_t* row_map;
+  const float* row_scale;
+  void* out;
+  int64_t out_rows, ldo;
+} awqb_fp4_gemm_args;
+int awqb_fp4_gemm(const awqb_fp4_gemm_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
  * Tensor-parallel all-reduce. Replaces NCCLWrapper (create_nccl_uid, ctor,
  * all_reduce), kernels/csrc/src/pynccl.cu:75-189, used through
  * PyNCCLDistributedImpl.all_reduce, srt/distributed/communicator.py:62-65.

@@ -33,6 +33,8 @@ SOURCES = [
     "awqb_group.cu",
     "awqb_grouped_gemm.cu",
     "awqb_lora.cu",
+    "awqb_fp4_rows.cu",
+    "awqb_fp4_gemm.cu",
     "awqb_nccl.cpp",
 ]
 

@@ -71,6 +71,10 @@ _SIGNATURES = {
     "awqb_grouped_gemm": (c_int, [ctypes.c_char_p, c_vp]),
     "awqb_lora_workspace_bytes": (c_int, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64p]),
     "awqb_lora": (c_int, [ctypes.c_char_p, c_vp]),
+    "awqb_fp4_quantize": (c_int, [ctypes.c_char_p, c_vp]),
+    "awqb_fp4_dequantize": (c_int, [ctypes.c_char_p, c_vp]),
+    "awqb_fp4_add_rmsnorm": (c_int, [ctypes.c_char_p, c_vp]),
+    "awqb_fp4_gemm": (c_int, [ctypes.c_char_p, c_vp]),
     "awqb_moe_topk_sum": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_vp, c_vp]),
     "awqb_nccl_unique_id_bytes": (c_int, []),
     "awqb_nccl_get_unique_id": (c_int, [c_vp]),
@@ -101,6 +105,14 @@ ARGS = {
     "awqb_rotary": struct.Struct("@PqqqPqqqPiPqqqifPPfPqqPqqi0q"),
     "awqb_grouped_gemm": struct.Struct("@PqqPqqqPiiPPPqq0q"),
     "awqb_lora": struct.Struct("@PqqqPPqqqqqqqqPPPPqPqiPq0q"),
+}
+
+# The same for the entry points of microscaled 4-bit floating point.
+FP4_ARGS = {
+    "awqb_fp4_quantize": struct.Struct("@PqqqiiPPqPqPP0q"),
+    "awqb_fp4_dequantize": struct.Struct("@PPqqiiPPq0q"),
+    "awqb_fp4_add_rmsnorm": struct.Struct("@PqPqPPqqqfiiPPP0q"),
+    "awqb_fp4_gemm": struct.Struct("@PPqqPPqqPiiPPPiPPPqq0q"),
 }
 
 _lock = threading.Lock()

@@ -52,12 +52,14 @@ __device__ __forceinline__ Tile find_tile(const Groups& g, const P& p, int t) {
   return r;
 }
 
-// Builds the tables of the groups from the offsets (clamped to the rows); all
-// threads, with a barrier still to come before they are read.
+// Builds the tables of the groups from the offsets (clamped to the rows; without
+// offsets, one group of all rows); all threads, with a barrier still to come before
+// they are read.
 template <typename C, typename P>
 __device__ __forceinline__ void build_groups(const Groups& g, const P& p) {
   for (int e = threadIdx.x; e < p.E; e += C::kThreads) {
-    const int r0 = min(max(p.offsets[e], 0), p.rows), r1 = min(max(p.offsets[e + 1], 0), p.rows);
+    const int r0 = p.offsets ? min(max(p.offsets[e], 0), p.rows) : 0;
+    const int r1 = p.offsets ? min(max(p.offsets[e + 1], 0), p.rows) : p.rows;
     g.row0[e] = r0;
     g.row0[p.E + e] = max(r1 - r0, 0);
   }

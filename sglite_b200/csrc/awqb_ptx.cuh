@@ -466,6 +466,56 @@ __device__ __forceinline__ void tma_load_4d_pair(uint32_t dst, const void* tmap,
       "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar), "l"(policy)
       : "memory");
 }
+// ---------------------------------------------------------------- block-scaled 4-bit products
+// Instruction descriptor of e2m1 operands with a scale per block along K, fp32
+// accumulation, both operands K-major: kNv, an e4m3 scale for 16 values; else an e8m0
+// scale for 32. The second format's two scales of an instruction's 64 k are half a
+// word of tensor memory; `half` says which.
+__host__ __device__ constexpr uint32_t make_idesc_fp4(int m, int n, bool nv, int half) {
+  return ((uint32_t)(2 * half) << 4)      // B scales: byte of the word
+         | (1u << 7)                      // A format: e2m1
+         | (1u << 10)                     // B format: e2m1
+         | ((uint32_t)(n >> 3) << 17)     // N >> 3
+         | ((nv ? 0u : 1u) << 23)         // scale format: e4m3 or e8m0
+         | ((uint32_t)(m >> 7) << 27)     // M >> 7
+         | ((uint32_t)(2 * half) << 29);  // A scales: byte of the word
+}
+// D[tmem] (+)= A[smem] * B[smem]^T over 64 k, A's and B's scales in tensor memory.
+#define AWQB_FP4_MMA(group, kind, vec)                                                                         \
+  asm volatile(                                                                                                \
+      "{\n\t.reg .pred p;\n\t"                                                                                 \
+      "setp.ne.b32 p, %6, 0;\n\t"                                                                              \
+      "tcgen05.mma.cta_group::" group ".kind::" kind ".block_scale.scale_vec::" vec                            \
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),                                                  \
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)                      \
+      : "memory")
+template <bool kNv, bool kPair>
+__device__ __forceinline__ void tc_mma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t a_scales, uint32_t b_scales, uint32_t accumulate) {
+  if (kNv && kPair)
+    AWQB_FP4_MMA("2", "mxf4nvf4", "4X");
+  else if (kNv)
+    AWQB_FP4_MMA("1", "mxf4nvf4", "4X");
+  else if (kPair)
+    AWQB_FP4_MMA("2", "mxf4", "2X");
+  else
+    AWQB_FP4_MMA("1", "mxf4", "2X");
+}
+#undef AWQB_FP4_MMA
+// 32 rows of 16 bytes from shared to tensor memory (four columns), the same for each
+// quarter of its lanes; for a pair, in both CTAs. In order with the products that the
+// same thread issues afterwards.
+template <bool kPair>
+__device__ __forceinline__ void tc_copy_scales(uint32_t d_tmem, uint32_t smem_addr) {
+  // no swizzle, K-major: 8-row groups 128 bytes apart
+  const uint64_t desc = (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)(128u >> 4) << 16 |
+                        (uint64_t)(128u >> 4) << 32 | (uint64_t)1 << 46;
+  if (kPair)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(d_tmem), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(d_tmem), "l"(desc) : "memory");
+}
+
 // Arrive on a barrier anywhere in the cluster (a shared::cluster address).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");

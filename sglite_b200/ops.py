@@ -15,7 +15,7 @@ from typing import Dict, Optional, Tuple
 
 import torch
 
-from ._lib import ARGS, c_i64, call, check, lib
+from ._lib import ARGS, FP4_ARGS, c_i64, call, check, lib
 
 DTYPE_CODE = {torch.float16: 0, torch.bfloat16: 1}
 
@@ -571,7 +571,8 @@ def _entry(name: str):
     """(C function, packer of its argument structure)."""
     fn = _FN.get(name)
     if fn is None:
-        fn = _FN[name] = (getattr(lib(), name), ARGS[name].pack if name in ARGS else None)
+        layout = ARGS.get(name) or FP4_ARGS.get(name)
+        fn = _FN[name] = (getattr(lib(), name), layout.pack if layout else None)
     return fn
 
 
@@ -797,6 +798,23 @@ def group_rows(ids: torch.Tensor, num_groups: int, begin: int = 0) -> Tuple[torc
     return order, offsets
 
 
+def _row_map_scale(row_map: Optional[torch.Tensor], row_scale: Optional[torch.Tensor], rows: int, out_rows: int,
+                   di: int) -> Tuple[int, int]:
+    """Pointers of a grouped product's row_map and row_scale, checked."""
+    pm = ps = 0
+    if row_map is not None:
+        if row_map.dtype != torch.int32 or row_map.numel() != rows or not row_map.is_contiguous() \
+                or row_map.get_device() != di:
+            raise ValueError("row_map must be a contiguous int32 [rows] tensor on x's device")
+        pm = row_map.data_ptr()
+    if row_scale is not None:
+        if row_scale.dtype != torch.float32 or row_scale.numel() != out_rows or not row_scale.is_contiguous() \
+                or row_scale.get_device() != di:
+            raise ValueError("row_scale must be a contiguous float32 tensor on x's device, one value per row of out")
+        ps = row_scale.data_ptr()
+    return pm, ps
+
+
 def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out: Optional[torch.Tensor] = None,
                  silu_mul: bool = False, row_map: Optional[torch.Tensor] = None,
                  row_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -828,17 +846,7 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out
     elif out.dim() != 2 or out.shape[1] != n_out or out.dtype != dtype or out.get_device() != di:
         raise ValueError(f"out must be a [rows, {n_out}] tensor of x's dtype on its device")
     out_rows = out.shape[0]
-    pm = ps = 0
-    if row_map is not None:
-        if row_map.dtype != torch.int32 or row_map.numel() != rows or not row_map.is_contiguous() \
-                or row_map.get_device() != di:
-            raise ValueError("row_map must be a contiguous int32 [rows] tensor on x's device")
-        pm = row_map.data_ptr()
-    if row_scale is not None:
-        if row_scale.dtype != torch.float32 or row_scale.numel() != out_rows or not row_scale.is_contiguous() \
-                or row_scale.get_device() != di:
-            raise ValueError("row_scale must be a contiguous float32 tensor on x's device, one value per row of out")
-        ps = row_scale.data_ptr()
+    pm, ps = _row_map_scale(row_map, row_scale, rows, out_rows, di)
     fn, pack = _entry("awqb_grouped_gemm")
     _run(fn, di, pack(x.data_ptr(), rows, _row_stride(x, K, "x"), w.data_ptr(), E, K, N, offsets.data_ptr(), code,
                       silu_mul, pm, ps, out.data_ptr(), out_rows, _row_stride(out, n_out, "out")))
@@ -905,4 +913,245 @@ def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, order: torch.Tensor,
     _run(fn, di, pack(x.data_ptr(), M, _row_stride(x, K, "x"), K, a.data_ptr(), b.data_ptr(), L, rank, N, parts, w[0], w[1],
                       w[2], w[3], order.data_ptr(), offsets.data_ptr(), ps, base.data_ptr(),
                       _row_stride(base, N, "base"), out.data_ptr(), _row_stride(out, N, "out"), code, ws.data_ptr(), nb))
+    return out
+
+
+# ---------------------------------------------------------------- microscaled 4-bit floating point
+# Values of a block of 4-bit numbers, codes of the formats and their blocks.
+FP4_FORMATS = {"nvfp4": 0, "mxfp4": 1}
+FP4_BLOCK = {"nvfp4": 16, "mxfp4": 32}
+
+
+def _fp4_format(fmt: str) -> int:
+    code = FP4_FORMATS.get(fmt)
+    if code is None:
+        raise ValueError(f"4-bit format {fmt!r}: one of {tuple(FP4_FORMATS)}")
+    return code
+
+
+def _fp4_scale(scale: Optional[torch.Tensor], n: int, fmt: str, di: int, name: str) -> int:
+    """Pointer of an fp32 scale of n values, 0 without one."""
+    if scale is None:
+        return 0
+    if fmt != "nvfp4":
+        raise ValueError(f"{name}: only nvfp4 has a scale beside its blocks' scales")
+    if scale.dtype != torch.float32 or scale.numel() != n or not scale.is_contiguous() or scale.get_device() != di:
+        raise ValueError(f"{name} must be a contiguous float32 [{n}] tensor on the same device")
+    return scale.data_ptr()
+
+
+def fp4_rows_empty(rows: int, K: int, fmt: str, device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Room for ``rows`` quantised rows of K values: codes uint8 [rows, K / 2] and scales
+    uint8 [granules, rows, 16], 16 scales of a row side by side (256 k of nvfp4, 512 of mxfp4)."""
+    granules = -(-K // (16 * FP4_BLOCK[fmt]))
+    return (torch.empty((rows, K // 2), dtype=torch.uint8, device=device),
+            torch.empty((granules, rows, 16), dtype=torch.uint8, device=device))
+
+
+def _fp4_rows(codes: torch.Tensor, scales: torch.Tensor, fmt: str, di: int) -> Tuple[int, int]:
+    """(rows, K) of quantised rows, checked."""
+    if codes.dim() != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous() or codes.get_device() != di:
+        raise ValueError("codes must be a contiguous uint8 [rows, K / 2] CUDA tensor")
+    rows, half = codes.shape
+    K = 2 * half
+    if scales.shape != (-(-K // (16 * FP4_BLOCK[fmt])), rows, 16) or scales.dtype != torch.uint8 \
+            or not scales.is_contiguous() or scales.get_device() != di:
+        raise ValueError(f"scales {tuple(scales.shape)} must be the contiguous uint8 [granules, rows, 16] tensor of "
+                         f"{rows} {fmt} rows of K={K}, on the codes' device")
+    return rows, K
+
+
+def fp4_quantize(x: torch.Tensor, fmt: str, *, scale: Optional[torch.Tensor] = None,
+                 index: Optional[torch.Tensor] = None, per_row: int = 1, count: Optional[torch.Tensor] = None,
+                 out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows of x [.., K] (fp16 or bf16, K a multiple of 32) in 4 bits: (codes, scales), as
+    ``fp4_rows_empty`` shapes them. fmt "nvfp4": blocks of 16 with an e4m3 scale each, and
+    ``scale`` (fp32 [1], positive; 1 without) for all: a code stands for code * block
+    scale * scale. "mxfp4": blocks of 32 with a power of two each. Roundings to nearest,
+    ties to even; what is too large saturates; a block that holds an infinity or a NaN gets
+    the scale NaN.
+
+    index (int32 [rows]): row r is x's row index[r] // per_row (an expert-sorted list of
+    (token, choice) pairs, with per_row choices a token); rows whose index is outside x, and
+    rows from ``count`` (int32 [1], on the device) on, are left as they were."""
+    code = _dtype_code(x.dtype)
+    fc = _fp4_format(fmt)
+    di = _device_of(x)
+    if x.dim() == 0:
+        raise ValueError("x must have rows of K values")
+    K = x.shape[-1]
+    rows_in = x.numel() // K if K else 0
+    pi = pc = 0
+    rows = rows_in
+    if index is not None:
+        if index.dtype != torch.int32 or index.dim() != 1 or not index.is_contiguous() or index.get_device() != di:
+            raise ValueError("index must be a contiguous int32 [rows] tensor on x's device")
+        pi, rows = index.data_ptr(), index.numel()
+    elif per_row != 1:
+        raise ValueError("per_row needs an index")
+    if count is not None:
+        if count.dtype != torch.int32 or count.numel() != 1 or count.get_device() != di:
+            raise ValueError("count must be an int32 [1] tensor on x's device")
+        pc = count.data_ptr()
+    ps = _fp4_scale(scale, 1, fmt, di, "scale")
+    if out is None:
+        out = fp4_rows_empty(rows, K, fmt, x.device)
+    elif _fp4_rows(out[0], out[1], fmt, di) != (rows, K):
+        raise ValueError(f"out must hold {rows} rows of K={K}")
+    fn, pack = _entry("awqb_fp4_quantize")
+    _run(fn, di, pack(x.data_ptr(), rows_in, _row_stride(x, K, "x"), K, fc, code, ps, pi, per_row, pc, rows,
+                      out[0].data_ptr(), out[1].data_ptr()))
+    return out
+
+
+def fp4_dequantize(codes: torch.Tensor, scales: torch.Tensor, fmt: str, dtype: torch.dtype, *,
+                   scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The values [rows, K] that quantised rows stand for, rounded to ``dtype``."""
+    code = _dtype_code(dtype)
+    fc = _fp4_format(fmt)
+    di = _device_of(codes)
+    rows, K = _fp4_rows(codes, scales, fmt, di)
+    if out is None:
+        out = torch.empty((rows, K), dtype=dtype, device=codes.device)
+    elif out.shape != (rows, K) or out.dtype != dtype or out.get_device() != di:
+        raise ValueError(f"out must be a [{rows}, {K}] tensor of {dtype} on the codes' device")
+    fn, pack = _entry("awqb_fp4_dequantize")
+    _run(fn, di, pack(codes.data_ptr(), scales.data_ptr(), rows, K, fc, code, _fp4_scale(scale, 1, fmt, di, "scale"),
+                      out.data_ptr(), _row_stride(out, K, "out")))
+    return out
+
+
+def fp4_add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float, fmt: str, *,
+                    scale: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None,
+                    out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The residual-add RMSNorm in front of a 4-bit projection: h = x + residual,
+    y = h * rsqrt(mean(h^2) + eps) * weight, quantised as ``fp4_quantize`` does, straight
+    from fp32. Returns (codes, scales, h), h rounded to x's dtype; without a residual h is x.
+    ``residual_out`` may be residual (in place) or x. K is at most 16384."""
+    dtype = x.dtype
+    code = _dtype_code(dtype)
+    fc = _fp4_format(fmt)
+    di = _device_of(x)
+    if x.dim() == 0:
+        raise ValueError("x must have rows of K values")
+    K = x.shape[-1]
+    rows = x.numel() // K if K else 0
+    if weight.numel() != K or weight.dtype != dtype or not weight.is_contiguous() or weight.get_device() != di:
+        raise ValueError("weight must be a contiguous [K] tensor in the activation dtype on x's device")
+    pr = po = ldr = ldo = 0
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != dtype or residual.get_device() != di:
+            raise ValueError("residual must have the shape, dtype and device of x")
+        if residual_out is None:
+            residual_out = torch.empty_like(residual)
+        elif residual_out.shape != x.shape or residual_out.dtype != dtype or residual_out.get_device() != di:
+            raise ValueError("residual_out must have the shape, dtype and device of residual")
+        pr, ldr = residual.data_ptr(), _row_stride(residual, K, "residual")
+        po, ldo = residual_out.data_ptr(), _row_stride(residual_out, K, "residual_out")
+    elif residual_out is not None:
+        raise ValueError("residual_out needs residual")
+    ps = _fp4_scale(scale, 1, fmt, di, "scale")
+    if out is None:
+        out = fp4_rows_empty(rows, K, fmt, x.device)
+    elif _fp4_rows(out[0], out[1], fmt, di) != (rows, K):
+        raise ValueError(f"out must hold {rows} rows of K={K}")
+    fn, pack = _entry("awqb_fp4_add_rmsnorm")
+    _run(fn, di, pack(x.data_ptr(), _row_stride(x, K, "x"), pr, ldr, weight.data_ptr(), po, ldo, rows, K, eps, fc, code,
+                      ps, out[0].data_ptr(), out[1].data_ptr()))
+    return out[0], out[1], (x if residual is None else residual_out)
+
+
+def fp4_lay_out_scales(scales: torch.Tensor, fmt: str) -> torch.Tensor:
+    """A weight's block scales [.., N, K / 16 (nvfp4) or K / 32 (mxfp4)], as bytes in the
+    order of a checkpoint, laid out for the tensor cores (once, at load): uint8
+    [.., ceil(N / 128), ceil(K / 256), 4 or 2, 32, 4, 4], tiles of 128 rows by four scales,
+    rows r, r + 32, r + 64 and r + 96 of a tile side by side, zero past N and K."""
+    _fp4_format(fmt)
+    if scales.dim() < 2 or scales.element_size() != 1:
+        raise ValueError("scales must be one-byte values [.., N, K / block]")
+    s = scales.view(torch.uint8)
+    lead, (N, n) = s.shape[:-2], s.shape[-2:]
+    per = 256 // FP4_BLOCK[fmt]  # scales of a stage of 256 k
+    s = torch.nn.functional.pad(s, (0, -n % per, 0, -N % 128))
+    s = s.reshape(*lead, s.shape[-2] // 128, 4, 32, s.shape[-1] // per, per // 4, 4)
+    d = len(lead)
+    return s.permute(*range(d), d, d + 3, d + 4, d + 2, d + 1, d + 5).contiguous()
+
+
+def _fp4_weight(w: torch.Tensor, w_scales: torch.Tensor, K: int, fmt: str, di: int) -> int:
+    """N of quantised weights [.., N, K / 2], checked with their laid-out scales."""
+    if w.dtype != torch.uint8 or w.shape[-1] * 2 != K or not w.is_contiguous() or w.get_device() != di:
+        raise ValueError(f"w {tuple(w.shape)} must be a contiguous uint8 [.., N, K / 2] tensor, K={K}, on the rows' device")
+    N = w.shape[-2]
+    want = (*w.shape[:-2], -(-N // 128), -(-K // 256), 64 // FP4_BLOCK[fmt], 32, 4, 4)
+    if w_scales.shape != want or w_scales.dtype != torch.uint8 or not w_scales.is_contiguous() \
+            or w_scales.get_device() != di:
+        raise ValueError(f"w_scales {tuple(w_scales.shape)} must be {want}: fp4_lay_out_scales of the weight's scales")
+    return N
+
+
+def fp4_gemm(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, fmt: str,
+             dtype: torch.dtype, *, x_scale: Optional[torch.Tensor] = None, w_scale: Optional[torch.Tensor] = None,
+             bias: Optional[torch.Tensor] = None, silu_mul: bool = False, out: Optional[torch.Tensor] = None
+             ) -> torch.Tensor:
+    """y = x @ w.T (+ bias) of quantised rows (codes, scales) and a quantised weight w uint8
+    [N, K / 2] with ``fp4_lay_out_scales``'s w_scales, both of format fmt, fp32 sums,
+    rounded to ``dtype``; x_scale, w_scale: their fp32 [1] scales (nvfp4). silu_mul: w's
+    rows (and bias) are gate and up by turns, y = silu(gate) * up [rows, N / 2]."""
+    code = _dtype_code(dtype)
+    fc = _fp4_format(fmt)
+    di = _device_of(codes)
+    rows, K = _fp4_rows(codes, scales, fmt, di)
+    if w.dim() != 2:
+        raise ValueError("w must be a [N, K / 2] tensor")
+    N = _fp4_weight(w, w_scales, K, fmt, di)
+    pb = 0
+    if bias is not None:
+        if bias.dtype != dtype or bias.numel() != N or not bias.is_contiguous() or bias.get_device() != di:
+            raise ValueError(f"bias must be a contiguous [{N}] tensor of {dtype} on the rows' device")
+        pb = bias.data_ptr()
+    n_out = N // 2 if silu_mul else N
+    if out is None:
+        out = torch.empty((rows, n_out), dtype=dtype, device=codes.device)
+    elif out.shape != (rows, n_out) or out.dtype != dtype or out.get_device() != di:
+        raise ValueError(f"out must be a [{rows}, {n_out}] tensor of {dtype} on the rows' device")
+    fn, pack = _entry("awqb_fp4_gemm")
+    _run(fn, di, pack(codes.data_ptr(), scales.data_ptr(), rows, K, w.data_ptr(), w_scales.data_ptr(), 1, N, 0, fc, code,
+                      _fp4_scale(x_scale, 1, fmt, di, "x_scale"), _fp4_scale(w_scale, 1, fmt, di, "w_scale"), pb,
+                      silu_mul, 0, 0, out.data_ptr(), rows, _row_stride(out, n_out, "out")))
+    return out
+
+
+def fp4_grouped_gemm(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
+                     offsets: torch.Tensor, fmt: str, dtype: torch.dtype, *, x_scale: Optional[torch.Tensor] = None,
+                     w_scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, silu_mul: bool = False,
+                     row_map: Optional[torch.Tensor] = None, row_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``fp4_gemm`` grouped by expert: ``y[r] = x[r] @ w[e].T`` for ``offsets[e] <= r <
+    offsets[e + 1]``, w uint8 [E, N, K / 2], w_scale fp32 [E] (nvfp4). offsets, out,
+    row_map and row_scale as in ``grouped_gemm``; with silu_mul w's rows are gate and up
+    by turns."""
+    code = _dtype_code(dtype)
+    fc = _fp4_format(fmt)
+    di = _device_of(codes)
+    rows, K = _fp4_rows(codes, scales, fmt, di)
+    if w.dim() != 3:
+        raise ValueError("w must be a [E, N, K / 2] tensor")
+    N = _fp4_weight(w, w_scales, K, fmt, di)
+    E = w.shape[0]
+    if offsets.dtype != torch.int32 or offsets.numel() != E + 1 or not offsets.is_contiguous() \
+            or offsets.get_device() != di:
+        raise ValueError("offsets must be a contiguous int32 [experts + 1] tensor on the rows' device")
+    n_out = N // 2 if silu_mul else N
+    if out is None:
+        out = torch.empty((rows, n_out), dtype=dtype, device=codes.device)
+    elif out.dim() != 2 or out.shape[1] != n_out or out.dtype != dtype or out.get_device() != di:
+        raise ValueError(f"out must be a [rows, {n_out}] tensor of {dtype} on the rows' device")
+    out_rows = out.shape[0]
+    pm, ps = _row_map_scale(row_map, row_scale, rows, out_rows, di)
+    fn, pack = _entry("awqb_fp4_gemm")
+    _run(fn, di, pack(codes.data_ptr(), scales.data_ptr(), rows, K, w.data_ptr(), w_scales.data_ptr(), E, N,
+                      offsets.data_ptr(), fc, code, _fp4_scale(x_scale, 1, fmt, di, "x_scale"),
+                      _fp4_scale(w_scale, E, fmt, di, "w_scale"), 0, silu_mul, pm, ps, out.data_ptr(), out_rows,
+                      _row_stride(out, n_out, "out")))
     return out

@@ -1,0 +1,216 @@
+"""Microscaled 4-bit floating point without a GPU: the oracle's own formats, the layout
+of weight scales, argument structures and refusals. Every refusal of the C entry points
+comes before any GPU work, so made-up addresses are never read."""
+
+import os
+import struct
+import subprocess
+
+import pytest
+import torch
+
+from oracle.fp4_ref import BLOCK, E4M3, GRID, nearest, pack, quantize_ref, values_ref
+from sglite_b200 import _lib, ops
+
+P = 256  # an aligned address that nothing reads
+
+
+def _refused(name, args, change, text):
+    args = list(args)
+    for k, v in change.items():
+        args[int(k[1:])] = v
+    fn = getattr(_lib.lib(), name)
+    assert fn(_lib.FP4_ARGS[name].pack(*(0 if v is None else v for v in args)), None) == 1
+    assert text in _lib.lib().awqb_last_error()
+
+
+Q = [P, 8, 256, 256, 0, 1, P, None, 1, None, 8, P, P]
+
+
+@pytest.mark.parametrize("change,text", [
+    ({"_3": 240}, b"K="), ({"_3": 0}, b"K="), ({"_3": -32}, b"K="), ({"_4": 2}, b"format"), ({"_4": -1}, b"format"),
+    ({"_5": 2}, b"dtype"), ({"_2": 248}, b"row stride"), ({"_2": 260}, b"row stride"), ({"_10": 9}, b"index"),
+    ({"_1": -1, "_10": -1}, b"rows"), ({"_8": 0, "_7": P}, b"per_row"), ({"_0": None}, b"null"), ({"_11": None}, b"null"),
+    ({"_12": None}, b"null"), ({"_0": 8}, b"16-byte"), ({"_11": 8}, b"16-byte"), ({"_12": 8}, b"16-byte"),
+    ({"_4": 1}, b"scale")])
+def test_quantize_refusals(change, text):
+    _refused("awqb_fp4_quantize", Q, change, text)
+
+
+D = [P, P, 8, 256, 0, 1, P, P, 256]
+
+
+@pytest.mark.parametrize("change,text", [
+    ({"_3": 48}, b"K="), ({"_4": 7}, b"format"), ({"_5": -1}, b"dtype"), ({"_8": 252}, b"row stride"), ({"_8": 8}, b"row stride"),
+    ({"_2": -1}, b"rows"), ({"_0": None}, b"null"), ({"_1": None}, b"null"), ({"_7": None}, b"null"), ({"_7": 24}, b"16-byte"),
+    ({"_4": 1}, b"scale")])
+def test_dequantize_refusals(change, text):
+    _refused("awqb_fp4_dequantize", D, change, text)
+
+
+NORM = [P, 256, P, 256, P, P, 256, 8, 256, 1e-6, 0, 1, P, P, P]
+
+
+@pytest.mark.parametrize("change,text", [
+    ({"_8": 250}, b"K="), ({"_8": 16416, "_1": 16416, "_3": 16416, "_6": 16416}, b"at most"), ({"_1": 8}, b"row strides"),
+    ({"_3": 255}, b"row strides"), ({"_6": 0}, b"row strides"), ({"_9": -1.0}, b"eps"), ({"_9": float("nan")}, b"eps"),
+    ({"_10": 3}, b"format"), ({"_11": 3}, b"dtype"), ({"_0": None}, b"null"), ({"_4": None}, b"null"),
+    ({"_5": None}, b"null"), ({"_13": None}, b"null"), ({"_14": None}, b"null"), ({"_4": 8}, b"16-byte"), ({"_7": -1}, b"rows"),
+    ({"_10": 1}, b"scale")])
+def test_add_rmsnorm_refusals(change, text):
+    _refused("awqb_fp4_add_rmsnorm", NORM, change, text)
+
+
+G = [P, P, 64, 256, P, P, 8, 512, P, 0, 1, P, P, None, 0, None, None, P, 64, 512]
+
+
+@pytest.mark.parametrize("change,text", [
+    ({"_3": 264}, b"K="), ({"_3": 0}, b"K="), ({"_7": 516}, b"N="), ({"_7": 0}, b"N="), ({"_7": 520, "_14": 1}, b"multiple of 16"),
+    ({"_6": 0}, b"experts"), ({"_6": 1025}, b"experts"), ({"_8": None}, b"offsets"), ({"_13": P}, b"bias"),
+    ({"_19": 504}, b"row stride"), ({"_19": 516}, b"row stride"), ({"_18": 63}, b"out has"), ({"_2": -1}, b"row count"),
+    ({"_9": 2}, b"format"), ({"_10": 2}, b"dtype"), ({"_0": None}, b"null"), ({"_1": None}, b"null"), ({"_4": None}, b"null"),
+    ({"_5": None}, b"null"), ({"_17": None}, b"null"), ({"_0": 8}, b"16-byte"), ({"_1": 8}, b"16-byte"), ({"_4": 8}, b"16-byte"),
+    ({"_5": 8}, b"16-byte"), ({"_17": 8}, b"16-byte"), ({"_7": 1 << 29}, b"N="), ({"_9": 1}, b"scale")])
+def test_gemm_refusals(change, text):
+    _refused("awqb_fp4_gemm", G, change, text)
+
+
+def test_null_arguments_are_refused():
+    for name in _lib.FP4_ARGS:
+        assert getattr(_lib.lib(), name)(None, None) == 1
+
+
+def test_packed_structures_have_the_size_that_c_reads(tmp_path):
+    names = {n: (f"{n}_args", last) for n, last in
+             (("awqb_fp4_quantize", "scales"), ("awqb_fp4_dequantize", "ldo"), ("awqb_fp4_add_rmsnorm", "scales"),
+              ("awqb_fp4_gemm", "ldo"))}
+    assert set(names) == set(_lib.FP4_ARGS)
+    lines = [f'printf("{k} %zu %zu\\n", sizeof({t}), offsetof({t}, {last}));' for k, (t, last) in names.items()]
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "awqb200.h"\nint main(void) {\n' + "\n".join(lines)
+                   + "\nreturn 0;\n}\n")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-I", include, str(src), "-o", str(tmp_path / "sizes")], check=True)
+    for line in subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout.splitlines():
+        name, size, last = line.split()
+        fields = _lib.FP4_ARGS[name].format.removesuffix("0q")
+        assert _lib.FP4_ARGS[name].size == int(size), name
+        assert struct.calcsize(fields) - struct.calcsize("@" + fields[-1]) == int(last), name
+
+
+# ---------------------------------------------------------------- the oracle and the layouts
+def test_oracle_formats():
+    assert torch.equal(E4M3.float(), torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).float())
+    v = torch.tensor([0.25, 0.2500001, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 5.0000001, 100.0], dtype=torch.float64)
+    assert GRID[nearest(v, GRID)].tolist() == [0, 0.5, 1, 1, 2, 2, 4, 4, 6, 6]
+    s = torch.rand(5000, dtype=torch.float64) * 448
+    assert torch.equal(E4M3[nearest(s.float().double(), E4M3)].float(), s.float().to(torch.float8_e4m3fn).float())
+    for fmt in BLOCK:
+        x = torch.randn(7, 96) * 3
+        values, byte = quantize_ref(x, fmt)
+        assert torch.equal(values_ref(pack(values, byte, fmt), byte, fmt), values)
+        assert float((values - x).norm() / x.norm()) < 0.2
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("shape", [(8, 32), (128, 256), (200, 800), (3, 136, 96)])
+def test_laid_out_scales(fmt, shape):
+    N, K = shape[-2:]
+    b = BLOCK[fmt]
+    s = torch.randint(1, 256, (*shape[:-1], K // b), dtype=torch.uint8)
+    t = ops.fp4_lay_out_scales(s, fmt)
+    assert t.shape == (*shape[:-2], -(-N // 128), -(-K // 256), 64 // b, 32, 4, 4) and t.is_contiguous()
+    flat, want = t.reshape(-1, *t.shape[len(shape) - 2:]), s.reshape(-1, N, K // b)
+    n, k = torch.meshgrid(torch.arange(N), torch.arange(K // b), indexing="ij")
+    k0 = k * b
+    got = flat[:, n // 128, k0 // 256, k0 % 256 // (4 * b), n % 32, n % 128 // 32, k % 4]
+    assert torch.equal(got, want)
+    assert int(t.count_nonzero()) == s.numel()  # zero everywhere else
+    assert torch.equal(ops.fp4_lay_out_scales(s.view(torch.int8), fmt), t)
+
+
+@pytest.mark.parametrize("bad", [torch.zeros(4, dtype=torch.uint8), torch.zeros((4, 4))])
+def test_scales_to_lay_out_are_bytes(bad):
+    with pytest.raises(ValueError):
+        ops.fp4_lay_out_scales(bad, "nvfp4")
+
+
+# ---------------------------------------------------------------- refusals of the wrappers
+@pytest.fixture
+def here(monkeypatch):
+    """Lets CPU tensors pass for CUDA ones up to the call itself, which must not be reached."""
+    def reached(*a):
+        raise AssertionError("the call was made")
+    monkeypatch.setattr(ops, "_device_of", lambda t: -1)
+    monkeypatch.setattr(ops, "_run", reached)
+
+
+def _rows(M, K, fmt):
+    c, s = ops.fp4_rows_empty(M, K, fmt, "cpu")
+    return c.zero_(), s.zero_()
+
+
+def test_wrappers_refuse(here):
+    T = torch.bfloat16
+    x = torch.zeros((4, 64), dtype=T)
+    one = torch.ones(1)
+    i32 = torch.zeros(4, dtype=torch.int32)
+    for kw in ({"fmt": "fp4"}, {"fmt": "mxfp4", "scale": one}, {"scale": one.double()}, {"scale": torch.ones(2)},
+               {"index": i32.long()}, {"index": i32[::2]}, {"per_row": 2}, {"count": i32}, {"count": torch.zeros(1)},
+               {"out": _rows(3, 64, "nvfp4")}, {"out": _rows(4, 96, "nvfp4")}, {"out": _rows(4, 64, "nvfp4")[::-1]}):
+        with pytest.raises(ValueError):
+            ops.fp4_quantize(x, kw.pop("fmt", "nvfp4"), **kw)
+    with pytest.raises(ValueError):
+        ops.fp4_quantize(x.float(), "nvfp4")
+    with pytest.raises(ValueError):
+        ops.fp4_quantize(x.T, "nvfp4")
+    c, s = _rows(4, 64, "nvfp4")
+    for args in ((c.int(), s), (c, s[:, :3]), (c, s.int()), (c[:, ::2], s)):
+        with pytest.raises(ValueError):
+            ops.fp4_dequantize(*args, "nvfp4", T)
+    with pytest.raises(ValueError):
+        ops.fp4_dequantize(c, s, "nvfp4", torch.float32)
+    with pytest.raises(ValueError):
+        ops.fp4_dequantize(c, s, "nvfp4", T, out=torch.zeros((4, 60), dtype=T))
+    w = torch.zeros(64, dtype=T)
+    for args, kw in (((x, x.half(), w), {}), ((x, x[:2], w), {}), ((x, x, w[:32]), {}), ((x, x, w.half()), {}),
+                     ((x, None, w), {"residual_out": x}), ((x, x, w), {"residual_out": x.half()}), ((x, x, w), {"scale": w})):
+        with pytest.raises(ValueError):
+            ops.fp4_add_rmsnorm(*args, 1e-6, "nvfp4", **kw)
+
+
+def test_products_refuse(here):
+    T = torch.bfloat16
+    c, s = _rows(4, 64, "nvfp4")
+    w = torch.zeros((32, 32), dtype=torch.uint8)
+    ws = ops.fp4_lay_out_scales(torch.zeros((32, 4), dtype=torch.uint8), "nvfp4")
+    for args, kw in (((c, s, w[:, :16], ws), {}), ((c, s, w.int(), ws), {}), ((c, s, w, ws[..., :2]), {}),
+                     ((c, s, w[None], ws[None]), {}), ((c, s, w, ws), {"bias": torch.zeros(32)}),
+                     ((c, s, w, ws), {"bias": torch.zeros(16, dtype=T)}), ((c, s, w, ws), {"x_scale": torch.ones(2)}),
+                     ((c, s, w, ws), {"w_scale": torch.ones(1, dtype=T)}), ((c, s, w, ws), {"out": torch.zeros((4, 16), dtype=T)}),
+                     ((c, s, w, ws), {"out": torch.zeros((4, 32), dtype=T), "silu_mul": True}), ((c, s[:, :2], w, ws), {})):
+        with pytest.raises(ValueError):
+            ops.fp4_gemm(*args, "nvfp4", T, **kw)
+    with pytest.raises(ValueError):  # laid out for the other format
+        ops.fp4_gemm(c, s, w, ws, "mxfp4", T)
+    w3, ws3 = w.expand(2, 32, 32).contiguous(), ws.expand(2, *ws.shape).contiguous()
+    off = torch.zeros(3, dtype=torch.int32)
+    for args, kw in (((c, s, w, ws, off), {}), ((c, s, w3, ws3, off[:2]), {}), ((c, s, w3, ws3, off.long()), {}),
+                     ((c, s, w3, ws, off), {}), ((c, s, w3, ws3, off), {"w_scale": torch.ones(1)}),
+                     ((c, s, w3, ws3, off), {"row_map": off}), ((c, s, w3, ws3, off), {"row_scale": torch.ones(3)}),
+                     ((c, s, w3, ws3, off), {"out": torch.zeros((4, 16), dtype=T)})):
+        with pytest.raises(ValueError):
+            ops.fp4_grouped_gemm(*args, "nvfp4", T, **kw)
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros((2, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.fp4_quantize(x, "nvfp4")
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.fp4_add_rmsnorm(x, None, x[0], 1e-6, "mxfp4")
+    c, s = _rows(2, 64, "nvfp4")
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.fp4_dequantize(c, s, "nvfp4", torch.float16)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.fp4_gemm(c, s, c, s, "nvfp4", torch.float16)
