@@ -44,21 +44,23 @@ struct Params {
   uint32_t* err;
   int64_t ldo, out_rows;
   int rows, E, K, N, n_out, silu, feat_tiles, tile_out;  // tile_out: weight rows of a tile
+  int split;  // CTAs (pairs) of a cluster that share a tile's K; above 1, a cluster has one tile
 };
 
+// One CTA per tile of 128 weight rows x kTok tokens, two CTAs to an SM. Of a stage:
+// weights, rows (both swizzled: 1024-byte aligned), the weights' and the rows' scales.
+// Tensor memory: two accumulators, two sets of scales.
+template <int kTokens>
 struct Few {
-  static constexpr int kTok = 64;   // tokens per tile
+  static constexpr int kTok = kTokens;
   static constexpr int kRound = 16;
-  static constexpr int kStages = 6;
+  static constexpr int kStages = kTok > 32 ? 3 : 4;
   static constexpr int kEpiWarps = 4;
   static constexpr int kThreads = 32 * (kEpiWarps + 3);
-  // of a stage: weights, rows (both swizzled: 1024-byte aligned), the weights' and the rows' scales
   static constexpr int kAtX = kWBytes, kAtWs = kAtX + kTok * kK / 2, kAtXs = kAtWs + 2048;
   static constexpr int kStageBytes = kAtXs + 2048;
-  // tensor memory: two accumulators, two sets of scales
-  static constexpr int kSets = 2 * kTok, kSetColumns = 32, kColumns = 256;
+  static constexpr int kSets = 2 * kTok, kSetColumns = 32, kColumns = kTok > 32 ? 256 : 128;
 };
-
 // A CTA pair; each loads its 128 weight rows and half the tokens, and the scales of all tokens.
 struct Many {
   static constexpr int kTok = 224;  // two accumulators and the scales fill tensor memory
@@ -83,8 +85,19 @@ __device__ __forceinline__ int first_word(int kb) { return kNv ? 0 : 2 * (kb & 1
 
 // Rows of 16 bytes of scales, as they stand in memory, into tiles of 32 x 16 bytes, in
 // place: of 128 rows, lane l holds l, l + 32, l + 64 and l + 96, four words each; word w
-// of the four goes to tile w.
+// of the four goes to tile w. (Tiles of up to 32 rows take it too: an instruction's scales
+// have to begin at a column that is a multiple of four, so a row's four words cannot be
+// left in neighbouring columns.)
 __device__ __forceinline__ void turn_scales(uint8_t* at, int rows, int lane) {
+  if (rows <= 32) {
+    const uint4 a = reinterpret_cast<uint4*>(at)[lane];
+    uint32_t* p = reinterpret_cast<uint32_t*>(at) + 4 * lane;
+    p[0] = a.x;
+    p[128] = a.y;
+    p[256] = a.z;
+    p[384] = a.w;
+    return;
+  }
   for (int r = 0; r < rows; r += 128, at += 2048) {
     uint4* p = reinterpret_cast<uint4*>(at) + lane;
     const uint4 a = p[0], b = p[32], c = p[64], d = p[96];
@@ -95,17 +108,54 @@ __device__ __forceinline__ void turn_scales(uint8_t* at, int rows, int lane) {
   }
 }
 
-template <typename T, bool kNv>
-__global__ void __launch_bounds__(Few::kThreads, 1)
+// Stores a weight row's values of tokens c and c + 1, or, where rows are gate and up by
+// turns, the pair of lanes' two products.
+template <typename T>
+__device__ __forceinline__ void store_two(const Params& p, float (&y)[2], const int* to, const float* factor, int c,
+                                          int rows, bool real, int odd, T* out) {
+  if (p.silu) {
+    const float got = __shfl_xor_sync(0xffffffffu, odd ? y[0] : y[1], 1);
+    y[0] = y[1] = odd ? silu_mul(got, y[1]) : silu_mul(y[0], got);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (!real || c + i >= rows || to[c + i] < 0 || (p.silu && i != odd)) continue;
+    out[(int64_t)to[c + i] * p.ldo] = (T)(p.row_scale ? y[i] * factor[c + i] : y[i]);
+  }
+}
+
+// The out row and the factor of a tile's row i, by one thread each, a tile ahead of use.
+struct RowTo {
+  int to;
+  float factor;
+};
+__device__ __forceinline__ RowTo row_to(const Params& p, const Tile& tile, int i) {
+  RowTo r = {-1, 0.f};
+  if (i >= tile.rows) return r;
+  const int to = p.row_map ? p.row_map[tile.row0 + i] : tile.row0 + i;
+  if (to < 0 || to >= p.out_rows) return r;
+  r.to = to;
+  if (p.row_scale) r.factor = p.row_scale[to];
+  return r;
+}
+
+// Stages of K that part `part` of p.split works on.
+__device__ __forceinline__ void stages_of(const Params& p, int nk, int part, int* first, int* last) {
+  *first = nk * part / p.split;
+  *last = nk * (part + 1) / p.split;
+}
+
+template <typename T, bool kNv, int kTok>
+__global__ void __launch_bounds__(Few<kTok>::kThreads, 2)
 fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ TokenMaps tm_x,
                     const __grid_constant__ Params p) {
-  using C = Few;
+  using C = Few<kTok>;
   extern __shared__ uint8_t raw[];
   uint8_t* ring = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
   int* dst = reinterpret_cast<int*>(ring + C::kStages * C::kStageBytes);  // [2][kTok] out row of a token
-  float* scl = reinterpret_cast<float*>(dst + 2 * C::kTok);               // [2][kTok]
+  float* scl = reinterpret_cast<float*>(dst + 2 * kTok);                  // [2][kTok]
   Groups g;
-  g.row0 = reinterpret_cast<int*>(scl + 2 * C::kTok);  // [E] first rows, [E] row counts
+  g.row0 = reinterpret_cast<int*>(scl + 2 * kTok);  // [E] first rows, [E] row counts
   g.tile0 = g.row0 + 2 * p.E;
   __shared__ uint64_t full[C::kStages], raw_scales[C::kStages], scaled[C::kStages], empty[C::kStages];
   __shared__ uint64_t acc_full[2], acc_empty[2];
@@ -113,6 +163,11 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   __shared__ int failed;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = p.split > 1 ? (int)cluster_ctarank() : 0;
+  const int first_tile = blockIdx.x / p.split, tile_step = gridDim.x / p.split;
+  const int nk = (p.K + kK - 1) / kK;
+  int kb0, kb1;
+  stages_of(p, nk, part, &kb0, &kb1);
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(smem_u32(&full[s]), 1);
@@ -126,150 +181,162 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     }
     failed = 0;
     fence_barrier_init();
-    prefetch_tmap(&tm_w);
   }
   if (warp == C::kEpiWarps + 1) {
     tmem_alloc(smem_u32(&tmem_slot), C::kColumns);
     tmem_relinquish();
   }
-  grid_dep_wait();
   grid_dep_launch();
+  if (p.offsets == nullptr && warp == C::kEpiWarps && elect_one()) {
+    // The weights' first stages on their way to L2 while the kernel in front ends. (Its
+    // outputs, this product's rows, are not touched before the wait.)
+    prefetch_tmap(&tm_w);
+    const int feat = first_tile / ((p.rows + kTok - 1) / kTok) * kFeat;
+    for (int kb = kb0; kb < min(kb1, kb0 + C::kStages); ++kb) tma_prefetch_2d(&tm_w, kb * kK / 2, feat);
+  }
+  __syncwarp();
+  grid_dep_wait();
   build_groups<C>(g, p);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const int total = g.tile0[p.E];
-  const int nk = (p.K + kK - 1) / kK;
   bool ok = true;
 
   if (warp == C::kEpiWarps) {  // ------------------------------------- producer
     const uint64_t keep = policy_evict_normal(), once = policy_evict_first();
     int it = 0;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+    for (int t = first_tile; t < total && ok; t += tile_step) {
       const Tile tile = find_tile<C>(g, p, t);
-      const int box = box_of(tile.n, C::kTok);
+      const int box = box_of(tile.n, kTok);
       // weights that one token tile reads once need not stay in L2
       const uint64_t wpol = tile.rows == g.row0[p.E + tile.e] ? once : keep;
       const int wrow = tile.e * p.N + tile.feat;
       const uint8_t* ws = p.w_scales + ((int64_t)tile.e * p.feat_tiles + tile.feat / kFeat) * nk * kWsBytes<kNv>;
       const int scale_rows = min(tile.n, p.rows - tile.row0);
-      for (int kb = 0; kb < nk; ++kb, ++it) {
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int s = it % C::kStages;
         ok = mbar_wait(smem_u32(&empty[s]), ((it / C::kStages) & 1) ^ 1);
         if (!ok) break;
         if (elect_one()) {
-          const uint32_t base = smem_u32(ring + s * C::kStageBytes);
-          const uint32_t bar = smem_u32(&full[s]), sbar = smem_u32(&raw_scales[s]);
-          mbar_arrive_expect_tx(bar, kWBytes + kWsBytes<kNv> + (C::kTok >> (2 - box)) * kK / 2);
+          const uint32_t base = smem_u32(ring + s * C::kStageBytes), bar = smem_u32(&full[s]);
+          const uint32_t sbar = smem_u32(&raw_scales[s]);
+          mbar_arrive_expect_tx(bar, kWBytes + kWsBytes<kNv> + (kTok >> (2 - box)) * kK / 2);
+          mbar_arrive_expect_tx(sbar, scale_rows * 16);
           tma_load_2d(base, &tm_w, kb * kK / 2, wrow, bar, wpol);
           bulk_g2s(base + C::kAtWs, ws + (int64_t)kb * kWsBytes<kNv>, kWsBytes<kNv>, bar, wpol);
-          tma_load_2d(base + C::kAtX, &tm_x.box[box], kb * kK / 2, tile.row0, bar, keep);
-          mbar_arrive_expect_tx(sbar, scale_rows * 16);
           bulk_g2s(base + C::kAtXs, p.x_scales + ((int64_t)granule_of<kNv>(kb) * p.rows + tile.row0) * 16,
                    scale_rows * 16, sbar, keep);
+          tma_load_2d(base + C::kAtX, &tm_x.box[box], kb * kK / 2, tile.row0, bar, keep);
         }
         __syncwarp();
       }
     }
   } else if (warp == C::kEpiWarps + 2) {  // ---------------------------- scales of the rows
     int it = 0;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      for (int kb = 0; kb < nk; ++kb, ++it) {
+    for (int t = first_tile; t < total && ok; t += tile_step) {
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int s = it % C::kStages;
-        ok = mbar_wait(smem_u32(&raw_scales[s]), (it / C::kStages) & 1);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&raw_scales[s]), (it / C::kStages) & 1));
         if (!ok) break;
-        turn_scales(ring + s * C::kStageBytes + C::kAtXs, C::kTok, lane);
+        turn_scales(ring + s * C::kStageBytes + C::kAtXs, kTok, lane);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&scaled[s]));
       }
     }
   } else if (warp == C::kEpiWarps + 1) {  // ---------------------------- MMA
+    const uint32_t issue = elect_one();
+    // (what the compiler cannot see to be the same for all lanes)
+    const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem, 0), ring0 = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
     int it = 0, n_tile = 0;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++n_tile) {
+    for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
       const Tile tile = find_tile<C>(g, p, t);
       const int b = n_tile & 1;
       ok = mbar_wait(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1);
       tc_fence_after();
-      const uint32_t d = tmem + b * C::kTok;
-      for (int kb = 0; kb < nk && ok; ++kb, ++it) {
+      const uint32_t d = tmem0 + b * kTok;
+      const uint32_t idesc = make_idesc_fp4(kFeat, __shfl_sync(0xffffffffu, tile.n, 0), kNv, 0);
+      for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
         const int s = it % C::kStages;
         ok = mbar_wait(smem_u32(&full[s]), (it / C::kStages) & 1) && mbar_wait(smem_u32(&scaled[s]), (it / C::kStages) & 1);
         if (!ok) break;
         tc_fence_after();
-        if (elect_one()) {
-          const uint32_t base = smem_u32(ring + s * C::kStageBytes);
-          const uint64_t ad = make_sw128_kmajor_desc(base), bd = make_sw128_kmajor_desc(base + C::kAtX);
-          const uint32_t sa = tmem + C::kSets + (it & 1) * C::kSetColumns, sb = sa + 16;
-          const int steps = min(kK, p.K - kb * kK + 63) / 64;
-          const int words = kNv ? steps : (steps + 1) / 2;
-          for (int j = 0; j < words; ++j) {
-            tc_copy_scales<false>(sa + 4 * j, base + C::kAtWs + 512 * j);
-            tc_copy_scales<false>(sb + 4 * j, base + C::kAtXs + 512 * (first_word<kNv>(kb) + j));
-          }
-          for (int j = 0; j < steps; ++j) {
-            const int w = kNv ? j : j >> 1, half = kNv ? 0 : j & 1;
-            tc_mma_fp4<kNv, false>(d, ad + 2 * j, bd + 2 * j, make_idesc_fp4(kFeat, tile.n, kNv, half), sa + 4 * w,
-                                   sb + 4 * w, kb + j > 0);
-          }
-          tc_commit(smem_u32(&empty[s]));
-          if (kb == nk - 1) tc_commit(smem_u32(&acc_full[b]));
+        const uint32_t base = ring0 + s * C::kStageBytes;
+        const uint32_t ad = desc_low(base), bd = desc_low(base + C::kAtX);
+        const uint32_t sa = tmem0 + C::kSets + (it & 1) * C::kSetColumns, sb = sa + 16;
+        const int steps = min(kK, p.K - kb * kK + 63) / 64;
+        const int words = kNv ? steps : (steps + 1) / 2;
+#pragma unroll
+        for (int j = 0; j < (kNv ? 4 : 2); ++j) {
+          const uint32_t want = issue && j < words;
+          tc_copy_scales<false>(want, sa + 4 * j, base + C::kAtWs + 512 * j);
+          tc_copy_scales<false>(want, sb + 4 * j, base + C::kAtXs + 512 * (first_word<kNv>(kb) + j));
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int w = kNv ? j : j >> 1, half = kNv ? 0 : j & 1;
+          tc_mma_fp4<kNv, false>(issue && j < steps, d, ad + 2 * j, bd + 2 * j, idesc | make_idesc_fp4(0, 0, kNv, half),
+                                 sa + 4 * w, sb + 4 * w, kb > kb0 || j > 0);
+        }
+        tc_commit_if(issue, smem_u32(&empty[s]));
+        tc_commit_if(issue && kb == kb1 - 1, smem_u32(&acc_full[b]));
         __syncwarp();
       }
     }
-  } else {  // -------------------------------------------------------- epilogue
+  } else if (warp < C::kEpiWarps) {  // --------------------------------- epilogue
     // A lane holds a weight row's tokens. Neighbouring lanes write neighbouring features
-    // of a token. With silu_mul even lanes hold gate and odd lanes up rows: a lane keeps
-    // eight of 16 tokens and gives its neighbour the others.
+    // of a token. With silu_mul even lanes hold gate and odd lanes up rows: of a pair of
+    // tokens a lane keeps one and gives its neighbour the other. A tile whose K is shared
+    // is summed after the barrier below: each CTA leaves its part in its ring, [token][row].
     const int tid = threadIdx.x, odd = lane & 1;
-    const float xs = p.x_scale ? *p.x_scale : 1.f;
     int n_tile = 0;
-    for (int t = blockIdx.x; t < total; t += gridDim.x, ++n_tile) {
-      const Tile tile = find_tile<C>(g, p, t);
+    Tile tile = {};
+    if (first_tile < total) {
+      tile = find_tile<C>(g, p, first_tile);
+      const RowTo r = row_to(p, tile, tid);
+      if (tid < kTok) dst[tid] = r.to, scl[tid] = r.factor;
+    }
+    const float xs = p.x_scale ? *p.x_scale : 1.f;
+    for (int t = first_tile; t < total; t += tile_step, ++n_tile) {
       const int b = n_tile & 1;
-      int* rows = dst + b * C::kTok;
-      float* scales = scl + b * C::kTok;
-      load_rows(p, tile, tid, 128, rows, scales);
+      Tile next = {};
+      if (t + tile_step < total) next = find_tile<C>(g, p, t + tile_step);
+      const RowTo r = row_to(p, next, tid);
       const int row = tile.feat + tid;  // of the weights
       const float alpha = xs * (p.w_scale ? p.w_scale[tile.e] : 1.f);
       const float bias = p.bias && row < p.N ? (float)static_cast<const T*>(p.bias)[row] : 0.f;
       ok = named_bar_and(1, 128, mbar_wait(smem_u32(&acc_full[b]), (n_tile >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
+      const int* to = dst + b * kTok;
+      const float* factor = scl + b * kTok;
       T* out = static_cast<T*>(p.out) + (p.silu ? row / 2 : row);
-      for (int c = 0; c < tile.n; c += 16) {
+      for (int c = 0; c < tile.rows; c += 16) {
         uint32_t v[16];
-        tmem_ld16(tmem + b * C::kTok + c + ((uint32_t)warp << 21), v);
+        tmem_ld16(tmem + b * kTok + c + ((uint32_t)warp << 21), v);
         tmem_ld_wait();
-        if (c + 16 >= tile.n) {  // the accumulator is read: the MMA warp may reuse it
+        if (p.split > 1) {
+          float* mine = reinterpret_cast<float*>(ring) + c * kFeat + tid;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) mine[j * kFeat] = __uint_as_float(v[j]);
+          continue;
+        }
+        if (c + 16 >= tile.rows) {  // the accumulator is read: the MMA warp may reuse it
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&acc_empty[b]));
         }
-        float y[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(v[j]) * alpha + bias;
-        const int count = p.silu ? 8 : 16, first = p.silu ? c + 8 * odd : c;
-        if (p.silu) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float keep = odd ? y[8 + j] : y[j];
-            const float got = __shfl_xor_sync(0xffffffffu, odd ? y[j] : y[8 + j], 1);
-            y[j] = odd ? silu_mul(got, keep) : silu_mul(keep, got);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (j >= count || first + j >= tile.rows || row >= p.N) continue;
-          const int to = rows[first + j];
-          if (to < 0) continue;
-          const float w = p.row_scale ? y[j] * scales[first + j] : y[j];
-          out[(int64_t)to * p.ldo] = (T)w;
+        for (int j = 0; j < 16; j += 2) {
+          if (c + j >= tile.rows) break;
+          float y[2] = {__uint_as_float(v[j]) * alpha + bias, __uint_as_float(v[j + 1]) * alpha + bias};
+          store_two<T>(p, y, to, factor, c + j, tile.rows, row < p.N, odd, out);
         }
       }
+      tile = next;
+      if (tid < kTok) dst[(b ^ 1) * kTok + tid] = r.to, scl[(b ^ 1) * kTok + tid] = r.factor;
     }
   }
   if (!ok && lane == 0) {
@@ -277,6 +344,29 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     atomicOr(p.err, kErrWait);
   }
   __syncwarp();
+  if (p.split > 1) {
+    // Two tokens at a time by turns: CTA `part` adds the parts in their order.
+    cluster_sync_all();
+    if (warp < C::kEpiWarps && first_tile < total) {
+      const Tile tile = find_tile<C>(g, p, first_tile);
+      const int tid = threadIdx.x, odd = lane & 1, row = tile.feat + tid;
+      const float alpha = (p.x_scale ? *p.x_scale : 1.f) * (p.w_scale ? p.w_scale[0] : 1.f);
+      const float bias = p.bias && row < p.N ? (float)static_cast<const T*>(p.bias)[row] : 0.f;
+      T* out = static_cast<T*>(p.out) + (p.silu ? row / 2 : row);
+      const uint32_t mine = smem_u32(ring) + tid * 4;
+      for (int c = 2 * part; c < tile.rows; c += 2 * p.split) {
+        float sum[2] = {0.f, 0.f};
+        for (int q = 0; q < p.split; ++q) {
+          const uint32_t at = mapa_shared(mine, q) + c * kFeat * 4;
+          sum[0] += ld_dsmem_f32(at);
+          sum[1] += ld_dsmem_f32(at + kFeat * 4);
+        }
+        float y[2] = {sum[0] * alpha + bias, sum[1] * alpha + bias};
+        store_two<T>(p, y, dst, scl, c, tile.rows, row < p.N, odd, out);
+      }
+    }
+    cluster_sync_all();  // the parts are read
+  }
   __syncthreads();
   if (failed) linger();
   tc_fence_before();
@@ -286,6 +376,51 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     tmem_dealloc(tmem, C::kColumns);
   }
 }
+
+// Stores 32 tokens of a warp's 32 weight rows. A lane holds a row's tokens; eight lanes
+// transpose eight tokens among them in registers, so that each writes eight features of a
+// token. Where even lanes hold gate and odd lanes up rows, a lane keeps 16 tokens and gives
+// its neighbour the other 16.
+template <typename T>
+struct ManyStore {
+  float alpha, bias;
+  int f, lane;  // the first of the eight features that this lane writes
+  __device__ __forceinline__ ManyStore(const Params& p, const Tile& tile, int rank, int quarter, int lane_) : lane(lane_) {
+    const int row = tile.feat + rank * kFeat + quarter * 32;  // of the weights, the warp's first
+    alpha = (p.x_scale ? *p.x_scale : 1.f) * (p.w_scale ? p.w_scale[tile.e] : 1.f);
+    bias = p.bias && row + lane < p.N ? (float)static_cast<const T*>(p.bias)[row + lane] : 0.f;
+    f = p.silu ? (row + (lane & 16)) / 2 : row + (lane & 24);
+  }
+  __device__ __forceinline__ void put(const Params& p, const Tile& tile, uint4 o, int i, const int* rows) const {
+    const int to = rows[i];
+    if (i < tile.rows && to >= 0 && f < p.n_out)
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)to * p.ldo + f) = o;
+  }
+  __device__ __forceinline__ void operator()(const Params& p, const Tile& tile, float (&v)[32], int c, const int* rows,
+                                             const float* factor) const {
+    const int odd = lane & 1;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = v[j] * alpha + bias;
+    if (p.silu) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float own = odd ? v[16 + j] : v[j];
+        const float got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[16 + j], 1);
+        v[j] = silu_mul(odd ? got : own, odd ? own : got);
+        if (p.row_scale) v[j] *= factor[c + 16 * odd + j];
+      }
+#pragma unroll
+      for (int j = 0; j < 16; j += 8)
+        put(p, tile, transpose8<T, 2>(v + j, lane), c + 16 * odd + j + ((lane >> 1) & 7), rows);
+    } else {
+      if (p.row_scale)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= factor[c + j];
+#pragma unroll
+      for (int j = 0; j < 32; j += 8) put(p, tile, transpose8<T, 1>(v + j, lane), c + j + (lane & 7), rows);
+    }
+  }
+};
 
 template <typename T, bool kNv>
 __global__ void __launch_bounds__(Many::kThreads, 1)
@@ -305,7 +440,14 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   __shared__ int failed;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();
+  // a cluster is p.split pairs; rank: in the pair, whose leader is CTA `leader` of the cluster
+  const uint32_t rank = cluster_ctarank() & 1, leader = cluster_ctarank() & ~1u;
+  const int part = cluster_ctarank() >> 1;
+  const uint16_t pair_mask = (uint16_t)(3u << leader);
+  const int first_tile = blockIdx.x / (2 * p.split), tile_step = gridDim.x / (2 * p.split);
+  const int nk = (p.K + kK - 1) / kK;
+  int kb0, kb1;
+  stages_of(p, nk, part, &kb0, &kb1);
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(smem_u32(&full[s]), 1);
@@ -319,14 +461,20 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     }
     failed = 0;
     fence_barrier_init();
-    prefetch_tmap(&tm_w);
   }
   if (warp == C::kEpiWarps + 1) {
     tmem_alloc_pair(smem_u32(&tmem_slot), C::kColumns);
     tmem_relinquish_pair();
   }
-  grid_dep_wait();
   grid_dep_launch();
+  if (p.offsets == nullptr && warp == C::kEpiWarps && elect_one()) {
+    // as in the kernel above, to L2 only
+    prefetch_tmap(&tm_w);
+    const int feat = first_tile / ((p.rows + C::kTok - 1) / C::kTok) * 2 * kFeat + (int)rank * kFeat;
+    for (int kb = kb0; kb < min(kb1, kb0 + C::kStages); ++kb) tma_prefetch_2d(&tm_w, kb * kK / 2, feat);
+  }
+  __syncwarp();
+  grid_dep_wait();
   build_groups<C>(g, p);
   tc_fence_before();
   cluster_sync_all();  // the peer's barriers are ready before anything arrives on them
@@ -334,15 +482,13 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const int total = g.tile0[p.E];
-  const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
-  const int nk = (p.K + kK - 1) / kK;
   bool ok = true;
 
   if (warp == C::kEpiWarps) {  // ------------------------------------- producer
     const uint64_t keep = policy_evict_normal(), once = policy_evict_first();
     const int scale_tiles = (p.N + kFeat - 1) / kFeat;
     int it = 0;
-    for (int t = pair; t < total && ok; t += pairs) {
+    for (int t = first_tile; t < total && ok; t += tile_step) {
       const Tile tile = find_tile<C>(g, p, t);
       const int box = box_of(tile.n / 2, C::kTok / 2);
       // weights that one token tile reads once need not stay in L2
@@ -353,12 +499,12 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
           p.w_scales + ((int64_t)tile.e * scale_tiles + min(feat / kFeat, scale_tiles - 1)) * nk * kWsBytes<kNv>;
       const int scale_rows = min(tile.n, p.rows - tile.row0);
       const uint32_t bytes = 2 * (kWBytes + (C::kTok / 2 >> (2 - box)) * kK / 2);
-      for (int kb = 0; kb < nk; ++kb, ++it) {
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int s = it % C::kStages;
         ok = mbar_wait(smem_u32(&empty[s]), ((it / C::kStages) & 1) ^ 1);
         if (!ok) break;
         if (elect_one()) {
-          const uint32_t base = smem_u32(ring + s * C::kStageBytes), bar = mapa_shared(smem_u32(&full[s]), 0);
+          const uint32_t base = smem_u32(ring + s * C::kStageBytes), bar = mapa_shared(smem_u32(&full[s]), leader);
           const uint32_t sbar = smem_u32(&raw_scales[s]);
           mbar_arrive_expect_tx(sbar, kWsBytes<kNv> + scale_rows * 16);
           bulk_g2s(base + C::kAtXs, p.x_scales + ((int64_t)granule_of<kNv>(kb) * p.rows + tile.row0) * 16,
@@ -376,117 +522,111 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       ok = mbar_wait(smem_u32(&empty[i % C::kStages]), (i / C::kStages) & 1);
   } else if (warp == C::kEpiWarps + 2) {  // ---------------------------- scales of the rows
     int it = 0;
-    for (int t = pair; t < total && ok; t += pairs) {
+    for (int t = first_tile; t < total && ok; t += tile_step) {
       const Tile tile = find_tile<C>(g, p, t);
-      for (int kb = 0; kb < nk; ++kb, ++it) {
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int s = it % C::kStages;
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&raw_scales[s]), (it / C::kStages) & 1));
         if (!ok) break;
         turn_scales(ring + s * C::kStageBytes + C::kAtXs, tile.n, lane);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive_peer(mapa_shared(smem_u32(&scaled[s]), 0));
+        if (lane == 0) mbar_arrive_peer(mapa_shared(smem_u32(&scaled[s]), leader));
       }
     }
   } else if (warp == C::kEpiWarps + 1) {  // ---------------------------- MMA, the leader's
+    const uint32_t issue = elect_one();
+    // (what the compiler cannot see to be the same for all lanes)
+    const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem, 0), ring0 = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
     int it = 0, n_tile = 0;
-    for (int t = pair; t < total && ok && rank == 0; t += pairs, ++n_tile) {
+    for (int t = first_tile; t < total && ok && rank == 0; t += tile_step, ++n_tile) {
       const Tile tile = find_tile<C>(g, p, t);
       const int b = n_tile & 1;
       ok = mbar_wait(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1);
       tc_fence_after();
-      const uint32_t sa = tmem + C::kSets, sb = sa + 16;  // a word's column of row scales: 8 for 256 rows
-      for (int kb = 0; kb < nk && ok; ++kb, ++it) {
+      const int n = __shfl_sync(0xffffffffu, tile.n, 0);
+      const uint32_t d = tmem0 + b * C::kTok, idesc = make_idesc_fp4(2 * kFeat, n, kNv, 0);
+      const uint32_t sa = tmem0 + C::kSets, sb = sa + 16;  // a word's columns of row scales: 8 for 256 rows
+      for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
         const int s = it % C::kStages;
         ok = mbar_wait(smem_u32(&full[s]), (it / C::kStages) & 1) && mbar_wait(smem_u32(&scaled[s]), (it / C::kStages) & 1);
         if (!ok) break;
         tc_fence_after();
-        if (elect_one()) {
-          const uint32_t base = smem_u32(ring + s * C::kStageBytes);
-          const uint64_t ad = make_sw128_kmajor_desc(base), bd = make_sw128_kmajor_desc(base + C::kAtX);
-          const int steps = min(kK, p.K - kb * kK + 63) / 64;
-          const int words = kNv ? steps : (steps + 1) / 2;
-          for (int j = 0; j < words; ++j) {
-            tc_copy_scales<true>(sa + 4 * j, base + C::kAtWs + 512 * j);
-            const uint32_t at = base + C::kAtXs + 512 * (first_word<kNv>(kb) + j);
-            tc_copy_scales<true>(sb + 8 * j, at);
-            if (tile.n > 128) tc_copy_scales<true>(sb + 8 * j + 4, at + 2048);
-          }
-          for (int j = 0; j < steps; ++j) {
-            const int w = kNv ? j : j >> 1, half = kNv ? 0 : j & 1;
-            tc_mma_fp4<kNv, true>(tmem + b * C::kTok, ad + 2 * j, bd + 2 * j, make_idesc_fp4(2 * kFeat, tile.n, kNv, half),
-                                  sa + 4 * w, sb + 8 * w, kb + j > 0);
-          }
-          tc_commit_pair(smem_u32(&empty[s]));
-          if (kb == nk - 1) tc_commit_pair(smem_u32(&acc_full[b]));
+        const uint32_t base = ring0 + s * C::kStageBytes;
+        const uint32_t ad = desc_low(base), bd = desc_low(base + C::kAtX);
+        const int steps = min(kK, p.K - kb * kK + 63) / 64;
+        const int words = kNv ? steps : (steps + 1) / 2;
+#pragma unroll
+        for (int j = 0; j < (kNv ? 4 : 2); ++j) {
+          const uint32_t want = issue && j < words;
+          const uint32_t at = base + C::kAtXs + 512 * (first_word<kNv>(kb) + j);
+          tc_copy_scales<true>(want, sa + 4 * j, base + C::kAtWs + 512 * j);
+          tc_copy_scales<true>(want, sb + 8 * j, at);
+          tc_copy_scales<true>(want && n > 128, sb + 8 * j + 4, at + 2048);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int w = kNv ? j : j >> 1, half = kNv ? 0 : j & 1;
+          tc_mma_fp4<kNv, true>(issue && j < steps, d, ad + 2 * j, bd + 2 * j, idesc | make_idesc_fp4(0, 0, kNv, half),
+                                sa + 4 * w, sb + 8 * w, kb > kb0 || j > 0);
+        }
+        tc_commit_pair_if(issue, smem_u32(&empty[s]), pair_mask);
+        tc_commit_pair_if(issue && kb == kb1 - 1, smem_u32(&acc_full[b]), pair_mask);
         __syncwarp();
       }
     }
   } else {  // -------------------------------------------------------- epilogue
-    // Two groups of four warps take turns over 32 tokens. A lane holds a weight row's
-    // tokens; eight lanes transpose eight tokens among them in registers, so that each
-    // writes eight features of a token. With silu_mul even lanes hold gate and odd lanes
-    // up rows: a lane keeps 16 tokens and gives its neighbour the other 16.
-    const int group = warp >> 2, quarter = warp & 3, odd = lane & 1;
+    // Two groups of four warps take turns over 32 tokens.
+    const int quarter = warp & 3;
     const uint32_t at = tmem + ((uint32_t)quarter << 21);
-    const float xs = p.x_scale ? *p.x_scale : 1.f;
     int n_tile = 0;
-    for (int t = pair; t < total; t += pairs, ++n_tile) {
-      const Tile tile = find_tile<C>(g, p, t);
+    Tile tile = {};
+    if (first_tile < total) {
+      tile = find_tile<C>(g, p, first_tile);
+      const RowTo r = row_to(p, tile, threadIdx.x);
+      if (threadIdx.x < C::kTok) dst[threadIdx.x] = r.to, scl[threadIdx.x] = r.factor;
+    }
+    for (int t = first_tile; t < total; t += tile_step, ++n_tile) {
       const int b = n_tile & 1;
-      int* rows = dst + b * C::kTok;
-      float* scales = scl + b * C::kTok;
-      load_rows(p, tile, threadIdx.x, 32 * C::kEpiWarps, rows, scales);
-      const int row = tile.feat + (int)rank * kFeat + quarter * 32;  // of the weights, the warp's first
-      const float alpha = xs * (p.w_scale ? p.w_scale[tile.e] : 1.f);
-      const float bias = p.bias && row + lane < p.N ? (float)static_cast<const T*>(p.bias)[row + lane] : 0.f;
+      Tile next = {};
+      if (t + tile_step < total) next = find_tile<C>(g, p, t + tile_step);
+      const RowTo r = row_to(p, next, threadIdx.x);
+      const ManyStore<T> store(p, tile, (int)rank, quarter, lane);
       ok = named_bar_and(1, 32 * C::kEpiWarps, mbar_wait(smem_u32(&acc_full[b]), (n_tile >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
-      const int f = p.silu ? (row + (lane & 16)) / 2 : row + (lane & 24);
-      const auto put = [&](uint4 o, int i) {  // token i's features f ..
-        const int to = rows[i];
-        if (i < tile.rows && to >= 0 && f < p.n_out)
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)to * p.ldo + f) = o;
-      };
-      for (int c = group * 32; c < tile.rows; c += 64) {
+      for (int c = (warp >> 2) * 32; c < tile.rows; c += 64) {
         uint32_t lo[16], hi[16];
         tmem_ld16(at + b * C::kTok + c, lo);
         tmem_ld16(at + b * C::kTok + c + 16, hi);
         tmem_ld_wait();
+        if (p.split > 1) {  // left in the ring, [token][row], for the sum below
+          float* mine = reinterpret_cast<float*>(ring) + c * kFeat + quarter * 32 + lane;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            mine[j * kFeat] = __uint_as_float(lo[j]);
+            mine[(j + 16) * kFeat] = __uint_as_float(hi[j]);
+          }
+          continue;
+        }
         if (c + 64 >= tile.rows) {  // this warp has read its part of the accumulator
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_peer(mapa_shared(smem_u32(&acc_empty[b]), 0));
+          if (lane == 0) mbar_arrive_peer(mapa_shared(smem_u32(&acc_empty[b]), leader));
         }
         float v[32];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          v[j] = __uint_as_float(lo[j]) * alpha + bias;
-          v[16 + j] = __uint_as_float(hi[j]) * alpha + bias;
-        }
-        if (p.silu) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float own = odd ? v[16 + j] : v[j];
-            const float got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[16 + j], 1);
-            v[j] = silu_mul(odd ? got : own, odd ? own : got);
-            if (p.row_scale) v[j] *= scales[c + 16 * odd + j];
-          }
-#pragma unroll
-          for (int j = 0; j < 16; j += 8) put(transpose8<T, 2>(v + j, lane), c + 16 * odd + j + ((lane >> 1) & 7));
-        } else {
-          if (p.row_scale)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= scales[c + j];
-#pragma unroll
-          for (int j = 0; j < 32; j += 8) put(transpose8<T, 1>(v + j, lane), c + j + (lane & 7));
-        }
+        for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(lo[j]), v[16 + j] = __uint_as_float(hi[j]);
+        store(p, tile, v, c, dst + b * C::kTok, scl + b * C::kTok);
       }
-      if (group * 32 >= tile.rows) {  // no tokens for this group
+      if ((warp >> 2) * 32 >= tile.rows) {  // no tokens for this group
         __syncwarp();
-        if (lane == 0) mbar_arrive_peer(mapa_shared(smem_u32(&acc_empty[b]), 0));
+        if (lane == 0) mbar_arrive_peer(mapa_shared(smem_u32(&acc_empty[b]), leader));
+      }
+      tile = next;
+      if (threadIdx.x < C::kTok) {
+        dst[(b ^ 1) * C::kTok + threadIdx.x] = r.to;
+        scl[(b ^ 1) * C::kTok + threadIdx.x] = r.factor;
       }
     }
   }
@@ -495,6 +635,25 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     atomicOr(p.err, kErrWait);
   }
   __syncwarp();
+  if (p.split > 1) {
+    // 32 tokens at a time by turns of the parts and the groups of warps, added in the parts' order
+    cluster_sync_all();
+    if (warp < C::kEpiWarps && first_tile < total) {
+      const Tile tile = find_tile<C>(g, p, first_tile);
+      const int quarter = warp & 3;
+      const ManyStore<T> store(p, tile, (int)rank, quarter, lane);
+      const uint32_t mine = smem_u32(ring) + (quarter * 32 + lane) * 4;
+      for (int c = (2 * part + (warp >> 2)) * 32; c < tile.rows; c += 64 * p.split) {
+        float v[32] = {};
+        for (int q = 0; q < p.split; ++q) {
+          const uint32_t at = mapa_shared(mine, 2 * q + rank) + c * kFeat * 4;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += ld_dsmem_f32(at + j * kFeat * 4);
+        }
+        store(p, tile, v, c, dst, scl);
+      }
+    }
+  }
   __syncthreads();
   if (failed) linger();
   tc_fence_before();
@@ -506,12 +665,10 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   }
 }
 
-template <typename T, bool kNv, bool kMany>
-int launch(const void* codes, const void* w, Params p, cudaStream_t stream) {
-  using C = typename std::conditional<kMany, Many, Few>::type;
-  const auto kernel = kMany ? fp4_gemm_many_kernel<T, kNv> : fp4_gemm_few_kernel<T, kNv>;
-  constexpr int kCluster = kMany ? 2 : 1, kTokCta = C::kTok / kCluster;
-  p.tile_out = kFeat * kCluster;
+template <typename C, typename Kernel>
+int launch(Kernel kernel, int pair, const void* codes, const void* w, Params p, int max_split, cudaStream_t stream) {
+  const int tok_cta = C::kTok / pair;
+  p.tile_out = kFeat * pair;
   p.feat_tiles = (p.N + p.tile_out - 1) / p.tile_out;
   CUtensorMap tw;
   TokenMaps tx;
@@ -519,32 +676,44 @@ int launch(const void* codes, const void* w, Params p, cudaStream_t stream) {
   int st = make_bytes_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, (int64_t)p.E * p.N, row_bytes, row_bytes, kFeat);
   for (int i = 0; i < 3 && st == kOk; ++i)
     st = make_bytes_map(&tx.box[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, p.rows, row_bytes, row_bytes,
-                        kTokCta >> (2 - i));
+                        tok_cta >> (2 - i));
   if (st != kOk) return st;
   const auto smem_for = [](int E) { return 1024 + C::kStages * C::kStageBytes + 4 * C::kTok * 4 + (3 * E + 1) * 4; };
   // (the most that any call wants: another thread's call may set it before this launch)
   AWQB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_for(kMaxExperts)));
+  // all of it, so that two CTAs of the few-rows kernel fit an SM
+  AWQB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kCluster);
   cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = smem_for(p.E);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kCluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  static std::atomic<int> cached[64];
-  int64_t clusters = 0;
-  st = max_clusters(kernel, cfg, cached, &clusters);
-  if (st != kOk) return st;
   // every tile there could be: a group adds at most one partly filled token tile
   const int64_t tiles = ((p.rows + C::kTok - 1) / C::kTok + (p.offsets ? std::min<int64_t>(p.E, p.rows) : 0)) * p.feat_tiles;
   AWQB_REQUIRE(tiles < (1ll << 31), kUnsupported, "too many tiles (%lld)", (long long)tiles);
-  cfg.gridDim = dim3((unsigned)(std::min(tiles, clusters) * kCluster));
+  // K is shared by as many CTAs (pairs) as leave each tile a cluster of its own at once, and
+  // each of them two stages
+  static std::atomic<int> cached[4][64];
+  const int nk = (p.K + kK - 1) / kK;
+  int64_t clusters = 0;
+  int log = 3;
+  if (p.offsets != nullptr) max_split = 1;
+  for (;; --log) {
+    p.split = 1 << log;
+    if (p.split > max_split || (p.split > 1 && nk < 2 * p.split)) continue;
+    attr[0].val.clusterDim.x = (unsigned)(pair * p.split);
+    cfg.gridDim = dim3((unsigned)(pair * p.split));
+    cfg.numAttrs = 1;
+    st = max_clusters(kernel, cfg, cached[log], &clusters);
+    if (st != kOk) return st;
+    if (log == 0 || tiles <= clusters) break;
+  }
+  cfg.gridDim = dim3((unsigned)(std::min(tiles, clusters) * pair * p.split));
   cfg.numAttrs = 2;
   AWQB_CUDA(cudaLaunchKernelEx(&cfg, kernel, tw, tx, p));
   return kOk;
@@ -552,8 +721,20 @@ int launch(const void* codes, const void* w, Params p, cudaStream_t stream) {
 
 template <typename T, bool kNv>
 int pick(const void* codes, const void* w, const Params& p, cudaStream_t stream) {
-  if (p.rows > 24 * p.E) return launch<T, kNv, true>(codes, w, p, stream);
-  return launch<T, kNv, false>(codes, w, p, stream);
+  const int64_t rows = (p.rows + p.E - 1) / p.E;  // of a group, on average
+#ifdef TUNE
+  const char* f = getenv("FP4K");
+  const char* sp = getenv("FP4S");
+  if (f) {
+    const int ms = sp ? atoi(sp) : 1;
+    if (f[0] == 'm') return launch<Many>(fp4_gemm_many_kernel<T, kNv>, 2, codes, w, p, ms, stream);
+    if (f[0] == 's') return launch<Few<32>>(fp4_gemm_few_kernel<T, kNv, 32>, 1, codes, w, p, ms, stream);
+    return launch<Few<64>>(fp4_gemm_few_kernel<T, kNv, 64>, 1, codes, w, p, ms, stream);
+  }
+#endif
+  if (rows > 64) return launch<Many>(fp4_gemm_many_kernel<T, kNv>, 2, codes, w, p, 4, stream);
+  if (rows > 16) return launch<Few<64>>(fp4_gemm_few_kernel<T, kNv, 64>, 1, codes, w, p, 8, stream);
+  return launch<Few<32>>(fp4_gemm_few_kernel<T, kNv, 32>, 1, codes, w, p, 8, stream);
 }
 
 }  // namespace

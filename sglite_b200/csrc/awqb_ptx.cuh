@@ -137,6 +137,13 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, int3
       : "memory");
 }
 
+// The same box into L2 only: no shared memory, no barrier, and nothing that a later
+// write could leave stale.
+__device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int32_t c0, int32_t c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(tmap), "r"(c0), "r"(c1)
+               : "memory");
+}
+
 // 3-D tiled TMA load (no multicast); c0 is the innermost coordinate.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, int32_t c0, int32_t c1, int32_t c2,
                                             uint32_t bar, uint64_t policy) {
@@ -480,17 +487,29 @@ __host__ __device__ constexpr uint32_t make_idesc_fp4(int m, int n, bool nv, int
          | ((uint32_t)(m >> 7) << 27)     // M >> 7
          | ((uint32_t)(2 * half) << 29);  // A scales: byte of the word
 }
-// D[tmem] (+)= A[smem] * B[smem]^T over 64 k, A's and B's scales in tensor memory.
+// The lower half of a K-major operand's descriptor (128-byte swizzle); the upper half is
+// kDescHigh for all.
+__device__ __forceinline__ uint32_t desc_low(uint32_t smem_addr) { return ((smem_addr & 0x3FFFFu) >> 4) | 1u << 16; }
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+
+// The following are issued by the lane whose `pred` is set, in code that the whole warp
+// runs: a branch around them would take their operands off the uniform registers.
+//
+// D[tmem] (+)= A[smem] * B[smem]^T over 64 k, A's and B's scales in tensor memory (at
+// columns that are multiples of four).
 #define AWQB_FP4_MMA(group, kind, vec)                                                                         \
   asm volatile(                                                                                                \
-      "{\n\t.reg .pred p;\n\t"                                                                                 \
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"                                                           \
       "setp.ne.b32 p, %6, 0;\n\t"                                                                              \
-      "tcgen05.mma.cta_group::" group ".kind::" kind ".block_scale.scale_vec::" vec                            \
-      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),                                                  \
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)                      \
+      "setp.ne.b32 q, %7, 0;\n\t"                                                                              \
+      "mov.b64 a, {%1, %8};\n\t"                                                                               \
+      "mov.b64 b, {%2, %8};\n\t"                                                                               \
+      "@q tcgen05.mma.cta_group::" group ".kind::" kind ".block_scale.scale_vec::" vec                         \
+      " [%0], a, b, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),                                                    \
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate), "r"(pred), "n"(kDescHigh) \
       : "memory")
 template <bool kNv, bool kPair>
-__device__ __forceinline__ void tc_mma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+__device__ __forceinline__ void tc_mma_fp4(uint32_t pred, uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc,
                                            uint32_t a_scales, uint32_t b_scales, uint32_t accumulate) {
   if (kNv && kPair)
     AWQB_FP4_MMA("2", "mxf4nvf4", "4X");
@@ -504,16 +523,39 @@ __device__ __forceinline__ void tc_mma_fp4(uint32_t d_tmem, uint64_t a_desc, uin
 #undef AWQB_FP4_MMA
 // 32 rows of 16 bytes from shared to tensor memory (four columns), the same for each
 // quarter of its lanes; for a pair, in both CTAs. In order with the products that the
-// same thread issues afterwards.
+// same thread issues afterwards. No swizzle, K-major: 8-row groups 128 bytes apart.
 template <bool kPair>
-__device__ __forceinline__ void tc_copy_scales(uint32_t d_tmem, uint32_t smem_addr) {
-  // no swizzle, K-major: 8-row groups 128 bytes apart
-  const uint64_t desc = (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)(128u >> 4) << 16 |
-                        (uint64_t)(128u >> 4) << 32 | (uint64_t)1 << 46;
+__device__ __forceinline__ void tc_copy_scales(uint32_t pred, uint32_t d_tmem, uint32_t smem_addr) {
+  const uint32_t low = ((smem_addr & 0x3FFFFu) >> 4) | (128u >> 4) << 16;
+#define AWQB_SCALES_CP(group)                                                          \
+  asm volatile(                                                                        \
+      "{\n\t.reg .pred q;\n\t.reg .b64 a;\n\t"                                         \
+      "setp.ne.b32 q, %2, 0;\n\t"                                                      \
+      "mov.b64 a, {%1, %3};\n\t"                                                       \
+      "@q tcgen05.cp.cta_group::" group ".32x128b.warpx4 [%0], a;\n\t}" ::"r"(d_tmem), \
+      "r"(low), "r"(pred), "n"((128u >> 4) | 1u << 14)                                 \
+      : "memory")
   if (kPair)
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(d_tmem), "l"(desc) : "memory");
+    AWQB_SCALES_CP("2");
   else
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(d_tmem), "l"(desc) : "memory");
+    AWQB_SCALES_CP("1");
+#undef AWQB_SCALES_CP
+}
+// tc_commit and tc_commit_pair by the lane whose `pred` is set.
+__device__ __forceinline__ void tc_commit_if(uint32_t pred, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(pred)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit_pair_if(uint32_t pred, uint32_t bar, uint16_t mask) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(
+          bar),
+      "h"(mask), "r"(pred)
+      : "memory");
 }
 
 // Arrive on a barrier anywhere in the cluster (a shared::cluster address).

@@ -243,6 +243,15 @@ def test_gemm_epilogues(cuda, M, K, N, fmt, silu, bias):
     _product(cuda, M, K, N, fmt, torch.bfloat16, silu, bias, ldo=8)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M", [1, 5, 31, 33, 64, 65, 100, 230, 333, 449])
+@pytest.mark.parametrize("K,N,silu", [(1056, 264, False), (4128, 136, False), (8192, 400, True), (2304, 16, True)])
+def test_gemm_shared_k(cuda, M, K, N, silu, fmt):
+    """Few tiles and a long K, which several CTAs then share."""
+    got = _product(cuda, M, K, N, fmt, torch.bfloat16, silu, bias=True, ldo=8)
+    assert torch.equal(got, _product(cuda, M, K, N, fmt, torch.bfloat16, silu, bias=True, ldo=8))
+
+
 @pytest.mark.parametrize("M", [1, 2, 8, 15, 16, 31, 32, 48, 63, 96, 127, 129, 255, 256, 257, 400, 511, 600])
 def test_gemm_row_counts(cuda, M):
     _product(cuda, M, 320, 272, "nvfp4", torch.bfloat16)
