@@ -44,6 +44,7 @@ struct Params {
   uint32_t* err;
   int64_t ldo, out_rows;
   int rows, E, K, N, n_out, silu, feat_tiles, tile_out;  // tile_out: weight rows of a tile
+  int box;    // of all tiles, or -1: by their rows
   int split;  // CTAs (pairs) of a cluster that share a tile's K; above 1, a cluster has one tile
 };
 
@@ -56,21 +57,33 @@ struct Few {
   static constexpr int kRound = 16;
   static constexpr int kStages = kTok > 32 ? 3 : 4;
   static constexpr int kEpiWarps = 4;
-  static constexpr int kThreads = 32 * (kEpiWarps + 3);
+  static constexpr int kThreads = 32 * (kEpiWarps + 4);
+  static constexpr int kPlans = 4, kCtasPerSm = 2;
   static constexpr int kAtX = kWBytes, kAtWs = kAtX + kTok * kK / 2, kAtXs = kAtWs + 2048;
   static constexpr int kStageBytes = kAtXs + 2048;
   static constexpr int kSets = 2 * kTok, kSetColumns = 32, kColumns = kTok > 32 ? 256 : 128;
 };
-// A CTA pair; each loads its 128 weight rows and half the tokens, and the scales of all tokens.
+// A CTA pair; each loads its 128 weight rows and half the tokens, and the scales of all
+// tokens. The accumulators and scales of 208 tokens fill tensor memory.
 struct Many {
-  static constexpr int kTok = 224;  // two accumulators and the scales fill tensor memory
-  static constexpr int kRound = 32;
-  static constexpr int kStages = 5;
+  static constexpr int kTok = 208;
+  static constexpr int kRound = 16;
+  static constexpr int kStages = 6;
   static constexpr int kEpiWarps = 8;
-  static constexpr int kThreads = 32 * (kEpiWarps + 3);
+  static constexpr int kThreads = 32 * (kEpiWarps + 5);
+  static constexpr int kPlans = 2, kCtasPerSm = 1;
   static constexpr int kAtX = kWBytes, kAtWs = kAtX + kTok / 2 * kK / 2, kAtXs = kAtWs + 2048;
   static constexpr int kStageBytes = kAtXs + 4096;
-  static constexpr int kSets = 2 * kTok, kColumns = 512;
+  static constexpr int kSets = 2 * kTok, kSetColumns = 48, kColumns = 512;
+};
+
+// What the roles need to know of a tile, found by one warp ahead of them: the tile, then
+// (a barrier later, since they come from memory) where its rows go.
+template <typename C>
+struct Plans {
+  uint64_t tile_full[C::kPlans], rows_full[C::kPlans], free[C::kPlans];
+  Tile tile[C::kPlans];
+  float alpha[C::kPlans];
 };
 
 // Bytes of a stage's weight scales.
@@ -88,23 +101,31 @@ __device__ __forceinline__ int first_word(int kb) { return kNv ? 0 : 2 * (kb & 1
 // of the four goes to tile w. (Tiles of up to 32 rows take it too: an instruction's scales
 // have to begin at a column that is a multiple of four, so a row's four words cannot be
 // left in neighbouring columns.)
+template <int kBlocks>
 __device__ __forceinline__ void turn_scales(uint8_t* at, int rows, int lane) {
+  uint4* p = reinterpret_cast<uint4*>(at) + lane;
   if (rows <= 32) {
-    const uint4 a = reinterpret_cast<uint4*>(at)[lane];
-    uint32_t* p = reinterpret_cast<uint32_t*>(at) + 4 * lane;
-    p[0] = a.x;
-    p[128] = a.y;
-    p[256] = a.z;
-    p[384] = a.w;
-    return;
-  }
-  for (int r = 0; r < rows; r += 128, at += 2048) {
-    uint4* p = reinterpret_cast<uint4*>(at) + lane;
-    const uint4 a = p[0], b = p[32], c = p[64], d = p[96];
-    p[0] = make_uint4(a.x, b.x, c.x, d.x);
-    p[32] = make_uint4(a.y, b.y, c.y, d.y);
-    p[64] = make_uint4(a.z, b.z, c.z, d.z);
-    p[96] = make_uint4(a.w, b.w, c.w, d.w);
+    const uint4 a = p[0];
+    uint32_t* q = reinterpret_cast<uint32_t*>(p);
+    q[0] = a.x, q[128] = a.y, q[256] = a.z, q[384] = a.w;
+  } else if (rows <= 64) {
+    const uint4 a = p[0], b = p[32];
+    uint2* q = reinterpret_cast<uint2*>(p);
+    q[0] = make_uint2(a.x, b.x), q[64] = make_uint2(a.y, b.y), q[128] = make_uint2(a.z, b.z), q[192] = make_uint2(a.w, b.w);
+  } else {
+    uint4 v[kBlocks][4];  // all loads before the first store
+#pragma unroll
+    for (int i = 0; i < 4 * kBlocks; ++i)
+      if (i < 4 || rows > 128) v[i / 4][i % 4] = p[32 * i];
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) {
+      if (i > 0 && rows <= 128) break;
+      const uint4 a = v[i][0], b = v[i][1], c = v[i][2], d = v[i][3];
+      p[128 * i] = make_uint4(a.x, b.x, c.x, d.x);
+      p[128 * i + 32] = make_uint4(a.y, b.y, c.y, d.y);
+      p[128 * i + 64] = make_uint4(a.z, b.z, c.z, d.z);
+      p[128 * i + 96] = make_uint4(a.w, b.w, c.w, d.w);
+    }
   }
 }
 
@@ -124,19 +145,65 @@ __device__ __forceinline__ void store_two(const Params& p, float (&y)[2], const 
   }
 }
 
-// The out row and the factor of a tile's row i, by one thread each, a tile ahead of use.
-struct RowTo {
-  int to;
-  float factor;
-};
-__device__ __forceinline__ RowTo row_to(const Params& p, const Tile& tile, int i) {
-  RowTo r = {-1, 0.f};
-  if (i >= tile.rows) return r;
-  const int to = p.row_map ? p.row_map[tile.row0 + i] : tile.row0 + i;
-  if (to < 0 || to >= p.out_rows) return r;
-  r.to = to;
-  if (p.row_scale) r.factor = p.row_scale[to];
-  return r;
+template <typename C>
+__device__ __forceinline__ void init_plans(Plans<C>& plans) {
+  for (int i = 0; i < C::kPlans; ++i) {
+    mbar_init(smem_u32(&plans.tile_full[i]), 1);
+    mbar_init(smem_u32(&plans.rows_full[i]), 1);
+    mbar_init(smem_u32(&plans.free[i]), C::kEpiWarps);
+  }
+}
+
+// The planning warp: tiles first_tile, first_tile + tile_step .. A plan is free again when
+// the epilogue, its last reader, is done with it.
+template <typename C>
+__device__ __forceinline__ bool plan_tiles(Plans<C>& plans, const Groups& g, const Params& p, int first_tile,
+                                           int tile_step, int* dst, float* scl, int lane) {
+  const int total = g.tile0[p.E];
+  int i = 0;
+  for (int t = first_tile; t < total; t += tile_step, ++i) {
+    const int at = i % C::kPlans;
+    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&plans.free[at]), ((i / C::kPlans) & 1) ^ 1))) return false;
+    const Tile tile = find_tile<C>(g, p, t);
+    if (lane == 0) {
+      plans.tile[at] = tile;
+      mbar_arrive(smem_u32(&plans.tile_full[at]));
+    }
+    float alpha = p.x_scale ? *p.x_scale : 1.f;
+    if (p.w_scale) alpha *= p.w_scale[tile.e];
+    constexpr int kMine = (C::kTok + 31) / 32;  // rows of a lane: all their loads in flight
+    int to[kMine];
+    float factor[kMine];
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      const int r = 32 * j + lane;
+      to[j] = r >= tile.rows ? -1 : p.row_map ? p.row_map[tile.row0 + r] : tile.row0 + r;
+    }
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      if (to[j] >= p.out_rows) to[j] = -1;
+      factor[j] = p.row_scale && to[j] >= 0 ? p.row_scale[to[j]] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < kMine; ++j)
+      if (32 * j + lane < C::kTok) {
+        dst[at * C::kTok + 32 * j + lane] = to[j];
+        scl[at * C::kTok + 32 * j + lane] = factor[j];
+      }
+    if (lane == 0) plans.alpha[at] = alpha;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&plans.rows_full[at]));
+  }
+  return true;
+}
+
+// A role's turn to tile number i of this CTA (false: the wait gave up).
+template <typename C>
+__device__ __forceinline__ bool next_tile(Plans<C>& plans, int i, Tile* tile) {
+  const int at = i % C::kPlans;
+  if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&plans.tile_full[at]), (i / C::kPlans) & 1))) return false;
+  *tile = plans.tile[at];
+  return true;
 }
 
 // Stages of K that part `part` of p.split works on.
@@ -146,19 +213,20 @@ __device__ __forceinline__ void stages_of(const Params& p, int nk, int part, int
 }
 
 template <typename T, bool kNv, int kTok>
-__global__ void __launch_bounds__(Few<kTok>::kThreads, 2)
+__global__ void __launch_bounds__(Few<kTok>::kThreads, Few<kTok>::kCtasPerSm)
 fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ TokenMaps tm_x,
                     const __grid_constant__ Params p) {
   using C = Few<kTok>;
   extern __shared__ uint8_t raw[];
   uint8_t* ring = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
-  int* dst = reinterpret_cast<int*>(ring + C::kStages * C::kStageBytes);  // [2][kTok] out row of a token
-  float* scl = reinterpret_cast<float*>(dst + 2 * kTok);                  // [2][kTok]
+  int* dst = reinterpret_cast<int*>(ring + C::kStages * C::kStageBytes);  // [kPlans][kTok] out row of a token
+  float* scl = reinterpret_cast<float*>(dst + C::kPlans * kTok);          // [kPlans][kTok] its factor
   Groups g;
-  g.row0 = reinterpret_cast<int*>(scl + 2 * kTok);  // [E] first rows, [E] row counts
+  g.row0 = reinterpret_cast<int*>(scl + C::kPlans * kTok);  // [E] first rows, [E] row counts
   g.tile0 = g.row0 + 2 * p.E;
-  __shared__ uint64_t full[C::kStages], raw_scales[C::kStages], scaled[C::kStages], empty[C::kStages];
+  __shared__ uint64_t full[C::kStages], raw_scales[C::kStages], empty[C::kStages];
   __shared__ uint64_t acc_full[2], acc_empty[2];
+  __shared__ Plans<C> plans;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
 
@@ -170,15 +238,15 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   stages_of(p, nk, part, &kb0, &kb1);
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&full[s]), 2);  // the producer's expectation and the turned scales
       mbar_init(smem_u32(&raw_scales[s]), 1);
-      mbar_init(smem_u32(&scaled[s]), 1);
       mbar_init(smem_u32(&empty[s]), 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&acc_full[b]), 1);
       mbar_init(smem_u32(&acc_empty[b]), C::kEpiWarps);
     }
+    init_plans(plans);
     failed = 0;
     fence_barrier_init();
   }
@@ -201,15 +269,17 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int total = g.tile0[p.E];
+  const int total = __shfl_sync(0xffffffffu, g.tile0[p.E], 0);
   bool ok = true;
 
   if (warp == C::kEpiWarps) {  // ------------------------------------- producer
     const uint64_t keep = policy_evict_normal(), once = policy_evict_first();
-    int it = 0;
-    for (int t = first_tile; t < total && ok; t += tile_step) {
-      const Tile tile = find_tile<C>(g, p, t);
-      const int box = box_of(tile.n, kTok);
+    int it = 0, n_tile = 0;
+    for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
+      Tile tile;
+      ok = next_tile(plans, n_tile, &tile);
+      if (!ok) break;
+      const int box = p.box >= 0 ? p.box : box_of(tile.n, kTok);
       // weights that one token tile reads once need not stay in L2
       const uint64_t wpol = tile.rows == g.row0[p.E + tile.e] ? once : keep;
       const int wrow = tile.e * p.N + tile.feat;
@@ -234,16 +304,19 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       }
     }
   } else if (warp == C::kEpiWarps + 2) {  // ---------------------------- scales of the rows
-    int it = 0;
-    for (int t = first_tile; t < total && ok; t += tile_step) {
+    int it = 0, n_tile = 0;
+    for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
+      Tile tile;
+      ok = next_tile(plans, n_tile, &tile);
+      if (!ok) break;
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int s = it % C::kStages;
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&raw_scales[s]), (it / C::kStages) & 1));
         if (!ok) break;
-        turn_scales(ring + s * C::kStageBytes + C::kAtXs, kTok, lane);
+        turn_scales<1>(ring + s * C::kStageBytes + C::kAtXs, tile.n, lane);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&scaled[s]));
+        if (lane == 0) mbar_arrive(smem_u32(&full[s]));
       }
     }
   } else if (warp == C::kEpiWarps + 1) {  // ---------------------------- MMA
@@ -252,15 +325,17 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem, 0), ring0 = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
     int it = 0, n_tile = 0;
     for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
-      const Tile tile = find_tile<C>(g, p, t);
+      Tile tile;
       const int b = n_tile & 1;
-      ok = mbar_wait(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1);
+      ok = next_tile(plans, n_tile, &tile) &&
+           __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1));
+      if (!ok) break;
       tc_fence_after();
       const uint32_t d = tmem0 + b * kTok;
       const uint32_t idesc = make_idesc_fp4(kFeat, __shfl_sync(0xffffffffu, tile.n, 0), kNv, 0);
-      for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int s = it % C::kStages;
-        ok = mbar_wait(smem_u32(&full[s]), (it / C::kStages) & 1) && mbar_wait(smem_u32(&scaled[s]), (it / C::kStages) & 1);
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[s]), (it / C::kStages) & 1));
         if (!ok) break;
         tc_fence_after();
         const uint32_t base = ring0 + s * C::kStageBytes;
@@ -285,33 +360,27 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
         __syncwarp();
       }
     }
-  } else if (warp < C::kEpiWarps) {  // --------------------------------- epilogue
+  } else if (warp == C::kEpiWarps + 3) {  // ---------------------------- plans
+    ok = plan_tiles(plans, g, p, first_tile, tile_step, dst, scl, lane);
+  } else {  // -------------------------------------------------------- epilogue
     // A lane holds a weight row's tokens. Neighbouring lanes write neighbouring features
     // of a token. With silu_mul even lanes hold gate and odd lanes up rows: of a pair of
     // tokens a lane keeps one and gives its neighbour the other. A tile whose K is shared
     // is summed after the barrier below: each CTA leaves its part in its ring, [token][row].
     const int tid = threadIdx.x, odd = lane & 1;
     int n_tile = 0;
-    Tile tile = {};
-    if (first_tile < total) {
-      tile = find_tile<C>(g, p, first_tile);
-      const RowTo r = row_to(p, tile, tid);
-      if (tid < kTok) dst[tid] = r.to, scl[tid] = r.factor;
-    }
-    const float xs = p.x_scale ? *p.x_scale : 1.f;
     for (int t = first_tile; t < total; t += tile_step, ++n_tile) {
-      const int b = n_tile & 1;
-      Tile next = {};
-      if (t + tile_step < total) next = find_tile<C>(g, p, t + tile_step);
-      const RowTo r = row_to(p, next, tid);
+      const int b = n_tile & 1, at = n_tile % C::kPlans;
+      ok = mbar_wait(smem_u32(&plans.rows_full[at]), (n_tile / C::kPlans) & 1);
+      const Tile tile = plans.tile[at];
+      const float alpha = plans.alpha[at];
       const int row = tile.feat + tid;  // of the weights
-      const float alpha = xs * (p.w_scale ? p.w_scale[tile.e] : 1.f);
       const float bias = p.bias && row < p.N ? (float)static_cast<const T*>(p.bias)[row] : 0.f;
-      ok = named_bar_and(1, 128, mbar_wait(smem_u32(&acc_full[b]), (n_tile >> 1) & 1));
+      ok = named_bar_and(1, 128, ok && mbar_wait(smem_u32(&acc_full[b]), (n_tile >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
-      const int* to = dst + b * kTok;
-      const float* factor = scl + b * kTok;
+      const int* to = dst + at * kTok;
+      const float* factor = scl + at * kTok;
       T* out = static_cast<T*>(p.out) + (p.silu ? row / 2 : row);
       for (int c = 0; c < tile.rows; c += 16) {
         uint32_t v[16];
@@ -335,8 +404,9 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
           store_two<T>(p, y, to, factor, c + j, tile.rows, row < p.N, odd, out);
         }
       }
-      tile = next;
-      if (tid < kTok) dst[(b ^ 1) * kTok + tid] = r.to, scl[(b ^ 1) * kTok + tid] = r.factor;
+      if (p.split > 1) break;  // (the plan stays, for the sum)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&plans.free[at]));
     }
   }
   if (!ok && lane == 0) {
@@ -348,9 +418,9 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     // Two tokens at a time by turns: CTA `part` adds the parts in their order.
     cluster_sync_all();
     if (warp < C::kEpiWarps && first_tile < total) {
-      const Tile tile = find_tile<C>(g, p, first_tile);
+      const Tile tile = plans.tile[0];
       const int tid = threadIdx.x, odd = lane & 1, row = tile.feat + tid;
-      const float alpha = (p.x_scale ? *p.x_scale : 1.f) * (p.w_scale ? p.w_scale[0] : 1.f);
+      const float alpha = plans.alpha[0];
       const float bias = p.bias && row < p.N ? (float)static_cast<const T*>(p.bias)[row] : 0.f;
       T* out = static_cast<T*>(p.out) + (p.silu ? row / 2 : row);
       const uint32_t mine = smem_u32(ring) + tid * 4;
@@ -385,9 +455,9 @@ template <typename T>
 struct ManyStore {
   float alpha, bias;
   int f, lane;  // the first of the eight features that this lane writes
-  __device__ __forceinline__ ManyStore(const Params& p, const Tile& tile, int rank, int quarter, int lane_) : lane(lane_) {
+  __device__ __forceinline__ ManyStore(const Params& p, const Tile& tile, float alpha_, int rank, int quarter, int lane_)
+      : alpha(alpha_), lane(lane_) {
     const int row = tile.feat + rank * kFeat + quarter * 32;  // of the weights, the warp's first
-    alpha = (p.x_scale ? *p.x_scale : 1.f) * (p.w_scale ? p.w_scale[tile.e] : 1.f);
     bias = p.bias && row + lane < p.N ? (float)static_cast<const T*>(p.bias)[row + lane] : 0.f;
     f = p.silu ? (row + (lane & 16)) / 2 : row + (lane & 24);
   }
@@ -429,13 +499,14 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   using C = Many;
   extern __shared__ uint8_t raw[];
   uint8_t* ring = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
-  int* dst = reinterpret_cast<int*>(ring + C::kStages * C::kStageBytes);  // [2][kTok] out row of a token
-  float* scl = reinterpret_cast<float*>(dst + 2 * C::kTok);               // [2][kTok]
+  int* dst = reinterpret_cast<int*>(ring + C::kStages * C::kStageBytes);  // [kPlans][kTok] out row of a token
+  float* scl = reinterpret_cast<float*>(dst + C::kPlans * C::kTok);       // [kPlans][kTok] its factor
   Groups g;
-  g.row0 = reinterpret_cast<int*>(scl + 2 * C::kTok);
+  g.row0 = reinterpret_cast<int*>(scl + C::kPlans * C::kTok);
   g.tile0 = g.row0 + 2 * p.E;
-  __shared__ uint64_t full[C::kStages], raw_scales[C::kStages], scaled[C::kStages], empty[C::kStages];
+  __shared__ uint64_t full[C::kStages], raw_scales[C::kStages], empty[C::kStages];
   __shared__ uint64_t acc_full[2], acc_empty[2];
+  __shared__ Plans<C> plans;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
 
@@ -450,15 +521,15 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   stages_of(p, nk, part, &kb0, &kb1);
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&full[s]), 3);  // the leader's expectation and both CTAs' turned scales
       mbar_init(smem_u32(&raw_scales[s]), 1);
-      mbar_init(smem_u32(&scaled[s]), 2);  // both CTAs' scales
       mbar_init(smem_u32(&empty[s]), 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&acc_full[b]), 1);
       mbar_init(smem_u32(&acc_empty[b]), 2 * C::kEpiWarps);
     }
+    init_plans(plans);
     failed = 0;
     fence_barrier_init();
   }
@@ -481,16 +552,18 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int total = g.tile0[p.E];
+  const int total = __shfl_sync(0xffffffffu, g.tile0[p.E], 0);
   bool ok = true;
 
   if (warp == C::kEpiWarps) {  // ------------------------------------- producer
     const uint64_t keep = policy_evict_normal(), once = policy_evict_first();
     const int scale_tiles = (p.N + kFeat - 1) / kFeat;
-    int it = 0;
-    for (int t = first_tile; t < total && ok; t += tile_step) {
-      const Tile tile = find_tile<C>(g, p, t);
-      const int box = box_of(tile.n / 2, C::kTok / 2);
+    int it = 0, n_tile = 0;
+    for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
+      Tile tile;
+      ok = next_tile(plans, n_tile, &tile);
+      if (!ok) break;
+      const int box = p.box >= 0 ? p.box : box_of(tile.n / 2, C::kTok / 2);
       // weights that one token tile reads once need not stay in L2
       const uint64_t wpol = tile.rows == g.row0[p.E + tile.e] ? once : keep;
       const int feat = tile.feat + (int)rank * kFeat, row = tile.row0 + (int)rank * (tile.n / 2);
@@ -520,18 +593,22 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     // the last stages' releases arrive from the pair's leader before this CTA may leave
     for (int i = max(0, it - C::kStages); i < it && ok; ++i)
       ok = mbar_wait(smem_u32(&empty[i % C::kStages]), (i / C::kStages) & 1);
-  } else if (warp == C::kEpiWarps + 2) {  // ---------------------------- scales of the rows
-    int it = 0;
-    for (int t = first_tile; t < total && ok; t += tile_step) {
-      const Tile tile = find_tile<C>(g, p, t);
+  } else if (warp == C::kEpiWarps + 2 || warp == C::kEpiWarps + 4) {  // -- scales of the rows, by turns
+    const int odd = warp == C::kEpiWarps + 4;
+    int it = 0, n_tile = 0;
+    for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
+      Tile tile;
+      ok = next_tile(plans, n_tile, &tile);
+      if (!ok) break;
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        if ((it & 1) != odd) continue;
         const int s = it % C::kStages;
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&raw_scales[s]), (it / C::kStages) & 1));
         if (!ok) break;
-        turn_scales(ring + s * C::kStageBytes + C::kAtXs, tile.n, lane);
+        turn_scales<2>(ring + s * C::kStageBytes + C::kAtXs, tile.n, lane);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive_peer(mapa_shared(smem_u32(&scaled[s]), leader));
+        if (lane == 0) mbar_arrive_peer(mapa_shared(smem_u32(&full[s]), leader));
       }
     }
   } else if (warp == C::kEpiWarps + 1) {  // ---------------------------- MMA, the leader's
@@ -540,20 +617,23 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem, 0), ring0 = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
     int it = 0, n_tile = 0;
     for (int t = first_tile; t < total && ok && rank == 0; t += tile_step, ++n_tile) {
-      const Tile tile = find_tile<C>(g, p, t);
+      Tile tile;
       const int b = n_tile & 1;
-      ok = mbar_wait(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1);
+      ok = next_tile(plans, n_tile, &tile) &&
+           __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1));
+      if (!ok) break;
       tc_fence_after();
       const int n = __shfl_sync(0xffffffffu, tile.n, 0);
       const uint32_t d = tmem0 + b * C::kTok, idesc = make_idesc_fp4(2 * kFeat, n, kNv, 0);
-      const uint32_t sa = tmem0 + C::kSets, sb = sa + 16;  // a word's columns of row scales: 8 for 256 rows
-      for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int s = it % C::kStages;
-        ok = mbar_wait(smem_u32(&full[s]), (it / C::kStages) & 1) && mbar_wait(smem_u32(&scaled[s]), (it / C::kStages) & 1);
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[s]), (it / C::kStages) & 1));
         if (!ok) break;
         tc_fence_after();
         const uint32_t base = ring0 + s * C::kStageBytes;
         const uint32_t ad = desc_low(base), bd = desc_low(base + C::kAtX);
+        // a word's columns of row scales: 8, for up to 256 rows
+        const uint32_t sa = tmem0 + C::kSets + (it & 1) * C::kSetColumns, sb = sa + 16;
         const int steps = min(kK, p.K - kb * kK + 63) / 64;
         const int words = kNv ? steps : (steps + 1) / 2;
 #pragma unroll
@@ -575,24 +655,19 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
         __syncwarp();
       }
     }
+  } else if (warp == C::kEpiWarps + 3) {  // ---------------------------- plans
+    ok = plan_tiles(plans, g, p, first_tile, tile_step, dst, scl, lane);
   } else {  // -------------------------------------------------------- epilogue
     // Two groups of four warps take turns over 32 tokens.
     const int quarter = warp & 3;
     const uint32_t at = tmem + ((uint32_t)quarter << 21);
     int n_tile = 0;
-    Tile tile = {};
-    if (first_tile < total) {
-      tile = find_tile<C>(g, p, first_tile);
-      const RowTo r = row_to(p, tile, threadIdx.x);
-      if (threadIdx.x < C::kTok) dst[threadIdx.x] = r.to, scl[threadIdx.x] = r.factor;
-    }
     for (int t = first_tile; t < total; t += tile_step, ++n_tile) {
-      const int b = n_tile & 1;
-      Tile next = {};
-      if (t + tile_step < total) next = find_tile<C>(g, p, t + tile_step);
-      const RowTo r = row_to(p, next, threadIdx.x);
-      const ManyStore<T> store(p, tile, (int)rank, quarter, lane);
-      ok = named_bar_and(1, 32 * C::kEpiWarps, mbar_wait(smem_u32(&acc_full[b]), (n_tile >> 1) & 1));
+      const int b = n_tile & 1, slot = n_tile % C::kPlans;
+      ok = mbar_wait(smem_u32(&plans.rows_full[slot]), (n_tile / C::kPlans) & 1);
+      const Tile tile = plans.tile[slot];
+      const ManyStore<T> store(p, tile, plans.alpha[slot], (int)rank, quarter, lane);
+      ok = named_bar_and(1, 32 * C::kEpiWarps, ok && mbar_wait(smem_u32(&acc_full[b]), (n_tile >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
       for (int c = (warp >> 2) * 32; c < tile.rows; c += 64) {
@@ -617,17 +692,15 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
         float v[32];
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(lo[j]), v[16 + j] = __uint_as_float(hi[j]);
-        store(p, tile, v, c, dst + b * C::kTok, scl + b * C::kTok);
+        store(p, tile, v, c, dst + slot * C::kTok, scl + slot * C::kTok);
       }
       if ((warp >> 2) * 32 >= tile.rows) {  // no tokens for this group
         __syncwarp();
         if (lane == 0) mbar_arrive_peer(mapa_shared(smem_u32(&acc_empty[b]), leader));
       }
-      tile = next;
-      if (threadIdx.x < C::kTok) {
-        dst[(b ^ 1) * C::kTok + threadIdx.x] = r.to;
-        scl[(b ^ 1) * C::kTok + threadIdx.x] = r.factor;
-      }
+      if (p.split > 1) break;  // (the plan stays, for the sum)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&plans.free[slot]));
     }
   }
   if (!ok && lane == 0) {
@@ -639,9 +712,9 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     // 32 tokens at a time by turns of the parts and the groups of warps, added in the parts' order
     cluster_sync_all();
     if (warp < C::kEpiWarps && first_tile < total) {
-      const Tile tile = find_tile<C>(g, p, first_tile);
+      const Tile tile = plans.tile[0];
       const int quarter = warp & 3;
-      const ManyStore<T> store(p, tile, (int)rank, quarter, lane);
+      const ManyStore<T> store(p, tile, plans.alpha[0], (int)rank, quarter, lane);
       const uint32_t mine = smem_u32(ring) + (quarter * 32 + lane) * 4;
       for (int c = (2 * part + (warp >> 2)) * 32; c < tile.rows; c += 64 * p.split) {
         float v[32] = {};
@@ -665,8 +738,8 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   }
 }
 
-template <typename C, typename Kernel>
-int launch(Kernel kernel, int pair, const void* codes, const void* w, Params p, int max_split, cudaStream_t stream) {
+template <typename C, auto kernel>
+int launch(int pair, const void* codes, const void* w, Params p, int max_split, cudaStream_t stream) {
   const int tok_cta = C::kTok / pair;
   p.tile_out = kFeat * pair;
   p.feat_tiles = (p.N + p.tile_out - 1) / p.tile_out;
@@ -674,15 +747,25 @@ int launch(Kernel kernel, int pair, const void* codes, const void* w, Params p, 
   TokenMaps tx;
   const int64_t row_bytes = p.K / 2;
   int st = make_bytes_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, (int64_t)p.E * p.N, row_bytes, row_bytes, kFeat);
+  // without groups all tiles take the first, largest tile's box
+  const int tok_tiles = (p.rows + C::kTok - 1) / C::kTok;
+  const int n = ((p.rows + tok_tiles - 1) / tok_tiles + C::kRound - 1) / C::kRound * C::kRound;
+  p.box = p.offsets ? -1 : box_of(n / pair, tok_cta);
   for (int i = 0; i < 3 && st == kOk; ++i)
-    st = make_bytes_map(&tx.box[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, p.rows, row_bytes, row_bytes,
-                        tok_cta >> (2 - i));
+    if (p.box < 0 || i == p.box)
+      st = make_bytes_map(&tx.box[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, p.rows, row_bytes, row_bytes,
+                          tok_cta >> (2 - i));
   if (st != kOk) return st;
-  const auto smem_for = [](int E) { return 1024 + C::kStages * C::kStageBytes + 4 * C::kTok * 4 + (3 * E + 1) * 4; };
-  // (the most that any call wants: another thread's call may set it before this launch)
-  AWQB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_for(kMaxExperts)));
-  // all of it, so that two CTAs of the few-rows kernel fit an SM
-  AWQB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
+  const auto smem_for = [](int E) { return 1024 + C::kStages * C::kStageBytes + 2 * C::kPlans * C::kTok * 4 + (3 * E + 1) * 4; };
+  static std::atomic<bool> ready[64];  // the kernel's attributes, set once for a device
+  int dev = 0;
+  AWQB_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !ready[dev].load()) {
+    AWQB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_for(kMaxExperts)));
+    // all of it, so that two CTAs of the few-rows kernel fit an SM
+    AWQB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
+    if (dev < 64) ready[dev].store(true);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = smem_for(p.E);
@@ -701,7 +784,7 @@ int launch(Kernel kernel, int pair, const void* codes, const void* w, Params p, 
   static std::atomic<int> cached[4][64];
   const int nk = (p.K + kK - 1) / kK;
   int64_t clusters = 0;
-  int log = 3;
+  int log = 3;  // up to 8
   if (p.offsets != nullptr) max_split = 1;
   for (;; --log) {
     p.split = 1 << log;
@@ -711,6 +794,7 @@ int launch(Kernel kernel, int pair, const void* codes, const void* w, Params p, 
     cfg.numAttrs = 1;
     st = max_clusters(kernel, cfg, cached[log], &clusters);
     if (st != kOk) return st;
+    clusters *= C::kCtasPerSm;  // (the query counts one for kernels with tensor memory)
     if (log == 0 || tiles <= clusters) break;
   }
   cfg.gridDim = dim3((unsigned)(std::min(tiles, clusters) * pair * p.split));
@@ -727,14 +811,14 @@ int pick(const void* codes, const void* w, const Params& p, cudaStream_t stream)
   const char* sp = getenv("FP4S");
   if (f) {
     const int ms = sp ? atoi(sp) : 1;
-    if (f[0] == 'm') return launch<Many>(fp4_gemm_many_kernel<T, kNv>, 2, codes, w, p, ms, stream);
-    if (f[0] == 's') return launch<Few<32>>(fp4_gemm_few_kernel<T, kNv, 32>, 1, codes, w, p, ms, stream);
-    return launch<Few<64>>(fp4_gemm_few_kernel<T, kNv, 64>, 1, codes, w, p, ms, stream);
+    if (f[0] == 'm') return launch<Many, fp4_gemm_many_kernel<T, kNv>>(2, codes, w, p, ms, stream);
+    if (f[0] == 's') return launch<Few<32>, fp4_gemm_few_kernel<T, kNv, 32>>(1, codes, w, p, ms, stream);
+    return launch<Few<64>, fp4_gemm_few_kernel<T, kNv, 64>>(1, codes, w, p, ms, stream);
   }
 #endif
-  if (rows > 64) return launch<Many>(fp4_gemm_many_kernel<T, kNv>, 2, codes, w, p, 4, stream);
-  if (rows > 16) return launch<Few<64>>(fp4_gemm_few_kernel<T, kNv, 64>, 1, codes, w, p, 8, stream);
-  return launch<Few<32>>(fp4_gemm_few_kernel<T, kNv, 32>, 1, codes, w, p, 8, stream);
+  if (rows > 64) return launch<Many, fp4_gemm_many_kernel<T, kNv>>(2, codes, w, p, 4, stream);
+  if (rows > 16) return launch<Few<64>, fp4_gemm_few_kernel<T, kNv, 64>>(1, codes, w, p, 8, stream);
+  return launch<Few<32>, fp4_gemm_few_kernel<T, kNv, 32>>(1, codes, w, p, 8, stream);
 }
 
 }  // namespace

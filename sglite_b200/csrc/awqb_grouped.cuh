@@ -123,7 +123,7 @@ __device__ __forceinline__ uint4 transpose8(const float* v, int lane) {
 }
 
 // The smallest box that holds `rows` token rows.
-__device__ __forceinline__ int box_of(int rows, int most) { return rows * 4 <= most ? 0 : rows * 2 <= most ? 1 : 2; }
+__host__ __device__ __forceinline__ int box_of(int rows, int most) { return rows * 4 <= most ? 0 : rows * 2 <= most ? 1 : 2; }
 
 // Clusters that run at once (a GPC with an odd number of SMs leaves one idle),
 // per device; the persistent grid must not exceed it.
