@@ -17,6 +17,8 @@
 
 #include <cstdint>
 
+#include "awqb_vec.cuh"
+
 namespace awqb {
 
 // Scales of a row that stand side by side in a granule of 16 bytes.
@@ -86,41 +88,81 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
 template <bool kNv>
 __device__ __forceinline__ uint32_t block_scale(float most) {
   if (!(most <= 3.402823466e38f)) return kNv ? 0x7fu : 0xffu;
-  if (kNv) return e4m3_byte(fminf(__fdiv_rn(most, 6.f), 448.f));
+  if (kNv) {  // most / 6, correctly rounded as in block_codes
+    const float sixth = 1.f / 6.f, q = most * sixth;
+    return e4m3_byte(fminf(fmaf(fmaf(-q, 6.f, most), sixth, q), 448.f));
+  }
   const int e = (int)(__float_as_uint(most) >> 23) - 2;
   return (uint32_t)max(e, 0);
 }
 
-// 16 values of one block (mxfp4: half of one) over its scale, as codes.
-template <bool kNv>
-__device__ __forceinline__ uint2 block_codes(const float (&u)[16], uint32_t byte) {
-  float v[16];
+// 8 L values of a block over its scale, as codes.
+template <bool kNv, int L>
+__device__ __forceinline__ void block_codes(const float (&u)[8 * L], uint32_t byte, uint32_t (&codes)[L]) {
+  float v[8 * L];
+  const bool none = kNv ? byte == 0u || byte == 0x7fu : byte == 0xffu;
   if (kNv) {
-    if (byte == 0u || byte == 0x7fu) return make_uint2(0u, 0u);
     // u / s, correctly rounded: s has few bits, so one correction of u * (1 / s) is enough
     const float s = e4m3_value(byte), r = __frcp_rn(s);
+    const float2 rr = make_float2(r, r), minus = make_float2(-s, -s);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float y = u[j] * r;
-      v[j] = fmaf(fmaf(-y, s, u[j]), r, y);
+    for (int j = 0; j < 8 * L; j += 2) {
+      const float2 x = make_float2(u[j], u[j + 1]), y = mul2(x, rr), z = fma2(fma2(y, minus, x), rr, y);
+      v[j] = z.x, v[j + 1] = z.y;
     }
   } else {
-    if (byte == 0xffu) return make_uint2(0u, 0u);
     // 1 / s = 2^(127 - byte); byte <= 252, so this is a normal number. The product is exact
     // (or far below the smallest value's half)
     const float r = __uint_as_float((254u - byte) << 23);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = u[j] * r;
+    for (int j = 0; j < 8 * L; ++j) v[j] = u[j] * r;
   }
-  return make_uint2(e2m1x8(v), e2m1x8(v + 8));
+#pragma unroll
+  for (int i = 0; i < L; ++i) {
+    const uint32_t c = e2m1x8(v + 8 * i);
+    codes[i] = none ? 0u : c;
+  }
 }
 
-// Where the scales of a row's 16 values number `item` (of 16) stand: granules of 16
-// bytes, [granule][row][16]. mxfp4: the second half of a block shares the first one's.
-template <bool kNv>
-__device__ __forceinline__ int64_t scale_at(int64_t rows, int64_t row, int item) {
-  const int i = kNv ? item : item >> 1;
-  return ((int64_t)(i / kGranule) * rows + row) * kGranule + i % kGranule;
+// A row is worked on in vectors of 8 L values, by neighbouring lanes: kBlock of them make
+// a block. kPer vectors go with a granule of scales.
+template <bool kNv, int L>
+struct Vectors {
+  static constexpr int kBlock = (kNv ? 2 : 4) / L;
+  static constexpr int kPer = kBlock * kGranule;
+  // of a row of K values, whole granules
+  static __host__ __device__ constexpr int count(int K) { return (K / (8 * L) + kPer - 1) / kPer * kPer; }
+  // the byte of vector v's scale, [granule][row][16]
+  static __device__ __forceinline__ int64_t at(int64_t rows, int64_t row, int v) {
+    const int i = v / kBlock;
+    return ((int64_t)(i / kGranule) * rows + row) * kGranule + i % kGranule;
+  }
+};
+
+// A vector's codes and, by the first of the lanes whose blocks' four scales make a word,
+// those. All lanes of a warp; `most` is the vector's own largest magnitude.
+template <bool kNv, int L>
+__device__ __forceinline__ void store_vector(const float (&u)[8 * L], float most, void* codes, uint8_t* scales,
+                                             int64_t rows, int64_t row, int K, int v, bool real) {
+  using V = Vectors<kNv, L>;
+#pragma unroll
+  for (int o = 1; o < V::kBlock; o *= 2) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const bool inside = v * 8 * L < K;
+  const uint32_t byte = inside ? block_scale<kNv>(most) : 0u;
+  uint32_t w = byte << (8 * (v / V::kBlock % 4));
+  w |= __shfl_xor_sync(0xffffffffu, w, V::kBlock);
+  w |= __shfl_xor_sync(0xffffffffu, w, 2 * V::kBlock);
+  if (!real) return;
+  if (inside) {
+    uint32_t c[L];
+    block_codes<kNv, L>(u, byte, c);
+    uint32_t* to = static_cast<uint32_t*>(codes) + row * (K / 8) + v * L;
+    if (L == 2)
+      *reinterpret_cast<uint2*>(to) = make_uint2(c[0], c[L - 1]);
+    else
+      *to = c[0];
+  }
+  if (v % (4 * V::kBlock) == 0) *reinterpret_cast<uint32_t*>(scales + V::at(rows, row, v)) = w;
 }
 
 }  // namespace awqb

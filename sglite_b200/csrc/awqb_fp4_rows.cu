@@ -2,8 +2,9 @@
 // residual-add RMSNorm that writes its result in four bits (awqb_fp4.cuh has the
 // formats).
 //
-// All three are bound by HBM. A thread takes 16 values: two 16-byte loads, eight bytes
-// of codes; four scales leave as one word.
+// All three are bound by HBM. A lane takes vectors of eight values (16-byte loads, whole
+// sectors by neighbouring lanes); all of a thread's loads are issued before the first is
+// used. Launched with programmatic dependent launch, like the other norms.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -19,11 +20,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Threads of a row: one per 16 values, rounded up to whole granules of scales.
-__host__ __device__ constexpr int items_of(int K, bool nv) {
-  return nv ? (K + 255) / 256 * 16 : (K + 511) / 512 * 32;
-}
-
 struct RowsArgs {
   const void* x;
   const float* scale;
@@ -31,54 +27,89 @@ struct RowsArgs {
   void* codes;
   uint8_t* scales;
   int64_t ldx, rows_in, rows;
-  int K, items, per_row;
+  int K, vecs, per_row;
 };
 
-// Stores a thread's codes and, by the first of four (mxfp4: eight) neighbours, four scales.
-template <bool kNv>
-__device__ __forceinline__ void store_block(void* codes, uint8_t* scales, int64_t rows, int64_t row, int K, int item,
-                                            uint2 c, uint32_t byte, bool real) {
-  constexpr int kStep = kNv ? 1 : 2;
-  uint32_t w = byte << (8 * (item / kStep % 4));
-  w |= __shfl_xor_sync(0xffffffffu, w, kStep);
-  w |= __shfl_xor_sync(0xffffffffu, w, 2 * kStep);
-  if (!real) return;
-  if (item * 16 < K) reinterpret_cast<uint2*>(codes)[row * (K / 16) + item] = c;
-  if (item % (4 * kStep) == 0) *reinterpret_cast<uint32_t*>(scales + scale_at<kNv>(rows, row, item)) = w;
+// Threads (x: vectors, y: rows) of a CTA of about kThreads, and CTAs over a row.
+struct Shape {
+  int x, y, over;
+};
+inline Shape shape_of(int vecs) {
+  Shape s;
+  s.over = (vecs + kThreads - 1) / kThreads;
+  s.x = ((vecs + s.over - 1) / s.over + 31) / 32 * 32;
+  s.y = std::max(1, kThreads / s.x);
+  return s;
 }
 
-template <typename T, bool kNv>
+// The largest magnitude of the 16-bit values of some words, NaN if one is.
+template <typename T>
+struct Most;
+template <>
+struct Most<__half> {
+  static __device__ __forceinline__ uint32_t pair(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7fff7fffu), "r"(b & 0x7fff7fffu));
+    return r;
+  }
+};
+template <>
+struct Most<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pair(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7fff7fffu), "r"(b & 0x7fff7fffu));
+    return r;
+  }
+};
+
+// kRows rows of a CTA's thread, blockDim.y apart, 16 values of each. The largest magnitude
+// is taken of the 16-bit values, two at a time: multiplying by 1 / scale rounds, and
+// rounding keeps the order.
+template <typename T, bool kNv, int kRows>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const __grid_constant__ RowsArgs a) {
   grid_dep_wait();
   grid_dep_launch();
-  const int64_t t = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t row = t / a.items;
-  const int item = (int)(t - row * a.items);
-  int64_t from = row;
-  bool real = row < a.rows && (a.count == nullptr || row < *a.count);
-  if (real && a.index != nullptr) {
-    from = a.index[row];
-    real = from >= 0;
-    from /= a.per_row;
-  }
-  real = real && from < a.rows_in;
-  float u[16] = {}, most = 0.f;
-  if (real && item * 16 < a.K) {
-    const uint4* xp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + from * a.ldx) + 2 * item;
-    const uint4 x0 = xp[0], x1 = xp[1];
-    float f[2][8];
-    unpack_vec<T>(x0, f[0]);
-    unpack_vec<T>(x1, f[1]);
-    const float inv = kNv && a.scale != nullptr ? __frcp_rn(*a.scale) : 1.f;
+  const int v = blockIdx.y * blockDim.x + threadIdx.x;
+  const int64_t row0 = (int64_t)blockIdx.x * (kRows * blockDim.y) + threadIdx.y;
+  bool real[kRows];
+  uint4 x[kRows][2];
+  const int64_t limit = a.count != nullptr ? min(a.rows, (int64_t)*a.count) : a.rows;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      u[j] = f[j / 8][j % 8] * inv;
-      most = max_nan(most, fabsf(u[j]));
+  for (int i = 0; i < kRows; ++i) {
+    const int64_t row = row0 + i * blockDim.y;
+    real[i] = row < limit && v < a.vecs;
+    int64_t from = row;
+    if (a.index != nullptr && real[i]) {
+      from = a.index[row];
+      real[i] = from >= 0;
+      from = (uint32_t)from / (uint32_t)a.per_row;
+    }
+    real[i] = real[i] && from < a.rows_in;
+    x[i][0] = x[i][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (real[i] && v * 16 < a.K) {
+      const uint4* xp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + from * a.ldx) + 2 * v;
+      x[i][0] = xp[0];
+      x[i][1] = xp[1];
     }
   }
-  if (!kNv) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, 1));
-  const uint32_t byte = item * 16 < a.K ? block_scale<kNv>(most) : 0u;
-  store_block<kNv>(a.codes, a.scales, a.rows, row, a.K, item, block_codes<kNv>(u, byte), byte, real);
+  const float inv = kNv && a.scale != nullptr ? __frcp_rn(*a.scale) : 1.f;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    float f[2][8], u[16];
+    unpack_vec<T>(x[i][0], f[0]);
+    unpack_vec<T>(x[i][1], f[1]);
+    const uint4 p = x[i][0], q = x[i][1];
+    const uint32_t m = Most<T>::pair(Most<T>::pair(Most<T>::pair(p.x, p.y), Most<T>::pair(p.z, p.w)),
+                                     Most<T>::pair(Most<T>::pair(q.x, q.y), Most<T>::pair(q.z, q.w)));
+    const float2 both = Pair<T>::unpack(m);
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float2 t = make_float2(f[j / 8][j % 8], f[j / 8][j % 8 + 1]), s = kNv ? mul2(t, make_float2(inv, inv)) : t;
+      u[j] = s.x, u[j + 1] = s.y;
+    }
+    const float most = max_nan(both.x, both.y);
+    store_vector<kNv, 2>(u, kNv ? most * inv : most, a.codes, a.scales, a.rows, row0 + i * blockDim.y, a.K, v, real[i]);
+  }
 }
 
 struct BackArgs {
@@ -90,26 +121,33 @@ struct BackArgs {
   int K;
 };
 
-template <typename T, bool kNv>
+template <typename T, bool kNv, int kRows>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const __grid_constant__ BackArgs a) {
   grid_dep_wait();
   grid_dep_launch();
-  const int64_t t = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int items = a.K / 16;
-  const int64_t row = t / items;
-  const int item = (int)(t - row * items);
-  if (row >= a.rows) return;
-  const uint2 c = reinterpret_cast<const uint2*>(a.codes)[row * items + item];
-  const float s = scale_value<kNv>(a.scales[scale_at<kNv>(a.rows, row, item)]);
+  const int v = blockIdx.y * blockDim.x + threadIdx.x;
+  if (v * 8 >= a.K) return;
+  const int64_t row0 = (int64_t)blockIdx.x * (kRows * blockDim.y) + threadIdx.y;
+  uint32_t codes[kRows], byte[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int64_t row = row0 + i * blockDim.y;
+    if (row < a.rows) {
+      codes[i] = static_cast<const uint32_t*>(a.codes)[row * (a.K / 8) + v];
+      byte[i] = a.scales[Vectors<kNv, 1>::at(a.rows, row, v)];
+    }
+  }
   const float scale = kNv && a.scale != nullptr ? *a.scale : 1.f;
-  uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.ldo) + 2 * item;
-  float v[8];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    e2m1x8_values(h ? c.y : c.x, v);
+  for (int i = 0; i < kRows; ++i) {
+    const int64_t row = row0 + i * blockDim.y;
+    if (row >= a.rows) return;
+    const float s = scale_value<kNv>(byte[i]);
+    float f[8];
+    e2m1x8_values(codes[i], f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = v[j] * s * scale;  // v * s is exact
-    to[h] = pack_vec<T>(v);
+    for (int j = 0; j < 8; ++j) f[j] = f[j] * s * scale;  // f * s is exact
+    reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.ldo)[v] = pack_vec<T>(f);
   }
 }
 
@@ -119,103 +157,138 @@ struct NormArgs {
   void *residual_out, *codes;
   uint8_t* scales;
   int64_t ldx, ldr, ldro, rows;
-  int K, items;
+  int K, vecs;
   float eps;
+  double inv_K;
 };
 
 constexpr int kNormThreads = 512;
-constexpr int kNormVec = 2;
-constexpr int kNormMaxK = kNormThreads * kNormVec * 16;
+constexpr int kNormVec = 4;  // vectors per thread
+constexpr int kNormMaxK = kNormThreads * kNormVec * 8;
 
 // A CTA takes a row and holds it in registers between the sum of squares and the
 // quantisation. h = x + residual is stored rounded; the norm is of the unrounded sum and
-// goes from fp32 into four bits with no rounding between. The threads' sums of squares
-// are added in 64 bits, so that a row's factor is right to its last bits: a block's
-// codes then differ from the exact ones only within 2^-23 of a border.
+// goes into four bits with no rounding to 16 bits between. A code depends on which side of
+// a border its value lies, so the value is rounded once only: the threads' sums of squares
+// are added in 64 bits, the row's factor (over the tensor's scale) is kept as two fp32
+// numbers, and so is h * weight.
+// h of the thread's vector v, stored; returns its sum of squares.
+template <typename T>
+__device__ __forceinline__ float add_vector(const NormArgs& a, int64_t row, int v, const uint4& x, const uint4& r,
+                                            float (&h)[8]) {
+  unpack_vec<T>(x, h);
+  if (a.residual != nullptr) {
+    float f[8];
+    unpack_vec<T>(r, f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] += f[j];
+    reinterpret_cast<uint4*>(static_cast<T*>(a.residual_out) + row * a.ldro)[v] = pack_vec<T>(h);
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ss += h[j] * h[j];
+  return ss;
+}
+
+// 1 / x to about 2^-44, from its fp32 approximation by one Newton step.
+__device__ __forceinline__ double inverse(float x) {
+  const double y = (double)__fdividef(1.f, x);
+  return fma(fma(-(double)x, y, 1.0), y, y);
+}
+
+// 1 / (rms * scale) of the row, as two fp32 numbers; over: 1 / scale. Each warp adds the
+// warps' sums for itself, so that one barrier is enough.
+__device__ __forceinline__ float2 row_factor(const NormArgs& a, float ss, double over, float* red) {
+  const int warps = blockDim.x / 32, lane = threadIdx.x & 31;
+  ss = warp_sum(ss);
+  if (lane == 0) red[threadIdx.x >> 5] = ss;
+  __syncthreads();
+  double sum = (lane & 15) < warps ? (double)red[lane & 15] : 0.0;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  // 1 / sqrt(m), from its fp32 approximation by one Newton step
+  const double m = fma(sum, a.inv_K, (double)a.eps), y = (double)rsqrtf((float)m);
+  const double f = fma(fma(-m * y, y, 1.0), 0.5 * y, y) * over;
+  const float high = (float)f;
+  return make_float2(high, (float)(f - (double)high));
+}
+
+template <typename T, bool kNv>
+__device__ __forceinline__ void norm_vector(const NormArgs& a, int64_t row, int v, const float (&h)[8], const uint4& w,
+                                            float2 factor) {
+  float u[8] = {}, most = 0.f;
+  if (v * 8 < a.K) {
+    float f[8];
+    unpack_vec<T>(w, f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float p = h[j] * f[j], rest = fmaf(h[j], f[j], -p);
+      u[j] = fmaf(p, factor.x, fmaf(rest, factor.x, p * factor.y));
+      most = max_nan(most, fabsf(u[j]));
+    }
+  }
+  store_vector<kNv, 1>(u, most, a.codes, a.scales, a.rows, row, a.K, v, v < a.vecs);
+}
+
 template <typename T, bool kNv, int kVec>
-__global__ void __launch_bounds__(kNormThreads, kVec == 1 ? 2 : 1) norm_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ double red[kNormThreads / 32];
+__global__ void __launch_bounds__(kNormThreads, kVec <= 2 ? 2 : 1) norm_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float red[kNormThreads / 32];
   grid_dep_wait();
   grid_dep_launch();
   const int64_t row = blockIdx.x;
-  const int nreal = a.K / 16;
-  const T* xp = static_cast<const T*>(a.x) + row * a.ldx;
-  const T* rp = static_cast<const T*>(a.residual) + row * a.ldr;
-  float h[kVec][16];
-  float ss = 0.f;
+  const int nvec = a.K / 8;
+  const uint4* xp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ldx);
+  const uint4* rp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.residual) + row * a.ldr);
+  const double over = kNv && a.scale != nullptr ? inverse(*a.scale) : 1.0;
+  uint4 x[kVec], r[kVec], w[kVec];
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
-    const int item = i * blockDim.x + threadIdx.x;
-    if (item < nreal) {
-      const uint4* xv = reinterpret_cast<const uint4*>(xp) + 2 * item;
-      const uint4 x0 = xv[0], x1 = xv[1];
-      float f[2][8];
-      unpack_vec<T>(x0, f[0]);
-      unpack_vec<T>(x1, f[1]);
-      if (a.residual != nullptr) {
-        const uint4* rv = reinterpret_cast<const uint4*>(rp) + 2 * item;
-        const uint4 r0 = rv[0], r1 = rv[1];
-        float r[2][8];
-        unpack_vec<T>(r0, r[0]);
-        unpack_vec<T>(r1, r[1]);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) f[j / 8][j % 8] += r[j / 8][j % 8];
-        uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.residual_out) + row * a.ldro) + 2 * item;
-        to[0] = pack_vec<T>(f[0]);
-        to[1] = pack_vec<T>(f[1]);
-      }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        h[i][j] = f[j / 8][j % 8];
-        ss += h[i][j] * h[i][j];
-      }
+    const int v = i * blockDim.x + threadIdx.x;
+    if (v < nvec) {
+      x[i] = xp[v];
+      if (a.residual != nullptr) r[i] = rp[v];
     }
   }
-  double sum = ss;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
-  __syncthreads();
-  sum = 0.0;
-  for (int w = 0; w < (int)blockDim.x / 32; ++w) sum += red[w];
-  const float rms = (float)(1.0 / sqrt(sum / a.K + (double)a.eps));
-  const float inv = kNv && a.scale != nullptr ? __frcp_rn(*a.scale) : 1.f;
+  float h[kVec][8], ss = 0.f;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
-    const int item = i * blockDim.x + threadIdx.x;
-    float most = 0.f;
-    if (item < nreal) {
-      const uint4* wv = static_cast<const uint4*>(a.weight) + 2 * item;
-      const uint4 w0 = wv[0], w1 = wv[1];
-      float w[2][8];
-      unpack_vec<T>(w0, w[0]);
-      unpack_vec<T>(w1, w[1]);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        h[i][j] = h[i][j] * rms * w[j / 8][j % 8] * inv;
-        most = max_nan(most, fabsf(h[i][j]));
-      }
+    const int v = i * blockDim.x + threadIdx.x;
+    if (v < nvec) {
+      ss += add_vector<T>(a, row, v, x[i], r[i], h[i]);
     }
-    if (!kNv) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    const uint32_t byte = item < nreal ? block_scale<kNv>(most) : 0u;
-    store_block<kNv>(a.codes, a.scales, a.rows, row, a.K, item, block_codes<kNv>(h[i], byte), byte, item < a.items);
+  }
+  const float2 factor = row_factor(a, ss, over, red);
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int v = i * blockDim.x + threadIdx.x;
+    if (v < nvec) w[i] = static_cast<const uint4*>(a.weight)[v];
+    norm_vector<T, kNv>(a, row, v, h[i], w[i], factor);
   }
 }
 
 template <typename Kernel, typename A>
-int launch(Kernel kernel, const A& a, int64_t blocks, int threads, void* stream) {
-  AWQB_REQUIRE(blocks <= 0x7fffffff, kUnsupported, "too many rows");
+int launch(Kernel kernel, dim3 grid, dim3 threads, void* stream, const A& a) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3((unsigned)threads);
+  cfg.gridDim = grid;
+  cfg.blockDim = threads;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   AWQB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
   return kOk;
+}
+
+// The row kernels' grid: CTAs of a shape, so many rows to a thread as leave every SM
+// several CTAs.
+constexpr int kQuantizeRows = 2, kBackRows = 4;
+inline bool many_rows(const Shape& s, int64_t rows, int per_thread) {
+  return rows * s.over >= (int64_t)8 * per_thread * s.y * device_sm_count();
+}
+inline dim3 grid_of(const Shape& s, int64_t rows, int per_thread) {
+  return dim3((unsigned)((rows + s.y * per_thread - 1) / (s.y * per_thread)), (unsigned)s.over);
 }
 
 // kernel<T, kNv> of the dtype and format, with further template arguments behind.
@@ -248,9 +321,13 @@ extern "C" int awqb_fp4_quantize(const awqb_fp4_quantize_args* args, void* strea
   AWQB_REQUIRE((x || rows_in == 0) && codes && scales, kInvalidArgument, "null pointer");
   AWQB_REQUIRE(aligned16(x) && aligned16(codes) && aligned16(scales), kInvalidArgument, "tensors must be 16-byte aligned");
   const bool nv = format == AWQB_FP4_NV;
-  const int items = items_of((int)K, nv);
-  const RowsArgs a = {x, scale, index, count, codes, scales, ldx, rows_in, rows, (int)K, items, (int)per_row};
-  return launch(AWQB_FP4_PICK(quantize_kernel), a, (rows * items + kThreads - 1) / kThreads, kThreads, stream);
+  const int vecs = nv ? Vectors<true, 2>::count((int)K) : Vectors<false, 2>::count((int)K);
+  const RowsArgs a = {x, scale, index, count, codes, scales, ldx, rows_in, rows, (int)K, vecs, (int)per_row};
+  const Shape s = shape_of(vecs);
+  const dim3 threads(s.x, s.y);
+  if (many_rows(s, rows, kQuantizeRows))
+    return launch(AWQB_FP4_PICK(quantize_kernel, , kQuantizeRows), grid_of(s, rows, kQuantizeRows), threads, stream, a);
+  return launch(AWQB_FP4_PICK(quantize_kernel, , 1), grid_of(s, rows, 1), threads, stream, a);
 }
 
 extern "C" int awqb_fp4_dequantize(const awqb_fp4_dequantize_args* args, void* stream) {
@@ -265,7 +342,11 @@ extern "C" int awqb_fp4_dequantize(const awqb_fp4_dequantize_args* args, void* s
                "tensors must be 16-byte aligned");
   const bool nv = format == AWQB_FP4_NV;
   const BackArgs a = {codes, scales, scale, out, ldo, rows, (int)K};
-  return launch(AWQB_FP4_PICK(dequantize_kernel), a, (rows * (K / 16) + kThreads - 1) / kThreads, kThreads, stream);
+  const Shape s = shape_of((int)K / 8);
+  const dim3 threads(s.x, s.y);
+  if (many_rows(s, rows, kBackRows))
+    return launch(AWQB_FP4_PICK(dequantize_kernel, , kBackRows), grid_of(s, rows, kBackRows), threads, stream, a);
+  return launch(AWQB_FP4_PICK(dequantize_kernel, , 1), grid_of(s, rows, 1), threads, stream, a);
 }
 
 extern "C" int awqb_fp4_add_rmsnorm(const awqb_fp4_add_rmsnorm_args* args, void* stream) {
@@ -285,8 +366,15 @@ extern "C" int awqb_fp4_add_rmsnorm(const awqb_fp4_add_rmsnorm_args* args, void*
                    aligned16(scales),
                kInvalidArgument, "tensors must be 16-byte aligned");
   const bool nv = format == AWQB_FP4_NV;
-  const int items = items_of((int)K, nv);
-  const NormArgs a = {x, residual, weight, scale, residual_out, codes, scales, ldx, ldr, ldro, rows, (int)K, items, eps};
-  if (items <= kNormThreads) return launch(AWQB_FP4_PICK(norm_kernel, , 1), a, rows, (items + 31) / 32 * 32, stream);
-  return launch(AWQB_FP4_PICK(norm_kernel, , 2), a, rows, (items / 2 + 31) / 32 * 32, stream);
+  const int vecs = nv ? Vectors<true, 1>::count((int)K) : Vectors<false, 1>::count((int)K);
+  const NormArgs a = {x, residual, weight, scale, residual_out, codes, scales, ldx, ldr, ldro, rows, (int)K, vecs, eps,
+                      1.0 / (double)K};
+  // Vectors per thread: many rows want small CTAs, more of them to an SM (8192 rows of 4096
+  // features: 48.0 us with one, 40.1 with two; 16 rows of 2048: 2.2 and 2.6)
+  const bool few = rows <= 2 * device_sm_count();
+  const int per = vecs <= (few ? kNormThreads : 128) ? 1 : vecs <= 2 * kNormThreads ? 2 : 4;
+  const dim3 grid((unsigned)rows), threads((vecs + per - 1) / per + 31 & ~31);
+  if (per == 1) return launch(AWQB_FP4_PICK(norm_kernel, , 1), grid, threads, stream, a);
+  if (per == 2) return launch(AWQB_FP4_PICK(norm_kernel, , 2), grid, threads, stream, a);
+  return launch(AWQB_FP4_PICK(norm_kernel, , 4), grid, threads, stream, a);
 }

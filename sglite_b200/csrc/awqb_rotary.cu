@@ -64,19 +64,6 @@ __device__ __forceinline__ int64_t position_of(const Args& a, int64_t m) {
   return a.pos64 ? static_cast<const int64_t*>(a.positions)[m] : (int64_t) static_cast<const int32_t*>(a.positions)[m];
 }
 
-// Two fp32 values per instruction.
-__device__ __forceinline__ uint64_t bits(float2 v) { return *reinterpret_cast<const uint64_t*>(&v); }
-__device__ __forceinline__ float2 floats(uint64_t v) { return *reinterpret_cast<const float2*>(&v); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
-  return floats(d);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
-  return floats(d);
-}
 // (x, y) turned by the angles of cosine c and sine s.
 __device__ __forceinline__ void turn2(float2& x, float2& y, float2 c, float2 s) {
   const float2 minus = make_float2(-s.x, -s.y), p = x;

@@ -929,10 +929,8 @@ def _fp4_format(fmt: str) -> int:
     return code
 
 
-def _fp4_scale(scale: Optional[torch.Tensor], n: int, fmt: str, di: int, name: str) -> int:
-    """Pointer of an fp32 scale of n values, 0 without one."""
-    if scale is None:
-        return 0
+def _fp4_scale(scale: torch.Tensor, n: int, fmt: str, di: int, name: str) -> int:
+    """Pointer of an fp32 scale of n values."""
     if fmt != "nvfp4":
         raise ValueError(f"{name}: only nvfp4 has a scale beside its blocks' scales")
     if scale.dtype != torch.float32 or scale.numel() != n or not scale.is_contiguous() or scale.get_device() != di:
@@ -943,9 +941,13 @@ def _fp4_scale(scale: Optional[torch.Tensor], n: int, fmt: str, di: int, name: s
 def fp4_rows_empty(rows: int, K: int, fmt: str, device) -> Tuple[torch.Tensor, torch.Tensor]:
     """Room for ``rows`` quantised rows of K values: codes uint8 [rows, K / 2] and scales
     uint8 [granules, rows, 16], 16 scales of a row side by side (256 k of nvfp4, 512 of mxfp4)."""
-    granules = -(-K // (16 * FP4_BLOCK[fmt]))
-    return (torch.empty((rows, K // 2), dtype=torch.uint8, device=device),
-            torch.empty((granules, rows, 16), dtype=torch.uint8, device=device))
+    _fp4_format(fmt)
+    return _fp4_rows_new(torch.empty(0, dtype=torch.uint8, device=device), rows, K, fmt)
+
+
+def _fp4_rows_new(like: torch.Tensor, rows: int, K: int, fmt: str) -> Tuple[torch.Tensor, torch.Tensor]:
+    codes = like.new_empty(rows, K // 2, dtype=torch.uint8)  # (sizes one by one: half a microsecond less)
+    return codes, codes.new_empty(-(-K // (16 * FP4_BLOCK[fmt])), rows, 16)
 
 
 def _fp4_rows(codes: torch.Tensor, scales: torch.Tensor, fmt: str, di: int) -> Tuple[int, int]:
@@ -953,12 +955,11 @@ def _fp4_rows(codes: torch.Tensor, scales: torch.Tensor, fmt: str, di: int) -> T
     if codes.dim() != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous() or codes.get_device() != di:
         raise ValueError("codes must be a contiguous uint8 [rows, K / 2] CUDA tensor")
     rows, half = codes.shape
-    K = 2 * half
-    if scales.shape != (-(-K // (16 * FP4_BLOCK[fmt])), rows, 16) or scales.dtype != torch.uint8 \
+    if scales.shape != (-(-half // (8 * FP4_BLOCK[fmt])), rows, 16) or scales.dtype != torch.uint8 \
             or not scales.is_contiguous() or scales.get_device() != di:
         raise ValueError(f"scales {tuple(scales.shape)} must be the contiguous uint8 [granules, rows, 16] tensor of "
-                         f"{rows} {fmt} rows of K={K}, on the codes' device")
-    return rows, K
+                         f"{rows} {fmt} rows of K={2 * half}, on the codes' device")
+    return rows, 2 * half
 
 
 def fp4_quantize(x: torch.Tensor, fmt: str, *, scale: Optional[torch.Tensor] = None,
@@ -993,9 +994,9 @@ def fp4_quantize(x: torch.Tensor, fmt: str, *, scale: Optional[torch.Tensor] = N
         if count.dtype != torch.int32 or count.numel() != 1 or count.get_device() != di:
             raise ValueError("count must be an int32 [1] tensor on x's device")
         pc = count.data_ptr()
-    ps = _fp4_scale(scale, 1, fmt, di, "scale")
+    ps = 0 if scale is None else _fp4_scale(scale, 1, fmt, di, "scale")
     if out is None:
-        out = fp4_rows_empty(rows, K, fmt, x.device)
+        out = _fp4_rows_new(x, rows, K, fmt)
     elif _fp4_rows(out[0], out[1], fmt, di) != (rows, K):
         raise ValueError(f"out must hold {rows} rows of K={K}")
     fn, pack = _entry("awqb_fp4_quantize")
@@ -1011,13 +1012,16 @@ def fp4_dequantize(codes: torch.Tensor, scales: torch.Tensor, fmt: str, dtype: t
     fc = _fp4_format(fmt)
     di = _device_of(codes)
     rows, K = _fp4_rows(codes, scales, fmt, di)
+    ps = 0 if scale is None else _fp4_scale(scale, 1, fmt, di, "scale")
     if out is None:
-        out = torch.empty((rows, K), dtype=dtype, device=codes.device)
+        out = codes.new_empty(rows, K, dtype=dtype)
+        ldo = K
     elif out.shape != (rows, K) or out.dtype != dtype or out.get_device() != di:
         raise ValueError(f"out must be a [{rows}, {K}] tensor of {dtype} on the codes' device")
+    else:
+        ldo = _row_stride(out, K, "out")
     fn, pack = _entry("awqb_fp4_dequantize")
-    _run(fn, di, pack(codes.data_ptr(), scales.data_ptr(), rows, K, fc, code, _fp4_scale(scale, 1, fmt, di, "scale"),
-                      out.data_ptr(), _row_stride(out, K, "out")))
+    _run(fn, di, pack(codes.data_ptr(), scales.data_ptr(), rows, K, fc, code, ps, out.data_ptr(), ldo))
     return out
 
 
@@ -1051,9 +1055,9 @@ def fp4_add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: t
         po, ldo = residual_out.data_ptr(), _row_stride(residual_out, K, "residual_out")
     elif residual_out is not None:
         raise ValueError("residual_out needs residual")
-    ps = _fp4_scale(scale, 1, fmt, di, "scale")
+    ps = 0 if scale is None else _fp4_scale(scale, 1, fmt, di, "scale")
     if out is None:
-        out = fp4_rows_empty(rows, K, fmt, x.device)
+        out = _fp4_rows_new(x, rows, K, fmt)
     elif _fp4_rows(out[0], out[1], fmt, di) != (rows, K):
         raise ValueError(f"out must hold {rows} rows of K={K}")
     fn, pack = _entry("awqb_fp4_add_rmsnorm")
@@ -1079,16 +1083,14 @@ def fp4_lay_out_scales(scales: torch.Tensor, fmt: str) -> torch.Tensor:
     return s.permute(*range(d), d, d + 3, d + 4, d + 2, d + 1, d + 5).contiguous()
 
 
-def _fp4_weight(w: torch.Tensor, w_scales: torch.Tensor, K: int, fmt: str, di: int) -> int:
-    """N of quantised weights [.., N, K / 2], checked with their laid-out scales."""
-    if w.dtype != torch.uint8 or w.shape[-1] * 2 != K or not w.is_contiguous() or w.get_device() != di:
-        raise ValueError(f"w {tuple(w.shape)} must be a contiguous uint8 [.., N, K / 2] tensor, K={K}, on the rows' device")
-    N = w.shape[-2]
-    want = (*w.shape[:-2], -(-N // 128), -(-K // 256), 64 // FP4_BLOCK[fmt], 32, 4, 4)
+def _fp4_weight(w: torch.Tensor, w_scales: torch.Tensor, lead: Tuple[int, ...], K: int, fmt: str, di: int) -> None:
+    """Checks quantised weights [*lead, N, K / 2] and their laid-out scales."""
+    if w.dtype != torch.uint8 or not w.is_contiguous() or w.get_device() != di:
+        raise ValueError("w must be a contiguous uint8 [.., N, K / 2] tensor on the rows' device")
+    want = (*lead, -(-w.size(-2) // 128), -(-K // 256), 64 // FP4_BLOCK[fmt], 32, 4, 4)
     if w_scales.shape != want or w_scales.dtype != torch.uint8 or not w_scales.is_contiguous() \
             or w_scales.get_device() != di:
         raise ValueError(f"w_scales {tuple(w_scales.shape)} must be {want}: fp4_lay_out_scales of the weight's scales")
-    return N
 
 
 def fp4_gemm(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, fmt: str,
@@ -1103,23 +1105,29 @@ def fp4_gemm(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_scale
     fc = _fp4_format(fmt)
     di = _device_of(codes)
     rows, K = _fp4_rows(codes, scales, fmt, di)
-    if w.dim() != 2:
-        raise ValueError("w must be a [N, K / 2] tensor")
-    N = _fp4_weight(w, w_scales, K, fmt, di)
-    pb = 0
+    if w.dim() != 2 or 2 * w.size(1) != K:
+        raise ValueError(f"w {tuple(w.shape)} must be a [N, K / 2] tensor, K={K}")
+    N = w.size(0)
+    _fp4_weight(w, w_scales, (), K, fmt, di)
+    pb = px = pw = 0
     if bias is not None:
         if bias.dtype != dtype or bias.numel() != N or not bias.is_contiguous() or bias.get_device() != di:
             raise ValueError(f"bias must be a contiguous [{N}] tensor of {dtype} on the rows' device")
         pb = bias.data_ptr()
-    n_out = N // 2 if silu_mul else N
+    if x_scale is not None:
+        px = _fp4_scale(x_scale, 1, fmt, di, "x_scale")
+    if w_scale is not None:
+        pw = _fp4_scale(w_scale, 1, fmt, di, "w_scale")
+    ldo = n_out = N // 2 if silu_mul else N
     if out is None:
-        out = torch.empty((rows, n_out), dtype=dtype, device=codes.device)
+        out = codes.new_empty(rows, n_out, dtype=dtype)
     elif out.shape != (rows, n_out) or out.dtype != dtype or out.get_device() != di:
         raise ValueError(f"out must be a [{rows}, {n_out}] tensor of {dtype} on the rows' device")
+    else:
+        ldo = _row_stride(out, n_out, "out")
     fn, pack = _entry("awqb_fp4_gemm")
     _run(fn, di, pack(codes.data_ptr(), scales.data_ptr(), rows, K, w.data_ptr(), w_scales.data_ptr(), 1, N, 0, fc, code,
-                      _fp4_scale(x_scale, 1, fmt, di, "x_scale"), _fp4_scale(w_scale, 1, fmt, di, "w_scale"), pb,
-                      silu_mul, 0, 0, out.data_ptr(), rows, _row_stride(out, n_out, "out")))
+                      px, pw, pb, silu_mul, 0, 0, out.data_ptr(), rows, ldo))
     return out
 
 
@@ -1135,23 +1143,24 @@ def fp4_grouped_gemm(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor,
     fc = _fp4_format(fmt)
     di = _device_of(codes)
     rows, K = _fp4_rows(codes, scales, fmt, di)
-    if w.dim() != 3:
-        raise ValueError("w must be a [E, N, K / 2] tensor")
-    N = _fp4_weight(w, w_scales, K, fmt, di)
-    E = w.shape[0]
+    if w.dim() != 3 or 2 * w.size(2) != K:
+        raise ValueError(f"w {tuple(w.shape)} must be a [E, N, K / 2] tensor, K={K}")
+    E, N, _ = w.shape
+    _fp4_weight(w, w_scales, (E,), K, fmt, di)
+    px = 0 if x_scale is None else _fp4_scale(x_scale, 1, fmt, di, "x_scale")
+    pw = 0 if w_scale is None else _fp4_scale(w_scale, E, fmt, di, "w_scale")
     if offsets.dtype != torch.int32 or offsets.numel() != E + 1 or not offsets.is_contiguous() \
             or offsets.get_device() != di:
         raise ValueError("offsets must be a contiguous int32 [experts + 1] tensor on the rows' device")
     n_out = N // 2 if silu_mul else N
     if out is None:
-        out = torch.empty((rows, n_out), dtype=dtype, device=codes.device)
+        out = codes.new_empty(rows, n_out, dtype=dtype)
     elif out.dim() != 2 or out.shape[1] != n_out or out.dtype != dtype or out.get_device() != di:
         raise ValueError(f"out must be a [rows, {n_out}] tensor of {dtype} on the rows' device")
     out_rows = out.shape[0]
     pm, ps = _row_map_scale(row_map, row_scale, rows, out_rows, di)
     fn, pack = _entry("awqb_fp4_gemm")
     _run(fn, di, pack(codes.data_ptr(), scales.data_ptr(), rows, K, w.data_ptr(), w_scales.data_ptr(), E, N,
-                      offsets.data_ptr(), fc, code, _fp4_scale(x_scale, 1, fmt, di, "x_scale"),
-                      _fp4_scale(w_scale, E, fmt, di, "w_scale"), 0, silu_mul, pm, ps, out.data_ptr(), out_rows,
+                      offsets.data_ptr(), fc, code, px, pw, 0, silu_mul, pm, ps, out.data_ptr(), out_rows,
                       _row_stride(out, n_out, "out")))
     return out
