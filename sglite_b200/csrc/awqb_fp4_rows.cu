@@ -172,6 +172,7 @@ constexpr int kNormMaxK = kNormThreads * kNormVec * 8;
 // a border its value lies, so the value is rounded once only: the threads' sums of squares
 // are added in 64 bits, the row's factor (over the tensor's scale) is kept as two fp32
 // numbers, and so is h * weight.
+
 // h of the thread's vector v, stored; returns its sum of squares.
 template <typename T>
 __device__ __forceinline__ float add_vector(const NormArgs& a, int64_t row, int v, const uint4& x, const uint4& r,
@@ -192,7 +193,7 @@ __device__ __forceinline__ float add_vector(const NormArgs& a, int64_t row, int 
 
 // 1 / x to about 2^-44, from its fp32 approximation by one Newton step.
 __device__ __forceinline__ double inverse(float x) {
-  const double y = (double)__fdividef(1.f, x);
+  const double y = (double)__frcp_rn(x);
   return fma(fma(-(double)x, y, 1.0), y, y);
 }
 
