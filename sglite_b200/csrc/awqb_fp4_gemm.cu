@@ -44,24 +44,29 @@ struct Params {
   uint32_t* err;
   int64_t ldo, out_rows;
   int rows, E, K, N, n_out, silu, feat_tiles, tile_out;  // tile_out: weight rows of a tile
+  int tok_tiles, tok_per;  // without offsets: token tiles, rows of each
   int box;    // of all tiles, or -1: by their rows
   int split;  // CTAs (pairs) of a cluster that share a tile's K; above 1, a cluster has one tile
 };
 
 // One CTA per tile of 128 weight rows x kTok tokens, two CTAs to an SM. Of a stage:
 // weights, rows (both swizzled: 1024-byte aligned), the weights' and the rows' scales.
-// Tensor memory: two accumulators, two sets of scales.
+// Tensor memory: two accumulators, two sets of scales. Where K is shared, the parts of a
+// tile's sum land behind the stages, of which there are fewer then.
 template <int kTokens>
 struct Few {
   static constexpr int kTok = kTokens;
   static constexpr int kRound = 16;
-  static constexpr int kStages = kTok > 32 ? 3 : 4;
+  static constexpr int kStages = kTok > 32 ? 3 : 4, kSplitStages = kTok > 32 ? 2 : 3;
   static constexpr int kEpiWarps = 4;
   static constexpr int kThreads = 32 * (kEpiWarps + 4);
   static constexpr int kPlans = 4, kCtasPerSm = 2;
   static constexpr int kAtX = kWBytes, kAtWs = kAtX + kTok * kK / 2, kAtXs = kAtWs + 2048;
   static constexpr int kStageBytes = kAtXs + 2048;
   static constexpr int kSets = 2 * kTok, kSetColumns = 32, kColumns = kTok > 32 ? 256 : 128;
+  static __host__ __device__ constexpr int ring_bytes(int split) {
+    return split > 1 ? kSplitStages * kStageBytes + kTok * kFeat * 4 : kStages * kStageBytes;
+  }
 };
 // A CTA pair; each loads its 128 weight rows and half the tokens, and the scales of all
 // tokens. The accumulators and scales of 208 tokens fill tensor memory.
@@ -75,6 +80,7 @@ struct Many {
   static constexpr int kAtX = kWBytes, kAtWs = kAtX + kTok / 2 * kK / 2, kAtXs = kAtWs + 2048;
   static constexpr int kStageBytes = kAtXs + 4096;
   static constexpr int kSets = 2 * kTok, kSetColumns = 48, kColumns = 512;
+  static __host__ __device__ constexpr int ring_bytes(int) { return kStages * kStageBytes; }
 };
 
 // What the roles need to know of a tile, found by one warp ahead of them: the tile, then
@@ -129,42 +135,68 @@ __device__ __forceinline__ void turn_scales(uint8_t* at, int rows, int lane) {
   }
 }
 
-// Stores a weight row's values of tokens c and c + 1, or, where rows are gate and up by
-// turns, the pair of lanes' two products.
-template <typename T>
-__device__ __forceinline__ void store_two(const Params& p, float (&y)[2], const int* to, const float* factor, int c,
-                                          int rows, bool real, int odd, T* out) {
-  if (p.silu) {
-    const float got = __shfl_xor_sync(0xffffffffu, odd ? y[0] : y[1], 1);
-    y[0] = y[1] = odd ? silu_mul(got, y[1]) : silu_mul(y[0], got);
+// Stores a weight row's values of 2 kPairs tokens from c on. Neighbouring lanes write
+// neighbouring features of a token. Where rows are gate and up by turns, of each two tokens
+// a lane keeps one and gives its neighbour the other.
+template <typename T, int kPairs>
+__device__ __forceinline__ void store_tokens(const Params& p, float (&y)[2 * kPairs], const int* to, const float* factor,
+                                             int c, int rows, bool real, int odd, T* out) {
+  int at[2 * kPairs];
+  float f[2 * kPairs];
+#pragma unroll
+  for (int i = 0; i < 2 * kPairs; ++i) {  // (all of them before the first store)
+    at[i] = to[c + i];
+    f[i] = p.row_scale ? factor[c + i] : 1.f;
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (!real || c + i >= rows || to[c + i] < 0 || (p.silu && i != odd)) continue;
-    out[(int64_t)to[c + i] * p.ldo] = (T)(p.row_scale ? y[i] * factor[c + i] : y[i]);
+  for (int i = 0; i < 2 * kPairs; i += 2) {
+    if (c + i >= rows) break;
+    if (p.silu) {
+      const float got = __shfl_xor_sync(0xffffffffu, odd ? y[i] : y[i + 1], 1);
+      y[i] = y[i + 1] = odd ? silu_mul(got, y[i + 1]) : silu_mul(y[i], got);
+    }
+#pragma unroll
+    for (int k = i; k < i + 2; ++k) {
+      if (!real || at[k] < 0 || (p.silu && k - i != odd)) continue;  // (-1 behind the rows)
+      out[(int64_t)at[k] * p.ldo] = (T)(y[k] * f[k]);
+    }
   }
 }
 
+// Initialises `n` barriers by one warp's lanes.
+__device__ __forceinline__ void init_barriers(uint64_t* bars, int n, uint32_t count, int lane) {
+  for (int i = lane; i < n; i += 32) mbar_init(smem_u32(bars + i), count);
+}
 template <typename C>
-__device__ __forceinline__ void init_plans(Plans<C>& plans) {
-  for (int i = 0; i < C::kPlans; ++i) {
-    mbar_init(smem_u32(&plans.tile_full[i]), 1);
-    mbar_init(smem_u32(&plans.rows_full[i]), 1);
-    mbar_init(smem_u32(&plans.free[i]), C::kEpiWarps);
-  }
+__device__ __forceinline__ void init_plans(Plans<C>& plans, int lane) {
+  init_barriers(plans.tile_full, C::kPlans, 1, lane);
+  init_barriers(plans.rows_full, C::kPlans, 1, lane);
+  init_barriers(plans.free, C::kPlans, C::kEpiWarps, lane);
+}
+
+// Tile t where all rows are one group.
+template <typename C>
+__device__ __forceinline__ Tile whole_tile(const Params& p, int t) {
+  const int ft = p.tok_tiles == 1 ? t : t / p.tok_tiles, tt = t - ft * p.tok_tiles;
+  Tile r;
+  r.e = 0;
+  r.row0 = tt * p.tok_per;
+  r.rows = min(p.tok_per, p.rows - r.row0);
+  r.n = (r.rows + C::kRound - 1) / C::kRound * C::kRound;
+  r.feat = ft * p.tile_out;
+  return r;
 }
 
 // The planning warp: tiles first_tile, first_tile + tile_step .. A plan is free again when
 // the epilogue, its last reader, is done with it.
 template <typename C>
 __device__ __forceinline__ bool plan_tiles(Plans<C>& plans, const Groups& g, const Params& p, int first_tile,
-                                           int tile_step, int* dst, float* scl, int lane) {
-  const int total = g.tile0[p.E];
+                                           int tile_step, int total, int* dst, float* scl, int lane) {
   int i = 0;
   for (int t = first_tile; t < total; t += tile_step, ++i) {
     const int at = i % C::kPlans;
     if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&plans.free[at]), ((i / C::kPlans) & 1) ^ 1))) return false;
-    const Tile tile = find_tile<C>(g, p, t);
+    const Tile tile = p.offsets ? find_tile<C>(g, p, t) : whole_tile<C>(p, t);
     if (lane == 0) {
       plans.tile[at] = tile;
       mbar_arrive(smem_u32(&plans.tile_full[at]));
@@ -197,14 +229,37 @@ __device__ __forceinline__ bool plan_tiles(Plans<C>& plans, const Groups& g, con
   return true;
 }
 
-// A role's turn to tile number i of this CTA (false: the wait gave up).
+// A role's turn to tile t, number i of this CTA (false: the wait gave up). Without groups
+// it is known at once.
 template <typename C>
-__device__ __forceinline__ bool next_tile(Plans<C>& plans, int i, Tile* tile) {
+__device__ __forceinline__ bool next_tile(Plans<C>& plans, const Params& p, int t, int i, Tile* tile) {
+  if (p.offsets == nullptr) {
+    *tile = whole_tile<C>(p, t);
+    return true;
+  }
   const int at = i % C::kPlans;
   if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&plans.tile_full[at]), (i / C::kPlans) & 1))) return false;
   *tile = plans.tile[at];
   return true;
 }
+
+// The number of tiles; builds the groups' tables where there are groups. All threads, a
+// barrier among them, but for one group.
+template <typename C>
+__device__ __forceinline__ void find_groups(const Groups& g, const Params& p) {
+  if (p.offsets != nullptr) build_groups<C>(g, p);
+}
+__device__ __forceinline__ int count_tiles(const Groups& g, const Params& p) {
+  return __shfl_sync(0xffffffffu, p.offsets ? g.tile0[p.E] : p.tok_tiles * p.feat_tiles, 0);
+}
+
+// A role's place in the ring of stages.
+struct Place {
+  int s = 0, lap = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++s == stages) s = 0, lap ^= 1;
+  }
+};
 
 // Stages of K that part `part` of p.split works on.
 __device__ __forceinline__ void stages_of(const Params& p, int nk, int part, int* first, int* last) {
@@ -219,13 +274,13 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   using C = Few<kTok>;
   extern __shared__ uint8_t raw[];
   uint8_t* ring = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
-  int* dst = reinterpret_cast<int*>(ring + C::kStages * C::kStageBytes);  // [kPlans][kTok] out row of a token
+  int* dst = reinterpret_cast<int*>(ring + C::ring_bytes(p.split));  // [kPlans][kTok] out row of a token
   float* scl = reinterpret_cast<float*>(dst + C::kPlans * kTok);          // [kPlans][kTok] its factor
   Groups g;
   g.row0 = reinterpret_cast<int*>(scl + C::kPlans * kTok);  // [E] first rows, [E] row counts
   g.tile0 = g.row0 + 2 * p.E;
   __shared__ uint64_t full[C::kStages], raw_scales[C::kStages], empty[C::kStages];
-  __shared__ uint64_t acc_full[2], acc_empty[2];
+  __shared__ uint64_t acc_full[2], acc_empty[2], landed;
   __shared__ Plans<C> plans;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
@@ -236,19 +291,25 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   const int nk = (p.K + kK - 1) / kK;
   int kb0, kb1;
   stages_of(p, nk, part, &kb0, &kb1);
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(smem_u32(&full[s]), 2);  // the producer's expectation and the turned scales
-      mbar_init(smem_u32(&raw_scales[s]), 1);
-      mbar_init(smem_u32(&empty[s]), 1);
+  const int stages = p.split > 1 ? C::kSplitStages : C::kStages;
+  // Where K is shared: token pairs go by turns to the parts; this one's, and where they land
+  const int pairs = p.split > 1 ? (whole_tile<C>(p, first_tile).rows + 1) / 2 : 0;
+  const int my_pairs = (pairs - part + p.split - 1) / p.split;
+  float2* landing = reinterpret_cast<float2*>(ring + C::kSplitStages * C::kStageBytes);  // [pair][part][feature]
+  if (warp == C::kEpiWarps) {
+    init_barriers(full, stages, 2, lane);  // the producer's expectation and the turned scales
+    init_barriers(raw_scales, stages, 1, lane);
+    init_barriers(empty, stages, 1, lane);
+    init_barriers(acc_full, 2, 1, lane);
+    init_barriers(acc_empty, 2, C::kEpiWarps, lane);
+    init_plans(plans, lane);
+    if (lane == 0) {
+      mbar_init(smem_u32(&landed), 1);
+      failed = 0;
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(smem_u32(&acc_full[b]), 1);
-      mbar_init(smem_u32(&acc_empty[b]), C::kEpiWarps);
-    }
-    init_plans(plans);
-    failed = 0;
     fence_barrier_init();
+    __syncwarp();
+    if (p.split > 1 && lane == 0) mbar_arrive_expect_tx(smem_u32(&landed), my_pairs * p.split * kFeat * 8);
   }
   if (warp == C::kEpiWarps + 1) {
     tmem_alloc(smem_u32(&tmem_slot), C::kColumns);
@@ -259,35 +320,37 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     // The weights' first stages on their way to L2 while the kernel in front ends. (Its
     // outputs, this product's rows, are not touched before the wait.)
     prefetch_tmap(&tm_w);
-    const int feat = first_tile / ((p.rows + kTok - 1) / kTok) * kFeat;
+    const int feat = whole_tile<C>(p, first_tile).feat;
     for (int kb = kb0; kb < min(kb1, kb0 + C::kStages); ++kb) tma_prefetch_2d(&tm_w, kb * kK / 2, feat);
   }
   __syncwarp();
+  if (p.split > 1) cluster_arrive();  // the barrier for landing parts is ready
   grid_dep_wait();
-  build_groups<C>(g, p);
+  find_groups<C>(g, p);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int total = __shfl_sync(0xffffffffu, g.tile0[p.E], 0);
-  bool ok = true;
+  const int total = count_tiles(g, p);
+  bool ok = true, waited = p.split == 1;
 
   if (warp == C::kEpiWarps) {  // ------------------------------------- producer
     const uint64_t keep = policy_evict_normal(), once = policy_evict_first();
-    int it = 0, n_tile = 0;
+    Place at;
+    int n_tile = 0;
     for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
       Tile tile;
-      ok = next_tile(plans, n_tile, &tile);
+      ok = next_tile(plans, p, t, n_tile, &tile);
       if (!ok) break;
       const int box = p.box >= 0 ? p.box : box_of(tile.n, kTok);
       // weights that one token tile reads once need not stay in L2
-      const uint64_t wpol = tile.rows == g.row0[p.E + tile.e] ? once : keep;
+      const uint64_t wpol = (p.offsets ? tile.rows == g.row0[p.E + tile.e] : p.tok_tiles == 1) ? once : keep;
       const int wrow = tile.e * p.N + tile.feat;
       const uint8_t* ws = p.w_scales + ((int64_t)tile.e * p.feat_tiles + tile.feat / kFeat) * nk * kWsBytes<kNv>;
       const int scale_rows = min(tile.n, p.rows - tile.row0);
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % C::kStages;
-        ok = mbar_wait(smem_u32(&empty[s]), ((it / C::kStages) & 1) ^ 1);
+      for (int kb = kb0; kb < kb1; ++kb, at.next(stages)) {
+        const int s = at.s, lap = at.lap;
+        ok = mbar_wait(smem_u32(&empty[s]), lap ^ 1);
         if (!ok) break;
         if (elect_one()) {
           const uint32_t base = smem_u32(ring + s * C::kStageBytes), bar = smem_u32(&full[s]);
@@ -304,14 +367,15 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       }
     }
   } else if (warp == C::kEpiWarps + 2) {  // ---------------------------- scales of the rows
-    int it = 0, n_tile = 0;
+    Place at;
+    int n_tile = 0;
     for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
       Tile tile;
-      ok = next_tile(plans, n_tile, &tile);
+      ok = next_tile(plans, p, t, n_tile, &tile);
       if (!ok) break;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % C::kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&raw_scales[s]), (it / C::kStages) & 1));
+      for (int kb = kb0; kb < kb1; ++kb, at.next(stages)) {
+        const int s = at.s, lap = at.lap;
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&raw_scales[s]), lap));
         if (!ok) break;
         turn_scales<1>(ring + s * C::kStageBytes + C::kAtXs, tile.n, lane);
         fence_proxy_async_smem();
@@ -323,19 +387,20 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     const uint32_t issue = elect_one();
     // (what the compiler cannot see to be the same for all lanes)
     const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem, 0), ring0 = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
+    Place at;
     int it = 0, n_tile = 0;
     for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
       Tile tile;
       const int b = n_tile & 1;
-      ok = next_tile(plans, n_tile, &tile) &&
+      ok = next_tile(plans, p, t, n_tile, &tile) &&
            __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1));
       if (!ok) break;
       tc_fence_after();
       const uint32_t d = tmem0 + b * kTok;
       const uint32_t idesc = make_idesc_fp4(kFeat, __shfl_sync(0xffffffffu, tile.n, 0), kNv, 0);
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % C::kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[s]), (it / C::kStages) & 1));
+      for (int kb = kb0; kb < kb1; ++kb, ++it, at.next(stages)) {
+        const int s = at.s, lap = at.lap;
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[s]), lap));
         if (!ok) break;
         tc_fence_after();
         const uint32_t base = ring0 + s * C::kStageBytes;
@@ -361,12 +426,10 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       }
     }
   } else if (warp == C::kEpiWarps + 3) {  // ---------------------------- plans
-    ok = plan_tiles(plans, g, p, first_tile, tile_step, dst, scl, lane);
+    ok = plan_tiles(plans, g, p, first_tile, tile_step, total, dst, scl, lane);
   } else {  // -------------------------------------------------------- epilogue
-    // A lane holds a weight row's tokens. Neighbouring lanes write neighbouring features
-    // of a token. With silu_mul even lanes hold gate and odd lanes up rows: of a pair of
-    // tokens a lane keeps one and gives its neighbour the other. A tile whose K is shared
-    // is summed after the barrier below: each CTA leaves its part in its ring, [token][row].
+    // A lane holds a weight row's tokens. Where K is shared, each pair of tokens is sent to
+    // the part whose turn it is, which adds what landed in the parts' order.
     const int tid = threadIdx.x, odd = lane & 1;
     int n_tile = 0;
     for (int t = first_tile; t < total; t += tile_step, ++n_tile) {
@@ -382,14 +445,20 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       const int* to = dst + at * kTok;
       const float* factor = scl + at * kTok;
       T* out = static_cast<T*>(p.out) + (p.silu ? row / 2 : row);
+      if (!waited) cluster_wait();
+      waited = true;
       for (int c = 0; c < tile.rows; c += 16) {
         uint32_t v[16];
         tmem_ld16(tmem + b * kTok + c + ((uint32_t)warp << 21), v);
         tmem_ld_wait();
         if (p.split > 1) {
-          float* mine = reinterpret_cast<float*>(ring) + c * kFeat + tid;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) mine[j * kFeat] = __uint_as_float(v[j]);
+          for (int j = 0; j < 16; j += 2) {
+            const int pair = (c + j) / 2, turn = pair / p.split, who = pair - turn * p.split;
+            if (pair < pairs)
+              st_async_v2(mapa_shared(smem_u32(landing + (turn * p.split + part) * kFeat + tid), who),
+                          __uint_as_float(v[j]), __uint_as_float(v[j + 1]), mapa_shared(smem_u32(&landed), who));
+          }
           continue;
         }
         if (c + 16 >= tile.rows) {  // the accumulator is read: the MMA warp may reuse it
@@ -397,14 +466,25 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&acc_empty[b]));
         }
+        float y[16];
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          if (c + j >= tile.rows) break;
-          float y[2] = {__uint_as_float(v[j]) * alpha + bias, __uint_as_float(v[j + 1]) * alpha + bias};
-          store_two<T>(p, y, to, factor, c + j, tile.rows, row < p.N, odd, out);
-        }
+        for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(v[j]) * alpha + bias;
+        store_tokens<T, 8>(p, y, to, factor, c, tile.rows, row < p.N, odd, out);
       }
-      if (p.split > 1) break;  // (the plan stays, for the sum)
+      if (p.split > 1) {
+        ok = named_bar_and(1, 128, mbar_wait(smem_u32(&landed), 0));
+        if (!ok) break;
+        for (int turn = 0; turn < my_pairs; ++turn) {
+          float2 sum = make_float2(0.f, 0.f);
+          for (int q = 0; q < p.split; ++q) {
+            const float2 v = landing[(turn * p.split + q) * kFeat + tid];
+            sum.x += v.x, sum.y += v.y;
+          }
+          float y[2] = {sum.x * alpha + bias, sum.y * alpha + bias};
+          store_tokens<T, 1>(p, y, to, factor, 2 * (turn * p.split + part), tile.rows, row < p.N, odd, out);
+        }
+        break;
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&plans.free[at]));
     }
@@ -414,31 +494,10 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     atomicOr(p.err, kErrWait);
   }
   __syncwarp();
-  if (p.split > 1) {
-    // Two tokens at a time by turns: CTA `part` adds the parts in their order.
-    cluster_sync_all();
-    if (warp < C::kEpiWarps && first_tile < total) {
-      const Tile tile = plans.tile[0];
-      const int tid = threadIdx.x, odd = lane & 1, row = tile.feat + tid;
-      const float alpha = plans.alpha[0];
-      const float bias = p.bias && row < p.N ? (float)static_cast<const T*>(p.bias)[row] : 0.f;
-      T* out = static_cast<T*>(p.out) + (p.silu ? row / 2 : row);
-      const uint32_t mine = smem_u32(ring) + tid * 4;
-      for (int c = 2 * part; c < tile.rows; c += 2 * p.split) {
-        float sum[2] = {0.f, 0.f};
-        for (int q = 0; q < p.split; ++q) {
-          const uint32_t at = mapa_shared(mine, q) + c * kFeat * 4;
-          sum[0] += ld_dsmem_f32(at);
-          sum[1] += ld_dsmem_f32(at + kFeat * 4);
-        }
-        float y[2] = {sum[0] * alpha + bias, sum[1] * alpha + bias};
-        store_two<T>(p, y, dst, scl, c, tile.rows, row < p.N, odd, out);
-      }
-    }
-    cluster_sync_all();  // the parts are read
-  }
+  if (!waited) cluster_wait();
   __syncthreads();
-  if (failed) linger();
+  // (where K is shared, until nobody can still be sending a part here)
+  for (int i = 0; failed && i < (p.split > 1 ? 250 : 1); ++i) linger();
   tc_fence_before();
   __syncthreads();
   if (warp == C::kEpiWarps + 1) {
@@ -519,18 +578,14 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   const int nk = (p.K + kK - 1) / kK;
   int kb0, kb1;
   stages_of(p, nk, part, &kb0, &kb1);
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(smem_u32(&full[s]), 3);  // the leader's expectation and both CTAs' turned scales
-      mbar_init(smem_u32(&raw_scales[s]), 1);
-      mbar_init(smem_u32(&empty[s]), 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(smem_u32(&acc_full[b]), 1);
-      mbar_init(smem_u32(&acc_empty[b]), 2 * C::kEpiWarps);
-    }
-    init_plans(plans);
-    failed = 0;
+  if (warp == C::kEpiWarps) {
+    init_barriers(full, C::kStages, 3, lane);  // the leader's expectation and both CTAs' turned scales
+    init_barriers(raw_scales, C::kStages, 1, lane);
+    init_barriers(empty, C::kStages, 1, lane);
+    init_barriers(acc_full, 2, 1, lane);
+    init_barriers(acc_empty, 2, 2 * C::kEpiWarps, lane);
+    init_plans(plans, lane);
+    if (lane == 0) failed = 0;
     fence_barrier_init();
   }
   if (warp == C::kEpiWarps + 1) {
@@ -541,18 +596,18 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   if (p.offsets == nullptr && warp == C::kEpiWarps && elect_one()) {
     // as in the kernel above, to L2 only
     prefetch_tmap(&tm_w);
-    const int feat = first_tile / ((p.rows + C::kTok - 1) / C::kTok) * 2 * kFeat + (int)rank * kFeat;
+    const int feat = whole_tile<C>(p, first_tile).feat + (int)rank * kFeat;
     for (int kb = kb0; kb < min(kb1, kb0 + C::kStages); ++kb) tma_prefetch_2d(&tm_w, kb * kK / 2, feat);
   }
   __syncwarp();
   grid_dep_wait();
-  build_groups<C>(g, p);
+  find_groups<C>(g, p);
   tc_fence_before();
   cluster_sync_all();  // the peer's barriers are ready before anything arrives on them
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int total = __shfl_sync(0xffffffffu, g.tile0[p.E], 0);
+  const int total = count_tiles(g, p);
   bool ok = true;
 
   if (warp == C::kEpiWarps) {  // ------------------------------------- producer
@@ -561,11 +616,11 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     int it = 0, n_tile = 0;
     for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
       Tile tile;
-      ok = next_tile(plans, n_tile, &tile);
+      ok = next_tile(plans, p, t, n_tile, &tile);
       if (!ok) break;
       const int box = p.box >= 0 ? p.box : box_of(tile.n / 2, C::kTok / 2);
       // weights that one token tile reads once need not stay in L2
-      const uint64_t wpol = tile.rows == g.row0[p.E + tile.e] ? once : keep;
+      const uint64_t wpol = (p.offsets ? tile.rows == g.row0[p.E + tile.e] : p.tok_tiles == 1) ? once : keep;
       const int feat = tile.feat + (int)rank * kFeat, row = tile.row0 + (int)rank * (tile.n / 2);
       // (rows past N are multiplied, by whatever scales, and not stored)
       const uint8_t* ws =
@@ -598,7 +653,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     int it = 0, n_tile = 0;
     for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
       Tile tile;
-      ok = next_tile(plans, n_tile, &tile);
+      ok = next_tile(plans, p, t, n_tile, &tile);
       if (!ok) break;
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         if ((it & 1) != odd) continue;
@@ -619,7 +674,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     for (int t = first_tile; t < total && ok && rank == 0; t += tile_step, ++n_tile) {
       Tile tile;
       const int b = n_tile & 1;
-      ok = next_tile(plans, n_tile, &tile) &&
+      ok = next_tile(plans, p, t, n_tile, &tile) &&
            __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1));
       if (!ok) break;
       tc_fence_after();
@@ -656,7 +711,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       }
     }
   } else if (warp == C::kEpiWarps + 3) {  // ---------------------------- plans
-    ok = plan_tiles(plans, g, p, first_tile, tile_step, dst, scl, lane);
+    ok = plan_tiles(plans, g, p, first_tile, tile_step, total, dst, scl, lane);
   } else {  // -------------------------------------------------------- epilogue
     // Two groups of four warps take turns over 32 tokens.
     const int quarter = warp & 3;
@@ -748,27 +803,29 @@ int launch(int pair, const void* codes, const void* w, Params p, int max_split, 
   const int64_t row_bytes = p.K / 2;
   int st = make_bytes_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, (int64_t)p.E * p.N, row_bytes, row_bytes, kFeat);
   // without groups all tiles take the first, largest tile's box
-  const int tok_tiles = (p.rows + C::kTok - 1) / C::kTok;
-  const int n = ((p.rows + tok_tiles - 1) / tok_tiles + C::kRound - 1) / C::kRound * C::kRound;
-  p.box = p.offsets ? -1 : box_of(n / pair, tok_cta);
+  p.tok_tiles = (p.rows + C::kTok - 1) / C::kTok;
+  p.tok_per = ((p.rows + p.tok_tiles - 1) / p.tok_tiles + C::kRound - 1) / C::kRound * C::kRound;
+  p.box = p.offsets ? -1 : box_of(p.tok_per / pair, tok_cta);
   for (int i = 0; i < 3 && st == kOk; ++i)
     if (p.box < 0 || i == p.box)
       st = make_bytes_map(&tx.box[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, p.rows, row_bytes, row_bytes,
                           tok_cta >> (2 - i));
   if (st != kOk) return st;
-  const auto smem_for = [](int E) { return 1024 + C::kStages * C::kStageBytes + 2 * C::kPlans * C::kTok * 4 + (3 * E + 1) * 4; };
+  const auto smem_for = [](int E, int split) {
+    return 1024 + C::ring_bytes(split) + 2 * C::kPlans * C::kTok * 4 + (3 * E + 1) * 4;
+  };
   static std::atomic<bool> ready[64];  // the kernel's attributes, set once for a device
   int dev = 0;
   AWQB_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !ready[dev].load()) {
-    AWQB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_for(kMaxExperts)));
+    AWQB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   std::max(smem_for(kMaxExperts, 1), smem_for(1, 2))));
     // all of it, so that two CTAs of the few-rows kernel fit an SM
     AWQB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
     if (dev < 64) ready[dev].store(true);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(C::kThreads);
-  cfg.dynamicSmemBytes = smem_for(p.E);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -777,7 +834,7 @@ int launch(int pair, const void* codes, const void* w, Params p, int max_split, 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   // every tile there could be: a group adds at most one partly filled token tile
-  const int64_t tiles = ((p.rows + C::kTok - 1) / C::kTok + (p.offsets ? std::min<int64_t>(p.E, p.rows) : 0)) * p.feat_tiles;
+  const int64_t tiles = (p.tok_tiles + (p.offsets ? std::min<int64_t>(p.E, p.rows) : 0)) * p.feat_tiles;
   AWQB_REQUIRE(tiles < (1ll << 31), kUnsupported, "too many tiles (%lld)", (long long)tiles);
   // K is shared by as many CTAs (pairs) as leave each tile a cluster of its own at once, and
   // each of them two stages
@@ -792,6 +849,7 @@ int launch(int pair, const void* codes, const void* w, Params p, int max_split, 
     attr[0].val.clusterDim.x = (unsigned)(pair * p.split);
     cfg.gridDim = dim3((unsigned)(pair * p.split));
     cfg.numAttrs = 1;
+    cfg.dynamicSmemBytes = smem_for(p.E, p.split);
     st = max_clusters(kernel, cfg, cached[log], &clusters);
     if (st != kOk) return st;
     clusters *= C::kCtasPerSm;  // (the query counts one for kernels with tensor memory)
