@@ -195,7 +195,7 @@ __device__ __forceinline__ bool plan_tiles(Plans<C>& plans, const Groups& g, con
   int i = 0;
   for (int t = first_tile; t < total; t += tile_step, ++i) {
     const int at = i % C::kPlans;
-    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&plans.free[at]), ((i / C::kPlans) & 1) ^ 1))) return false;
+    if (!(mbar_wait_warp(smem_u32(&plans.free[at]), ((i / C::kPlans) & 1) ^ 1))) return false;
     const Tile tile = p.offsets ? find_tile<C>(g, p, t) : whole_tile<C>(p, t);
     if (lane == 0) {
       plans.tile[at] = tile;
@@ -238,7 +238,7 @@ __device__ __forceinline__ bool next_tile(Plans<C>& plans, const Params& p, int 
     return true;
   }
   const int at = i % C::kPlans;
-  if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&plans.tile_full[at]), (i / C::kPlans) & 1))) return false;
+  if (!(mbar_wait_warp(smem_u32(&plans.tile_full[at]), (i / C::kPlans) & 1))) return false;
   *tile = plans.tile[at];
   return true;
 }
@@ -285,17 +285,18 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (from lane 0: the compiler then takes the roles' code as the whole warp's)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int part = p.split > 1 ? (int)cluster_ctarank() : 0;
   const int first_tile = blockIdx.x / p.split, tile_step = gridDim.x / p.split;
   const int nk = (p.K + kK - 1) / kK;
   int kb0, kb1;
   stages_of(p, nk, part, &kb0, &kb1);
   const int stages = p.split > 1 ? C::kSplitStages : C::kStages;
-  // Where K is shared: token pairs go by turns to the parts; this one's, and where they land
-  const int pairs = p.split > 1 ? (whole_tile<C>(p, first_tile).rows + 1) / 2 : 0;
-  const int my_pairs = (pairs - part + p.split - 1) / p.split;
-  float2* landing = reinterpret_cast<float2*>(ring + C::kSplitStages * C::kStageBytes);  // [pair][part][feature]
+  // Where K is shared: four tokens at a time go by turns to the parts; this one's, and where they land
+  const int fours = p.split > 1 ? (whole_tile<C>(p, first_tile).rows + 3) / 4 : 0;
+  const int my_fours = (fours - part + p.split - 1) / p.split;
+  float4* landing = reinterpret_cast<float4*>(ring + C::kSplitStages * C::kStageBytes);  // [turn][part][weight row]
   if (warp == C::kEpiWarps) {
     init_barriers(full, stages, 2, lane);  // the producer's expectation and the turned scales
     init_barriers(raw_scales, stages, 1, lane);
@@ -309,7 +310,7 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     }
     fence_barrier_init();
     __syncwarp();
-    if (p.split > 1 && lane == 0) mbar_arrive_expect_tx(smem_u32(&landed), my_pairs * p.split * kFeat * 8);
+    if (p.split > 1 && lane == 0) mbar_arrive_expect_tx(smem_u32(&landed), my_fours * p.split * kFeat * 16);
   }
   if (warp == C::kEpiWarps + 1) {
     tmem_alloc(smem_u32(&tmem_slot), C::kColumns);
@@ -375,7 +376,7 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       if (!ok) break;
       for (int kb = kb0; kb < kb1; ++kb, at.next(stages)) {
         const int s = at.s, lap = at.lap;
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&raw_scales[s]), lap));
+        ok = (mbar_wait_warp(smem_u32(&raw_scales[s]), lap));
         if (!ok) break;
         turn_scales<1>(ring + s * C::kStageBytes + C::kAtXs, tile.n, lane);
         fence_proxy_async_smem();
@@ -393,14 +394,14 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       Tile tile;
       const int b = n_tile & 1;
       ok = next_tile(plans, p, t, n_tile, &tile) &&
-           __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1));
+           (mbar_wait_warp(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1));
       if (!ok) break;
       tc_fence_after();
       const uint32_t d = tmem0 + b * kTok;
       const uint32_t idesc = make_idesc_fp4(kFeat, __shfl_sync(0xffffffffu, tile.n, 0), kNv, 0);
       for (int kb = kb0; kb < kb1; ++kb, ++it, at.next(stages)) {
         const int s = at.s, lap = at.lap;
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[s]), lap));
+        ok = (mbar_wait_warp(smem_u32(&full[s]), lap));
         if (!ok) break;
         tc_fence_after();
         const uint32_t base = ring0 + s * C::kStageBytes;
@@ -421,14 +422,13 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
                                  sa + 4 * w, sb + 4 * w, kb > kb0 || j > 0);
         }
         tc_commit_if(issue, smem_u32(&empty[s]));
-        tc_commit_if(issue && kb == kb1 - 1, smem_u32(&acc_full[b]));
-        __syncwarp();
       }
+      if (ok) tc_commit_if(issue, smem_u32(&acc_full[b]));
     }
   } else if (warp == C::kEpiWarps + 3) {  // ---------------------------- plans
     ok = plan_tiles(plans, g, p, first_tile, tile_step, total, dst, scl, lane);
   } else {  // -------------------------------------------------------- epilogue
-    // A lane holds a weight row's tokens. Where K is shared, each pair of tokens is sent to
+    // A lane holds a weight row's tokens. Where K is shared, each four tokens are sent to
     // the part whose turn it is, which adds what landed in the parts' order.
     const int tid = threadIdx.x, odd = lane & 1;
     int n_tile = 0;
@@ -453,11 +453,11 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
         tmem_ld_wait();
         if (p.split > 1) {
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            const int pair = (c + j) / 2, turn = pair / p.split, who = pair - turn * p.split;
-            if (pair < pairs)
-              st_async_v2(mapa_shared(smem_u32(landing + (turn * p.split + part) * kFeat + tid), who),
-                          __uint_as_float(v[j]), __uint_as_float(v[j + 1]), mapa_shared(smem_u32(&landed), who));
+          for (int j = 0; j < 16; j += 4) {
+            const int four = (c + j) / 4, turn = four / p.split, who = four - turn * p.split;
+            if (four < fours)
+              st_async_v4(mapa_shared(smem_u32(landing + (turn * p.split + part) * kFeat + tid), who), v + j,
+                          mapa_shared(smem_u32(&landed), who));
           }
           continue;
         }
@@ -474,14 +474,15 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       if (p.split > 1) {
         ok = named_bar_and(1, 128, mbar_wait(smem_u32(&landed), 0));
         if (!ok) break;
-        for (int turn = 0; turn < my_pairs; ++turn) {
-          float2 sum = make_float2(0.f, 0.f);
-          for (int q = 0; q < p.split; ++q) {
-            const float2 v = landing[(turn * p.split + q) * kFeat + tid];
-            sum.x += v.x, sum.y += v.y;
+        for (int turn = 0; turn < my_fours; ++turn) {
+          const float4* part0 = landing + turn * p.split * kFeat + tid;
+          float4 sum = part0[0];
+          for (int q = 1; q < p.split; ++q) {
+            const float4 v = part0[q * kFeat];
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
           }
-          float y[2] = {sum.x * alpha + bias, sum.y * alpha + bias};
-          store_tokens<T, 1>(p, y, to, factor, 2 * (turn * p.split + part), tile.rows, row < p.N, odd, out);
+          float y[4] = {sum.x * alpha + bias, sum.y * alpha + bias, sum.z * alpha + bias, sum.w * alpha + bias};
+          store_tokens<T, 2>(p, y, to, factor, 4 * (turn * p.split + part), tile.rows, row < p.N, odd, out);
         }
         break;
       }
@@ -569,7 +570,8 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (from lane 0: the compiler then takes the roles' code as the whole warp's)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // a cluster is p.split pairs; rank: in the pair, whose leader is CTA `leader` of the cluster
   const uint32_t rank = cluster_ctarank() & 1, leader = cluster_ctarank() & ~1u;
   const int part = cluster_ctarank() >> 1;
@@ -658,7 +660,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         if ((it & 1) != odd) continue;
         const int s = it % C::kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&raw_scales[s]), (it / C::kStages) & 1));
+        ok = (mbar_wait_warp(smem_u32(&raw_scales[s]), (it / C::kStages) & 1));
         if (!ok) break;
         turn_scales<2>(ring + s * C::kStageBytes + C::kAtXs, tile.n, lane);
         fence_proxy_async_smem();
@@ -675,14 +677,14 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       Tile tile;
       const int b = n_tile & 1;
       ok = next_tile(plans, p, t, n_tile, &tile) &&
-           __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1));
+           (mbar_wait_warp(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1));
       if (!ok) break;
       tc_fence_after();
       const int n = __shfl_sync(0xffffffffu, tile.n, 0);
       const uint32_t d = tmem0 + b * C::kTok, idesc = make_idesc_fp4(2 * kFeat, n, kNv, 0);
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int s = it % C::kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[s]), (it / C::kStages) & 1));
+        ok = (mbar_wait_warp(smem_u32(&full[s]), (it / C::kStages) & 1));
         if (!ok) break;
         tc_fence_after();
         const uint32_t base = ring0 + s * C::kStageBytes;
@@ -706,9 +708,8 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
                                 sa + 4 * w, sb + 8 * w, kb > kb0 || j > 0);
         }
         tc_commit_pair_if(issue, smem_u32(&empty[s]), pair_mask);
-        tc_commit_pair_if(issue && kb == kb1 - 1, smem_u32(&acc_full[b]), pair_mask);
-        __syncwarp();
       }
+      if (ok) tc_commit_pair_if(issue, smem_u32(&acc_full[b]), pair_mask);
     }
   } else if (warp == C::kEpiWarps + 3) {  // ---------------------------- plans
     ok = plan_tiles(plans, g, p, first_tile, tile_step, total, dst, scl, lane);

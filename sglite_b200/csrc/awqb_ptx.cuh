@@ -91,6 +91,16 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
   }
 }
 
+// The same by a whole warp, with votes for branches: the code behind stays the warp's.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t i = 1;; ++i) {
+    if (__all_sync(0xffffffffu, mbar_try_wait_hint(bar, parity, 20000u))) return true;
+    if ((i & 15u) == 0 && __any_sync(0xffffffffu, globaltimer_ns() - t0 > AWQB_WAIT_TIMEOUT_NS)) return false;
+  }
+}
+
 // After a wait gave up: copies and products in flight get time to end.
 __device__ __forceinline__ void linger() {
   const uint64_t t0 = globaltimer_ns();
@@ -431,11 +441,12 @@ __device__ __forceinline__ float ld_dsmem_f32(uint32_t addr) {
   return v;
 }
 
-// Two words into the shared memory of a CTA of the cluster, counted by a barrier there.
-__device__ __forceinline__ void st_async_v2(uint32_t addr, float a, float b, uint32_t bar) {
-  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(addr),
-               "r"(__float_as_uint(a)), "r"(__float_as_uint(b)), "r"(bar)
-               : "memory");
+// Four values into the shared memory of a CTA of the cluster, counted by a barrier there.
+__device__ __forceinline__ void st_async_v4(uint32_t addr, const uint32_t* v, uint32_t bar) {
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(bar)
+      : "memory");
 }
 
 // ---------------------------------------------------------------- CTA pairs
