@@ -195,7 +195,7 @@ __device__ __forceinline__ bool plan_tiles(Plans<C>& plans, const Groups& g, con
   int i = 0;
   for (int t = first_tile; t < total; t += tile_step, ++i) {
     const int at = i % C::kPlans;
-    if (!(mbar_wait_warp(smem_u32(&plans.free[at]), ((i / C::kPlans) & 1) ^ 1))) return false;
+    if (!mbar_wait_warp(smem_u32(&plans.free[at]), ((i / C::kPlans) & 1) ^ 1)) return false;
     const Tile tile = p.offsets ? find_tile<C>(g, p, t) : whole_tile<C>(p, t);
     if (lane == 0) {
       plans.tile[at] = tile;
@@ -238,7 +238,7 @@ __device__ __forceinline__ bool next_tile(Plans<C>& plans, const Params& p, int 
     return true;
   }
   const int at = i % C::kPlans;
-  if (!(mbar_wait_warp(smem_u32(&plans.tile_full[at]), (i / C::kPlans) & 1))) return false;
+  if (!mbar_wait_warp(smem_u32(&plans.tile_full[at]), (i / C::kPlans) & 1)) return false;
   *tile = plans.tile[at];
   return true;
 }
@@ -351,7 +351,7 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       const int scale_rows = min(tile.n, p.rows - tile.row0);
       for (int kb = kb0; kb < kb1; ++kb, at.next(stages)) {
         const int s = at.s, lap = at.lap;
-        ok = mbar_wait(smem_u32(&empty[s]), lap ^ 1);
+        ok = mbar_wait_warp(smem_u32(&empty[s]), lap ^ 1);
         if (!ok) break;
         if (elect_one()) {
           const uint32_t base = smem_u32(ring + s * C::kStageBytes), bar = smem_u32(&full[s]);
@@ -376,7 +376,7 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       if (!ok) break;
       for (int kb = kb0; kb < kb1; ++kb, at.next(stages)) {
         const int s = at.s, lap = at.lap;
-        ok = (mbar_wait_warp(smem_u32(&raw_scales[s]), lap));
+        ok = mbar_wait_warp(smem_u32(&raw_scales[s]), lap);
         if (!ok) break;
         turn_scales<1>(ring + s * C::kStageBytes + C::kAtXs, tile.n, lane);
         fence_proxy_async_smem();
@@ -394,14 +394,14 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       Tile tile;
       const int b = n_tile & 1;
       ok = next_tile(plans, p, t, n_tile, &tile) &&
-           (mbar_wait_warp(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1));
+           mbar_wait_warp(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1);
       if (!ok) break;
       tc_fence_after();
       const uint32_t d = tmem0 + b * kTok;
       const uint32_t idesc = make_idesc_fp4(kFeat, __shfl_sync(0xffffffffu, tile.n, 0), kNv, 0);
       for (int kb = kb0; kb < kb1; ++kb, ++it, at.next(stages)) {
         const int s = at.s, lap = at.lap;
-        ok = (mbar_wait_warp(smem_u32(&full[s]), lap));
+        ok = mbar_wait_warp(smem_u32(&full[s]), lap);
         if (!ok) break;
         tc_fence_after();
         const uint32_t base = ring0 + s * C::kStageBytes;
@@ -615,7 +615,8 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   if (warp == C::kEpiWarps) {  // ------------------------------------- producer
     const uint64_t keep = policy_evict_normal(), once = policy_evict_first();
     const int scale_tiles = (p.N + kFeat - 1) / kFeat;
-    int it = 0, n_tile = 0;
+    Place at;
+    int n_tile = 0;
     for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
       Tile tile;
       ok = next_tile(plans, p, t, n_tile, &tile);
@@ -629,9 +630,9 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
           p.w_scales + ((int64_t)tile.e * scale_tiles + min(feat / kFeat, scale_tiles - 1)) * nk * kWsBytes<kNv>;
       const int scale_rows = min(tile.n, p.rows - tile.row0);
       const uint32_t bytes = 2 * (kWBytes + (C::kTok / 2 >> (2 - box)) * kK / 2);
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % C::kStages;
-        ok = mbar_wait(smem_u32(&empty[s]), ((it / C::kStages) & 1) ^ 1);
+      for (int kb = kb0; kb < kb1; ++kb, at.next(C::kStages)) {
+        const int s = at.s, lap = at.lap;
+        ok = mbar_wait_warp(smem_u32(&empty[s]), lap ^ 1);
         if (!ok) break;
         if (elect_one()) {
           const uint32_t base = smem_u32(ring + s * C::kStageBytes), bar = mapa_shared(smem_u32(&full[s]), leader);
@@ -648,19 +649,20 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       }
     }
     // the last stages' releases arrive from the pair's leader before this CTA may leave
-    for (int i = max(0, it - C::kStages); i < it && ok; ++i)
-      ok = mbar_wait(smem_u32(&empty[i % C::kStages]), (i / C::kStages) & 1);
+    for (int i = 0; i < C::kStages && ok; ++i, at.next(C::kStages))
+      ok = mbar_wait_warp(smem_u32(&empty[at.s]), at.lap ^ 1);
   } else if (warp == C::kEpiWarps + 2 || warp == C::kEpiWarps + 4) {  // -- scales of the rows, by turns
     const int odd = warp == C::kEpiWarps + 4;
+    Place at;
     int it = 0, n_tile = 0;
     for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
       Tile tile;
       ok = next_tile(plans, p, t, n_tile, &tile);
       if (!ok) break;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+      for (int kb = kb0; kb < kb1; ++kb, ++it, at.next(C::kStages)) {
         if ((it & 1) != odd) continue;
-        const int s = it % C::kStages;
-        ok = (mbar_wait_warp(smem_u32(&raw_scales[s]), (it / C::kStages) & 1));
+        const int s = at.s, lap = at.lap;
+        ok = mbar_wait_warp(smem_u32(&raw_scales[s]), lap);
         if (!ok) break;
         turn_scales<2>(ring + s * C::kStageBytes + C::kAtXs, tile.n, lane);
         fence_proxy_async_smem();
@@ -672,19 +674,20 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     const uint32_t issue = elect_one();
     // (what the compiler cannot see to be the same for all lanes)
     const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem, 0), ring0 = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
+    Place at;
     int it = 0, n_tile = 0;
     for (int t = first_tile; t < total && ok && rank == 0; t += tile_step, ++n_tile) {
       Tile tile;
       const int b = n_tile & 1;
       ok = next_tile(plans, p, t, n_tile, &tile) &&
-           (mbar_wait_warp(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1));
+           mbar_wait_warp(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1);
       if (!ok) break;
       tc_fence_after();
       const int n = __shfl_sync(0xffffffffu, tile.n, 0);
       const uint32_t d = tmem0 + b * C::kTok, idesc = make_idesc_fp4(2 * kFeat, n, kNv, 0);
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % C::kStages;
-        ok = (mbar_wait_warp(smem_u32(&full[s]), (it / C::kStages) & 1));
+      for (int kb = kb0; kb < kb1; ++kb, ++it, at.next(C::kStages)) {
+        const int s = at.s, lap = at.lap;
+        ok = mbar_wait_warp(smem_u32(&full[s]), lap);
         if (!ok) break;
         tc_fence_after();
         const uint32_t base = ring0 + s * C::kStageBytes;
