@@ -267,6 +267,19 @@ __device__ __forceinline__ void stages_of(const Params& p, int nk, int part, int
   *last = nk * (part + 1) / p.split;
 }
 
+// The first stages of weight rows feat .. on their way to L2 while the kernel in front ends,
+// where there are no groups to wait for. (Its outputs, this product's rows, are not
+// touched before the wait.) One thread.
+template <bool kNv>
+__device__ __forceinline__ void prefetch_weights(const CUtensorMap* tm_w, const CUtensorMap* tm_x, const Params& p,
+                                                 int feat, int nk, int kb0, int kb1) {
+  prefetch_tmap(tm_w);
+  prefetch_tmap(tm_x);
+  if (feat >= p.N) return;
+  bulk_prefetch(p.w_scales + ((int64_t)(feat / kFeat) * nk + kb0) * kWsBytes<kNv>, (kb1 - kb0) * kWsBytes<kNv>);
+  for (int kb = kb0; kb < kb1; ++kb) tma_prefetch_2d(tm_w, kb * kK / 2, feat);
+}
+
 template <typename T, bool kNv, int kTok>
 __global__ void __launch_bounds__(Few<kTok>::kThreads, Few<kTok>::kCtasPerSm)
 fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ TokenMaps tm_x,
@@ -317,13 +330,9 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     tmem_relinquish();
   }
   grid_dep_launch();
-  if (p.offsets == nullptr && warp == C::kEpiWarps && elect_one()) {
-    // The weights' first stages on their way to L2 while the kernel in front ends. (Its
-    // outputs, this product's rows, are not touched before the wait.)
-    prefetch_tmap(&tm_w);
-    const int feat = whole_tile<C>(p, first_tile).feat;
-    for (int kb = kb0; kb < min(kb1, kb0 + C::kStages); ++kb) tma_prefetch_2d(&tm_w, kb * kK / 2, feat);
-  }
+  if (p.offsets == nullptr && warp == C::kEpiWarps && elect_one())
+    prefetch_weights<kNv>(&tm_w, &tm_x.box[p.box], p, whole_tile<C>(p, first_tile).feat, nk, kb0,
+                          min(kb1, kb0 + C::kStages));
   __syncwarp();
   if (p.split > 1) cluster_arrive();  // the barrier for landing parts is ready
   grid_dep_wait();
@@ -507,10 +516,10 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   }
 }
 
-// Stores 32 tokens of a warp's 32 weight rows. A lane holds a row's tokens; eight lanes
+// Stores tokens of a warp's 32 weight rows. A lane holds a row's tokens; eight lanes
 // transpose eight tokens among them in registers, so that each writes eight features of a
-// token. Where even lanes hold gate and odd lanes up rows, a lane keeps 16 tokens and gives
-// its neighbour the other 16.
+// token. Where even lanes hold gate and odd lanes up rows, a lane keeps half of the tokens
+// and gives its neighbour the others.
 template <typename T>
 struct ManyStore {
   float alpha, bias;
@@ -526,28 +535,31 @@ struct ManyStore {
     if (i < tile.rows && to >= 0 && f < p.n_out)
       *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)to * p.ldo + f) = o;
   }
-  __device__ __forceinline__ void operator()(const Params& p, const Tile& tile, float (&v)[32], int c, const int* rows,
-                                             const float* factor) const {
+  // tokens c .. c + kTokens - 1
+  template <int kTokens>
+  __device__ __forceinline__ void tokens(const Params& p, const Tile& tile, float (&v)[kTokens], int c, const int* rows,
+                                         const float* factor) const {
+    constexpr int kHalf = kTokens / 2;
     const int odd = lane & 1;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = v[j] * alpha + bias;
+    for (int j = 0; j < kTokens; ++j) v[j] = v[j] * alpha + bias;
     if (p.silu) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float own = odd ? v[16 + j] : v[j];
-        const float got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[16 + j], 1);
+      for (int j = 0; j < kHalf; ++j) {
+        const float own = odd ? v[kHalf + j] : v[j];
+        const float got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[kHalf + j], 1);
         v[j] = silu_mul(odd ? got : own, odd ? own : got);
-        if (p.row_scale) v[j] *= factor[c + 16 * odd + j];
+        if (p.row_scale) v[j] *= factor[c + kHalf * odd + j];
       }
 #pragma unroll
-      for (int j = 0; j < 16; j += 8)
-        put(p, tile, transpose8<T, 2>(v + j, lane), c + 16 * odd + j + ((lane >> 1) & 7), rows);
+      for (int j = 0; j < kHalf; j += 8)
+        put(p, tile, transpose8<T, 2>(v + j, lane), c + kHalf * odd + j + ((lane >> 1) & 7), rows);
     } else {
       if (p.row_scale)
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] *= factor[c + j];
+        for (int j = 0; j < kTokens; ++j) v[j] *= factor[c + j];
 #pragma unroll
-      for (int j = 0; j < 32; j += 8) put(p, tile, transpose8<T, 1>(v + j, lane), c + j + (lane & 7), rows);
+      for (int j = 0; j < kTokens; j += 8) put(p, tile, transpose8<T, 1>(v + j, lane), c + j + (lane & 7), rows);
     }
   }
 };
@@ -565,7 +577,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   g.row0 = reinterpret_cast<int*>(scl + C::kPlans * C::kTok);
   g.tile0 = g.row0 + 2 * p.E;
   __shared__ uint64_t full[C::kStages], raw_scales[C::kStages], empty[C::kStages];
-  __shared__ uint64_t acc_full[2], acc_empty[2];
+  __shared__ uint64_t acc_full[2], acc_empty[2], landed;
   __shared__ Plans<C> plans;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
@@ -580,6 +592,11 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   const int nk = (p.K + kK - 1) / kK;
   int kb0, kb1;
   stages_of(p, nk, part, &kb0, &kb1);
+  // Where K is shared: 16 tokens at a time go by turns to the parts, this one's among them,
+  // and land in the ring, [turn][part, without this one][four][weight row][4 tokens]
+  const int turns = p.split > 1 ? (whole_tile<C>(p, first_tile).rows + 15) / 16 : 0;
+  const int my_turns = (turns - part + p.split - 1) / p.split;
+  float4* landing = reinterpret_cast<float4*>(ring);
   if (warp == C::kEpiWarps) {
     init_barriers(full, C::kStages, 3, lane);  // the leader's expectation and both CTAs' turned scales
     init_barriers(raw_scales, C::kStages, 1, lane);
@@ -587,20 +604,23 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     init_barriers(acc_full, 2, 1, lane);
     init_barriers(acc_empty, 2, 2 * C::kEpiWarps, lane);
     init_plans(plans, lane);
-    if (lane == 0) failed = 0;
+    if (lane == 0) {
+      mbar_init(smem_u32(&landed), 1);
+      failed = 0;
+    }
     fence_barrier_init();
+    __syncwarp();
+    if (p.split > 1 && lane == 0)
+      mbar_arrive_expect_tx(smem_u32(&landed), my_turns * (p.split - 1) * 16 * kFeat * 4);
   }
   if (warp == C::kEpiWarps + 1) {
     tmem_alloc_pair(smem_u32(&tmem_slot), C::kColumns);
     tmem_relinquish_pair();
   }
   grid_dep_launch();
-  if (p.offsets == nullptr && warp == C::kEpiWarps && elect_one()) {
-    // as in the kernel above, to L2 only
-    prefetch_tmap(&tm_w);
-    const int feat = whole_tile<C>(p, first_tile).feat + (int)rank * kFeat;
-    for (int kb = kb0; kb < min(kb1, kb0 + C::kStages); ++kb) tma_prefetch_2d(&tm_w, kb * kK / 2, feat);
-  }
+  if (p.offsets == nullptr && warp == C::kEpiWarps && elect_one())
+    prefetch_weights<kNv>(&tm_w, &tm_x.box[p.box], p, whole_tile<C>(p, first_tile).feat + (int)rank * kFeat, nk, kb0,
+                          min(kb1, kb0 + C::kStages));
   __syncwarp();
   grid_dep_wait();
   find_groups<C>(g, p);
@@ -729,20 +749,12 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       ok = named_bar_and(1, 32 * C::kEpiWarps, ok && mbar_wait(smem_u32(&acc_full[b]), (n_tile >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
+      if (p.split > 1) break;  // the accumulator is summed below
       for (int c = (warp >> 2) * 32; c < tile.rows; c += 64) {
         uint32_t lo[16], hi[16];
         tmem_ld16(at + b * C::kTok + c, lo);
         tmem_ld16(at + b * C::kTok + c + 16, hi);
         tmem_ld_wait();
-        if (p.split > 1) {  // left in the ring, [token][row], for the sum below
-          float* mine = reinterpret_cast<float*>(ring) + c * kFeat + quarter * 32 + lane;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            mine[j * kFeat] = __uint_as_float(lo[j]);
-            mine[(j + 16) * kFeat] = __uint_as_float(hi[j]);
-          }
-          continue;
-        }
         if (c + 64 >= tile.rows) {  // this warp has read its part of the accumulator
           tc_fence_before();
           __syncwarp();
@@ -751,13 +763,12 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
         float v[32];
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(lo[j]), v[16 + j] = __uint_as_float(hi[j]);
-        store(p, tile, v, c, dst + slot * C::kTok, scl + slot * C::kTok);
+        store.tokens(p, tile, v, c, dst + slot * C::kTok, scl + slot * C::kTok);
       }
       if ((warp >> 2) * 32 >= tile.rows) {  // no tokens for this group
         __syncwarp();
         if (lane == 0) mbar_arrive_peer(mapa_shared(smem_u32(&acc_empty[b]), leader));
       }
-      if (p.split > 1) break;  // (the plan stays, for the sum)
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&plans.free[slot]));
     }
@@ -768,21 +779,47 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   }
   __syncwarp();
   if (p.split > 1) {
-    // 32 tokens at a time by turns of the parts and the groups of warps, added in the parts' order
-    cluster_sync_all();
-    if (warp < C::kEpiWarps && first_tile < total) {
+    cluster_sync_all();  // every ring is idle: parts may land there
+    if (warp < C::kEpiWarps && first_tile < total && ok) {
       const Tile tile = plans.tile[0];
-      const int quarter = warp & 3;
-      const ManyStore<T> store(p, tile, plans.alpha[0], (int)rank, quarter, lane);
-      const uint32_t mine = smem_u32(ring) + (quarter * 32 + lane) * 4;
-      for (int c = (2 * part + (warp >> 2)) * 32; c < tile.rows; c += 64 * p.split) {
-        float v[32] = {};
-        for (int q = 0; q < p.split; ++q) {
-          const uint32_t at = mapa_shared(mine, 2 * q + rank) + c * kFeat * 4;
+      const int quarter = warp & 3, group = warp >> 2, row = quarter * 32 + lane;
+      const uint32_t at = tmem + ((uint32_t)quarter << 21);
+      tc_fence_after();
+      for (int i = group; i < turns; i += 2) {
+        const int turn = i / p.split, who = i - turn * p.split;
+        if (who == part) continue;
+        uint32_t v[16];
+        tmem_ld16(at + 16 * i, v);
+        tmem_ld_wait();
+        const int slot = turn * (p.split - 1) + (part < who ? part : part - 1);
+        const uint32_t to = mapa_shared(smem_u32(landing + slot * 4 * kFeat + row), 2 * who + rank);
+        const uint32_t bar = mapa_shared(smem_u32(&landed), 2 * who + rank);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] += ld_dsmem_f32(at + j * kFeat * 4);
+        for (int j = 0; j < 4; ++j) st_async_v4(to + j * kFeat * 16, v + 4 * j, bar);
+      }
+      const ManyStore<T> store(p, tile, plans.alpha[0], (int)rank, quarter, lane);
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&landed), 0));
+      for (int turn = group; turn < my_turns && ok; turn += 2) {
+        const int c = 16 * (turn * p.split + part);
+        uint32_t own[16];
+        tmem_ld16(at + c, own);
+        tmem_ld_wait();
+        float v[16] = {};
+        for (int q = 0; q < p.split; ++q) {  // in the parts' order
+          const float4* from = landing + (turn * (p.split - 1) + (q < part ? q : q - 1)) * 4 * kFeat + row;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float4 f = q == part ? make_float4(__uint_as_float(own[4 * j]), __uint_as_float(own[4 * j + 1]),
+                                                     __uint_as_float(own[4 * j + 2]), __uint_as_float(own[4 * j + 3]))
+                                       : from[j * kFeat];
+            v[4 * j] += f.x, v[4 * j + 1] += f.y, v[4 * j + 2] += f.z, v[4 * j + 3] += f.w;
+          }
         }
-        store(p, tile, v, c, dst, scl);
+        store.tokens(p, tile, v, c, dst, scl);
+      }
+      if (!ok && lane == 0) {
+        failed = 1;
+        atomicOr(p.err, kErrWait);
       }
     }
   }

@@ -154,6 +154,11 @@ __device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int32_t c0, in
                : "memory");
 }
 
+// The same for plain bytes; address and size multiples of 16.
+__device__ __forceinline__ void bulk_prefetch(const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
+
 // 3-D tiled TMA load (no multicast); c0 is the innermost coordinate.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, int32_t c0, int32_t c1, int32_t c2,
                                             uint32_t bar, uint64_t policy) {
