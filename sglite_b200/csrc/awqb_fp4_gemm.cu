@@ -73,14 +73,16 @@ struct Few {
 struct Many {
   static constexpr int kTok = 208;
   static constexpr int kRound = 16;
-  static constexpr int kStages = 6;
+  static constexpr int kStages = 5;
   static constexpr int kEpiWarps = 8;
   static constexpr int kThreads = 32 * (kEpiWarps + 5);
   static constexpr int kPlans = 2, kCtasPerSm = 1;
   static constexpr int kAtX = kWBytes, kAtWs = kAtX + kTok / 2 * kK / 2, kAtXs = kAtWs + 2048;
   static constexpr int kStageBytes = kAtXs + 4096;
   static constexpr int kSets = 2 * kTok, kSetColumns = 48, kColumns = 512;
-  static __host__ __device__ constexpr int ring_bytes(int) { return kStages * kStageBytes; }
+  static constexpr int kTurn = 32 * 272;  // bytes of a group's transposition
+  // the stages and the two groups' transpositions
+  static __host__ __device__ constexpr int ring_bytes(int) { return kStages * kStageBytes + 2 * kTurn; }
 };
 
 // What the roles need to know of a tile, found by one warp ahead of them: the tile, then
@@ -516,50 +518,91 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   }
 }
 
-// Stores tokens of a warp's 32 weight rows. A lane holds a row's tokens; eight lanes
-// transpose eight tokens among them in registers, so that each writes eight features of a
-// token. Where even lanes hold gate and odd lanes up rows, a lane keeps half of the tokens
-// and gives its neighbour the others.
+// Stores tokens of a group of four warps' 128 weight rows, 8 G at a time. The accumulator
+// comes as fragments (rows l / 4 and l / 4 + 8 of each half of a warp's rows, tokens
+// 2 (l % 4) and the next), which stmatrix transposes on the way through the group's
+// [32 tokens][128 features] of shared memory (rows of 272 bytes: no bank twice for eight of
+// them), so that a token's features leave as 256 contiguous bytes. (64 bytes a warp, without
+// the group's barriers, kept the stores at 14 bytes a clock and SM.) Where rows are gate and
+// up by turns, neighbouring rows are four lanes apart: the even one takes the first eight
+// rows' four products and the odd one the last eight's, which come out as features
+// 0, 4, 1, 5 .. and are put in order behind the transposition.
 template <typename T>
 struct ManyStore {
-  float alpha, bias;
-  int f, lane;  // the first of the eight features that this lane writes
-  __device__ __forceinline__ ManyStore(const Params& p, const Tile& tile, float alpha_, int rank, int quarter, int lane_)
-      : alpha(alpha_), lane(lane_) {
-    const int row = tile.feat + rank * kFeat + quarter * 32;  // of the weights, the warp's first
-    bias = p.bias && row + lane < p.N ? (float)static_cast<const T*>(p.bias)[row + lane] : 0.f;
-    f = p.silu ? (row + (lane & 16)) / 2 : row + (lane & 24);
+  static constexpr int kPitch = 272;
+  float alpha, bias[2][2];
+  int f, lane, quarter, group;  // f: the CTA's first feature
+  uint32_t turn;
+  __device__ __forceinline__ ManyStore(const Params& p, const Tile& tile, float alpha_, int rank, int warp, int lane_,
+                                       uint8_t* turn_)
+      : alpha(alpha_), lane(lane_), quarter(warp & 3), group(warp >> 2), turn(smem_u32(turn_)) {
+    const int row = tile.feat + rank * kFeat;  // of the weights, the CTA's first
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = row + 32 * quarter + 8 * i + (lane >> 2);
+      bias[i / 2][i % 2] = p.bias && r < p.N ? (float)static_cast<const T*>(p.bias)[r] : 0.f;
+    }
+    f = p.silu ? row / 2 : row;
   }
-  __device__ __forceinline__ void put(const Params& p, const Tile& tile, uint4 o, int i, const int* rows) const {
-    const int to = rows[i];
-    if (i < tile.rows && to >= 0 && f < p.n_out)
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)to * p.ldo + f) = o;
-  }
-  // tokens c .. c + kTokens - 1
-  template <int kTokens>
-  __device__ __forceinline__ void tokens(const Params& p, const Tile& tile, float (&v)[kTokens], int c, const int* rows,
+  // tokens c .. c + 8 G - 1 of the tile, v[half of the rows][eight tokens]
+  template <int G>
+  __device__ __forceinline__ void tokens(const Params& p, int rows, uint32_t (&v)[2][G][4], int c, const int* to,
                                          const float* factor) const {
-    constexpr int kHalf = kTokens / 2;
-    const int odd = lane & 1;
+    const int odd = (lane >> 2) & 1;
+    uint32_t m[G][4];
 #pragma unroll
-    for (int j = 0; j < kTokens; ++j) v[j] = v[j] * alpha + bias;
-    if (p.silu) {
+    for (int g = 0; g < G; ++g) {
+      float2 s = make_float2(1.f, 1.f);
+      if (p.row_scale) s = *reinterpret_cast<const float2*>(factor + c + 8 * g + 2 * (lane & 3));
 #pragma unroll
-      for (int j = 0; j < kHalf; ++j) {
-        const float own = odd ? v[kHalf + j] : v[j];
-        const float got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[kHalf + j], 1);
-        v[j] = silu_mul(odd ? got : own, odd ? own : got);
-        if (p.row_scale) v[j] *= factor[c + kHalf * odd + j];
+      for (int h = 0; h < 2; ++h) {
+        float y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = __uint_as_float(v[h][g][k]) * alpha + bias[h][k / 2];
+        if (p.silu) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {  // even lanes keep rows 0..7 (gate) and get their up; odd ones 8..15 (up) and get gate
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? y[k] : y[2 + k], 4);
+            y[k] = odd ? silu_mul(got, y[2 + k]) : silu_mul(y[k], got);
+          }
+          m[g][h] = Pair<T>::pack(y[0] * s.x, y[1] * s.y);
+        } else {
+          m[g][2 * h] = Pair<T>::pack(y[0] * s.x, y[1] * s.y);
+          m[g][2 * h + 1] = Pair<T>::pack(y[2] * s.x, y[3] * s.y);
+        }
       }
+    }
+    named_bar_sync(2 + group, 128);  // (the last tokens are read)
 #pragma unroll
-      for (int j = 0; j < kHalf; j += 8)
-        put(p, tile, transpose8<T, 2>(v + j, lane), c + kHalf * odd + j + ((lane >> 1) & 7), rows);
-    } else {
-      if (p.row_scale)
+    for (int g = 0; g < G; ++g) {
+      const uint32_t at = turn + (8 * g + (lane & 7)) * kPitch;
+      if (p.silu)  // two matrices of eight features
+        asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1, %2};" ::"r"(
+                         at + quarter * 32 + ((lane >> 3) & 1) * 16),
+                     "r"(m[g][0]), "r"(m[g][1])
+                     : "memory");
+      else
+        st_matrix_trans(at + quarter * 64 + (lane >> 3) * 16, m[g]);
+    }
+    named_bar_sync(2 + group, 128);
+    // vector `piece` of every step-th token from t0 on
+    const int tid = quarter * 32 + lane, shift = p.silu ? 3 : 4, t0 = tid >> shift, piece = tid & ((1 << shift) - 1);
+    const int step = 128 >> shift;
+    T* out = static_cast<T*>(p.out) + f + 8 * piece;
 #pragma unroll
-        for (int j = 0; j < kTokens; ++j) v[j] *= factor[c + j];
-#pragma unroll
-      for (int j = 0; j < kTokens; j += 8) put(p, tile, transpose8<T, 1>(v + j, lane), c + j + (lane & 7), rows);
+    for (int i = 0; i < G; ++i) {
+      const int t = step * i + t0;
+      if (step * i >= 8 * G || c + t >= rows || f + 8 * piece >= p.n_out) break;
+      const int row = to[c + t];
+      uint4 o;
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
+                   : "r"(turn + t * kPitch + piece * 16)
+                   : "memory");
+      if (p.silu)
+        o = make_uint4(__byte_perm(o.x, o.y, 0x5410), __byte_perm(o.z, o.w, 0x5410), __byte_perm(o.x, o.y, 0x7632),
+                       __byte_perm(o.z, o.w, 0x7632));
+      if (row >= 0) *reinterpret_cast<uint4*>(out + (int64_t)row * p.ldo) = o;
     }
   }
 };
@@ -571,10 +614,10 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   using C = Many;
   extern __shared__ uint8_t raw[];
   uint8_t* ring = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
-  int* dst = reinterpret_cast<int*>(ring + C::kStages * C::kStageBytes);  // [kPlans][kTok] out row of a token
-  float* scl = reinterpret_cast<float*>(dst + C::kPlans * C::kTok);       // [kPlans][kTok] its factor
+  int* dst = reinterpret_cast<int*>(ring + C::ring_bytes(1));  // [kPlans][kTok] out row of a token
+  float* scl = reinterpret_cast<float*>(dst + C::kPlans * C::kTok);  // [kPlans][kTok] its factor; 32 are read at a time
   Groups g;
-  g.row0 = reinterpret_cast<int*>(scl + C::kPlans * C::kTok);
+  g.row0 = reinterpret_cast<int*>(scl + C::kPlans * C::kTok + 32);
   g.tile0 = g.row0 + 2 * p.E;
   __shared__ uint64_t full[C::kStages], raw_scales[C::kStages], empty[C::kStages];
   __shared__ uint64_t acc_full[2], acc_empty[2], landed;
@@ -593,7 +636,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   int kb0, kb1;
   stages_of(p, nk, part, &kb0, &kb1);
   // Where K is shared: 16 tokens at a time go by turns to the parts, this one's among them,
-  // and land in the ring, [turn][part, without this one][four][weight row][4 tokens]
+  // and land in the ring, [turn][part, without this one][fragment][lane of the warps' 128]
   const int turns = p.split > 1 ? (whole_tile<C>(p, first_tile).rows + 15) / 16 : 0;
   const int my_turns = (turns - part + p.split - 1) / p.split;
   float4* landing = reinterpret_cast<float4*>(ring);
@@ -629,6 +672,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  uint8_t* turn_bytes = ring + C::kStages * C::kStageBytes + ((warp >> 2) & 1) * C::kTurn;
   const int total = count_tiles(g, p);
   bool ok = true;
 
@@ -671,17 +715,19 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     // the last stages' releases arrive from the pair's leader before this CTA may leave
     for (int i = 0; i < C::kStages && ok; ++i, at.next(C::kStages))
       ok = mbar_wait_warp(smem_u32(&empty[at.s]), at.lap ^ 1);
-  } else if (warp == C::kEpiWarps + 2 || warp == C::kEpiWarps + 4) {  // -- scales of the rows, by turns
+  } else if (warp == C::kEpiWarps + 2 || warp == C::kEpiWarps + 4) {  // -- scales of the rows
+    // A slot of the ring is always the same warp's: copies may land out of order, and a wait
+    // for a lap of a slot tells it from the one before only if that one has been seen to end.
     const int odd = warp == C::kEpiWarps + 4;
     Place at;
-    int it = 0, n_tile = 0;
+    int n_tile = 0;
     for (int t = first_tile; t < total && ok; t += tile_step, ++n_tile) {
       Tile tile;
       ok = next_tile(plans, p, t, n_tile, &tile);
       if (!ok) break;
-      for (int kb = kb0; kb < kb1; ++kb, ++it, at.next(C::kStages)) {
-        if ((it & 1) != odd) continue;
+      for (int kb = kb0; kb < kb1; ++kb, at.next(C::kStages)) {
         const int s = at.s, lap = at.lap;
+        if ((s & 1) != odd) continue;
         ok = mbar_wait_warp(smem_u32(&raw_scales[s]), lap);
         if (!ok) break;
         turn_scales<2>(ring + s * C::kStageBytes + C::kAtXs, tile.n, lane);
@@ -745,25 +791,22 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       const int b = n_tile & 1, slot = n_tile % C::kPlans;
       ok = mbar_wait(smem_u32(&plans.rows_full[slot]), (n_tile / C::kPlans) & 1);
       const Tile tile = plans.tile[slot];
-      const ManyStore<T> store(p, tile, plans.alpha[slot], (int)rank, quarter, lane);
+      const ManyStore<T> store(p, tile, plans.alpha[slot], (int)rank, warp, lane, turn_bytes);
       ok = named_bar_and(1, 32 * C::kEpiWarps, ok && mbar_wait(smem_u32(&acc_full[b]), (n_tile >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
       if (p.split > 1) break;  // the accumulator is summed below
       for (int c = (warp >> 2) * 32; c < tile.rows; c += 64) {
-        uint32_t lo[16], hi[16];
-        tmem_ld16(at + b * C::kTok + c, lo);
-        tmem_ld16(at + b * C::kTok + c + 16, hi);
+        uint32_t v[2][4][4];
+        tmem_ld_fragments(at + b * C::kTok + c, v[0]);
+        tmem_ld_fragments(at + b * C::kTok + c + (16u << 16), v[1]);
         tmem_ld_wait();
         if (c + 64 >= tile.rows) {  // this warp has read its part of the accumulator
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_peer(mapa_shared(smem_u32(&acc_empty[b]), leader));
         }
-        float v[32];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(lo[j]), v[16 + j] = __uint_as_float(hi[j]);
-        store.tokens(p, tile, v, c, dst + slot * C::kTok, scl + slot * C::kTok);
+        store.tokens(p, tile.rows, v, c, dst + slot * C::kTok, scl + slot * C::kTok);
       }
       if ((warp >> 2) * 32 >= tile.rows) {  // no tokens for this group
         __syncwarp();
@@ -782,40 +825,45 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     cluster_sync_all();  // every ring is idle: parts may land there
     if (warp < C::kEpiWarps && first_tile < total && ok) {
       const Tile tile = plans.tile[0];
-      const int quarter = warp & 3, group = warp >> 2, row = quarter * 32 + lane;
+      const int quarter = warp & 3, group = warp >> 2, place = quarter * 32 + lane;
       const uint32_t at = tmem + ((uint32_t)quarter << 21);
       tc_fence_after();
       for (int i = group; i < turns; i += 2) {
         const int turn = i / p.split, who = i - turn * p.split;
         if (who == part) continue;
-        uint32_t v[16];
-        tmem_ld16(at + 16 * i, v);
+        uint32_t v[2][2][4];
+        tmem_ld_fragments(at + 16 * i, v[0]);
+        tmem_ld_fragments(at + 16 * i + (16u << 16), v[1]);
         tmem_ld_wait();
         const int slot = turn * (p.split - 1) + (part < who ? part : part - 1);
-        const uint32_t to = mapa_shared(smem_u32(landing + slot * 4 * kFeat + row), 2 * who + rank);
+        const uint32_t to = mapa_shared(smem_u32(landing + slot * 4 * kFeat + place), 2 * who + rank);
         const uint32_t bar = mapa_shared(smem_u32(&landed), 2 * who + rank);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) st_async_v4(to + j * kFeat * 16, v + 4 * j, bar);
+        for (int j = 0; j < 4; ++j) st_async_v4(to + j * kFeat * 16, v[j / 2][j % 2], bar);
       }
-      const ManyStore<T> store(p, tile, plans.alpha[0], (int)rank, quarter, lane);
+      const ManyStore<T> store(p, tile, plans.alpha[0], (int)rank, warp, lane, turn_bytes);
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&landed), 0));
       for (int turn = group; turn < my_turns && ok; turn += 2) {
         const int c = 16 * (turn * p.split + part);
-        uint32_t own[16];
-        tmem_ld16(at + c, own);
+        uint32_t own[2][2][4];
+        tmem_ld_fragments(at + c, own[0]);
+        tmem_ld_fragments(at + c + (16u << 16), own[1]);
         tmem_ld_wait();
-        float v[16] = {};
+        float sum[4][4] = {};
         for (int q = 0; q < p.split; ++q) {  // in the parts' order
-          const float4* from = landing + (turn * (p.split - 1) + (q < part ? q : q - 1)) * 4 * kFeat + row;
+          const float4* from = landing + (turn * (p.split - 1) + (q < part ? q : q - 1)) * 4 * kFeat + place;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float4 f = q == part ? make_float4(__uint_as_float(own[4 * j]), __uint_as_float(own[4 * j + 1]),
-                                                     __uint_as_float(own[4 * j + 2]), __uint_as_float(own[4 * j + 3]))
+            const uint32_t* o = own[j / 2][j % 2];
+            const float4 f = q == part ? make_float4(__uint_as_float(o[0]), __uint_as_float(o[1]), __uint_as_float(o[2]),
+                                                     __uint_as_float(o[3]))
                                        : from[j * kFeat];
-            v[4 * j] += f.x, v[4 * j + 1] += f.y, v[4 * j + 2] += f.z, v[4 * j + 3] += f.w;
+            sum[j][0] += f.x, sum[j][1] += f.y, sum[j][2] += f.z, sum[j][3] += f.w;
           }
         }
-        store.tokens(p, tile, v, c, dst, scl);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) own[j / 8][j / 4 % 2][j % 4] = __float_as_uint(sum[j / 4][j % 4]);
+        store.tokens(p, tile.rows, own, c, dst, scl);
       }
       if (!ok && lane == 0) {
         failed = 1;
@@ -853,7 +901,7 @@ int launch(int pair, const void* codes, const void* w, Params p, int max_split, 
                           tok_cta >> (2 - i));
   if (st != kOk) return st;
   const auto smem_for = [](int E, int split) {
-    return 1024 + C::ring_bytes(split) + 2 * C::kPlans * C::kTok * 4 + (3 * E + 1) * 4;
+    return 1024 + C::ring_bytes(split) + (2 * C::kPlans * C::kTok + 32) * 4 + (3 * E + 1) * 4;
   };
   static std::atomic<bool> ready[64];  // the kernel's attributes, set once for a device
   int dev = 0;

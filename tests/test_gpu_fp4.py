@@ -252,6 +252,25 @@ def test_gemm_shared_k(cuda, M, K, N, silu, fmt):
     assert torch.equal(got, _product(cuda, M, K, N, fmt, torch.bfloat16, silu, bias=True, ldo=8))
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,K,N", [(128, 2048, 28672), (450, 1536, 9000), (9, 4096, 28672), (2000, 800, 2056)])
+def test_gemm_many_tiles_over_and_over(cuda, M, K, N, fmt):
+    """Several tiles to a CTA, back to back without waiting between: the same bits each time,
+    right on columns spread over the tiles."""
+    codes, scales, xs, x = _rows(cuda, M, K, fmt)
+    g = torch.Generator(device=cuda).manual_seed(3)
+    w = torch.randint(0, 256, (N, K // 2), generator=g, device=cuda, dtype=torch.uint8)
+    byte = torch.randint(40 if fmt == "nvfp4" else 118, 60 if fmt == "nvfp4" else 122, (N, K // BLOCK[fmt]), generator=g,
+                         device=cuda, dtype=torch.uint8)
+    laid = ops.fp4_lay_out_scales(byte, fmt)
+    y = [ops.fp4_gemm(codes, scales, w, laid, fmt, torch.bfloat16, x_scale=xs) for _ in range(30)]
+    assert ops.device_error() == 0
+    assert all(torch.equal(t, y[0]) for t in y[1:])
+    at = torch.arange(7, N, 97)
+    want, bound = product_ref(x, values_ref(w[at.to(cuda)], byte[at.to(cuda)], fmt), xs)
+    assert within(y[0][:, at.to(cuda)].cpu(), want, bound, torch.bfloat16) <= 0
+
+
 @pytest.mark.parametrize("M", [1, 2, 8, 15, 16, 31, 32, 48, 63, 96, 127, 129, 255, 256, 257, 400, 511, 600])
 def test_gemm_row_counts(cuda, M):
     _product(cuda, M, 320, 272, "nvfp4", torch.bfloat16)
