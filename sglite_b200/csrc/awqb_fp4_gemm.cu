@@ -45,25 +45,24 @@ struct Params {
   int64_t ldo, out_rows;
   int rows, E, K, N, n_out, silu, feat_tiles, tile_out;  // tile_out: weight rows of a tile
   int tok_tiles, tok_per;  // without offsets: token tiles, rows of each
-  int box;    // of all tiles, or -1: by their rows
+  int box_rows;  // without offsets: rows of the box that all tiles take
   int split;  // CTAs (pairs) of a cluster that share a tile's K; above 1, a cluster has one tile
 };
 
-// One CTA per tile of 128 weight rows x kTok tokens, two CTAs to an SM. Of a stage:
+// One CTA per tile of 128 weight rows x up to 32 tokens, two CTAs to an SM. Of a stage:
 // weights, rows (both swizzled: 1024-byte aligned), the weights' and the rows' scales.
 // Tensor memory: two accumulators, two sets of scales. Where K is shared, the parts of a
 // tile's sum land behind the stages, of which there are fewer then.
-template <int kTokens>
 struct Few {
-  static constexpr int kTok = kTokens;
+  static constexpr int kTok = 32;
   static constexpr int kRound = 16;
-  static constexpr int kStages = kTok > 32 ? 3 : 4, kSplitStages = kTok > 32 ? 2 : 3;
+  static constexpr int kStages = 4, kSplitStages = 3;
   static constexpr int kEpiWarps = 4;
   static constexpr int kThreads = 32 * (kEpiWarps + 4);
   static constexpr int kPlans = 4, kCtasPerSm = 2;
   static constexpr int kAtX = kWBytes, kAtWs = kAtX + kTok * kK / 2, kAtXs = kAtWs + 2048;
   static constexpr int kStageBytes = kAtXs + 2048;
-  static constexpr int kSets = 2 * kTok, kSetColumns = 32, kColumns = kTok > 32 ? 256 : 128;
+  static constexpr int kSets = 2 * kTok, kSetColumns = 32, kColumns = 128;
   static __host__ __device__ constexpr int ring_bytes(int split) {
     return split > 1 ? kSplitStages * kStageBytes + kTok * kFeat * 4 : kStages * kStageBytes;
   }
@@ -74,15 +73,15 @@ struct Many {
   static constexpr int kTok = 208;
   static constexpr int kRound = 16;
   static constexpr int kStages = 5;
-  static constexpr int kEpiWarps = 8;
+  static constexpr int kEpiWarps = 12, kGroups = kEpiWarps / 4;
   static constexpr int kThreads = 32 * (kEpiWarps + 5);
   static constexpr int kPlans = 2, kCtasPerSm = 1;
   static constexpr int kAtX = kWBytes, kAtWs = kAtX + kTok / 2 * kK / 2, kAtXs = kAtWs + 2048;
   static constexpr int kStageBytes = kAtXs + 4096;
   static constexpr int kSets = 2 * kTok, kSetColumns = 48, kColumns = 512;
-  static constexpr int kTurn = 32 * 272;  // bytes of a group's transposition
-  // the stages and the two groups' transpositions
-  static __host__ __device__ constexpr int ring_bytes(int) { return kStages * kStageBytes + 2 * kTurn; }
+  static constexpr int kTurn = 16 * 272;  // bytes of a group's transposition
+  // the stages and the groups' transpositions
+  static __host__ __device__ constexpr int ring_bytes(int) { return kStages * kStageBytes + kGroups * kTurn; }
 };
 
 // What the roles need to know of a tile, found by one warp ahead of them: the tile, then
@@ -282,17 +281,17 @@ __device__ __forceinline__ void prefetch_weights(const CUtensorMap* tm_w, const 
   for (int kb = kb0; kb < kb1; ++kb) tma_prefetch_2d(tm_w, kb * kK / 2, feat);
 }
 
-template <typename T, bool kNv, int kTok>
-__global__ void __launch_bounds__(Few<kTok>::kThreads, Few<kTok>::kCtasPerSm)
+template <typename T, bool kNv>
+__global__ void __launch_bounds__(Few::kThreads, Few::kCtasPerSm)
 fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ TokenMaps tm_x,
                     const __grid_constant__ Params p) {
-  using C = Few<kTok>;
+  using C = Few;
   extern __shared__ uint8_t raw[];
   uint8_t* ring = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
-  int* dst = reinterpret_cast<int*>(ring + C::ring_bytes(p.split));  // [kPlans][kTok] out row of a token
-  float* scl = reinterpret_cast<float*>(dst + C::kPlans * kTok);          // [kPlans][kTok] its factor
+  int* dst = reinterpret_cast<int*>(ring + C::ring_bytes(p.split));  // [kPlans][C::kTok] out row of a token
+  float* scl = reinterpret_cast<float*>(dst + C::kPlans * C::kTok);          // [kPlans][C::kTok] its factor
   Groups g;
-  g.row0 = reinterpret_cast<int*>(scl + C::kPlans * kTok);  // [E] first rows, [E] row counts
+  g.row0 = reinterpret_cast<int*>(scl + C::kPlans * C::kTok);  // [E] first rows, [E] row counts
   g.tile0 = g.row0 + 2 * p.E;
   __shared__ uint64_t full[C::kStages], raw_scales[C::kStages], empty[C::kStages];
   __shared__ uint64_t acc_full[2], acc_empty[2], landed;
@@ -333,7 +332,7 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   }
   grid_dep_launch();
   if (p.offsets == nullptr && warp == C::kEpiWarps && elect_one())
-    prefetch_weights<kNv>(&tm_w, &tm_x.box[p.box], p, whole_tile<C>(p, first_tile).feat, nk, kb0,
+    prefetch_weights<kNv>(&tm_w, &tm_x.box[0], p, whole_tile<C>(p, first_tile).feat, nk, kb0,
                           min(kb1, kb0 + C::kStages));
   __syncwarp();
   if (p.split > 1) cluster_arrive();  // the barrier for landing parts is ready
@@ -354,7 +353,8 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       Tile tile;
       ok = next_tile(plans, p, t, n_tile, &tile);
       if (!ok) break;
-      const int box = p.box >= 0 ? p.box : box_of(tile.n, kTok);
+      const int box = p.offsets ? box_of(tile.rows, C::kTok) : 0;
+      const uint32_t x_bytes = (p.offsets ? C::kTok >> (2 - box) : p.box_rows) * kK / 2;
       // weights that one token tile reads once need not stay in L2
       const uint64_t wpol = (p.offsets ? tile.rows == g.row0[p.E + tile.e] : p.tok_tiles == 1) ? once : keep;
       const int wrow = tile.e * p.N + tile.feat;
@@ -367,7 +367,7 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
         if (elect_one()) {
           const uint32_t base = smem_u32(ring + s * C::kStageBytes), bar = smem_u32(&full[s]);
           const uint32_t sbar = smem_u32(&raw_scales[s]);
-          mbar_arrive_expect_tx(bar, kWBytes + kWsBytes<kNv> + (kTok >> (2 - box)) * kK / 2);
+          mbar_arrive_expect_tx(bar, kWBytes + kWsBytes<kNv> + x_bytes);
           mbar_arrive_expect_tx(sbar, scale_rows * 16);
           tma_load_2d(base, &tm_w, kb * kK / 2, wrow, bar, wpol);
           bulk_g2s(base + C::kAtWs, ws + (int64_t)kb * kWsBytes<kNv>, kWsBytes<kNv>, bar, wpol);
@@ -408,11 +408,11 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
            mbar_wait_warp(smem_u32(&acc_empty[b]), ((n_tile >> 1) & 1) ^ 1);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t d = tmem0 + b * kTok;
+      const uint32_t d = tmem0 + b * C::kTok;
       const uint32_t idesc = make_idesc_fp4(kFeat, __shfl_sync(0xffffffffu, tile.n, 0), kNv, 0);
       for (int kb = kb0; kb < kb1; ++kb, ++it, at.next(stages)) {
-        const int s = at.s, lap = at.lap;
-        ok = mbar_wait_warp(smem_u32(&full[s]), lap);
+        const int s = at.s;
+        ok = mbar_wait_warp(smem_u32(&full[s]), at.lap);
         if (!ok) break;
         tc_fence_after();
         const uint32_t base = ring0 + s * C::kStageBytes;
@@ -453,14 +453,14 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       ok = named_bar_and(1, 128, ok && mbar_wait(smem_u32(&acc_full[b]), (n_tile >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
-      const int* to = dst + at * kTok;
-      const float* factor = scl + at * kTok;
+      const int* to = dst + at * C::kTok;
+      const float* factor = scl + at * C::kTok;
       T* out = static_cast<T*>(p.out) + (p.silu ? row / 2 : row);
       if (!waited) cluster_wait();
       waited = true;
       for (int c = 0; c < tile.rows; c += 16) {
         uint32_t v[16];
-        tmem_ld16(tmem + b * kTok + c + ((uint32_t)warp << 21), v);
+        tmem_ld16(tmem + b * C::kTok + c + ((uint32_t)warp << 21), v);
         tmem_ld_wait();
         if (p.split > 1) {
 #pragma unroll
@@ -521,7 +521,7 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
 // Stores tokens of a group of four warps' 128 weight rows, 8 G at a time. The accumulator
 // comes as fragments (rows l / 4 and l / 4 + 8 of each half of a warp's rows, tokens
 // 2 (l % 4) and the next), which stmatrix transposes on the way through the group's
-// [32 tokens][128 features] of shared memory (rows of 272 bytes: no bank twice for eight of
+// [16 tokens][128 features] of shared memory (rows of 272 bytes: no bank twice for eight of
 // them), so that a token's features leave as 256 contiguous bytes. (64 bytes a warp, without
 // the group's barriers, kept the stores at 14 bytes a clock and SM.) Where rows are gate and
 // up by turns, neighbouring rows are four lanes apart: the even one takes the first eight
@@ -662,7 +662,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   }
   grid_dep_launch();
   if (p.offsets == nullptr && warp == C::kEpiWarps && elect_one())
-    prefetch_weights<kNv>(&tm_w, &tm_x.box[p.box], p, whole_tile<C>(p, first_tile).feat + (int)rank * kFeat, nk, kb0,
+    prefetch_weights<kNv>(&tm_w, &tm_x.box[0], p, whole_tile<C>(p, first_tile).feat + (int)rank * kFeat, nk, kb0,
                           min(kb1, kb0 + C::kStages));
   __syncwarp();
   grid_dep_wait();
@@ -672,7 +672,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  uint8_t* turn_bytes = ring + C::kStages * C::kStageBytes + ((warp >> 2) & 1) * C::kTurn;
+  uint8_t* turn_bytes = ring + C::kStages * C::kStageBytes + (warp >> 2) % C::kGroups * C::kTurn;
   const int total = count_tiles(g, p);
   bool ok = true;
 
@@ -685,7 +685,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       Tile tile;
       ok = next_tile(plans, p, t, n_tile, &tile);
       if (!ok) break;
-      const int box = p.box >= 0 ? p.box : box_of(tile.n / 2, C::kTok / 2);
+      const int box = p.offsets ? box_of(min(tile.rows, tile.n / 2), C::kTok / 2) : 0;
       // weights that one token tile reads once need not stay in L2
       const uint64_t wpol = (p.offsets ? tile.rows == g.row0[p.E + tile.e] : p.tok_tiles == 1) ? once : keep;
       const int feat = tile.feat + (int)rank * kFeat, row = tile.row0 + (int)rank * (tile.n / 2);
@@ -693,7 +693,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       const uint8_t* ws =
           p.w_scales + ((int64_t)tile.e * scale_tiles + min(feat / kFeat, scale_tiles - 1)) * nk * kWsBytes<kNv>;
       const int scale_rows = min(tile.n, p.rows - tile.row0);
-      const uint32_t bytes = 2 * (kWBytes + (C::kTok / 2 >> (2 - box)) * kK / 2);
+      const uint32_t bytes = 2 * (kWBytes + (p.offsets ? C::kTok / 2 >> (2 - box) : p.box_rows) * kK / 2);
       for (int kb = kb0; kb < kb1; ++kb, at.next(C::kStages)) {
         const int s = at.s, lap = at.lap;
         ok = mbar_wait_warp(smem_u32(&empty[s]), lap ^ 1);
@@ -752,8 +752,8 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       const int n = __shfl_sync(0xffffffffu, tile.n, 0);
       const uint32_t d = tmem0 + b * C::kTok, idesc = make_idesc_fp4(2 * kFeat, n, kNv, 0);
       for (int kb = kb0; kb < kb1; ++kb, ++it, at.next(C::kStages)) {
-        const int s = at.s, lap = at.lap;
-        ok = mbar_wait_warp(smem_u32(&full[s]), lap);
+        const int s = at.s;
+        ok = mbar_wait_warp(smem_u32(&full[s]), at.lap);
         if (!ok) break;
         tc_fence_after();
         const uint32_t base = ring0 + s * C::kStageBytes;
@@ -783,7 +783,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   } else if (warp == C::kEpiWarps + 3) {  // ---------------------------- plans
     ok = plan_tiles(plans, g, p, first_tile, tile_step, total, dst, scl, lane);
   } else {  // -------------------------------------------------------- epilogue
-    // Two groups of four warps take turns over 32 tokens.
+    // The groups of four warps take turns over 16 tokens.
     const int quarter = warp & 3;
     const uint32_t at = tmem + ((uint32_t)quarter << 21);
     int n_tile = 0;
@@ -796,19 +796,19 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       if (!ok) break;
       tc_fence_after();
       if (p.split > 1) break;  // the accumulator is summed below
-      for (int c = (warp >> 2) * 32; c < tile.rows; c += 64) {
-        uint32_t v[2][4][4];
+      for (int c = (warp >> 2) * 16; c < tile.rows; c += 16 * C::kGroups) {
+        uint32_t v[2][2][4];
         tmem_ld_fragments(at + b * C::kTok + c, v[0]);
         tmem_ld_fragments(at + b * C::kTok + c + (16u << 16), v[1]);
         tmem_ld_wait();
-        if (c + 64 >= tile.rows) {  // this warp has read its part of the accumulator
+        if (c + 16 * C::kGroups >= tile.rows) {  // this warp has read its part of the accumulator
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_peer(mapa_shared(smem_u32(&acc_empty[b]), leader));
         }
         store.tokens(p, tile.rows, v, c, dst + slot * C::kTok, scl + slot * C::kTok);
       }
-      if ((warp >> 2) * 32 >= tile.rows) {  // no tokens for this group
+      if ((warp >> 2) * 16 >= tile.rows) {  // no tokens for this group
         __syncwarp();
         if (lane == 0) mbar_arrive_peer(mapa_shared(smem_u32(&acc_empty[b]), leader));
       }
@@ -828,7 +828,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       const int quarter = warp & 3, group = warp >> 2, place = quarter * 32 + lane;
       const uint32_t at = tmem + ((uint32_t)quarter << 21);
       tc_fence_after();
-      for (int i = group; i < turns; i += 2) {
+      for (int i = group; i < turns; i += C::kGroups) {
         const int turn = i / p.split, who = i - turn * p.split;
         if (who == part) continue;
         uint32_t v[2][2][4];
@@ -843,7 +843,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       }
       const ManyStore<T> store(p, tile, plans.alpha[0], (int)rank, warp, lane, turn_bytes);
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&landed), 0));
-      for (int turn = group; turn < my_turns && ok; turn += 2) {
+      for (int turn = group; turn < my_turns && ok; turn += C::kGroups) {
         const int c = 16 * (turn * p.split + part);
         uint32_t own[2][2][4];
         tmem_ld_fragments(at + c, own[0]);
@@ -894,11 +894,12 @@ int launch(int pair, const void* codes, const void* w, Params p, int max_split, 
   // without groups all tiles take the first, largest tile's box
   p.tok_tiles = (p.rows + C::kTok - 1) / C::kTok;
   p.tok_per = ((p.rows + p.tok_tiles - 1) / p.tok_tiles + C::kRound - 1) / C::kRound * C::kRound;
-  p.box = p.offsets ? -1 : box_of(p.tok_per / pair, tok_cta);
-  for (int i = 0; i < 3 && st == kOk; ++i)
-    if (p.box < 0 || i == p.box)
-      st = make_bytes_map(&tx.box[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, p.rows, row_bytes, row_bytes,
-                          tok_cta >> (2 - i));
+  // without groups, a box of just the rows of a tile: rows that a box reads past the last
+  // one cost as much as real ones and more (1 token 4096 -> 28672: 16.2 us in a box of 16, 14.0 in one of 8)
+  p.box_rows = std::min(p.rows, p.tok_per / pair);
+  for (int i = 0; i < (p.offsets ? 3 : 1) && st == kOk; ++i)
+    st = make_bytes_map(&tx.box[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, p.rows, row_bytes, row_bytes,
+                        p.offsets ? tok_cta >> (2 - i) : p.box_rows);
   if (st != kOk) return st;
   const auto smem_for = [](int E, int split) {
     return 1024 + C::ring_bytes(split) + (2 * C::kPlans * C::kTok + 32) * 4 + (3 * E + 1) * 4;
@@ -952,20 +953,17 @@ int launch(int pair, const void* codes, const void* w, Params p, int max_split, 
 
 template <typename T, bool kNv>
 int pick(const void* codes, const void* w, const Params& p, cudaStream_t stream) {
-  const int64_t rows = (p.rows + p.E - 1) / p.E;  // of a group, on average
-#ifdef TUNE
-  const char* f = getenv("FP4K");
-  const char* sp = getenv("FP4S");
-  if (f) {
-    const int ms = sp ? atoi(sp) : 1;
-    if (f[0] == 'm') return launch<Many, fp4_gemm_many_kernel<T, kNv>>(2, codes, w, p, ms, stream);
-    if (f[0] == 's') return launch<Few<32>, fp4_gemm_few_kernel<T, kNv, 32>>(1, codes, w, p, ms, stream);
-    return launch<Few<64>, fp4_gemm_few_kernel<T, kNv, 64>>(1, codes, w, p, ms, stream);
-  }
-#endif
-  if (rows > 64) return launch<Many, fp4_gemm_many_kernel<T, kNv>>(2, codes, w, p, 4, stream);
-  if (rows > 16) return launch<Few<64>, fp4_gemm_few_kernel<T, kNv, 64>>(1, codes, w, p, 8, stream);
-  return launch<Few<32>, fp4_gemm_few_kernel<T, kNv, 32>>(1, codes, w, p, 8, stream);
+  // Groups: by their mean rows, since the CTA pairs' epilogue and start cost more and are
+  // spread over K's stages (us, few-rows and many-rows kernel, 2048 -> 1536 x 128 experts: 39 and 40 for
+  // 12 rows, 43 and 41 for 16, 53 and 44 for 48; 768 -> 2048: 31 and 33 for 32, 39 and 36 for 48). One group:
+  // above 32 rows, unless the few-rows kernel's tiles are few as well (4096 -> 28672, 48 rows: 22
+  // and 17; 8192 -> 1024, 128 rows: 7.9 and 9.0).
+  const int nk = (p.K + kK - 1) / kK;
+  const int64_t mean = (p.rows + p.E - 1) / p.E;
+  const int64_t tiles = (int64_t)((p.N + kFeat - 1) / kFeat) * ((p.rows + Few::kTok - 1) / Few::kTok);
+  const bool many = p.offsets ? mean > (nk >= 4 ? 20 : 40) : p.rows > Few::kTok && tiles > device_sm_count() / 2;
+  if (many) return launch<Many, fp4_gemm_many_kernel<T, kNv>>(2, codes, w, p, 4, stream);
+  return launch<Few, fp4_gemm_few_kernel<T, kNv>>(1, codes, w, p, 8, stream);
 }
 
 }  // namespace
