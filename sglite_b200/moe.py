@@ -111,6 +111,56 @@ class DenseExpertWeights:
         return self.e_begin + self.num_experts
 
 
+@dataclass
+class FP4ExpertWeights:
+    """A rank's experts of one projection in microscaled 4-bit floating point
+    (``ops.fp4_grouped_gemm``). No counterpart in the reference, whose experts are
+    dense (layers/moe_layer.py:36-47)."""
+
+    w: torch.Tensor              # uint8 [E_local, N, K / 2]
+    w_scales: torch.Tensor       # their laid-out block scales (ops.fp4_lay_out_scales)
+    fmt: str                     # "nvfp4" or "mxfp4"
+    act_dtype: torch.dtype
+    w_scale: Optional[torch.Tensor] = None   # fp32 [E_local] (nvfp4)
+    x_scale: Optional[torch.Tensor] = None   # fp32 [1]: the scale of this projection's input (nvfp4)
+    e_begin: int = 0             # first global expert id held here
+    num_global_experts: Optional[int] = None
+
+    @property
+    def num_experts(self) -> int:
+        return self.w.shape[0]
+
+    @property
+    def N(self) -> int:
+        return self.w.shape[1]
+
+    @property
+    def K(self) -> int:
+        return 2 * self.w.shape[2]
+
+    @property
+    def e_end(self) -> int:
+        return self.e_begin + self.num_experts
+
+    @classmethod
+    def from_checkpoint(cls, w: torch.Tensor, scales: torch.Tensor, fmt: str, act_dtype: torch.dtype,
+                        w_scale: Optional[torch.Tensor] = None, x_scale: Optional[torch.Tensor] = None,
+                        e_begin: int = 0, num_global_experts: Optional[int] = None,
+                        gate_up: bool = False) -> "FP4ExpertWeights":
+        """w uint8 [E, N, K / 2] and block scales (bytes) [E, N, K / 16 or K / 32] as stacked
+        from a checkpoint, on the device. gate_up=True for the merged gate_up projection (the
+        gate's rows, then the up's): its rows are interleaved, as the SiLU-and-mul epilogue
+        wants them."""
+        if w.dim() != 3 or w.element_size() != 1 or scales.element_size() != 1 \
+                or scales.shape != (*w.shape[:2], 2 * w.shape[2] // ops.FP4_BLOCK[fmt]):
+            raise ValueError(f"w {tuple(w.shape)} and scales {tuple(scales.shape)} are not {fmt} experts")
+        w, scales = w.view(torch.uint8), scales.view(torch.uint8)
+        if gate_up:
+            w, scales = ops.fp4_interleave_gate_up(w), ops.fp4_interleave_gate_up(scales)
+        return cls(w.contiguous(), ops.fp4_lay_out_scales(scales, fmt), fmt, act_dtype, w_scale, x_scale, e_begin,
+                   num_global_experts)
+
+
 def choose_block_m(num_tokens: int, topk: int, num_experts: int) -> int:
     """Rows per expert block (the grouped GEMM's token tile), from the mean
     number of rows per expert. Measured on B200 (Qwen3-30B-A3B experts): a
@@ -128,13 +178,14 @@ def choose_block_m(num_tokens: int, topk: int, num_experts: int) -> int:
     return 128
 
 
-ExpertWeights = Union[AWQExpertWeights, DenseExpertWeights, torch.Tensor]
+ExpertWeights = Union[AWQExpertWeights, DenseExpertWeights, FP4ExpertWeights, torch.Tensor]
 
 
 class AWQB200MoeBackend(BaseMoeBackend):
     """MoE backend over AWQ int4 experts (registered as "awq_b200"). 16-bit experts
     (``DenseExpertWeights``, or the plain [E, N, K] tensors that the reference's
-    backends take) run on the grouped 16-bit kernel."""
+    backends take) run on the grouped 16-bit kernel, 4-bit floating-point ones
+    (``FP4ExpertWeights``, w1 with gate and up rows by turns) on the block-scaled one."""
 
     def forward(self, hidden_states: torch.Tensor, w1: ExpertWeights, w2: ExpertWeights,
                 gating_output: torch.Tensor, topk: int, renormalize: bool, activation: str = "silu",
@@ -162,10 +213,12 @@ class AWQB200MoeBackend(BaseMoeBackend):
             raise ValueError("w1 and w2 hold different experts")
         E_glob = w1.num_global_experts or w1.num_experts
         numel = M * topk
-        if isinstance(w1, DenseExpertWeights) != isinstance(w2, DenseExpertWeights):
-            raise ValueError("w1 and w2 must both be AWQ or both be 16-bit experts")
+        if any(isinstance(w1, kind) != isinstance(w2, kind) for kind in (DenseExpertWeights, FP4ExpertWeights)):
+            raise ValueError("w1 and w2 must both be AWQ, both 16-bit or both 4-bit floating-point experts")
         if isinstance(w1, DenseExpertWeights):
             return self._dense_experts(x, w1, w2, topk_weights, topk_ids)
+        if isinstance(w1, FP4ExpertWeights):
+            return self._fp4_experts(x, w1, w2, topk_weights, topk_ids)
         block_m = choose_block_m(M, topk, E_glob)
         sorted_ids, block_expert, npp = ops.moe_align(topk_ids, w1.e_begin, w1.e_end, block_m)
         rows = sorted_ids.numel()
@@ -202,6 +255,26 @@ class AWQB200MoeBackend(BaseMoeBackend):
         y3 = torch.empty((numel, H), dtype=x.dtype, device=x.device)
         ops.grouped_gemm(a, w2.w, offsets, out=y3, row_map=order, row_scale=topk_weights.reshape(-1).contiguous())
         # always by the ids: an id that no expert here has (another rank's, padding) wrote no row of y3
+        return ops.moe_topk_sum(y3, M, topk, topk_ids, w1.e_begin, w1.e_end, x)
+
+
+    def _fp4_experts(self, x: torch.Tensor, w1: FP4ExpertWeights, w2: FP4ExpertWeights,
+                     topk_weights: torch.Tensor, topk_ids: torch.Tensor) -> torch.Tensor:
+        """The same over 4-bit experts: rows are quantised as they are gathered, and again
+        between the two products."""
+        M, H = x.shape
+        topk = topk_ids.shape[1]
+        if M * topk == 0:
+            return x
+        order, offsets = ops.group_rows(topk_ids.reshape(-1), w1.num_experts, w1.e_begin)
+        held = offsets[-1:]  # rows of experts elsewhere come last
+        codes, scales = ops.fp4_quantize(x, w1.fmt, scale=w1.x_scale, index=order, per_row=topk, count=held)
+        a = ops.fp4_grouped_gemm(codes, scales, w1.w, w1.w_scales, offsets, w1.fmt, x.dtype, x_scale=w1.x_scale,
+                                 w_scale=w1.w_scale, silu_mul=True)
+        codes, scales = ops.fp4_quantize(a, w2.fmt, scale=w2.x_scale, count=held)
+        y3 = torch.empty((M * topk, H), dtype=x.dtype, device=x.device)
+        ops.fp4_grouped_gemm(codes, scales, w2.w, w2.w_scales, offsets, w2.fmt, x.dtype, x_scale=w2.x_scale,
+                             w_scale=w2.w_scale, out=y3, row_map=order, row_scale=topk_weights.reshape(-1).contiguous())
         return ops.moe_topk_sum(y3, M, topk, topk_ids, w1.e_begin, w1.e_end, x)
 
 

@@ -1,7 +1,7 @@
 """RMSNorm layers over the library's kernels, with the interface of the
 reference's ``srt/model_executor/layers/norm.py:10-47`` (``RMSNorm``,
-``RMSNormFused``), and ``RMSNormGated`` for blocks with norms on both sides, a
-gate or a residual scale. After a row-parallel projection whose all-reduce is fused
+``RMSNormFused``), ``RMSNormFP4`` in front of 4-bit projections, and ``RMSNormGated``
+for blocks with norms on both sides, a gate or a residual scale. After a row-parallel projection whose all-reduce is fused
 into the GEMM (``distributed.PeerExchange.gemm_allreduce``), the residual add
 and the norm run as one more kernel, launched so that it overlaps the GEMM's
 tail (programmatic dependent launch)."""
@@ -44,6 +44,26 @@ class RMSNormFused:
             return ops.rmsnorm(x, self.weight, self.eps), x
         ops.fused_add_rmsnorm(x, residual, self.weight, self.eps)
         return x, residual
+
+
+class RMSNormFP4:
+    """RMSNorm with the residual add whose result goes straight into four bits, for a
+    projection that takes quantised rows (``FP4B200LinearMethod``): ``RMSNormFused``
+    (``norm.py:28-47``) and the quantisation in one kernel, without the rounding to
+    16 bits between. fmt "nvfp4" or "mxfp4"; ``scale`` is the projection's input_scale
+    (nvfp4)."""
+
+    def __init__(self, size: int, eps: float, fmt: str, scale: Optional[torch.Tensor] = None) -> None:
+        self.eps, self.fmt, self.scale = eps, fmt, scale
+        self.weight = torch.empty(size)
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None
+                ) -> Tuple[Tuple[torch.Tensor, torch.Tensor], torch.Tensor]:
+        """((codes, scales), residual): without a residual of rmsnorm(x), and x; with one,
+        residual += x in place and of rmsnorm(residual)."""
+        codes, scales, h = ops.fp4_add_rmsnorm(x, residual, self.weight, self.eps, self.fmt, scale=self.scale,
+                                               residual_out=residual)
+        return (codes, scales), h
 
 
 class RMSNormGated:

@@ -1083,6 +1083,16 @@ def fp4_lay_out_scales(scales: torch.Tensor, fmt: str) -> torch.Tensor:
     return s.permute(*range(d), d, d + 3, d + 4, d + 2, d + 1, d + 5).contiguous()
 
 
+def fp4_interleave_gate_up(t: torch.Tensor, dim: int = -2) -> torch.Tensor:
+    """A merged gate_up tensor's rows (the gate's, then the up's; weight codes, block scales in
+    the order of a checkpoint, or with dim=-1 a bias) by turns, as ``silu_mul`` wants them."""
+    n = t.shape[dim]
+    if n % 2:
+        raise ValueError(f"{n} rows are not a gate's and an up's")
+    turn = torch.arange(n, device=t.device).view(2, n // 2).t().reshape(-1)
+    return t.index_select(dim, turn)
+
+
 def _fp4_weight(w: torch.Tensor, w_scales: torch.Tensor, lead: Tuple[int, ...], K: int, fmt: str, di: int) -> None:
     """Checks quantised weights [*lead, N, K / 2] and their laid-out scales."""
     if w.dtype != torch.uint8 or not w.is_contiguous() or w.get_device() != di:

@@ -1,7 +1,8 @@
 """Quantization registry for the B200 AWQ path.
 
 ``get_quantization_config`` mirrors the reference's registry
-(``layers/quantization/__init__.py:15-29``) and adds ``"awq_b200"``;
+(``layers/quantization/__init__.py:15-29``) and adds ``"awq_b200"`` and
+``"fp4_b200"`` (microscaled 4-bit floating point);
 ``select_awq_config`` mirrors ``_create_awq_config``
 (``model_executor/models/config.py:73-89``) with the B200 method first.
 """
@@ -20,7 +21,11 @@ def get_quantization_config(method_name: str) -> type:
         from .awq_b200 import AWQB200Config
 
         return AWQB200Config
-    raise ValueError(f"Unknown quantization method: {method_name!r}. Supported methods: ['awq_b200']")
+    if name == "fp4_b200":
+        from .fp4_b200 import FP4B200Config
+
+        return FP4B200Config
+    raise ValueError(f"Unknown quantization method: {method_name!r}. Supported methods: ['awq_b200', 'fp4_b200']")
 
 
 def select_awq_config(config_dict: Dict[str, Any]):

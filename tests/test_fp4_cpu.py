@@ -214,3 +214,57 @@ def test_cpu_tensors_are_refused():
         ops.fp4_dequantize(c, s, "nvfp4", torch.float16)
     with pytest.raises(ValueError, match="CUDA"):
         ops.fp4_gemm(c, s, c, s, "nvfp4", torch.float16)
+
+
+# ---------------------------------------------------------------- config and linear method
+def test_config():
+    from sglite_b200.quantization import get_quantization_config
+    from sglite_b200.quantization.fp4_b200 import FP4B200Config
+
+    assert get_quantization_config("FP4_B200") is FP4B200Config
+    for config, fmt in (({"quant_algo": "NVFP4", "group_size": 16}, "nvfp4"), ({"quant_method": "mxfp4"}, "mxfp4")):
+        c = FP4B200Config.from_config(config)
+        assert c.fmt == fmt and c.group_size == BLOCK[fmt] and c.get_name() == "fp4_b200"
+        assert torch.bfloat16 in c.get_supported_act_dtypes() and c.get_min_capability() == 100
+    for bad in ({"quant_algo": "FP8"}, {"quant_algo": "NVFP4", "group_size": 32}, {"group_size": 16}):
+        with pytest.raises(ValueError):
+            FP4B200Config.from_config(bad)
+    with pytest.raises(ValueError):
+        FP4B200Config("int4")
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_created_weights(fmt):
+    from sglite_b200.quantization.fp4_b200 import FP4B200Config
+
+    method = FP4B200Config(fmt).get_linear_method()
+    w = method.create_weights(96, 24)
+    assert w["weight"].shape == (24, 48) and w["weight_scale"].shape == (24, 96 // BLOCK[fmt])
+    assert w["weight"].packed_dim == 1 and w["weight"].pack_factor == 2 and w["weight_scale"].output_dim == 0
+    assert ("input_scale" in w) == (fmt == "nvfp4") == ("weight_scale_2" in w)
+    for sizes in ((80, 24), (96, 20)):
+        with pytest.raises(ValueError):
+            method.create_weights(*sizes)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        method.process_weights_after_loading(w)
+    with pytest.raises(RuntimeError, match="process_weights_after_loading"):
+        method.apply_weights(w, torch.zeros((1, 96), dtype=torch.bfloat16))
+
+
+def test_interleaved_gate_up():
+    t = torch.arange(12).view(6, 2)
+    assert ops.fp4_interleave_gate_up(t)[:, 0].tolist() == [0, 6, 2, 8, 4, 10]
+    assert ops.fp4_interleave_gate_up(torch.arange(4), dim=-1).tolist() == [0, 2, 1, 3]
+    with pytest.raises(ValueError):
+        ops.fp4_interleave_gate_up(torch.zeros(3, 2))
+
+
+def test_experts_from_a_checkpoint_are_checked():
+    from sglite_b200.moe import FP4ExpertWeights
+
+    w, s = torch.zeros((2, 16, 32), dtype=torch.uint8), torch.zeros((2, 16, 4), dtype=torch.uint8)
+    e = FP4ExpertWeights.from_checkpoint(w, s, "nvfp4", torch.bfloat16, e_begin=2, num_global_experts=8, gate_up=True)
+    assert (e.num_experts, e.N, e.K, e.e_end) == (2, 16, 64, 4)
+    for bad in ((w, s[:, :, :2]), (w[0], s[0]), (w.int(), s), (w, s.float())):
+        with pytest.raises(ValueError):
+            FP4ExpertWeights.from_checkpoint(*bad, "nvfp4", torch.bfloat16)
