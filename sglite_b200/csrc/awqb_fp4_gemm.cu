@@ -75,7 +75,7 @@ struct Many {
   static constexpr int kStages = 5;
   static constexpr int kEpiWarps = 12, kGroups = kEpiWarps / 4;
   static constexpr int kThreads = 32 * (kEpiWarps + 5);
-  static constexpr int kPlans = 2, kCtasPerSm = 1;
+  static constexpr int kPlans = 4, kCtasPerSm = 1;
   static constexpr int kAtX = kWBytes, kAtWs = kAtX + kTok / 2 * kK / 2, kAtXs = kAtWs + 2048;
   static constexpr int kStageBytes = kAtXs + 4096;
   static constexpr int kSets = 2 * kTok, kSetColumns = 48, kColumns = 512;
