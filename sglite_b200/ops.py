@@ -922,11 +922,30 @@ FP4_FORMATS = {"nvfp4": 0, "mxfp4": 1}
 FP4_BLOCK = {"nvfp4": 16, "mxfp4": 32}
 
 
+_FP4_CODE = {(fmt, dtype): (f, d) for fmt, f in FP4_FORMATS.items() for dtype, d in DTYPE_CODE.items()}
+
+
 def _fp4_format(fmt: str) -> int:
     code = FP4_FORMATS.get(fmt)
     if code is None:
         raise ValueError(f"4-bit format {fmt!r}: one of {tuple(FP4_FORMATS)}")
     return code
+
+
+def _fp4_code(fmt: str, dtype: torch.dtype) -> Tuple[int, int]:
+    """The library's codes of a format and a 16-bit dtype."""
+    both = _FP4_CODE.get((fmt, dtype))
+    return both if both is not None else (_fp4_format(fmt), _dtype_code(dtype))
+
+
+def _fp4_x(x: torch.Tensor) -> Tuple[int, int]:
+    """(rows, K) of x [.., K]."""
+    shape = x.shape
+    if len(shape) == 2:
+        return shape
+    if not shape:
+        raise ValueError("x must have rows of K values")
+    return (x.numel() // shape[-1] if shape[-1] else 0), shape[-1]
 
 
 def _fp4_scale(scale: torch.Tensor, n: int, fmt: str, di: int, name: str) -> int:
@@ -952,9 +971,10 @@ def _fp4_rows_new(like: torch.Tensor, rows: int, K: int, fmt: str) -> Tuple[torc
 
 def _fp4_rows(codes: torch.Tensor, scales: torch.Tensor, fmt: str, di: int) -> Tuple[int, int]:
     """(rows, K) of quantised rows, checked."""
-    if codes.dim() != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous() or codes.get_device() != di:
+    shape = codes.shape
+    if len(shape) != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous() or codes.get_device() != di:
         raise ValueError("codes must be a contiguous uint8 [rows, K / 2] CUDA tensor")
-    rows, half = codes.shape
+    rows, half = shape
     if scales.shape != (-(-half // (8 * FP4_BLOCK[fmt])), rows, 16) or scales.dtype != torch.uint8 \
             or not scales.is_contiguous() or scales.get_device() != di:
         raise ValueError(f"scales {tuple(scales.shape)} must be the contiguous uint8 [granules, rows, 16] tensor of "
@@ -975,15 +995,10 @@ def fp4_quantize(x: torch.Tensor, fmt: str, *, scale: Optional[torch.Tensor] = N
     index (int32 [rows]): row r is x's row index[r] // per_row (an expert-sorted list of
     (token, choice) pairs, with per_row choices a token); rows whose index is outside x, and
     rows from ``count`` (int32 [1], on the device) on, are left as they were."""
-    code = _dtype_code(x.dtype)
-    fc = _fp4_format(fmt)
+    fc, code = _fp4_code(fmt, x.dtype)
     di = _device_of(x)
-    if x.dim() == 0:
-        raise ValueError("x must have rows of K values")
-    K = x.shape[-1]
-    rows_in = x.numel() // K if K else 0
-    pi = pc = 0
-    rows = rows_in
+    rows, K = _fp4_x(x)
+    rows_in, pi, pc = rows, 0, 0
     if index is not None:
         if index.dtype != torch.int32 or index.dim() != 1 or not index.is_contiguous() or index.get_device() != di:
             raise ValueError("index must be a contiguous int32 [rows] tensor on x's device")
@@ -1008,8 +1023,7 @@ def fp4_quantize(x: torch.Tensor, fmt: str, *, scale: Optional[torch.Tensor] = N
 def fp4_dequantize(codes: torch.Tensor, scales: torch.Tensor, fmt: str, dtype: torch.dtype, *,
                    scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values [rows, K] that quantised rows stand for, rounded to ``dtype``."""
-    code = _dtype_code(dtype)
-    fc = _fp4_format(fmt)
+    fc, code = _fp4_code(fmt, dtype)
     di = _device_of(codes)
     rows, K = _fp4_rows(codes, scales, fmt, di)
     ps = 0 if scale is None else _fp4_scale(scale, 1, fmt, di, "scale")
@@ -1034,13 +1048,9 @@ def fp4_add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: t
     from fp32. Returns (codes, scales, h), h rounded to x's dtype; without a residual h is x.
     ``residual_out`` may be residual (in place) or x. K is at most 16384."""
     dtype = x.dtype
-    code = _dtype_code(dtype)
-    fc = _fp4_format(fmt)
+    fc, code = _fp4_code(fmt, dtype)
     di = _device_of(x)
-    if x.dim() == 0:
-        raise ValueError("x must have rows of K values")
-    K = x.shape[-1]
-    rows = x.numel() // K if K else 0
+    rows, K = _fp4_x(x)
     if weight.numel() != K or weight.dtype != dtype or not weight.is_contiguous() or weight.get_device() != di:
         raise ValueError("weight must be a contiguous [K] tensor in the activation dtype on x's device")
     pr = po = ldr = ldo = 0
@@ -1048,7 +1058,7 @@ def fp4_add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: t
         if residual.shape != x.shape or residual.dtype != dtype or residual.get_device() != di:
             raise ValueError("residual must have the shape, dtype and device of x")
         if residual_out is None:
-            residual_out = torch.empty_like(residual)
+            residual_out = torch.empty_like(residual)  # (padded rows give a contiguous result)
         elif residual_out.shape != x.shape or residual_out.dtype != dtype or residual_out.get_device() != di:
             raise ValueError("residual_out must have the shape, dtype and device of residual")
         pr, ldr = residual.data_ptr(), _row_stride(residual, K, "residual")
@@ -1093,11 +1103,11 @@ def fp4_interleave_gate_up(t: torch.Tensor, dim: int = -2) -> torch.Tensor:
     return t.index_select(dim, turn)
 
 
-def _fp4_weight(w: torch.Tensor, w_scales: torch.Tensor, lead: Tuple[int, ...], K: int, fmt: str, di: int) -> None:
+def _fp4_weight(w: torch.Tensor, w_scales: torch.Tensor, lead: Tuple[int, ...], N: int, K: int, fmt: str, di: int) -> None:
     """Checks quantised weights [*lead, N, K / 2] and their laid-out scales."""
     if w.dtype != torch.uint8 or not w.is_contiguous() or w.get_device() != di:
         raise ValueError("w must be a contiguous uint8 [.., N, K / 2] tensor on the rows' device")
-    want = (*lead, -(-w.size(-2) // 128), -(-K // 256), 64 // FP4_BLOCK[fmt], 32, 4, 4)
+    want = (*lead, -(-N // 128), -(-K // 256), 64 // FP4_BLOCK[fmt], 32, 4, 4)
     if w_scales.shape != want or w_scales.dtype != torch.uint8 or not w_scales.is_contiguous() \
             or w_scales.get_device() != di:
         raise ValueError(f"w_scales {tuple(w_scales.shape)} must be {want}: fp4_lay_out_scales of the weight's scales")
@@ -1111,14 +1121,14 @@ def fp4_gemm(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor, w_scale
     [N, K / 2] with ``fp4_lay_out_scales``'s w_scales, both of format fmt, fp32 sums,
     rounded to ``dtype``; x_scale, w_scale: their fp32 [1] scales (nvfp4). silu_mul: w's
     rows (and bias) are gate and up by turns, y = silu(gate) * up [rows, N / 2]."""
-    code = _dtype_code(dtype)
-    fc = _fp4_format(fmt)
+    fc, code = _fp4_code(fmt, dtype)
     di = _device_of(codes)
     rows, K = _fp4_rows(codes, scales, fmt, di)
-    if w.dim() != 2 or 2 * w.size(1) != K:
-        raise ValueError(f"w {tuple(w.shape)} must be a [N, K / 2] tensor, K={K}")
-    N = w.size(0)
-    _fp4_weight(w, w_scales, (), K, fmt, di)
+    shape = w.shape
+    if len(shape) != 2 or 2 * shape[1] != K:
+        raise ValueError(f"w {tuple(shape)} must be a [N, K / 2] tensor, K={K}")
+    N = shape[0]
+    _fp4_weight(w, w_scales, (), N, K, fmt, di)
     pb = px = pw = 0
     if bias is not None:
         if bias.dtype != dtype or bias.numel() != N or not bias.is_contiguous() or bias.get_device() != di:
@@ -1149,14 +1159,13 @@ def fp4_grouped_gemm(codes: torch.Tensor, scales: torch.Tensor, w: torch.Tensor,
     offsets[e + 1]``, w uint8 [E, N, K / 2], w_scale fp32 [E] (nvfp4). offsets, out,
     row_map and row_scale as in ``grouped_gemm``; with silu_mul w's rows are gate and up
     by turns."""
-    code = _dtype_code(dtype)
-    fc = _fp4_format(fmt)
+    fc, code = _fp4_code(fmt, dtype)
     di = _device_of(codes)
     rows, K = _fp4_rows(codes, scales, fmt, di)
     if w.dim() != 3 or 2 * w.size(2) != K:
         raise ValueError(f"w {tuple(w.shape)} must be a [E, N, K / 2] tensor, K={K}")
     E, N, _ = w.shape
-    _fp4_weight(w, w_scales, (E,), K, fmt, di)
+    _fp4_weight(w, w_scales, (E,), N, K, fmt, di)
     px = 0 if x_scale is None else _fp4_scale(x_scale, 1, fmt, di, "x_scale")
     pw = 0 if w_scale is None else _fp4_scale(w_scale, E, fmt, di, "w_scale")
     if offsets.dtype != torch.int32 or offsets.numel() != E + 1 or not offsets.is_contiguous() \

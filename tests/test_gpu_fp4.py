@@ -52,12 +52,9 @@ def _check_quantized(codes, scales, x, fmt, scale):
 # ---------------------------------------------------------------- rows
 @pytest.mark.parametrize("M,K", [(1, 32), (1, 4096), (3, 96), (7, 256), (5, 288), (33, 544), (2, 16384), (129, 768),
                                  (1000, 64), (17, 2880)])
-@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("fmt,scale", [("nvfp4", None), ("nvfp4", 0.0137), ("nvfp4", 2.0 ** -6), ("mxfp4", None)])
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("scale", [None, 0.0137, 2.0 ** -6])
 def test_quantize(cuda, M, K, fmt, dtype, scale):
-    if fmt == "mxfp4" and scale is not None:
-        pytest.skip("mxfp4 has no other scale")
     x = _normal(cuda, M, K, dtype)
     s = None if scale is None else torch.full((1,), scale, device=cuda)
     codes, scales = ops.fp4_quantize(x, fmt, scale=s)
@@ -93,12 +90,10 @@ def _edges(dtype, fmt):
     return torch.tensor(rows, dtype=torch.float64).flatten().to(dtype)
 
 
-@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("fmt,scale", [("nvfp4", None), ("nvfp4", 2.0 ** -3), ("nvfp4", 0.3), ("nvfp4", 1e-30),
+                                       ("mxfp4", None)])
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("scale", [None, 2.0 ** -3, 0.3, 1e-30])
 def test_quantize_edges(cuda, fmt, dtype, scale):
-    if fmt == "mxfp4" and scale is not None:
-        pytest.skip("mxfp4 has no other scale")
     x = _edges(dtype, fmt)[None].to(cuda)
     s = None if scale is None else torch.full((1,), scale, device=cuda)
     codes, scales = ops.fp4_quantize(x, fmt, scale=s)
@@ -151,6 +146,19 @@ def test_quantize_gathered(cuda, fmt, per_row):
     src = x[(index.long()[live] // per_row).to(cuda)]
     _check_quantized(codes[live.to(cuda)], scales[:, live.to(cuda)], src, fmt, s)
     assert bool((codes[~live.to(cuda)] == 77).all()) and bool((scales[:, ~live.to(cuda)] == 77).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("count", [-3, 0, 1, 6, 9, 100])
+def test_quantize_up_to_a_count_on_the_device(cuda, fmt, count):
+    x = _normal(cuda, 9, 96, torch.float16)
+    out = ops.fp4_rows_empty(9, 96, fmt, cuda)
+    for t in out:
+        t.fill_(77)
+    codes, scales = ops.fp4_quantize(x, fmt, count=torch.tensor([count], dtype=torch.int32, device=cuda), out=out)
+    n = min(max(count, 0), 9)
+    _check_quantized(codes[:n], scales[:, :n], x[:n], fmt, None)
+    assert bool((codes[n:] == 77).all()) and bool((scales[:, n:] == 77).all())
 
 
 # ---------------------------------------------------------------- norm
@@ -253,6 +261,27 @@ def test_gemm_shared_k(cuda, M, K, N, silu, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("silu,bias,dtype", [(False, True, torch.bfloat16), (True, False, torch.float16)])
+@pytest.mark.parametrize("M,K,N", [(65, 2304, 3712), (100, 4128, 3600), (40, 1056, 5008), (33, 8192, 9488), (209, 800, 2608),
+                                   (333, 2080, 2320), (208, 512, 2400), (416, 1312, 1936), (1000, 32, 1200),
+                                   (417, 96, 1040)])
+def test_gemm_many_rows(cuda, M, K, N, fmt, silu, bias, dtype):
+    """The kernel of CTA pairs at odd sizes, K whole and shared by two or four pairs."""
+    codes, scales, xs, x = _rows(cuda, M, K, fmt)
+    w, byte, wv, ws = _weight(cuda, 1, N, K, fmt)
+    b = torch.randn(N, generator=torch.Generator().manual_seed(9)).to(dtype).to(cuda) if bias else None
+    n_out = N // 2 if silu else N
+    out = torch.full((M + 1, n_out + 8), 3.0, dtype=dtype, device=cuda)
+    laid = ops.fp4_lay_out_scales(byte[0], fmt).to(cuda)
+    got = ops.fp4_gemm(codes, scales, w[0], laid, fmt, dtype, x_scale=xs, w_scale=ws, bias=b, silu_mul=silu,
+                       out=out[:M, :n_out])
+    y, bound = product_ref(x.to(cuda), wv[0].to(cuda), xs, ws, b, silu)
+    assert ops.device_error() == 0
+    assert within(got, y, bound, dtype) <= 0
+    assert bool((out[M] == 3).all()) and bool((out[:, n_out:] == 3).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("M,K,N", [(128, 2048, 28672), (450, 1536, 9000), (9, 4096, 28672), (2000, 800, 2056)])
 def test_gemm_many_tiles_over_and_over(cuda, M, K, N, fmt):
     """Several tiles to a CTA, back to back without waiting between: the same bits each time,
@@ -321,6 +350,40 @@ def test_grouped(cuda, sizes, K, N, fmt):
 @pytest.mark.parametrize("sizes", [[1, 0, 40, 2], [100, 300, 0, 33], [2, 1, 1, 1, 0, 0, 3]])
 def test_grouped_epilogues(cuda, sizes, silu, scatter, first, fmt):
     _grouped(cuda, sizes, 288, 272, fmt, torch.float16, silu, pad=9, first=first, scatter=scatter, ldo=8)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("sizes", [[1] * 1024, [0] * 1000 + [3] * 24, [100] + [0] * 1023])
+def test_grouped_of_a_thousand_experts(cuda, sizes, fmt):
+    _grouped(cuda, sizes, 64, 24, fmt, torch.float16, pad=2)
+
+
+@pytest.mark.parametrize("sizes", [[3, 0, 5], [90, 120]])
+def test_grouped_rows_that_map_nowhere(cuda, sizes):
+    """Rows whose place is outside out are dropped, and so is what offsets say past the rows."""
+    rows, K, N = sum(sizes), 128, 136
+    codes, scales, xs, x = _rows(cuda, rows, K, "nvfp4")
+    w, byte, wv, ws = _weight(cuda, len(sizes), N, K, "nvfp4")
+    to = torch.arange(rows, dtype=torch.int32).flip(0)
+    to[1], to[2], to[rows - 1] = -1, 2 ** 31 - 1, rows + 4
+    off = torch.tensor([0] + sizes).cumsum(0).to(torch.int32)
+    off[-1] += 1000
+    out = torch.full((rows + 4, N), 3.0, dtype=torch.bfloat16, device=cuda)
+    factor = torch.rand(rows + 4, generator=torch.Generator().manual_seed(4))
+    got = ops.fp4_grouped_gemm(codes, scales, w, ops.fp4_lay_out_scales(byte, "nvfp4").to(cuda), off.to(cuda), "nvfp4",
+                               torch.bfloat16, x_scale=xs, w_scale=ws, out=out, row_map=to.to(cuda),
+                               row_scale=factor.to(cuda)).cpu()
+    left = torch.ones(rows + 4, dtype=torch.bool)
+    for e in range(len(sizes)):
+        for r in range(int(off[e]), min(int(off[e + 1]), rows)):
+            at = int(to[r])
+            if not 0 <= at < rows + 4:
+                continue
+            y, bound = product_ref(x[r:r + 1], wv[e], xs, ws[e])
+            f = float(factor[at])
+            assert within(got[at:at + 1], y * f, bound * f + 2.0 ** -23 * (y * f).abs(), torch.bfloat16) <= 0
+            left[at] = False
+    assert bool((got[left] == 3).all())
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
