@@ -63,8 +63,9 @@ struct Few {
   static constexpr int kAtX = kWBytes, kAtWs = kAtX + kTok * kK / 2, kAtXs = kAtWs + 2048;
   static constexpr int kStageBytes = kAtXs + 2048;
   static constexpr int kSets = 2 * kTok, kSetColumns = 32, kColumns = 128;
+  static constexpr int kTurn = 16 * 272;  // bytes of the epilogue's transposition
   static __host__ __device__ constexpr int ring_bytes(int split) {
-    return split > 1 ? kSplitStages * kStageBytes + kTok * kFeat * 4 : kStages * kStageBytes;
+    return split > 1 ? kSplitStages * kStageBytes + kTok * kFeat * 4 : kStages * kStageBytes + kTurn;
   }
 };
 // A CTA pair; each loads its 128 weight rows and half the tokens, and the scales of all
@@ -268,6 +269,94 @@ __device__ __forceinline__ void stages_of(const Params& p, int nk, int part, int
   *last = nk * (part + 1) / p.split;
 }
 
+// Stores tokens of a group of four warps' 128 weight rows, 8 G at a time. The accumulator
+// comes as fragments (rows l / 4 and l / 4 + 8 of each half of a warp's rows, tokens
+// 2 (l % 4) and the next), which stmatrix transposes on the way through the group's
+// [16 tokens][128 features] of shared memory (rows of 272 bytes: no bank twice for eight of
+// them), so that a token's features leave as 256 contiguous bytes. (64 bytes a warp, without
+// the group's barriers, kept the stores at 14 bytes a clock and SM.) Where rows are gate and
+// up by turns, neighbouring rows are four lanes apart: the even one takes the first eight
+// rows' four products and the odd one the last eight's, which come out as features
+// 0, 4, 1, 5 .. and are put in order behind the transposition.
+template <typename T>
+struct TileStore {
+  static constexpr int kPitch = 272;
+  float alpha, bias[2][2];
+  int f, lane, quarter, group;  // f: the CTA's first feature
+  uint32_t turn;
+  // row: of the weights, the CTA's first
+  __device__ __forceinline__ TileStore(const Params& p, int row, float alpha_, int warp, int lane_, uint8_t* turn_)
+      : alpha(alpha_), lane(lane_), quarter(warp & 3), group(warp >> 2), turn(smem_u32(turn_)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = row + 32 * quarter + 8 * i + (lane >> 2);
+      bias[i / 2][i % 2] = p.bias && r < p.N ? (float)static_cast<const T*>(p.bias)[r] : 0.f;
+    }
+    f = p.silu ? row / 2 : row;
+  }
+  // tokens c .. c + 8 G - 1 of the tile, v[half of the rows][eight tokens]
+  template <int G>
+  __device__ __forceinline__ void tokens(const Params& p, int rows, uint32_t (&v)[2][G][4], int c, const int* to,
+                                         const float* factor) const {
+    const int odd = (lane >> 2) & 1;
+    uint32_t m[G][4];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float2 s = make_float2(1.f, 1.f);
+      if (p.row_scale) s = *reinterpret_cast<const float2*>(factor + c + 8 * g + 2 * (lane & 3));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = __uint_as_float(v[h][g][k]) * alpha + bias[h][k / 2];
+        if (p.silu) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {  // even lanes keep rows 0..7 (gate) and get their up; odd ones 8..15 (up) and get gate
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? y[k] : y[2 + k], 4);
+            y[k] = odd ? silu_mul(got, y[2 + k]) : silu_mul(y[k], got);
+          }
+          m[g][h] = Pair<T>::pack(y[0] * s.x, y[1] * s.y);
+        } else {
+          m[g][2 * h] = Pair<T>::pack(y[0] * s.x, y[1] * s.y);
+          m[g][2 * h + 1] = Pair<T>::pack(y[2] * s.x, y[3] * s.y);
+        }
+      }
+    }
+    named_bar_sync(2 + group, 128);  // (the last tokens are read)
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const uint32_t at = turn + (8 * g + (lane & 7)) * kPitch;
+      if (p.silu)  // two matrices of eight features
+        asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1, %2};" ::"r"(
+                         at + quarter * 32 + ((lane >> 3) & 1) * 16),
+                     "r"(m[g][0]), "r"(m[g][1])
+                     : "memory");
+      else
+        st_matrix_trans(at + quarter * 64 + (lane >> 3) * 16, m[g]);
+    }
+    named_bar_sync(2 + group, 128);
+    // vector `piece` of every step-th token from t0 on
+    const int tid = quarter * 32 + lane, shift = p.silu ? 3 : 4, t0 = tid >> shift, piece = tid & ((1 << shift) - 1);
+    const int step = 128 >> shift;
+    T* out = static_cast<T*>(p.out) + f + 8 * piece;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int t = step * i + t0;
+      if (step * i >= 8 * G || c + t >= rows || f + 8 * piece >= p.n_out) break;
+      const int row = to[c + t];
+      uint4 o;
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
+                   : "r"(turn + t * kPitch + piece * 16)
+                   : "memory");
+      if (p.silu)
+        o = make_uint4(__byte_perm(o.x, o.y, 0x5410), __byte_perm(o.z, o.w, 0x5410), __byte_perm(o.x, o.y, 0x7632),
+                       __byte_perm(o.z, o.w, 0x7632));
+      if (row >= 0) *reinterpret_cast<uint4*>(out + (int64_t)row * p.ldo) = o;
+    }
+  }
+};
+
 // The first stages of weight rows feat .. on their way to L2 while the kernel in front ends,
 // where there are no groups to wait for. (Its outputs, this product's rows, are not
 // touched before the wait.) One thread.
@@ -458,29 +547,17 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       T* out = static_cast<T*>(p.out) + (p.silu ? row / 2 : row);
       if (!waited) cluster_wait();
       waited = true;
-      for (int c = 0; c < tile.rows; c += 16) {
+      for (int c = 0; c < tile.rows && p.split > 1; c += 16) {
         uint32_t v[16];
         tmem_ld16(tmem + b * C::kTok + c + ((uint32_t)warp << 21), v);
         tmem_ld_wait();
-        if (p.split > 1) {
 #pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            const int four = (c + j) / 4, turn = four / p.split, who = four - turn * p.split;
-            if (four < fours)
-              st_async_v4(mapa_shared(smem_u32(landing + (turn * p.split + part) * kFeat + tid), who), v + j,
-                          mapa_shared(smem_u32(&landed), who));
-          }
-          continue;
+        for (int j = 0; j < 16; j += 4) {
+          const int four = (c + j) / 4, turn = four / p.split, who = four - turn * p.split;
+          if (four < fours)
+            st_async_v4(mapa_shared(smem_u32(landing + (turn * p.split + part) * kFeat + tid), who), v + j,
+                        mapa_shared(smem_u32(&landed), who));
         }
-        if (c + 16 >= tile.rows) {  // the accumulator is read: the MMA warp may reuse it
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&acc_empty[b]));
-        }
-        float y[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(v[j]) * alpha + bias;
-        store_tokens<T, 8>(p, y, to, factor, c, tile.rows, row < p.N, odd, out);
       }
       if (p.split > 1) {
         ok = named_bar_and(1, 128, mbar_wait(smem_u32(&landed), 0));
@@ -496,6 +573,20 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
           store_tokens<T, 2>(p, y, to, factor, 4 * (turn * p.split + part), tile.rows, row < p.N, odd, out);
         }
         break;
+      }
+      const TileStore<T> store(p, tile.feat, alpha, warp, lane, ring + C::kStages * C::kStageBytes);
+      for (int c = 0; c < tile.rows; c += 16) {
+        uint32_t v[2][2][4];
+        const uint32_t from = tmem + b * C::kTok + c + ((uint32_t)warp << 21);
+        tmem_ld_fragments(from, v[0]);
+        tmem_ld_fragments(from + (16u << 16), v[1]);
+        tmem_ld_wait();
+        if (c + 16 >= tile.rows) {  // the accumulator is read: the MMA warp may reuse it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&acc_empty[b]));
+        }
+        store.tokens(p, tile.rows, v, c, to, factor);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&plans.free[at]));
@@ -517,95 +608,6 @@ fp4_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     tmem_dealloc(tmem, C::kColumns);
   }
 }
-
-// Stores tokens of a group of four warps' 128 weight rows, 8 G at a time. The accumulator
-// comes as fragments (rows l / 4 and l / 4 + 8 of each half of a warp's rows, tokens
-// 2 (l % 4) and the next), which stmatrix transposes on the way through the group's
-// [16 tokens][128 features] of shared memory (rows of 272 bytes: no bank twice for eight of
-// them), so that a token's features leave as 256 contiguous bytes. (64 bytes a warp, without
-// the group's barriers, kept the stores at 14 bytes a clock and SM.) Where rows are gate and
-// up by turns, neighbouring rows are four lanes apart: the even one takes the first eight
-// rows' four products and the odd one the last eight's, which come out as features
-// 0, 4, 1, 5 .. and are put in order behind the transposition.
-template <typename T>
-struct ManyStore {
-  static constexpr int kPitch = 272;
-  float alpha, bias[2][2];
-  int f, lane, quarter, group;  // f: the CTA's first feature
-  uint32_t turn;
-  __device__ __forceinline__ ManyStore(const Params& p, const Tile& tile, float alpha_, int rank, int warp, int lane_,
-                                       uint8_t* turn_)
-      : alpha(alpha_), lane(lane_), quarter(warp & 3), group(warp >> 2), turn(smem_u32(turn_)) {
-    const int row = tile.feat + rank * kFeat;  // of the weights, the CTA's first
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = row + 32 * quarter + 8 * i + (lane >> 2);
-      bias[i / 2][i % 2] = p.bias && r < p.N ? (float)static_cast<const T*>(p.bias)[r] : 0.f;
-    }
-    f = p.silu ? row / 2 : row;
-  }
-  // tokens c .. c + 8 G - 1 of the tile, v[half of the rows][eight tokens]
-  template <int G>
-  __device__ __forceinline__ void tokens(const Params& p, int rows, uint32_t (&v)[2][G][4], int c, const int* to,
-                                         const float* factor) const {
-    const int odd = (lane >> 2) & 1;
-    uint32_t m[G][4];
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      float2 s = make_float2(1.f, 1.f);
-      if (p.row_scale) s = *reinterpret_cast<const float2*>(factor + c + 8 * g + 2 * (lane & 3));
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float y[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) y[k] = __uint_as_float(v[h][g][k]) * alpha + bias[h][k / 2];
-        if (p.silu) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {  // even lanes keep rows 0..7 (gate) and get their up; odd ones 8..15 (up) and get gate
-            const float got = __shfl_xor_sync(0xffffffffu, odd ? y[k] : y[2 + k], 4);
-            y[k] = odd ? silu_mul(got, y[2 + k]) : silu_mul(y[k], got);
-          }
-          m[g][h] = Pair<T>::pack(y[0] * s.x, y[1] * s.y);
-        } else {
-          m[g][2 * h] = Pair<T>::pack(y[0] * s.x, y[1] * s.y);
-          m[g][2 * h + 1] = Pair<T>::pack(y[2] * s.x, y[3] * s.y);
-        }
-      }
-    }
-    named_bar_sync(2 + group, 128);  // (the last tokens are read)
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const uint32_t at = turn + (8 * g + (lane & 7)) * kPitch;
-      if (p.silu)  // two matrices of eight features
-        asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1, %2};" ::"r"(
-                         at + quarter * 32 + ((lane >> 3) & 1) * 16),
-                     "r"(m[g][0]), "r"(m[g][1])
-                     : "memory");
-      else
-        st_matrix_trans(at + quarter * 64 + (lane >> 3) * 16, m[g]);
-    }
-    named_bar_sync(2 + group, 128);
-    // vector `piece` of every step-th token from t0 on
-    const int tid = quarter * 32 + lane, shift = p.silu ? 3 : 4, t0 = tid >> shift, piece = tid & ((1 << shift) - 1);
-    const int step = 128 >> shift;
-    T* out = static_cast<T*>(p.out) + f + 8 * piece;
-#pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const int t = step * i + t0;
-      if (step * i >= 8 * G || c + t >= rows || f + 8 * piece >= p.n_out) break;
-      const int row = to[c + t];
-      uint4 o;
-      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
-                   : "r"(turn + t * kPitch + piece * 16)
-                   : "memory");
-      if (p.silu)
-        o = make_uint4(__byte_perm(o.x, o.y, 0x5410), __byte_perm(o.z, o.w, 0x5410), __byte_perm(o.x, o.y, 0x7632),
-                       __byte_perm(o.z, o.w, 0x7632));
-      if (row >= 0) *reinterpret_cast<uint4*>(out + (int64_t)row * p.ldo) = o;
-    }
-  }
-};
 
 template <typename T, bool kNv>
 __global__ void __launch_bounds__(Many::kThreads, 1)
@@ -791,7 +793,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       const int b = n_tile & 1, slot = n_tile % C::kPlans;
       ok = mbar_wait(smem_u32(&plans.rows_full[slot]), (n_tile / C::kPlans) & 1);
       const Tile tile = plans.tile[slot];
-      const ManyStore<T> store(p, tile, plans.alpha[slot], (int)rank, warp, lane, turn_bytes);
+      const TileStore<T> store(p, tile.feat + (int)rank * kFeat, plans.alpha[slot], warp, lane, turn_bytes);
       ok = named_bar_and(1, 32 * C::kEpiWarps, ok && mbar_wait(smem_u32(&acc_full[b]), (n_tile >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
@@ -841,7 +843,7 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
 #pragma unroll
         for (int j = 0; j < 4; ++j) st_async_v4(to + j * kFeat * 16, v[j / 2][j % 2], bar);
       }
-      const ManyStore<T> store(p, tile, plans.alpha[0], (int)rank, warp, lane, turn_bytes);
+      const TileStore<T> store(p, tile.feat + (int)rank * kFeat, plans.alpha[0], warp, lane, turn_bytes);
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&landed), 0));
       for (int turn = group; turn < my_turns && ok; turn += C::kGroups) {
         const int c = 16 * (turn * p.split + part);
