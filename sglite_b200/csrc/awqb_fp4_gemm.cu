@@ -10,8 +10,30 @@
 // Scales. An instruction takes 64 k and wants row r's scales on lane r % 32 of column
 // r / 32. The weights' scales are laid out so once, at load. The rows' scales are kept
 // as rows, [granule][row][16 bytes], since a group may begin at any row: the copy of a
-// tile's scales then is one contiguous bulk copy, and one warp turns four rows' words
-// among a lane's registers, in place, on the way to tensor memory.
+// tile's scales then is one contiguous bulk copy, and a warp turns four rows' words
+// among a lane's registers, in place, on the way to tensor memory. A stage is 256 k, one
+// swizzled row of 128 bytes.
+//
+// Roles of a CTA's warps: a producer of copies, one that issues the tensor-core work, the
+// scale turners, one that finds tiles and where their rows go ahead of the others (the
+// rows' places come from memory, two loads one after the other: 256 tokens' experts 52 -> 29 us),
+// and the epilogue. A role's code and waits are a whole warp's, and the issuing lane is
+// a predicate: with branches around them each instruction's operands pass through a move
+// to the uniform registers (4096 tokens 8192 -> 28672: 461 -> 424 us for the predicates, 414 -> 378
+// for roles and waits by the whole warp).
+//
+// Two kernels. Few rows: the weights' bytes bound it; a CTA takes 128 weight rows x up to 32
+// tokens, two CTAs to an SM, eight stages of 18 KB in flight there. Where the tiles of a
+// product do not fill the GPU, two to eight CTAs of a cluster share a tile's K, and each adds
+// its share of the tokens from what the others send to its shared memory (1 token
+// 4096 -> 4096: 7.9 us whole, 5.6 by four). Many rows: a CTA pair takes 256 weight rows x up to
+// 208 tokens, what two accumulators and two sets of scales leave of tensor memory; K is
+// shared by two or four pairs where tiles are few. On a B200: 1 token 4096 -> 6144 in 6.1 us, 32
+// tokens 4096 -> 28672 with SiLU-and-mul in 14.1 (4.8 TB/s), 4096 tokens 8192 -> 28672 in 380
+// (5.1 PFLOP/s; 440 when repeated for seconds, at 1.35 GHz under the power cap). What bounds
+// the second one until the power does is the issue of a stage's four products and twelve
+// copies of scales (560 cycles where the products take 416): mxfp4, with six copies, takes
+// 355 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -69,7 +91,9 @@ struct Few {
   }
 };
 // A CTA pair; each loads its 128 weight rows and half the tokens, and the scales of all
-// tokens. The accumulators and scales of 208 tokens fill tensor memory.
+// tokens. The accumulators and scales of 208 tokens fill tensor memory. Three groups of
+// epilogue warps: a tile of few stages is bound by them (4096 tokens' experts 768 -> 2048:
+// 82 us with two, 77 with three or four).
 struct Many {
   static constexpr int kTok = 208;
   static constexpr int kRound = 16;
