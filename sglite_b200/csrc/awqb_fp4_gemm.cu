@@ -30,10 +30,8 @@
 // 208 tokens, what two accumulators and two sets of scales leave of tensor memory; K is
 // shared by two or four pairs where tiles are few. On a B200: 1 token 4096 -> 6144 in 6.1 us, 32
 // tokens 4096 -> 28672 with SiLU-and-mul in 14.1 (4.8 TB/s), 4096 tokens 8192 -> 28672 in 380
-// (5.1 PFLOP/s; 440 when repeated for seconds, at 1.35 GHz under the power cap). What bounds
-// the second one until the power does is the issue of a stage's four products and twelve
-// copies of scales (560 cycles where the products take 416): mxfp4, with six copies, takes
-// 355 us.
+// (5.1 PFLOP/s; 440 when repeated for seconds, at 1.35 GHz under the power cap). mxfp4, with half
+// the copies of scales, takes 355 us there (burst).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
