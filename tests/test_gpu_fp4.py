@@ -190,6 +190,27 @@ def test_add_rmsnorm(cuda, M, K, fmt, dtype, add):
     assert bool(((got == 0) | (torch.sign(got) == torch.sign(y))).all())
 
 
+@pytest.mark.parametrize("scale,weight,size", [(1.5 * 2.0 ** 126, 2.0 ** 126, 2.0 ** -6), (2.0 ** -120, 2.0 ** -118, 1.0),
+                                               (1.0, 1.0, 1.0)])
+def test_add_rmsnorm_scales_near_the_ends_of_fp32(cuda, scale, weight, size):
+    """1 / scale is right where a fast fp32 division gives zero. The factor's low half may
+    be subnormal here: off by 2^-149 where it is 2^-121, far within the 2^-19 allowed."""
+    x = (_normal(cuda, 5, 1024, torch.bfloat16).float() * size).to(torch.bfloat16)
+    g = torch.Generator(device=cuda).manual_seed(2)
+    w = ((torch.rand(1024, generator=g, device=cuda) + 0.5) * weight).to(torch.bfloat16)
+    codes, scales, _ = ops.fp4_add_rmsnorm(x, None, w, 1e-9, "nvfp4", scale=torch.full((1,), scale, device=cuda))
+    wide = x.double().cpu()
+    y = wide / (wide.pow(2).mean(-1, keepdim=True) + 1e-9).sqrt() * w.double().cpu() / scale
+    d = 2.0 ** -19
+    byte = rows_scales(scales, 1024, "nvfp4")
+    most = y.unflatten(-1, (-1, 16)).abs().amax(-1)
+    low, high = block_scales(most * (1 - d), "nvfp4"), block_scales(most * (1 + d), "nvfp4")
+    assert bool(((byte == low) | (byte == high)).all()) and bool((byte > 0).all())
+    sv = scale_values(byte, "nvfp4").repeat_interleave(16, dim=-1)
+    got, q = _held(codes, scales, "nvfp4").abs(), y.abs() / sv
+    assert bool(((got >= GRID[nearest(q * (1 - d), GRID)] * sv) & (got <= GRID[nearest(q * (1 + d), GRID)] * sv)).all())
+
+
 def test_add_rmsnorm_in_place_and_strided(cuda):
     x, r = _normal(cuda, 7, 512, torch.bfloat16)[:, :288], _normal(cuda, 7, 640, torch.bfloat16)[:, 64:352]
     w = torch.ones(288, dtype=torch.bfloat16, device=cuda)
