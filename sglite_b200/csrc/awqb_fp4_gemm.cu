@@ -16,22 +16,25 @@
 //
 // Roles of a CTA's warps: a producer of copies, one that issues the tensor-core work, the
 // scale turners, one that finds tiles and where their rows go ahead of the others (the
-// rows' places come from memory, two loads one after the other: 256 tokens' experts 52 -> 29 us),
+// rows' places come from memory, two loads one after the other; with that and two CTAs to an SM
+// 256 tokens' experts 768 -> 2048 went from 52 to 28 us),
 // and the epilogue. A role's code and waits are a whole warp's, and the issuing lane is
 // a predicate: with branches around them each instruction's operands pass through a move
-// to the uniform registers (4096 tokens 8192 -> 28672: 461 -> 424 us for the predicates, 414 -> 378
-// for roles and waits by the whole warp).
+// to the uniform registers (4096 tokens 8192 -> 28672: 414 -> 378 us for roles and waits by the whole
+// warp).
 //
 // Two kernels. Few rows: the weights' bytes bound it; a CTA takes 128 weight rows x up to 32
-// tokens, two CTAs to an SM, eight stages of 18 KB in flight there. Where the tiles of a
+// tokens, two CTAs to an SM, eight stages of 23 KB in flight there. Where the tiles of a
 // product do not fill the GPU, two to eight CTAs of a cluster share a tile's K, and each adds
 // its share of the tokens from what the others send to its shared memory (1 token
 // 4096 -> 4096: 7.9 us whole, 5.6 by four). Many rows: a CTA pair takes 256 weight rows x up to
 // 208 tokens, what two accumulators and two sets of scales leave of tensor memory; K is
 // shared by two or four pairs where tiles are few. On a B200: 1 token 4096 -> 6144 in 6.1 us, 32
-// tokens 4096 -> 28672 with SiLU-and-mul in 14.1 (4.8 TB/s), 4096 tokens 8192 -> 28672 in 380
-// (5.1 PFLOP/s; 440 when repeated for seconds, at 1.35 GHz under the power cap). mxfp4, with half
-// the copies of scales, takes 355 us there (burst).
+// tokens 4096 -> 28672 with SiLU-and-mul in 13.9 (4.8 TB/s), 4096 tokens 8192 -> 28672 in 375
+// (5.1 PFLOP/s; 441 when repeated for seconds, at 1.37 GHz under the power cap) and in 350 in
+// mxfp4. Copies of that kernel which leave work out: 321 us without the scales' copies to tensor
+// memory, 289 without the products, 323 without both; so no one of them bounds it, and the loop
+// around them takes most of what they take.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -639,9 +642,9 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   extern __shared__ uint8_t raw[];
   uint8_t* ring = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
   int* dst = reinterpret_cast<int*>(ring + C::ring_bytes(1));  // [kPlans][kTok] out row of a token
-  float* scl = reinterpret_cast<float*>(dst + C::kPlans * C::kTok);  // [kPlans][kTok] its factor; 32 are read at a time
+  float* scl = reinterpret_cast<float*>(dst + C::kPlans * C::kTok);  // [kPlans][kTok] its factor
   Groups g;
-  g.row0 = reinterpret_cast<int*>(scl + C::kPlans * C::kTok + 32);
+  g.row0 = reinterpret_cast<int*>(scl + C::kPlans * C::kTok);
   g.tile0 = g.row0 + 2 * p.E;
   __shared__ uint64_t full[C::kStages], raw_scales[C::kStages], empty[C::kStages];
   __shared__ uint64_t acc_full[2], acc_empty[2], landed;
@@ -926,7 +929,7 @@ int launch(int pair, const void* codes, const void* w, Params p, int max_split, 
                         p.offsets ? tok_cta >> (2 - i) : p.box_rows);
   if (st != kOk) return st;
   const auto smem_for = [](int E, int split) {
-    return 1024 + C::ring_bytes(split) + (2 * C::kPlans * C::kTok + 32) * 4 + (3 * E + 1) * 4;
+    return 1024 + C::ring_bytes(split) + 2 * C::kPlans * C::kTok * 4 + (3 * E + 1) * 4;
   };
   static std::atomic<bool> ready[64];  // the kernel's attributes, set once for a device
   int dev = 0;

@@ -5,9 +5,8 @@
 // All three are bound by HBM. A lane takes vectors of eight values (16-byte loads, whole
 // sectors by neighbouring lanes); all of a thread's loads are issued before the first is
 // used. Launched with programmatic dependent launch, like the other norms. On a B200, 4096
-// rows: mxfp4 of 14336 values quantised in 24.3 us (6.1 TB/s), nvfp4 in 30 (issue: the
-// correctly rounded division), read back in 25.4 (5.8); norms of 8192 values in 40 and 42.6
-// (5.4 and 5.2 TB/s).
+// bf16 rows of 14336: mxfp4 quantised in 24.4 us (6.1 TB/s), nvfp4 in 30.5 (4.9), read back in
+// 25.4 (5.9); norms of 8192 values in 38.7 in mxfp4 and 42.4 in nvfp4 (5.7 and 5.2 TB/s).
 #include <cuda_runtime.h>
 
 #include <algorithm>

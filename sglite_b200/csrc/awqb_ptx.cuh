@@ -265,7 +265,7 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
                : "r"(taddr)
                : "memory");
 }
-// 16 lanes x 8 G columns as fragments: four words for each eight columns, lane l / 4's and
+// 16 lanes x 16 columns as fragments: four words for each eight columns, lane l / 4's and
 // l / 4 + 8's at columns 2 (l % 4) and the next.
 __device__ __forceinline__ void tmem_ld_fragments(uint32_t taddr, uint32_t (&r)[2][4]) {
   asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -273,16 +273,6 @@ __device__ __forceinline__ void tmem_ld_fragments(uint32_t taddr, uint32_t (&r)[
                  "=r"(r[1][2]), "=r"(r[1][3])
                : "r"(taddr)
                : "memory");
-}
-__device__ __forceinline__ void tmem_ld_fragments(uint32_t taddr, uint32_t (&r)[4][4]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0][0]), "=r"(r[0][1]), "=r"(r[0][2]), "=r"(r[0][3]), "=r"(r[1][0]), "=r"(r[1][1]), "=r"(r[1][2]),
-        "=r"(r[1][3]), "=r"(r[2][0]), "=r"(r[2][1]), "=r"(r[2][2]), "=r"(r[2][3]), "=r"(r[3][0]), "=r"(r[3][1]),
-        "=r"(r[3][2]), "=r"(r[3][3])
-      : "r"(taddr)
-      : "memory");
 }
 // Four 8 x 8 matrices of 16-bit values, stored transposed: lane l's address is the row
 // l % 8 in memory of matrix l / 8.

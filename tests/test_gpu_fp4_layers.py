@@ -13,7 +13,7 @@ from sglite_b200.lora import LoraAdapters, LoraBatch
 from sglite_b200.moe import AWQB200MoeBackend, DenseExpertWeights, FP4ExpertWeights
 from sglite_b200.norm import RMSNormFP4
 from sglite_b200.quantization import get_quantization_config
-from sglite_b200.quantization.fp4_b200 import FP4B200Config, quantize_weight
+from sglite_b200.quantization.fp4_b200 import quantize_weight
 
 pytestmark = pytest.mark.gpu
 
