@@ -70,6 +70,25 @@ def test_linear_method(cuda, fmt, shape, dtype):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+def test_one_row_without_a_batch_and_rows_from_the_middle(cuda, fmt):
+    """x [K] as a row, and weights and x that start inside a larger tensor: the same bits."""
+    K, N = 288, 136
+    method, weights, _, _ = _linear(cuda, fmt, K, N, torch.bfloat16)
+    x = _normal(cuda, 3, K)
+    want = method.apply_weights(weights, x)
+    one = method.apply_weights(weights, x[1])
+    assert one.shape == (N,) and torch.equal(one, want[1])
+    room = torch.zeros((7, K + 64), dtype=torch.bfloat16, device=cuda)
+    room[2:5, 32:32 + K] = x
+    assert torch.equal(method.apply_weights(weights, room[2:5, 32:32 + K]), want)
+    more = torch.zeros((N + 3, K // 2), dtype=torch.uint8, device=cuda)
+    more[3:] = weights["weight"]
+    assert torch.equal(method.apply_weights(dict(weights, weight=more[3:]), x), want)
+    with pytest.raises(ValueError):  # not a copy of the row for each of its uses
+        ops.fp4_quantize(x[:1].expand(4, K).transpose(0, 1), fmt)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_gate_up_and_quantised_rows(cuda, fmt):
     """The norm's rows straight into gate_up with SiLU-and-mul; the gate and up halves of the
     plain projection give the same."""
