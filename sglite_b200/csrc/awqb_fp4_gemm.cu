@@ -82,7 +82,7 @@ struct Few {
   static constexpr int kStages = 4, kSplitStages = 3;
   static constexpr int kEpiWarps = 4;
   static constexpr int kThreads = 32 * (kEpiWarps + 4);
-  static constexpr int kPlans = 4, kCtasPerSm = 2;
+  static constexpr int kPlans = 4, kPlanReaders = kEpiWarps, kCtasPerSm = 2;
   static constexpr int kAtX = kWBytes, kAtWs = kAtX + kTok * kK / 2, kAtXs = kAtWs + 2048;
   static constexpr int kStageBytes = kAtXs + 2048;
   static constexpr int kSets = 2 * kTok, kSetColumns = 32, kColumns = 128;
@@ -101,7 +101,8 @@ struct Many {
   static constexpr int kStages = 5;
   static constexpr int kEpiWarps = 12, kGroups = kEpiWarps / 4;
   static constexpr int kThreads = 32 * (kEpiWarps + 5);
-  static constexpr int kPlans = 4, kCtasPerSm = 1;
+  // the epilogue, and the scale turners: a tile of few stages may need nothing of one of them
+  static constexpr int kPlans = 4, kPlanReaders = kEpiWarps + 2, kCtasPerSm = 1;
   static constexpr int kAtX = kWBytes, kAtWs = kAtX + kTok / 2 * kK / 2, kAtXs = kAtWs + 2048;
   static constexpr int kStageBytes = kAtXs + 4096;
   static constexpr int kSets = 2 * kTok, kSetColumns = 48, kColumns = 512;
@@ -198,7 +199,7 @@ template <typename C>
 __device__ __forceinline__ void init_plans(Plans<C>& plans, int lane) {
   init_barriers(plans.tile_full, C::kPlans, 1, lane);
   init_barriers(plans.rows_full, C::kPlans, 1, lane);
-  init_barriers(plans.free, C::kPlans, C::kEpiWarps, lane);
+  init_barriers(plans.free, C::kPlans, C::kPlanReaders, lane);
 }
 
 // Tile t where all rows are one group.
@@ -215,7 +216,8 @@ __device__ __forceinline__ Tile whole_tile(const Params& p, int t) {
 }
 
 // The planning warp: tiles first_tile, first_tile + tile_step .. A plan is free again when
-// the epilogue, its last reader, is done with it.
+// the epilogue is done with it, and whoever else may still have it to read: the roles that
+// every tile needs something of have read it before the epilogue gets the tile.
 template <typename C>
 __device__ __forceinline__ bool plan_tiles(Plans<C>& plans, const Groups& g, const Params& p, int first_tile,
                                            int tile_step, int total, int* dst, float* scl, int lane) {
@@ -745,6 +747,8 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
   } else if (warp == C::kEpiWarps + 2 || warp == C::kEpiWarps + 4) {  // -- scales of the rows
     // A slot of the ring is always the same warp's: copies may land out of order, and a wait
     // for a lap of a slot tells it from the one before only if that one has been seen to end.
+    // Where tiles have few stages, one may have none in this warp's slots and be done without
+    // it: the plan is read and given back all the same.
     const int odd = warp == C::kEpiWarps + 4;
     Place at;
     int n_tile = 0;
@@ -752,6 +756,8 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
       Tile tile;
       ok = next_tile(plans, p, t, n_tile, &tile);
       if (!ok) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&plans.free[n_tile % C::kPlans]));
       for (int kb = kb0; kb < kb1; ++kb, at.next(C::kStages)) {
         const int s = at.s, lap = at.lap;
         if ((s & 1) != odd) continue;

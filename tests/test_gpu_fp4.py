@@ -379,6 +379,31 @@ def test_grouped_of_a_thousand_experts(cuda, sizes, fmt):
     _grouped(cuda, sizes, 64, 24, fmt, torch.float16, pad=2)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("K", [32, 256, 512, 768])
+def test_grouped_many_short_tiles(cuda, K, fmt):
+    """Dozens of tiles of one to three stages to a CTA pair: tiles that one of the two warps
+    that turn scales has nothing to do for. The same bits each time, right on columns spread
+    over the tiles."""
+    E, N, per = 64, 16384, 50
+    codes, scales, xs, x = _rows(cuda, E * per, K, fmt)
+    g = torch.Generator(device=cuda).manual_seed(K)
+    w = torch.randint(0, 256, (E, N, K // 2), generator=g, device=cuda, dtype=torch.uint8)
+    byte = torch.randint(40 if fmt == "nvfp4" else 118, 60 if fmt == "nvfp4" else 122, (E, N, K // BLOCK[fmt]),
+                         generator=g, device=cuda, dtype=torch.uint8)
+    laid = ops.fp4_lay_out_scales(byte, fmt)
+    off = (torch.arange(E + 1, device=cuda) * per).to(torch.int32)
+    first = ops.fp4_grouped_gemm(codes, scales, w, laid, off, fmt, torch.bfloat16, x_scale=xs)
+    for _ in range(30):
+        assert torch.equal(ops.fp4_grouped_gemm(codes, scales, w, laid, off, fmt, torch.bfloat16, x_scale=xs), first)
+    assert ops.device_error() == 0
+    at = torch.arange(7, N, 397, device=cuda)
+    for e in range(E):
+        rows = slice(e * per, (e + 1) * per)
+        want, bound = product_ref(x[rows], values_ref(w[e][at], byte[e][at], fmt), xs)
+        assert within(first[rows][:, at].cpu(), want, bound, torch.bfloat16) <= 0
+
+
 @pytest.mark.parametrize("sizes", [[3, 0, 5], [90, 120]])
 def test_grouped_rows_that_map_nowhere(cuda, sizes):
     """Rows whose place is outside out are dropped, and so is what offsets say past the rows."""
