@@ -875,7 +875,8 @@ fp4_gemm_many_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
         for (int j = 0; j < 4; ++j) st_async_v4(to + j * kFeat * 16, v[j / 2][j % 2], bar);
       }
       const TileStore<T> store(p, tile.feat + (int)rank * kFeat, plans.alpha[0], warp, lane, turn_bytes);
-      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&landed), 0));
+      // (all of them or none: a group's warps meet at barriers when they store)
+      ok = named_bar_and(1, 32 * C::kEpiWarps, mbar_wait(smem_u32(&landed), 0));
       for (int turn = group; turn < my_turns && ok; turn += C::kGroups) {
         const int c = 16 * (turn * p.split + part);
         uint32_t own[2][2][4];

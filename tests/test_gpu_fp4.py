@@ -321,6 +321,23 @@ def test_gemm_many_tiles_over_and_over(cuda, M, K, N, fmt):
     assert within(y[0][:, at.to(cuda)].cpu(), want, bound, torch.bfloat16) <= 0
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,K,N", [(65, 2304, 3712), (80, 4096, 4096), (100, 2048, 3840), (208, 8192, 2048), (209, 1024, 6000)])
+def test_gemm_pairs_share_k_over_and_over(cuda, M, K, N, fmt):
+    """K shared by two or four CTA pairs, whose warps have one turn, two or none to sum:
+    the same bits each time, right on columns spread over the tiles."""
+    codes, scales, xs, x = _rows(cuda, M, K, fmt)
+    w, byte, wv, ws = _weight(cuda, 1, N, K, fmt)
+    laid = ops.fp4_lay_out_scales(byte[0], fmt).to(cuda)
+    first = ops.fp4_gemm(codes, scales, w[0], laid, fmt, torch.bfloat16, x_scale=xs, w_scale=ws)
+    for _ in range(50):
+        assert torch.equal(ops.fp4_gemm(codes, scales, w[0], laid, fmt, torch.bfloat16, x_scale=xs, w_scale=ws), first)
+    assert ops.device_error() == 0
+    at = torch.arange(3, N, 37)
+    want, bound = product_ref(x, wv[0][at], xs, ws)
+    assert within(first[:, at.to(cuda)].cpu(), want, bound, torch.bfloat16) <= 0
+
+
 @pytest.mark.parametrize("M", [1, 2, 8, 15, 16, 31, 32, 48, 63, 96, 127, 129, 255, 256, 257, 400, 511, 600])
 def test_gemm_row_counts(cuda, M):
     _product(cuda, M, 320, 272, "nvfp4", torch.bfloat16)
