@@ -203,9 +203,9 @@ __device__ __forceinline__ double inverse(float x) {
   return fma(fma(-(double)x, y, 1.0), y, y);
 }
 
-// 1 / (rms * scale) of the row, as two fp32 numbers; over: 1 / scale. Each warp adds the
-// warps' sums for itself, so that one barrier is enough.
-__device__ __forceinline__ float2 row_factor(const NormArgs& a, float ss, double over, float* red) {
+// The row's mean square plus eps. Each warp adds the warps' sums for itself, so that one
+// barrier is enough.
+__device__ __forceinline__ double mean_square(const NormArgs& a, float ss, double eps, float* red) {
   const int warps = blockDim.x / 32, lane = threadIdx.x & 31;
   ss = warp_sum(ss);
   if (lane == 0) red[threadIdx.x >> 5] = ss;
@@ -213,8 +213,13 @@ __device__ __forceinline__ float2 row_factor(const NormArgs& a, float ss, double
   double sum = (lane & 15) < warps ? (double)red[lane & 15] : 0.0;
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  // 1 / sqrt(m), from its fp32 approximation by one Newton step
-  const double m = fma(sum, a.inv_K, (double)a.eps), y = (double)rsqrtf((float)m);
+  return fma(sum, a.inv_K, eps);
+}
+
+// over / sqrt(m) as two fp32 numbers, the root from its fp32 approximation by one Newton
+// step; over: 1 / scale.
+__device__ __forceinline__ float2 row_factor(double m, double over) {
+  const double y = (double)rsqrtf((float)m);
   const double f = fma(fma(-m * y, y, 1.0), 0.5 * y, y) * over;
   const float high = (float)f;
   return make_float2(high, (float)(f - (double)high));
@@ -237,16 +242,18 @@ __device__ __forceinline__ void norm_vector(const NormArgs& a, int64_t row, int 
   store_vector<kNv, 1>(u, most, a.codes, a.scales, a.rows, row, a.K, v, v < a.vecs);
 }
 
+// (mxfp4, two vectors: registers for three CTAs to an SM, 4096 rows of 8192 features 45.2 -> 40.2
+// us; nvfp4 is better off with two CTAs and 48 registers: 8192 rows of 4096 features 41.5, 42.1 with three.)
 template <typename T, bool kNv, int kVec>
-__global__ void __launch_bounds__(kNormThreads, kVec <= 2 ? 2 : 1) norm_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float red[kNormThreads / 32];
+__global__ void __launch_bounds__(kNormThreads, kVec > 2 ? 1 : kVec == 2 && !kNv ? 3 : 2) norm_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float red[2][kNormThreads / 32];
   grid_dep_wait();
   grid_dep_launch();
   const int64_t row = blockIdx.x;
   const int nvec = a.K / 8;
   const uint4* xp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ldx);
   const uint4* rp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.residual) + row * a.ldr);
-  const double over = kNv && a.scale != nullptr ? inverse(*a.scale) : 1.0;
+  double over = kNv && a.scale != nullptr ? inverse(*a.scale) : 1.0;
   uint4 x[kVec], r[kVec], w[kVec];
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
@@ -264,7 +271,24 @@ __global__ void __launch_bounds__(kNormThreads, kVec <= 2 ? 2 : 1) norm_kernel(c
       ss += add_vector<T>(a, row, v, x[i], r[i], h[i]);
     }
   }
-  const float2 factor = row_factor(a, ss, over, red);
+  double m = mean_square(a, ss, a.eps, red[0]);
+  if (__builtin_expect(!((float)m >= 0x1p-90f && (float)m <= 0x1p120f), 0)) {
+    // bf16 reaches from 2^-133 to 2^128, where fp32 squares end at half of that: once more with h
+    // times a power of two, which the quotient does not see. (The same branch for the whole row.)
+    const float by = m < 1.0 ? 0x1p80f : 0x1p-80f;
+    ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        h[i][j] *= by;
+        if (i * blockDim.x + threadIdx.x < nvec) ss += h[i][j] * h[i][j];
+      }
+    }
+    m = mean_square(a, ss, (double)a.eps * by * by, red[1]);
+    if (m > 0x1p127) m = 1.0, over = 0.0;  // an infinity in the row: all else is 0
+  }
+  const float2 factor = row_factor(m, over);
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
     const int v = i * blockDim.x + threadIdx.x;

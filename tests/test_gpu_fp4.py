@@ -211,6 +211,48 @@ def test_add_rmsnorm_scales_near_the_ends_of_fp32(cuda, scale, weight, size):
     assert bool(((got >= GRID[nearest(q * (1 - d), GRID)] * sv) & (got <= GRID[nearest(q * (1 + d), GRID)] * sv)).all())
 
 
+@pytest.mark.parametrize("power,eps", [(-126, 0.0), (-100, 0.0), (-100, 2.0 ** -190), (-60, 2.0 ** -110), (-40, 0.0),
+                                       (58, 1e-6), (63, 1e-6), (66, 1e-6), (100, 1e-6), (120, 0.0)])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("K", [96, 2048, 16384])
+def test_add_rmsnorm_of_very_large_and_small_rows(cuda, K, fmt, power, eps):
+    """Squares past both ends of fp32, beside an ordinary row: the formula's values."""
+    x = _normal(cuda, 3, K, torch.bfloat16)
+    x[1:] = (x[1:].double() * 2.0 ** power).to(torch.bfloat16)
+    r = torch.zeros_like(x)
+    r[1] = (_normal(cuda, 1, K, torch.bfloat16, seed=5)[0].double() * 2.0 ** power).to(torch.bfloat16)
+    w = (torch.rand(K, generator=torch.Generator(device=cuda).manual_seed(2), device=cuda) + 0.5).to(torch.bfloat16)
+    s = _scale(cuda, fmt, 0.011)
+    codes, scales, h = ops.fp4_add_rmsnorm(x, r, w, eps, fmt, scale=s)
+    assert bool(torch.isfinite(h).all())
+    eps = float(torch.tensor(eps, dtype=torch.float32))  # as the call takes it: 2^-190 is 0 there
+    wide = x.double().cpu() + r.double().cpu()
+    y = wide / (wide.pow(2).mean(-1, keepdim=True) + eps).sqrt() * w.double().cpu() / (1.0 if s is None else float(s))
+    d = 2.0 ** -19
+    byte = rows_scales(scales, K, fmt)
+    most = y.unflatten(-1, (-1, BLOCK[fmt])).abs().amax(-1)
+    low, high = block_scales(most * (1 - d), fmt), block_scales(most * (1 + d), fmt)
+    assert bool(((byte == low) | (byte == high)).all())
+    sv = scale_values(byte, fmt).repeat_interleave(BLOCK[fmt], dim=-1)
+    got, q = _held(codes, scales, fmt).abs(), torch.where(sv > 0, y.abs() / sv, 0.0)
+    assert bool(((got >= GRID[nearest(q * (1 - d), GRID)] * sv) & (got <= GRID[nearest(q * (1 + d), GRID)] * sv)).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_add_rmsnorm_of_a_row_with_an_infinity(cuda, dtype, fmt):
+    """Over an infinite root mean square everything finite is 0 and an infinity is NaN, in
+    its block only; a NaN makes its whole row NaN."""
+    K = 544
+    x = _normal(cuda, 3, K, dtype)
+    x[0, 40], x[1, 100] = float("inf"), float("nan")
+    codes, scales, _ = ops.fp4_add_rmsnorm(x, None, torch.ones(K, dtype=dtype, device=cuda), 1e-6, fmt)
+    got = _held(codes, scales, fmt)
+    block = torch.arange(K) // BLOCK[fmt] == 40 // BLOCK[fmt]
+    assert bool(torch.isnan(got[0, block]).all()) and not got[0, ~block].any()
+    assert bool(torch.isnan(got[1]).all()) and bool(torch.isfinite(got[2]).all())
+
+
 def test_add_rmsnorm_in_place_and_strided(cuda):
     x, r = _normal(cuda, 7, 512, torch.bfloat16)[:, :288], _normal(cuda, 7, 640, torch.bfloat16)[:, 64:352]
     w = torch.ones(288, dtype=torch.bfloat16, device=cuda)
