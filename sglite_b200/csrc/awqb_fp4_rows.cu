@@ -345,7 +345,8 @@ extern "C" int awqb_fp4_quantize(const awqb_fp4_quantize_args* args, void* strea
   AWQB_FP4_CHECK(K, format, dtype, scale);
   AWQB_REQUIRE(rows >= 0 && rows <= 0x7fffffff && rows_in >= 0 && rows_in <= 0x7fffffff, kInvalidArgument,
                "too many rows (%lld)", (long long)rows);
-  AWQB_REQUIRE(index != nullptr || rows == rows_in, kInvalidArgument, "without an index, rows are those of x");
+  // (an empty index may have no address)
+  AWQB_REQUIRE(index != nullptr || rows == rows_in || rows == 0, kInvalidArgument, "without an index, rows are those of x");
   AWQB_REQUIRE(per_row >= 1 && per_row <= 0x7fffffff, kInvalidArgument, "per_row must be at least 1");
   AWQB_REQUIRE(ldx >= K && ldx % 8 == 0, kInvalidArgument, "the row stride of x must be >= K and a multiple of 8");
   if (rows == 0) return kOk;

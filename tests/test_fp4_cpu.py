@@ -37,6 +37,13 @@ def test_quantize_refusals(change, text):
     _refused("awqb_fp4_quantize", Q, change, text)
 
 
+def test_quantize_takes_an_empty_index():
+    """A list of no rows has no address; nothing is launched for it."""
+    args = list(Q)
+    args[10], args[11], args[12] = 0, None, None
+    assert _lib.lib().awqb_fp4_quantize(_lib.FP4_ARGS["awqb_fp4_quantize"].pack(*(0 if v is None else v for v in args)), None) == 0
+
+
 D = [P, P, 8, 256, 0, 1, P, P, 256]
 
 

@@ -149,6 +149,16 @@ def test_quantize_gathered(cuda, fmt, per_row):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_by_an_empty_index(cuda, fmt):
+    x = _normal(cuda, 5, 96, torch.float16)
+    index = torch.zeros(4, dtype=torch.int32, device=cuda)
+    for empty in (torch.empty(0, dtype=torch.int32, device=cuda), index[4:]):
+        for kw in ({}, {"per_row": 3, "count": index[:1]}):
+            codes, scales = ops.fp4_quantize(x, fmt, index=empty, **kw)
+            assert codes.shape == (0, 48) and scales.shape[1:] == (0, 16)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("count", [-3, 0, 1, 6, 9, 100])
 def test_quantize_up_to_a_count_on_the_device(cuda, fmt, count):
     x = _normal(cuda, 9, 96, torch.float16)
