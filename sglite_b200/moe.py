@@ -154,7 +154,7 @@ class FP4ExpertWeights:
         if w.dim() != 3 or w.element_size() != 1 or scales.element_size() != 1 \
                 or scales.shape != (*w.shape[:2], 2 * w.shape[2] // ops.FP4_BLOCK[fmt]):
             raise ValueError(f"w {tuple(w.shape)} and scales {tuple(scales.shape)} are not {fmt} experts")
-        w, scales = w.view(torch.uint8), scales.view(torch.uint8)
+        w, scales = (t.as_subclass(torch.Tensor).view(torch.uint8) for t in (w, scales))
         if gate_up:
             w, scales = ops.fp4_interleave_gate_up(w), ops.fp4_interleave_gate_up(scales)
         return cls(w.contiguous(), ops.fp4_lay_out_scales(scales, fmt), fmt, act_dtype, w_scale, x_scale, e_begin,

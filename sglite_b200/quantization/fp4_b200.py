@@ -24,6 +24,32 @@ from .base_config import LinearMethodBase, QuantizationConfig, set_weight_attrs
 FP4Rows = Tuple[torch.Tensor, torch.Tensor]
 
 
+class CheckpointBytes(torch.Tensor):
+    """Bytes that a loader fills from a checkpoint. uint8, but a checkpoint may type them
+    (scales as float8_e4m3fn or float8_e8m0fnu): copied into these, or into a slice of these,
+    they keep their bits, where a plain uint8 tensor would take their values (0.5 as 0)."""
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        kwargs = kwargs or {}
+        if func in (torch.Tensor.copy_, torch.Tensor.__setitem__):
+            args = (args[0], *map(_as_bytes, args[1:]))
+            kwargs = {k: _as_bytes(v) for k, v in kwargs.items()}
+        return super().__torch_function__(func, types, args, kwargs)
+
+
+def _as_bytes(value):
+    if not isinstance(value, torch.Tensor) or not value.is_floating_point():
+        return value
+    if value.element_size() != 1:
+        raise ValueError(f"bytes of a checkpoint cannot be taken from {value.dtype} values")
+    return value.view(torch.uint8)
+
+
+def _checkpoint_bytes(rows: int, columns: int) -> Parameter:
+    return Parameter(torch.empty(rows, columns, dtype=torch.uint8).as_subclass(CheckpointBytes), requires_grad=False)
+
+
 def tensor_scale(w: torch.Tensor) -> torch.Tensor:
     """The fp32 [1] scale under which the largest block scale of w is e4m3's largest value."""
     most = w.abs().amax().float().reshape(1)
@@ -94,8 +120,9 @@ class FP4B200LinearMethod(LinearMethodBase):
 
     def create_weights(self, input_size: int, output_size: int) -> Dict[str, Any]:
         """weight [N, K / 2] (uint8, the value with the even k in the low bits),
-        weight_scale [N, K / block] (bytes), and for nvfp4 weight_scale_2 and input_scale
-        (fp32 [1]; input_scale is the scale of the activations and starts at one)."""
+        weight_scale [N, K / block] (bytes, also where the checkpoint types them as 8-bit
+        floats: CheckpointBytes), and for nvfp4 weight_scale_2 and input_scale (fp32 [1];
+        input_scale is the scale of the activations and starts at one)."""
         block = self.quant_config.group_size
         if input_size % 32:
             raise ValueError(f"input_size={input_size} must be a multiple of 32. "
@@ -103,9 +130,9 @@ class FP4B200LinearMethod(LinearMethodBase):
         if output_size % 8:
             raise ValueError(f"output_size={output_size} must be a multiple of 8. "
                              "This can be caused by too large tensor parallel size.")
-        weight = Parameter(torch.empty(output_size, input_size // 2, dtype=torch.uint8), requires_grad=False)
+        weight = _checkpoint_bytes(output_size, input_size // 2)
         set_weight_attrs(weight, {"input_dim": 1, "output_dim": 0, "packed_dim": 1, "pack_factor": 2})
-        scale = Parameter(torch.empty(output_size, input_size // block, dtype=torch.uint8), requires_grad=False)
+        scale = _checkpoint_bytes(output_size, input_size // block)
         set_weight_attrs(scale, {"input_dim": 1, "output_dim": 0})
         weights = {"weight": weight, "weight_scale": scale, "_input_size": input_size, "_output_size": output_size,
                    "_weights_processed": False}
@@ -117,7 +144,7 @@ class FP4B200LinearMethod(LinearMethodBase):
     def process_weights_after_loading(self, weights: Dict[str, Any]) -> Dict[str, Any]:
         if weights.get("_weights_processed", False):
             return weights
-        weight, scale = weights["weight"].data, weights["weight_scale"].data
+        weight, scale = (weights[name].data.as_subclass(torch.Tensor) for name in ("weight", "weight_scale"))
         if weight.device.type != "cuda":
             raise RuntimeError("FP4 B200 weights must be loaded on a CUDA device before their scales are laid out")
         N, K = weights["_output_size"], weights["_input_size"]

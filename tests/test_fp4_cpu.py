@@ -258,6 +258,29 @@ def test_created_weights(fmt):
         method.apply_weights(w, torch.zeros((1, 96), dtype=torch.bfloat16))
 
 
+@pytest.mark.parametrize("fmt,kind", [("nvfp4", torch.float8_e4m3fn), ("mxfp4", torch.float8_e8m0fnu)])
+def test_typed_scales_of_a_checkpoint_keep_their_bits(fmt, kind):
+    """Block scales typed as 8-bit floats, copied in place as loaders do, whole and by shards."""
+    from sglite_b200.quantization.fp4_b200 import FP4B200Config
+
+    method = FP4B200Config(fmt).get_linear_method()
+    want = torch.randint(0, 255, (24, 96 // BLOCK[fmt]), dtype=torch.uint8)
+    typed = want.view(kind)
+    fills = [lambda p: p.data.copy_(typed), lambda p: p.copy_(typed), lambda p: p.copy_(other=typed),
+             lambda p: p.data[:8].copy_(typed[:8]) is p.data.narrow(0, 8, 16).copy_(typed.narrow(0, 8, 16)),
+             lambda p: p.data.__setitem__(slice(None), typed), lambda p: p.data.copy_(want), lambda p: p.data.copy_(want.int()),
+             lambda p: [p.data[:, k:k + 1].copy_(typed[:, k:k + 1]) for k in range(typed.shape[1])]]
+    for fill in fills:
+        w = method.create_weights(96, 24)
+        w["weight_scale"].data.zero_()
+        fill(w["weight_scale"])
+        assert isinstance(w["weight_scale"], torch.nn.Parameter) and w["weight_scale"].dtype == torch.uint8
+        assert torch.equal(w["weight_scale"].data, want)
+        assert torch.equal(ops.fp4_lay_out_scales(w["weight_scale"].data, fmt), ops.fp4_lay_out_scales(want, fmt))
+    with pytest.raises(ValueError, match="bytes"):
+        w["weight_scale"].data.copy_(want.float())
+
+
 def test_interleaved_gate_up():
     t = torch.arange(12).view(6, 2)
     assert ops.fp4_interleave_gate_up(t)[:, 0].tolist() == [0, 6, 2, 8, 4, 10]
