@@ -98,8 +98,13 @@ class FP4B200Config(QuantizationConfig):
 
     @classmethod
     def from_config(cls, config: Dict[str, Any]) -> "FP4B200Config":
-        """``quant_algo`` or ``quant_method`` names the format (NVFP4 / MXFP4, any case)."""
+        """``quant_algo``, ``format`` or ``quant_method`` names the format (NVFP4 / MXFP4, any
+        case; modelopt_fp4 is NVFP4), at the top or, as hf_quant_config.json has it, under
+        ``quantization``."""
+        inner = config.get("quantization")
+        config = inner if isinstance(inner, dict) else config
         fmt = str(cls.get_from_keys(config, ["quant_algo", "format", "quant_method"])).lower()
+        fmt = "nvfp4" if fmt == "modelopt_fp4" else fmt
         group = config.get("group_size")
         if group is not None and fmt in ops.FP4_BLOCK and group != ops.FP4_BLOCK[fmt]:
             raise ValueError(f"{fmt} has blocks of {ops.FP4_BLOCK[fmt]}, got group_size={group}")

@@ -240,6 +240,21 @@ def test_config():
         FP4B200Config("int4")
 
 
+def test_config_of_a_checkpoint_file():
+    """hf_quant_config.json keeps its entries under "quantization"."""
+    from sglite_b200.quantization.fp4_b200 import FP4B200Config
+
+    assert FP4B200Config.get_config_filenames()[0] == "hf_quant_config.json"
+    inner = {"quant_algo": "NVFP4", "kv_cache_quant_algo": None, "group_size": 16, "exclude_modules": ["lm_head"]}
+    assert FP4B200Config.from_config({"producer": {"name": "x", "version": "1"}, "quantization": inner}).fmt == "nvfp4"
+    assert FP4B200Config.from_config({"quant_method": "modelopt_fp4"}).fmt == "nvfp4"
+    for bad in ({**inner, "group_size": 32}, {**inner, "quant_algo": "FP8"}, {"group_size": 16}):
+        with pytest.raises(ValueError):
+            FP4B200Config.from_config({"quantization": bad})
+    with pytest.raises(ValueError):  # its tensors have other names, and its global scale is the reciprocal
+        FP4B200Config.from_config({"quant_method": "compressed-tensors", "format": "nvfp4-pack-quantized"})
+
+
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 def test_created_weights(fmt):
     from sglite_b200.quantization.fp4_b200 import FP4B200Config
