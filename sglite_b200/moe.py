@@ -125,6 +125,8 @@ class FP4ExpertWeights:
     x_scale: Optional[torch.Tensor] = None   # fp32 [1]: the scale of this projection's input (nvfp4)
     e_begin: int = 0             # first global expert id held here
     num_global_experts: Optional[int] = None
+    # gate and up rows by turns, as w1 has to have them; None: not recorded, the caller answers for it
+    gate_up_interleaved: Optional[bool] = None
 
     @property
     def num_experts(self) -> int:
@@ -146,11 +148,13 @@ class FP4ExpertWeights:
     def from_checkpoint(cls, w: torch.Tensor, scales: torch.Tensor, fmt: str, act_dtype: torch.dtype,
                         w_scale: Optional[torch.Tensor] = None, x_scale: Optional[torch.Tensor] = None,
                         e_begin: int = 0, num_global_experts: Optional[int] = None,
-                        gate_up: bool = False) -> "FP4ExpertWeights":
+                        gate_up: bool = False, gate_up_interleaved: bool = False) -> "FP4ExpertWeights":
         """w uint8 [E, N, K / 2] and block scales (bytes) [E, N, K / 16 or K / 32] as stacked
         from a checkpoint, on the device. gate_up=True for the merged gate_up projection (the
         gate's rows, then the up's): its rows are interleaved, as the SiLU-and-mul epilogue
-        wants them."""
+        wants them. gate_up_interleaved=True where the checkpoint's rows are by turns already."""
+        if gate_up and gate_up_interleaved:
+            raise ValueError("gate_up interleaves the rows: they cannot be by turns already")
         if w.dim() != 3 or w.element_size() != 1 or scales.element_size() != 1 \
                 or scales.shape != (*w.shape[:2], 2 * w.shape[2] // ops.FP4_BLOCK[fmt]):
             raise ValueError(f"w {tuple(w.shape)} and scales {tuple(scales.shape)} are not {fmt} experts")
@@ -158,7 +162,7 @@ class FP4ExpertWeights:
         if gate_up:
             w, scales = ops.fp4_interleave_gate_up(w), ops.fp4_interleave_gate_up(scales)
         return cls(w.contiguous(), ops.fp4_lay_out_scales(scales, fmt), fmt, act_dtype, w_scale, x_scale, e_begin,
-                   num_global_experts)
+                   num_global_experts, gate_up or gate_up_interleaved)
 
 
 def choose_block_m(num_tokens: int, topk: int, num_experts: int) -> int:
@@ -262,6 +266,9 @@ class AWQB200MoeBackend(BaseMoeBackend):
                      topk_weights: torch.Tensor, topk_ids: torch.Tensor) -> torch.Tensor:
         """The same over 4-bit experts: rows are quantised as they are gathered, and again
         between the two products."""
+        if w1.gate_up_interleaved is False or w2.gate_up_interleaved:
+            raise ValueError("w1's gate and up rows must be by turns, w2's rows in order: "
+                             "from_checkpoint(.., gate_up=True) for w1 only")
         M, H = x.shape
         topk = topk_ids.shape[1]
         if M * topk == 0:

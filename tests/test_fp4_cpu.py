@@ -313,3 +313,30 @@ def test_experts_from_a_checkpoint_are_checked():
     for bad in ((w, s[:, :, :2]), (w[0], s[0]), (w.int(), s), (w, s.float())):
         with pytest.raises(ValueError):
             FP4ExpertWeights.from_checkpoint(*bad, "nvfp4", torch.bfloat16)
+
+
+def test_experts_record_the_order_of_their_rows():
+    """Gate and up rows in the wrong order are refused, not multiplied to something else."""
+    from sglite_b200.moe import AWQB200MoeBackend, FP4ExpertWeights
+
+    E, H, I = 2, 64, 32
+    T = torch.bfloat16
+
+    def experts(N, K, **kw):
+        w, s = torch.zeros((E, N, K // 2), dtype=torch.uint8), torch.zeros((E, N, K // 16), dtype=torch.uint8)
+        return FP4ExpertWeights.from_checkpoint(w, s, "nvfp4", T, **kw)
+
+    by_turns, plain = experts(2 * I, H, gate_up=True), experts(2 * I, H)
+    assert by_turns.gate_up_interleaved and plain.gate_up_interleaved is False
+    already, down = experts(2 * I, H, gate_up_interleaved=True), experts(H, I)
+    assert already.gate_up_interleaved and torch.equal(already.w, plain.w)
+    with pytest.raises(ValueError):
+        experts(2 * I, H, gate_up=True, gate_up_interleaved=True)
+    backend, x = AWQB200MoeBackend(), torch.zeros((0, H), dtype=T)  # (no rows: no kernel runs)
+    none = torch.zeros((0, 2)), torch.zeros((0, 2), dtype=torch.int32)
+    made = FP4ExpertWeights(by_turns.w, by_turns.w_scales, "nvfp4", T)
+    for w1 in (by_turns, already, made):
+        assert backend.experts(x, w1, down, *none) is x
+    for w1, w2 in ((plain, down), (by_turns, experts(H, I, gate_up=True))):
+        with pytest.raises(ValueError, match="by turns"):
+            backend.experts(x, w1, w2, *none)
