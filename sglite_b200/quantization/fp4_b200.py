@@ -51,9 +51,11 @@ def _checkpoint_bytes(rows: int, columns: int) -> Parameter:
 
 
 def tensor_scale(w: torch.Tensor) -> torch.Tensor:
-    """The fp32 [1] scale under which the largest block scale of w is e4m3's largest value."""
-    most = w.abs().amax().float().reshape(1)
-    return torch.where(most > 0, most / (6.0 * 448.0), 1.0)
+    """The fp32 [1] scale under which the largest block scale of w's finite values is e4m3's
+    largest value. (An infinity would make it infinite and all other values 0, a NaN leave it
+    at 1, where small weights lose most of their bits.) At least 2^-126, so that 1 / scale is finite."""
+    most = torch.nan_to_num(w, nan=0.0, posinf=0.0, neginf=0.0).abs().amax().float().reshape(1)
+    return torch.where(most > 0, (most / (6.0 * 448.0)).clamp(min=2.0 ** -126), 1.0)
 
 
 def quantize_weight(w: torch.Tensor, fmt: str) -> Dict[str, torch.Tensor]:

@@ -296,6 +296,24 @@ def test_typed_scales_of_a_checkpoint_keep_their_bits(fmt, kind):
         w["weight_scale"].data.copy_(want.float())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scale_of_a_tensor_is_that_of_its_finite_values(dtype):
+    from sglite_b200.quantization.fp4_b200 import tensor_scale
+
+    w = (torch.randn((8, 64), generator=torch.Generator().manual_seed(1)) * 0.02).to(dtype)
+    want = w.abs().amax().float().reshape(1) / 2688
+    assert torch.equal(tensor_scale(w), want)
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        one = w.clone()
+        at = int(w.abs().flatten().argmin())
+        one.view(-1)[at] = bad
+        assert torch.equal(tensor_scale(one), want)
+    assert torch.equal(tensor_scale(torch.zeros_like(w)), torch.ones(1))
+    if dtype is torch.bfloat16:
+        tiny = tensor_scale((w.double() * 2.0 ** -125).to(dtype))
+        assert 0 < float(1 / tiny) < float("inf")
+
+
 def test_interleaved_gate_up():
     t = torch.arange(12).view(6, 2)
     assert ops.fp4_interleave_gate_up(t)[:, 0].tolist() == [0, 6, 2, 8, 4, 10]

@@ -69,6 +69,24 @@ def test_linear_method(cuda, fmt, shape, dtype):
     assert method.process_weights_after_loading(weights) is weights
 
 
+def test_quantised_weight_with_an_infinity_or_a_nan(cuda):
+    """The block is NaN, and the others are as they are without it; so are tiny weights."""
+    w = _normal(cuda, 16, 256, std=0.02)
+    clean = quantize_weight(w, "nvfp4")
+    for bad in (float("inf"), float("nan")):
+        one = w.clone()
+        one[3, 40] = bad
+        got = quantize_weight(one, "nvfp4")
+        values = values_ref(got["weight"], got["weight_scale"], "nvfp4") * float(got["weight_scale_2"])
+        want = values_ref(clean["weight"], clean["weight_scale"], "nvfp4") * float(clean["weight_scale_2"])
+        block = torch.zeros((16, 256), dtype=torch.bool)
+        block[3, 32:48] = True
+        assert bool(torch.isnan(values[block]).all()) and torch.equal(values[~block], want[~block])
+    tiny = quantize_weight((w.double() * 2.0 ** -120).to(w.dtype), "nvfp4")
+    values = values_ref(tiny["weight"], tiny["weight_scale"], "nvfp4") * float(tiny["weight_scale_2"])
+    assert bool(torch.isfinite(values).all()) and bool((values != 0).any())
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_one_row_without_a_batch_and_rows_from_the_middle(cuda, fmt):
     """x [K] as a row, and weights and x that start inside a larger tensor: the same bits."""
