@@ -1,7 +1,7 @@
 // What the kernels over ragged groups of rows share: a group's rows cut into equal
-// token tiles, tiles found on the device from the groups' offsets, and the epilogues'
-// small parts. P is a kernel's parameter structure (offsets, row_map, row_scale,
-// out_rows, rows, E, feat_tiles, tile_out), C its constants (kTok, kRound, kThreads).
+// token tiles, tiles found on the device from the groups' offsets, SiLU-and-mul. P is a
+// kernel's parameter structure (offsets, rows, E, feat_tiles, tile_out), C its
+// constants (kTok, kRound, kThreads).
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -10,7 +10,6 @@
 
 #include "awqb_common.h"
 #include "awqb_ptx.cuh"
-#include "awqb_vec.cuh"
 
 namespace awqb {
 namespace {
@@ -52,14 +51,12 @@ __device__ __forceinline__ Tile find_tile(const Groups& g, const P& p, int t) {
   return r;
 }
 
-// Builds the tables of the groups from the offsets (clamped to the rows; without
-// offsets, one group of all rows); all threads, with a barrier still to come before
-// they are read.
+// Builds the tables of the groups from the offsets (clamped to the rows); all
+// threads, with a barrier still to come before they are read.
 template <typename C, typename P>
 __device__ __forceinline__ void build_groups(const Groups& g, const P& p) {
   for (int e = threadIdx.x; e < p.E; e += C::kThreads) {
-    const int r0 = p.offsets ? min(max(p.offsets[e], 0), p.rows) : 0;
-    const int r1 = p.offsets ? min(max(p.offsets[e + 1], 0), p.rows) : p.rows;
+    const int r0 = min(max(p.offsets[e], 0), p.rows), r1 = min(max(p.offsets[e + 1], 0), p.rows);
     g.row0[e] = r0;
     g.row0[p.E + e] = max(r1 - r0, 0);
   }
@@ -81,49 +78,13 @@ __device__ __forceinline__ void build_groups(const Groups& g, const P& p) {
   }
 }
 
-// Where a tile's rows go in out, and their factors, into shared memory.
-template <typename P>
-__device__ __forceinline__ void load_rows(const P& p, const Tile& tile, int first, int step, int* dst, float* scl) {
-  for (int i = first; i < tile.rows; i += step) {
-    const int to = p.row_map ? p.row_map[tile.row0 + i] : tile.row0 + i;
-    const bool in = to >= 0 && to < p.out_rows;
-    dst[i] = in ? to : -1;
-    if (p.row_scale) scl[i] = in ? p.row_scale[to] : 0.f;
-  }
-}
-
 // silu(g) * u with the approximate exponential and division: right to
 // (6 + 1.173 |g|) 2^-23 of the value (1.2e-5 at g = -80; 16-bit results keep 2^-11 at
 // best), and 0 below g = -87.3, where |silu(g)| < 88 * 2^-126.
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
-// Eight lanes, kStep apart, hold eight values each: v[t] of feature l, l = 0..7 their
-// number. Afterwards lane l holds value l of all eight features, rounded to 16 bits.
-template <typename T, int kStep>
-__device__ __forceinline__ uint4 transpose8(const float* v, int lane) {
-  const bool b2 = lane & (4 * kStep), b1 = lane & (2 * kStep), b0 = lane & kStep;
-  uint32_t r[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = Pair<T>::pack(v[2 * i], v[2 * i + 1]);
-  // values 0..3 to the lower four lanes, 4..7 to the upper ones; x[feature bit 2][pair]
-  const uint32_t g0 = __shfl_xor_sync(0xffffffffu, b2 ? r[0] : r[2], 4 * kStep);
-  const uint32_t g1 = __shfl_xor_sync(0xffffffffu, b2 ? r[1] : r[3], 4 * kStep);
-  const uint32_t x00 = b2 ? g0 : r[0], x01 = b2 ? g1 : r[1], x10 = b2 ? r[2] : g0, x11 = b2 ? r[3] : g1;
-  // the pair of this lane's value; y[feature bit 2][feature bit 1]
-  const uint32_t h0 = __shfl_xor_sync(0xffffffffu, b1 ? x00 : x01, 2 * kStep);
-  const uint32_t h1 = __shfl_xor_sync(0xffffffffu, b1 ? x10 : x11, 2 * kStep);
-  const uint32_t y00 = b1 ? h0 : x00, y01 = b1 ? x01 : h0, y10 = b1 ? h1 : x10, y11 = b1 ? x11 : h1;
-  // the half of the pair; the neighbour's goes as the other feature of each word
-  const uint32_t send = b0 ? 0x5410u : 0x7632u;  // lower halves, or upper ones
-  const uint32_t k0 = __shfl_xor_sync(0xffffffffu, __byte_perm(y00, y01, send), kStep);
-  const uint32_t k1 = __shfl_xor_sync(0xffffffffu, __byte_perm(y10, y11, send), kStep);
-  const uint32_t low = b0 ? 0x3254u : 0x5410u, high = b0 ? 0x3276u : 0x7610u;
-  return make_uint4(__byte_perm(y00, k0, low), __byte_perm(y01, k0, high), __byte_perm(y10, k1, low),
-                    __byte_perm(y11, k1, high));
-}
-
 // The smallest box that holds `rows` token rows.
-__host__ __device__ __forceinline__ int box_of(int rows, int most) { return rows * 4 <= most ? 0 : rows * 2 <= most ? 1 : 2; }
+__device__ __forceinline__ int box_of(int rows, int most) { return rows * 4 <= most ? 0 : rows * 2 <= most ? 1 : 2; }
 
 // Clusters that run at once (a GPC with an odd number of SMs leaves one idle),
 // per device; the persistent grid must not exceed it.

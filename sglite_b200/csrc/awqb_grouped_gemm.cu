@@ -73,6 +73,41 @@ struct Params {
   int rows, E, K, N, n_out, silu, feat_tiles, tile_out;  // output features of a tile
 };
 
+// Where a tile's rows go in out, and their factors, into shared memory.
+__device__ __forceinline__ void load_rows(const Params& p, const Tile& tile, int first, int step, int* dst, float* scl) {
+  for (int i = first; i < tile.rows; i += step) {
+    const int to = p.row_map ? p.row_map[tile.row0 + i] : tile.row0 + i;
+    const bool in = to >= 0 && to < p.out_rows;
+    dst[i] = in ? to : -1;
+    if (p.row_scale) scl[i] = in ? p.row_scale[to] : 0.f;
+  }
+}
+
+// Eight lanes, kStep apart, hold eight values each: v[t] of feature l, l = 0..7 their
+// number. Afterwards lane l holds value l of all eight features, rounded to 16 bits.
+template <typename T, int kStep>
+__device__ __forceinline__ uint4 transpose8(const float* v, int lane) {
+  const bool b2 = lane & (4 * kStep), b1 = lane & (2 * kStep), b0 = lane & kStep;
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = Pair<T>::pack(v[2 * i], v[2 * i + 1]);
+  // values 0..3 to the lower four lanes, 4..7 to the upper ones; x[feature bit 2][pair]
+  const uint32_t g0 = __shfl_xor_sync(0xffffffffu, b2 ? r[0] : r[2], 4 * kStep);
+  const uint32_t g1 = __shfl_xor_sync(0xffffffffu, b2 ? r[1] : r[3], 4 * kStep);
+  const uint32_t x00 = b2 ? g0 : r[0], x01 = b2 ? g1 : r[1], x10 = b2 ? r[2] : g0, x11 = b2 ? r[3] : g1;
+  // the pair of this lane's value; y[feature bit 2][feature bit 1]
+  const uint32_t h0 = __shfl_xor_sync(0xffffffffu, b1 ? x00 : x01, 2 * kStep);
+  const uint32_t h1 = __shfl_xor_sync(0xffffffffu, b1 ? x10 : x11, 2 * kStep);
+  const uint32_t y00 = b1 ? h0 : x00, y01 = b1 ? x01 : h0, y10 = b1 ? h1 : x10, y11 = b1 ? x11 : h1;
+  // the half of the pair; the neighbour's goes as the other feature of each word
+  const uint32_t send = b0 ? 0x5410u : 0x7632u;  // lower halves, or upper ones
+  const uint32_t k0 = __shfl_xor_sync(0xffffffffu, __byte_perm(y00, y01, send), kStep);
+  const uint32_t k1 = __shfl_xor_sync(0xffffffffu, __byte_perm(y10, y11, send), kStep);
+  const uint32_t low = b0 ? 0x3254u : 0x5410u, high = b0 ? 0x3276u : 0x7610u;
+  return make_uint4(__byte_perm(y00, k0, low), __byte_perm(y01, k0, high), __byte_perm(y10, k1, low),
+                    __byte_perm(y11, k1, high));
+}
+
 template <typename T>
 __global__ void __launch_bounds__(Few::kThreads, 1)
 grouped_gemm_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ TokenMaps tm_x,
