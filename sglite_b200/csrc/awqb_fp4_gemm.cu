@@ -1019,8 +1019,10 @@ extern "C" int awqb_fp4_gemm(const awqb_fp4_gemm_args* args, void* stream) {
   AWQB_REQUIRE(offsets == nullptr || bias == nullptr, kInvalidArgument, "a bias is for a product without groups");
   AWQB_REQUIRE(K > 0 && K % 32 == 0 && K <= (1 << 20), kInvalidArgument, "K=%lld must be a positive multiple of 32",
                (long long)K);
-  AWQB_REQUIRE(N > 0 && N % (silu_mul ? 16 : 8) == 0 && E * N <= 0x7fffffff, kInvalidArgument,
-               "N=%lld must be a positive multiple of %d", (long long)N, silu_mul ? 16 : 8);
+  // (a pair's rows behind the last one still have 32-bit coordinates; N first, so that E * N cannot overflow)
+  AWQB_REQUIRE(N > 0 && N % (silu_mul ? 16 : 8) == 0 && N <= 0x7fffff00 && E * N <= 0x7fffff00, kInvalidArgument,
+               "N=%lld must be a positive multiple of %d, and all experts' rows fewer than 2^31 - 255", (long long)N,
+               silu_mul ? 16 : 8);
   AWQB_REQUIRE(rows >= 0 && rows <= (1 << 30) && out_rows >= 0, kInvalidArgument, "bad row count %lld", (long long)rows);
   const int64_t n_out = silu_mul ? N / 2 : N;
   AWQB_REQUIRE(ldo >= n_out && ldo % 8 == 0, kInvalidArgument, "the row stride of out must be >= %lld and a multiple of 8",

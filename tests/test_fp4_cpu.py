@@ -82,6 +82,12 @@ def test_gemm_refusals(change, text):
     _refused("awqb_fp4_gemm", G, change, text)
 
 
+@pytest.mark.parametrize("E,N", [(1, 0x7ffffff8), (1, 0x7fffff08), (8, 1 << 28), (1024, 1 << 60)])
+def test_weights_of_more_rows_than_coordinates_are_refused(E, N):
+    """Up to where the last tile's rows still count in 32 bits; E * N itself may pass 64."""
+    _refused("awqb_fp4_gemm", G, {"_6": E, "_7": N, "_19": N}, b"N=")
+
+
 def test_null_arguments_are_refused():
     for name in _lib.FP4_ARGS:
         assert getattr(_lib.lib(), name)(None, None) == 1
