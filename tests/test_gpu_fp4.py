@@ -443,6 +443,14 @@ def test_grouped_epilogues(cuda, sizes, silu, scatter, first, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("silu,scatter", [(False, True), (True, False)])
+@pytest.mark.parametrize("K,sizes", [(2048, [1, 0, 2, 1]), (288, [0, 3, 0, 0]), (1024, [0, 0, 0, 0])])
+def test_grouped_few_live_rows_of_a_large_buffer(cuda, K, sizes, silu, scatter, fmt):
+    """A rank whose experts got few of the buffer's rows: the kernel for many rows with a few."""
+    _grouped(cuda, sizes, K, 272, fmt, torch.bfloat16, silu, pad=500, scatter=scatter)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("sizes", [[1] * 1024, [0] * 1000 + [3] * 24, [100] + [0] * 1023])
 def test_grouped_of_a_thousand_experts(cuda, sizes, fmt):
     _grouped(cuda, sizes, 64, 24, fmt, torch.float16, pad=2)

@@ -107,6 +107,36 @@ def test_one_row_without_a_batch_and_rows_from_the_middle(cuda, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M", [1, 45, 200])
+def test_shards_of_a_projection(cuda, fmt, M):
+    """A rank's rows (column-parallel) or k (row-parallel) of weight and weight_scale, copied into
+    the tensors of create_weights: the product of just those."""
+    K, N, ranks, dtype = 1152, 528, 3, torch.bfloat16
+    block = ops.FP4_BLOCK[fmt]
+    loaded = quantize_weight(_normal(cuda, N, K, dtype=dtype, std=K ** -0.5), fmt)
+    values, ws = values_ref(loaded["weight"], loaded["weight_scale"], fmt), loaded.get("weight_scale_2")
+    x = _normal(cuda, M, K, dtype=dtype)
+    method = get_quantization_config("fp4_b200")(fmt).get_linear_method()
+
+    def shard(n, k):
+        w = method.create_weights(k.stop - k.start, n.stop - n.start)
+        for name, per in (("weight", 2), ("weight_scale", block)):
+            w[name] = torch.nn.Parameter(w[name].data.to(cuda), requires_grad=False)
+            w[name].data.copy_(loaded[name][n, k.start // per:k.stop // per])
+        if fmt == "nvfp4":
+            w["weight_scale_2"].data, w["input_scale"].data = ws.clone(), torch.full((1,), 0.01, device=cuda)
+        w = method.process_weights_after_loading(w)
+        xs = w.get("input_scale")
+        y, bound = product_ref(_held(x[:, k], fmt, xs), values[n, k], xs, ws)
+        got = method.apply_weights(w, x[:, k])
+        assert within(got.cpu(), y, bound, dtype) <= 0
+
+    for r in range(ranks):
+        shard(slice(N // ranks * r, N // ranks * (r + 1)), slice(0, K))
+        shard(slice(0, N), slice(K // ranks * r, K // ranks * (r + 1)))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_gate_up_and_quantised_rows(cuda, fmt):
     """The norm's rows straight into gate_up with SiLU-and-mul; the gate and up halves of the
     plain projection give the same."""
