@@ -433,7 +433,8 @@ typedef struct {
 int awqb_fp4_dequantize(const awqb_fp4_dequantize_args* args, void* stream);
 /* h = x + residual (stored to residual_out, rounded; residual null: h = x, and
  * nothing is stored), quantised h * rsqrt(mean(h^2) + eps) * weight, the norm over the
- * unrounded h and not rounded before its quantisation. residual_out may be residual.
+ * unrounded h and not rounded before its quantisation, for rows of any finite size; where
+ * a row holds an infinity, all finite values of it are 0. residual_out may be residual.
  * K <= 16384. */
 typedef struct {
   const void* x;
@@ -462,7 +463,7 @@ int awqb_fp4_add_rmsnorm(const awqb_fp4_add_rmsnorm_args* args, void* stream);
  * y[r] goes to row r of out, or to row_map[r] (rows that map outside 0..out_rows - 1
  * are dropped, no two to one), times row_scale[its row of out] if given; rows of out
  * that nothing maps to are left as they were. N is a multiple of 8 (16 with
- * silu_mul), ldo of 8. E <= 1024. out must not overlap the inputs. */
+ * silu_mul), ldo of 8. E <= 1024, E * N <= 2^31 - 256. out must not overlap the inputs. */
 typedef struct {
   const void* codes;
   const uint8_t* scales;

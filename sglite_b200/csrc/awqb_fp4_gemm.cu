@@ -27,14 +27,14 @@
 // tokens, two CTAs to an SM, eight stages of 23 KB in flight there. Where the tiles of a
 // product do not fill the GPU, two to eight CTAs of a cluster share a tile's K, and each adds
 // its share of the tokens from what the others send to its shared memory (1 token
-// 4096 -> 4096: 7.9 us whole, 5.6 by four). Many rows: a CTA pair takes 256 weight rows x up to
+// 4096 -> 4096: 7.7 us whole, 5.3 by four). Many rows: a CTA pair takes 256 weight rows x up to
 // 208 tokens, what two accumulators and two sets of scales leave of tensor memory; K is
 // shared by two or four pairs where tiles are few. On a B200: 1 token 4096 -> 6144 in 6.1 us, 32
-// tokens 4096 -> 28672 with SiLU-and-mul in 13.9 (4.8 TB/s), 4096 tokens 8192 -> 28672 in 375
-// (5.1 PFLOP/s; 441 when repeated for seconds, at 1.37 GHz under the power cap) and in 350 in
-// mxfp4. Copies of that kernel which leave work out: 321 us without the scales' copies to tensor
-// memory, 289 without the products, 323 without both; so no one of them bounds it, and the loop
-// around them takes most of what they take.
+// tokens 4096 -> 28672 with SiLU-and-mul in 13.8 (4.9 TB/s), 4096 tokens 8192 -> 28672 in 383
+// (5.0 PFLOP/s; 443 when repeated for seconds, under the power cap) and in 360 in mxfp4.
+// Copies of that kernel which leave work out (374 us whole on that GPU): 321 without the scales'
+// copies to tensor memory, 289 without the products, 323 without both. The last is slower than the
+// one before it, so the series says that neither alone bounds it, and not what the loop waits for.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -989,7 +989,9 @@ template <typename T, bool kNv>
 int pick(const void* codes, const void* w, const Params& p, cudaStream_t stream) {
   // Groups: by their mean rows, since the CTA pairs' epilogue and start cost more and are
   // spread over K's stages (us, few-rows and many-rows kernel, 2048 -> 1536 x 128 experts: 39 and 40 for
-  // 12 rows, 43 and 41 for 16, 53 and 44 for 48; 768 -> 2048: 31 and 33 for 32, 39 and 36 for 48). One group:
+  // 12 rows, 43 and 41 for 16, 53 and 44 for 48; 768 -> 2048: 31 and 33 for 32, 39 and 36 for 48. The
+  // border, 20, is past that of the first series: 16 rows take the slower kernel, by 5 %). The rows
+  // are the buffer's, the only count that the host has: rows behind the last group count too. One group:
   // above 32 rows, unless the few-rows kernel's tiles are few as well (4096 -> 28672, 48 rows: 22
   // and 17; 8192 -> 1024, 128 rows: 7.9 and 9.0).
   const int nk = (p.K + kK - 1) / kK;

@@ -3,10 +3,11 @@
 // formats).
 //
 // All three are bound by HBM. A lane takes vectors of eight values (16-byte loads, whole
-// sectors by neighbouring lanes); all of a thread's loads are issued before the first is
-// used. Launched with programmatic dependent launch, like the other norms. On a B200, 4096
-// bf16 rows of 14336: mxfp4 quantised in 24.4 us (6.1 TB/s), nvfp4 in 30.5 (4.9), read back in
-// 25.4 (5.9); norms of 8192 values in 38.7 in mxfp4 and 42.4 in nvfp4 (5.7 and 5.2 TB/s).
+// sectors by neighbouring lanes), two of them at a time where it only quantises; all of a
+// thread's loads are issued before the first is used. Launched with programmatic dependent
+// launch, like the other norms. On a B200, 4096 bf16 rows of 14336: mxfp4 quantised in 24.4 us
+// (6.1 TB/s), nvfp4 in 30.7 (4.9), read back in 26 (5.8); norms of 8192 values in 40.4 in mxfp4
+// and 43.6 in nvfp4 (5.4 and 5.1 TB/s).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -171,9 +172,12 @@ constexpr int kNormMaxK = kNormThreads * kNormVec * 8;
 // A CTA takes a row and holds it in registers between the sum of squares and the
 // quantisation. h = x + residual is stored rounded; the norm is of the unrounded sum and
 // goes into four bits with no rounding to 16 bits between. A code depends on which side of
-// a border its value lies, so the value is rounded once only: the threads' sums of squares
-// are added in 64 bits, the row's factor (over the tensor's scale) is kept as two fp32
-// numbers, and so is h * weight.
+// a border its value lies, so little is lost on the way: a thread adds its squares (at most
+// 32) and a warp its lanes' sums in fp32, the warps' sums are added in 64 bits; the row's
+// factor (over the tensor's scale) is kept as two fp32 numbers, and so is h * weight. h is
+// rounded to fp32. A square goes through at most 8 + 4 + 5 additions in fp32, 2^-24 each: less
+// than 2^-19.9 of the sum and half of that of its root. With h's rounding and the result's, what
+// is quantised is within 2^-20 of the exact value.
 // h of the thread's vector v, stored; returns its sum of squares.
 template <typename T>
 __device__ __forceinline__ float add_vector(const NormArgs& a, int64_t row, int v, const uint4& x, const uint4& r,
@@ -245,7 +249,8 @@ __device__ __forceinline__ void norm_vector(const NormArgs& a, int64_t row, int 
 // (mxfp4, two vectors: registers for three CTAs to an SM, 4096 rows of 8192 features 45.2 -> 40.2
 // us; nvfp4 is better off with two CTAs and 48 registers: 8192 rows of 4096 features 41.5, 42.1 with three.)
 template <typename T, bool kNv, int kVec>
-__global__ void __launch_bounds__(kNormThreads, kVec > 2 ? 1 : kVec == 2 && !kNv ? 3 : 2) norm_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(kNormThreads, kVec > 2 ? 1 : kVec == 2 && !kNv ? 3 : 2)
+norm_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float red[2][kNormThreads / 32];
   grid_dep_wait();
   grid_dep_launch();
@@ -402,7 +407,7 @@ extern "C" int awqb_fp4_add_rmsnorm(const awqb_fp4_add_rmsnorm_args* args, void*
   const NormArgs a = {x, residual, weight, scale, residual_out, codes, scales, ldx, ldr, ldro, rows, (int)K, vecs, eps,
                       1.0 / (double)K};
   // Vectors per thread: many rows want small CTAs, more of them to an SM (8192 rows of 4096
-  // features: 48.0 us with one, 40.1 with two; 16 rows of 2048: 2.2 and 2.6)
+  // features: 49.4 us with one, 41.8 with two; 16 rows of 2048: 2.15 and 2.56)
   const bool few = rows <= 2 * device_sm_count();
   const int per = vecs <= (few ? kNormThreads : 128) ? 1 : vecs <= 2 * kNormThreads ? 2 : 4;
   const dim3 grid((unsigned)rows), threads((vecs + per - 1) / per + 31 & ~31);

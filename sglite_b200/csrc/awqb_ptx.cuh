@@ -607,9 +607,12 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// The same, releasing at CTA scope only (1600 cycles less under load): for a peer that
-// issues tensor-core work on what this CTA's tensor core then reads, or reuses tensor
-// memory that this CTA has read; it does not read this CTA's memory itself.
+// The same, releasing at CTA scope only: for a peer that issues tensor-core work on what
+// this CTA's own tensor core then reads (written to this CTA's shared memory, and completed
+// for the async proxy by the fence in front of the arrival), or that reuses tensor memory
+// which this CTA has read; the peer does not read this CTA's memory itself. A release at
+// cluster scope from the warps that turn 4-bit scales, once a stage: 395 -> 629 us for 4096
+// tokens 8192 -> 28672.
 __device__ __forceinline__ void mbar_arrive_peer(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }

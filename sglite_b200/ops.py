@@ -1045,7 +1045,8 @@ def fp4_add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: t
                     ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The residual-add RMSNorm in front of a 4-bit projection: h = x + residual,
     y = h * rsqrt(mean(h^2) + eps) * weight, quantised as ``fp4_quantize`` does, straight
-    from fp32. Returns (codes, scales, h), h rounded to x's dtype; without a residual h is x.
+    from fp32, for rows of any finite size (a row with an infinity: finite values over it are 0);
+    eps is taken as fp32. Returns (codes, scales, h), h rounded to x's dtype; without a residual h is x.
     ``residual_out`` may be residual (in place) or x. K is at most 16384."""
     dtype = x.dtype
     fc, code = _fp4_code(fmt, dtype)
